@@ -396,6 +396,77 @@ int awq_w4a16_rmsnorm_gemm(const void* x, int64_t ldx, const void* norm_w, float
                            int32_t layout, int32_t act_dtype, int32_t norm_dtype, int32_t scale_dtype,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- microscaled fp4 (MXFP4) ------------------------------------------------------
+ * The format of the OCP Microscaling Formats specification 1.0: 32 consecutive values along K share a
+ * scale 2^(byte - 127) (byte 255: the whole block is NaN); a value is an e2m1 code (sign, two exponent
+ * bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6).  A [rows, K] matrix is codes [rows, K/2] bytes (the
+ * even index in the low four bits) and scales [rows, K/32] bytes, both dense: the layout of checkpoints,
+ * which the kernels read as it is.  K % 32 == 0; codes 16-byte aligned.  No counterpart in the
+ * reference, whose 4-bit weights are integers. */
+
+/* codes, scales = MXFP4(x): for a block with the largest magnitude m, 2^e with e = floor(log2 m) - 2 (at
+ * least -127), each x / 2^e rounded to the nearest code, ties to even, above 6 to 6.  A block of zeros
+ * takes scale byte 0; one that holds a NaN or an infinity byte 255 and codes 0.
+ *   x: [M, K] of dtype (F16, BF16 or F32), row stride ldx (a multiple of 8), 16-byte aligned. */
+int awq_w4a16_mxfp4_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t M, int64_t K,
+                             int32_t dtype, void* stream);
+
+/* out[M, K] (F16, BF16 or F32, dense, 16-byte aligned) = the values, each rounded once. */
+int awq_w4a16_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int64_t M, int64_t K,
+                               int32_t out_dtype, void* stream);
+
+/* Workspace bytes of awq_w4a16_mxfp4_gemm for an `a` that is not quantised yet (no zeroing needed). */
+size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+/* C[M, N] = A . W^T (+ bias), both operands MXFP4, sums and bias in fp32, one rounding to act_dtype (F16 or
+ * BF16).
+ *   a: with a_scales NULL [M, K] of act_dtype, row stride lda (a multiple of 8), quantised in the call
+ *      as awq_w4a16_mxfp4_quantize does; else codes [M, K/2] with a_scales [M, K/32] (lda and the workspace
+ *      are not used).
+ *   w: codes [N, K/2], w_scales [N, K/32];  bias: NULL or [N] of bias_dtype;  c: row stride ldc.
+ *   Any M, N >= 0.  Results are bitwise reproducible.  A NaN block makes NaN of every output that reads it.
+ *   workspace: 256-byte aligned; calls that may overlap must not share one. */
+int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, const uint8_t* w,
+                         const uint8_t* w_scales, const void* bias, void* c, int64_t ldc, int64_t M, int64_t N,
+                         int64_t K, int32_t act_dtype, int32_t bias_dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of awq_w4a16_mxfp4_moe (no zeroing needed). */
+size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k);
+
+/* awq_w4a16_moe over MXFP4 stacks: with e = ids[t, j],
+ *   h = MXFP4(act(g) * u) of the fp32 sums g, u = MXFP4(x[t]) . W1_e^T (rows 0 .. I-1 gate, I .. 2I-1 up),
+ *   out[t] = sum over j of w[t, j] * (h . W2_e^T), fp32 in slot order, one rounding.
+ *   gate_up: codes [E, 2I, H/2], scales [E, 2I, H/32];  down: codes [E, H, I/2], scales [E, H, I/32].
+ *   x: [T, H] act_dtype, row stride ldx (a multiple of 8);  out: row stride ldo.  Ids outside [0, E)
+ *   contribute nothing; an expert may occur twice in a token.  E <= 1024, H % 32 == 0, I % 32 == 0.
+ *   Results are bitwise reproducible.  workspace: 256-byte aligned. */
+int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_t ids_bits, const void* topk_weights,
+                        int32_t weights_dtype, const uint8_t* gate_up, const uint8_t* gate_up_scales,
+                        const uint8_t* down, const uint8_t* down_scales, void* out, int64_t ldo, int64_t T,
+                        int64_t H, int64_t I, int32_t E, int32_t top_k, int32_t activation, int32_t act_dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- balance of a router's experts --------------------------------------------------
+ * No counterpart in the reference, which does not train.  n = kept tokens (mask[t] != 0; all without a
+ * mask), counts[e] = routes of kept tokens to e (ids outside [0, E) are none), p = softmax(logits) in fp32:
+ *   loss = E * sum_e (counts[e] / (n top_k)) * (sum over kept t of p[t, e] / n)      (1 when even)
+ * No kept token: 0.  A row of nothing but -inf has p = 0.  What a masked row holds is not read.
+ *   logits: [T, ld] of logits_dtype;  topk_ids: [T, top_k] int32 or int64, dense;  mask: NULL or [T] bytes;
+ *   loss: 1 float;  counts: [E];  factor: [E] floats for awq_w4a16_moe_balance_grad.  E <= 1024.
+ *   Results are bitwise reproducible.  workspace: 16-byte aligned, no zeroing needed. */
+size_t awq_w4a16_moe_balance_workspace_bytes(int64_t T, int32_t E);
+int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, const void* topk_ids,
+                          int32_t ids_bits, const uint8_t* mask, int64_t T, int32_t E, int32_t top_k, float* loss,
+                          int32_t* counts, float* factor, void* workspace, size_t workspace_bytes, void* stream);
+
+/* grad[t, e] (dense [T, E] of logits_dtype) = upstream[0] * d loss / d logits[t, e], with the logits, mask
+ * and factor of the forward call: p (factor_e - sum_j factor_j p_j), 0 for a masked row.  The counts are
+ * piecewise constant and take no part. */
+int awq_w4a16_moe_balance_grad(const void* logits, int64_t ld, int32_t logits_dtype, const uint8_t* mask,
+                               const float* factor, const float* upstream, void* grad, int64_t T, int32_t E,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,15 @@ from .moe import (  # noqa: F401
     gemma4_moe_int4_prefill_grouped_fused,
     moe_route,
 )
+from .moe_balance import moe_balance_loss  # noqa: F401
+from .mxfp4 import (  # noqa: F401
+    MXFP4Experts,
+    MXFP4Weight,
+    mxfp4_dequantize,
+    mxfp4_gemm,
+    mxfp4_moe,
+    mxfp4_quantize,
+)
 from .rmsnorm_awq_fused import rmsnorm_awq_fused_linear  # noqa: F401
 from .tensor import AWQWeight, PackedInt4Weight  # noqa: F401
 

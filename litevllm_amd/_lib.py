@@ -87,6 +87,20 @@ SIGNATURES = {
     "awq_w4a16_rmsnorm_gemm": (ctypes.c_int, [_c_p, _c_i64, _c_p, ctypes.c_float, _c_p, _c_p, _c_p, _c_p,
                                               _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
                                               _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
+    "awq_w4a16_mxfp4_quantize": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_p]),
+    "awq_w4a16_mxfp4_dequantize": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i32, _c_p]),
+    "awq_w4a16_mxfp4_gemm_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64]),
+    "awq_w4a16_mxfp4_gemm": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64,
+                                            _c_i64, _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
+    "awq_w4a16_mxfp4_moe_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i32, _c_i32]),
+    "awq_w4a16_mxfp4_moe": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p,
+                                           _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_p,
+                                           _c_sz, _c_p]),
+    "awq_w4a16_moe_balance_workspace_bytes": (_c_sz, [_c_i64, _c_i32]),
+    "awq_w4a16_moe_balance": (ctypes.c_int, [_c_p, _c_i64, _c_i32, _c_p, _c_i32, _c_p, _c_i64, _c_i32, _c_i32, _c_p,
+                                             _c_p, _c_p, _c_p, _c_sz, _c_p]),
+    "awq_w4a16_moe_balance_grad": (ctypes.c_int, [_c_p, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,
+                                                  _c_p]),
 }
 
 MOE_ACT_SILU = 0

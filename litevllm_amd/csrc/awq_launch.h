@@ -131,4 +131,36 @@ struct MoeCall {
 };
 int launch_moe(const MoeCall& c, hipStream_t st);
 
+// ---- microscaled fp4 (awq_mx_*.hip) ----
+int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t M, int64_t K, int dtype, hipStream_t st);
+int launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int64_t M, int64_t K, int dtype, hipStream_t st);
+
+// Workspace of one call over expert stacks (byte offsets): the number of row tiles, the routes sorted by
+// expert, the tile table, the quantised tokens, the quantised intermediate and the per-route fp32 rows.
+struct MxMoeWorkspace {
+  int64_t order, tiles, x, xs, h, hs, y, total, max_tiles;
+};
+MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk);
+struct MxMoeCall {
+  const void* x;
+  int64_t ldx;
+  const void* ids;
+  int id64;
+  const void* weights;
+  int weights_dtype;
+  const uint8_t *gate_up, *gate_up_scales, *down, *down_scales;
+  void* out;
+  int64_t ldo, T, H, I;
+  int E, topk, act_kind, act_dtype;
+  void* workspace;
+};
+int launch_mx_moe(const MxMoeCall& c, hipStream_t st);
+
+// ---- balance of a router's experts (awq_moe_balance.hip) ----
+size_t balance_workspace_bytes(int64_t T, int E);
+int launch_moe_balance(const void* logits, int64_t ld, int dtype, const void* ids, int id64, const uint8_t* mask, int64_t T, int E,
+                       int topk, float* loss, int32_t* counts, float* factor, void* workspace, hipStream_t st);
+int launch_moe_balance_grad(const void* logits, int64_t ld, int dtype, const uint8_t* mask, const float* factor, const float* upstream,
+                            void* grad, int64_t T, int E, hipStream_t st);
+
 }  // namespace awq_host

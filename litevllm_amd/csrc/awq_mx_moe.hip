@@ -1,0 +1,158 @@
+// Mixture of experts over microscaled fp4 stacks: the places of the routes, the grouped products
+// (awq_mx_gemm.hip) and the weighted sum.
+#include <algorithm>
+
+#include "awq_launch.h"
+#include "awq_mx_common.h"
+
+namespace awq {
+
+constexpr int kOrderThreads = 1024;
+
+__device__ __forceinline__ int64_t route_id(const void* ids, int id64, int64_t r) {
+  return id64 ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];
+}
+
+// Sorts the routes by expert (one block): order[place] = route, and the table of row tiles, at most
+// `rows` places of one expert each.  The order inside an expert is that of the atomics; no result
+// depends on it, since every place's row is computed by itself and summed by its route.  Routes
+// without an expert get no place.
+__global__ void __launch_bounds__(kOrderThreads) mx_order_kernel(const void* __restrict__ ids, int id64, int R, int E, int rows,
+                                                                 int* __restrict__ order, int* __restrict__ tiles,
+                                                                 int* __restrict__ tile_count) {
+  extern __shared__ int sh[];
+  int *count = sh, *cursor = sh + E;
+  __shared__ int tot[2][kOrderThreads / 64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  for (int e = t; e < E; e += kOrderThreads) count[e] = 0;
+  __syncthreads();
+  for (int r = t; r < R; r += kOrderThreads) {
+    const int64_t e = route_id(ids, id64, r);
+    if (e >= 0 && e < E) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  // E <= kOrderThreads: one expert per thread; prefix sums of places and tiles
+  const int c = t < E ? count[t] : 0, nt = (c + rows - 1) / rows;
+  const int ic = wave_incl_scan_i32(c), it = wave_incl_scan_i32(nt);
+  if (lane == 63) tot[0][wave] = ic, tot[1][wave] = it;
+  __syncthreads();
+  int first = ic - c, ft = it - nt;
+  for (int w = 0; w < wave; ++w) first += tot[0][w], ft += tot[1][w];
+  if (t < E) {
+    cursor[t] = first;
+    for (int i = 0; i < nt; ++i) {
+      int* row = tiles + 3 * (ft + i);
+      row[0] = t;
+      row[1] = first + i * rows;
+      row[2] = min(rows, c - i * rows);
+    }
+  }
+  if (t == kOrderThreads - 1) tile_count[0] = ft + nt;
+  __syncthreads();
+  for (int r = t; r < R; r += kOrderThreads) {
+    const int64_t e = route_id(ids, id64, r);
+    if (e >= 0 && e < E) order[atomicAdd(&cursor[e], 1)] = r;
+  }
+}
+
+__device__ __forceinline__ float route_weight(const void* w, int dtype, int64_t r) {
+  if (dtype == AWQ_DTYPE_F32) return ((const float*)w)[r];
+  const uint16_t b = ((const uint16_t*)w)[r];
+  return dtype == AWQ_DTYPE_F16 ? h_bits2f(b) : bf_bits2f(b);
+}
+
+// out[t] = the sum over a token's slots, in slot order, of weight * y: fp32, one rounding.  A slot
+// without an expert adds nothing (its row of y was never written).
+template <typename T>
+__global__ void __launch_bounds__(256) mx_combine_kernel(const float* __restrict__ y, const void* __restrict__ ids, int id64,
+                                                         const void* __restrict__ w, int w_dtype, int E, int64_t T_, int H, int topk,
+                                                         uint16_t* __restrict__ out, int64_t ldo) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = i / (H / 4);
+  if (t >= T_) return;
+  const int c = (int)(i - t * (H / 4)) * 4;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < topk; ++j) {
+    const int64_t r = t * topk + j, e = route_id(ids, id64, r);
+    if (e < 0 || e >= E) continue;
+    const f32x4 v = *(const f32x4*)(y + r * H + c);
+    const float g = route_weight(w, w_dtype, r);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] = fmaf(v[u], g, s[u]);
+  }
+  u32x2 o = {pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
+  uint16_t* at = out + t * ldo + c;
+  if (((uintptr_t)at & 7) == 0) {
+    *(u32x2*)at = o;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at[u] = (uint16_t)(o[u >> 1] >> (16 * (u & 1)));
+  }
+}
+
+}  // namespace awq
+
+namespace awq_host {
+using namespace awq;
+
+// Rows of a row tile: what an expert gets on average, so that its weights are read about once.
+static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)16 * E ? 16 : 64; }
+
+MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk) {
+  MxMoeWorkspace w{};
+  const int64_t R = T * topk;
+  auto al = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  w.max_tiles = R / mx_moe_rows(R, E) + std::min<int64_t>(R, E);
+  w.order = 256;  // the tile count sits in front
+  w.tiles = al(w.order + R * 4);
+  w.x = al(w.tiles + w.max_tiles * 12);
+  w.xs = al(w.x + T * (H / 2));
+  w.h = al(w.xs + T * (H / 32));
+  w.hs = al(w.h + R * (I / 2));
+  w.y = al(w.hs + R * (I / 32));
+  w.total = al(w.y + R * H * 4);
+  return w;
+}
+
+int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
+  const int64_t R = c.T * c.topk;
+  if (R > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
+  const MxMoeWorkspace w = mx_moe_workspace(c.T, c.H, c.I, c.E, c.topk);
+  char* ws = (char*)c.workspace;
+  int* order = (int*)(ws + w.order);
+  int* tiles = (int*)(ws + w.tiles);
+  const int rows = mx_moe_rows(R, c.E);
+  mx_order_kernel<<<1, kOrderThreads, 2 * c.E * sizeof(int), st>>>(c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws);
+  if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
+  int rc = launch_mx_quantize(c.x, c.ldx, (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), c.T, c.H, c.act_dtype, st);
+  if (rc != AWQ_OK) return rc;
+
+  MxArgs g{};
+  g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);
+  g.w = c.gate_up, g.ws = c.gate_up_scales;
+  g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I;
+  g.tiles = tiles, g.tile_count = (const int*)ws, g.order = order;
+  g.topk = c.topk, g.act = c.act_kind;
+  g.h = (uint8_t*)(ws + w.h), g.hs = (uint8_t*)(ws + w.hs);
+  rc = launch_mx_grouped(g, true, rows, w.max_tiles, st);
+  if (rc != AWQ_OK) return rc;
+
+  MxArgs d = g;
+  d.a = g.h, d.as = g.hs;
+  d.w = c.down, d.ws = c.down_scales;
+  d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H;
+  d.y = (float*)(ws + w.y);
+  rc = launch_mx_grouped(d, false, rows, w.max_tiles, st);
+  if (rc != AWQ_OK) return rc;
+
+  const dim3 grid((unsigned)cdiv(c.T * (c.H / 4), 256));
+  if (c.act_dtype == AWQ_DTYPE_BF16)
+    mx_combine_kernel<bf16><<<grid, 256, 0, st>>>(d.y, c.ids, c.id64, c.weights, c.weights_dtype, c.E, c.T, (int)c.H, c.topk,
+                                                 (uint16_t*)c.out, c.ldo);
+  else
+    mx_combine_kernel<f16><<<grid, 256, 0, st>>>(d.y, c.ids, c.id64, c.weights, c.weights_dtype, c.E, c.T, (int)c.H, c.topk,
+                                                (uint16_t*)c.out, c.ldo);
+  return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
+}
+
+}  // namespace awq_host

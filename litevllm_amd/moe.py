@@ -23,6 +23,7 @@ import torch
 
 from . import ops
 from ._lib import AWQKernelError
+from .mxfp4 import MXFP4Experts, mxfp4_moe
 
 moe_route = ops.moe_route
 
@@ -263,16 +264,21 @@ def fused_moe(hidden_states: torch.Tensor, w1, w2, gating_output: torch.Tensor, 
       * ``w1``, ``w2`` int4 AWQ expert stacks (:class:`AWQExperts`), ``w1`` the gate_up stack
         ``[E, 2I, H]`` (unpacked orientation), ``w2`` the down stack ``[E, H, I]``: the grouped
         W4A16 kernels (gate, up, SiLU, down and the weighted sum, fp32 sums).
+      * ``w1``, ``w2`` MXFP4 expert stacks (:class:`MXFP4Experts`) of the same orientation: the grouped
+        MXFP4 kernels, which quantise the tokens and the intermediate (:func:`mxfp4_moe`).
       * ``w1`` an AWQ stack of ``I`` rows (the ungated form, ``fused_moe.py:52-53``): the experts
         are dequantized once by the HIP kernel (held on the stack) and run in the dense form.
       * dense ``w1 [E, 2I or I, H]`` / ``w2 [E, H, I]`` tensors (the materialised experts the
         reference's zero-point Gemma4 path passes, ``gemma4/moe.py:722-750, 788``): the
         reference's own expert loop on the device (dense GEMMs, not the int4 kernels)."""
     awq1, awq2 = isinstance(w1, AWQExperts), isinstance(w2, AWQExperts)
-    if awq1 != awq2:
-        raise TypeError("w1 and w2 must both be AWQExperts or both be dense expert tensors")
+    mx1, mx2 = isinstance(w1, MXFP4Experts), isinstance(w2, MXFP4Experts)
+    if awq1 != awq2 or mx1 != mx2:
+        raise TypeError("w1 and w2 must both be AWQExperts, both MXFP4Experts or both dense expert tensors")
     H = int(hidden_states.shape[1])
     tw, tid = moe_route(gating_output, topk, renormalize, flow="logits")
+    if mx1:
+        return mxfp4_moe(hidden_states, tw, tid, w1, w2, activation="silu")
     if awq1:
         _, _, n1 = w1.dims()
         _, inter, n2 = w2.dims()

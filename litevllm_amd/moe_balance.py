@@ -1,0 +1,75 @@
+"""The load-balancing loss of a mixture of experts and the routes per expert, beside :func:`moe_route`, whose
+logits and ids it takes."""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import ops
+from .mxfp4 import _call
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, mask, experts):
+        dev, t = logits.device, logits.shape[0]
+        dt = ops.dtype_code(logits.dtype)
+        ld = logits.stride(0) if t > 1 else experts
+        ws_bytes = L.load().awq_w4a16_moe_balance_workspace_bytes(t, experts)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        factor = torch.empty(experts, dtype=torch.float32, device=dev)
+        counts = torch.empty(experts, dtype=torch.int32, device=dev)
+        _call(dev, "awq_w4a16_moe_balance", logits.data_ptr(), ld, dt, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32,
+              ops._ptr(mask), t, experts, ids.shape[1], loss.data_ptr(), counts.data_ptr(), factor.data_ptr(), ws.data_ptr(),
+              ws_bytes)
+        ctx.save_for_backward(logits, mask, factor)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream, _):
+        logits, mask, factor = ctx.saved_tensors
+        t, experts = logits.shape
+        grad = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
+        if t:
+            upstream = upstream.contiguous()
+            _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
+                  ops.dtype_code(logits.dtype), ops._ptr(mask), factor.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t,
+                  experts)
+        return grad, None, None, None
+
+
+def moe_balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor,
+                     mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(loss, counts)`` of a router: ``loss`` an fp32 scalar, differentiable in ``router_logits``, ``counts`` int32
+    ``[E]``, the routes of every expert.
+
+    With ``n`` kept tokens (``mask [T]`` bool, True keeps; all without one), ``p = softmax(router_logits)`` in fp32::
+
+        loss = E * sum_e (counts[e] / (n * top_k)) * (sum over kept t of p[t, e] / n)
+
+    which is 1 for an even load.  ``router_logits``: fp16, bf16 or fp32 ``[T, E]`` (E up to 1024); ``topk_ids``: int32 or
+    int64 ``[T, top_k]``; ids outside ``[0, E)`` count nowhere.  What a masked row holds is not read and its
+    gradient is 0; without a kept token loss and gradient are 0.  A row of nothing but ``-inf`` has no
+    probabilities.  The gradient takes the counts as constants; it is not differentiable again."""
+    ops._require_device(router_logits, topk_ids, mask)
+    ops.dtype_code(router_logits.dtype)
+    if router_logits.dim() != 2 or topk_ids.dim() != 2 or topk_ids.shape[0] != router_logits.shape[0]:
+        raise ValueError(f"router_logits must be [T, E] and topk_ids [T, top_k], got {tuple(router_logits.shape)} and "
+                         f"{tuple(topk_ids.shape)}")
+    experts = router_logits.shape[1]
+    if not 1 <= experts <= 1024 or topk_ids.shape[1] < 1:
+        raise ValueError(f"1 to 1024 experts and at least one route a token, got {experts} and {topk_ids.shape[1]}")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.shape != router_logits.shape[:1]:
+            raise ValueError(f"mask must be bool [{router_logits.shape[0]}], got {mask.dtype} {tuple(mask.shape)}")
+        mask = mask.contiguous()
+    t = router_logits.shape[0]
+    if (router_logits.stride(1) != 1 and experts > 1) or (t > 1 and router_logits.stride(0) < experts):
+        router_logits = router_logits.contiguous()
+    return _BalanceLoss.apply(router_logits, topk_ids.contiguous(), mask, experts)
