@@ -13,6 +13,7 @@ bool dtype_float(int d) { return dtype_16(d) || d == AWQ_DTYPE_F32; }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 constexpr int64_t kIntMax = 0x7FFFFFFFLL;
+constexpr int64_t kOffsets = 0xFFFFFFFFLL;  // blocks of 32 in an operand that the kernels count in 32 bits
 }  // namespace
 
 extern "C" {
@@ -49,6 +50,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   if (M == 0 || N == 0) return AWQ_OK;
   if (!a || !w || !w_scales || !c) return AWQ_ERR_NULL;
   if (!dtype_16(act_dtype) || M > kIntMax || N > kIntMax || K > kIntMax) return AWQ_ERR_UNSUPPORTED;
+  if (M * (K / 32) > kOffsets || N * (K / 32) > kOffsets) return AWQ_ERR_UNSUPPORTED;
   if (bias ? !dtype_float(bias_dtype) : bias_dtype != AWQ_DTYPE_NONE) return AWQ_ERR_UNSUPPORTED;
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(c, 2) || ldc < N) return AWQ_ERR_STRIDE;
   MxArgs p{};
@@ -95,6 +97,7 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
   if (!dtype_16(act_dtype) || !dtype_float(weights_dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
   if (activation != AWQ_MOE_ACT_SILU && activation != AWQ_MOE_ACT_GELU_TANH) return AWQ_ERR_UNSUPPORTED;
   if (E > 1024 || H > kIntMax || 2 * I > kIntMax || T > kIntMax || T * top_k > kIntMax) return AWQ_ERR_UNSUPPORTED;
+  if (T * (H / 32) > kOffsets || T * top_k * (I / 32) > kOffsets || 2 * I * (H / 32) > kOffsets) return AWQ_ERR_UNSUPPORTED;
   if ((T > 1 && (ldx < H || (ldx % 8) != 0 || ldo < H)) || !aligned(x, 16) || !aligned(out, 2)) return AWQ_ERR_STRIDE;
   if (!aligned(gate_up, 16) || !aligned(down, 16)) return AWQ_ERR_STRIDE;
   if (!workspace || workspace_bytes < awq_w4a16_mxfp4_moe_workspace_bytes(T, H, I, E, top_k)) return AWQ_ERR_WORKSPACE;

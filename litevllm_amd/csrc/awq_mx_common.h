@@ -115,6 +115,8 @@ __device__ __forceinline__ int64_t mx_a_row(const MxArgs& p, const MxRows& t, in
 
 namespace awq_host {
 int launch_mx_gemm(const awq::MxArgs& p, hipStream_t st);
+int launch_mx_tile_gemm(const awq::MxArgs& p, hipStream_t st);
+int launch_mx_tile_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
 // gate_up or down product of the grouped routes in `row_tiles` (at most) row tiles of `rows` rows
 int launch_mx_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
 }  // namespace awq_host

@@ -130,23 +130,18 @@ static void launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
 }
 
 int launch_mx_gemm(const MxArgs& p, hipStream_t st) {
-  const int64_t t64 = cdiv(p.M, 64);
+  if (p.M > 64) return launch_mx_tile_gemm(p, st);
   if (p.M <= 16) launch_rows<kMxDense, 1, 1>(p, 1, st);
   else if (p.M <= 32) launch_rows<kMxDense, 2, 1>(p, 1, st);
-  else if (t64 > 65535) return AWQ_ERR_UNSUPPORTED;
-  else launch_rows<kMxDense, 4, 2>(p, t64, st);
+  else launch_rows<kMxDense, 4, 2>(p, 1, st);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
 int launch_mx_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
+  if (rows > 16) return launch_mx_tile_grouped(p, gate_up, rows, row_tiles, st);
   if (row_tiles > 65535) return AWQ_ERR_UNSUPPORTED;
-  if (gate_up) {
-    if (rows == 16) launch_rows<kMxGateUp, 1, 4>(p, row_tiles, st);
-    else launch_rows<kMxGateUp, 4, 4>(p, row_tiles, st);
-  } else {
-    if (rows == 16) launch_rows<kMxDown, 1, 2>(p, row_tiles, st);
-    else launch_rows<kMxDown, 4, 2>(p, row_tiles, st);
-  }
+  if (gate_up) launch_rows<kMxGateUp, 1, 4>(p, row_tiles, st);
+  else launch_rows<kMxDown, 1, 2>(p, row_tiles, st);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

@@ -96,7 +96,7 @@ namespace awq_host {
 using namespace awq;
 
 // Rows of a row tile: what an expert gets on average, so that its weights are read about once.
-static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)16 * E ? 16 : 64; }
+static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)16 * E ? 16 : (R <= (int64_t)128 * E ? 64 : 128); }
 
 MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk) {
   MxMoeWorkspace w{};

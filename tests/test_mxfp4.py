@@ -185,7 +185,7 @@ def test_quantize_refuses():
     (1, 16, 32, None), (1, 1, 64, "f32"), (1, 4096, 4096, None), (2, 333, 1056, "f16"), (5, 48, 96, None), (13, 1000, 2048, "bf16"),
     (16, 256, 12288, None), (17, 128, 512, None), (33, 517, 160, "f32"), (57, 1024, 4096, None), (64, 256, 1024, None),
     (65, 130, 2080, "f16"), (128, 512, 384, None), (200, 5001, 288, "bf16"), (300, 256, 4128, None), (513, 771, 1024, None),
-    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (8, 20000, 256, None), (129, 1, 32, None)])
+    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None)])
 def test_gemm(m, n, k, bias, dtype):
     from litevllm_amd import mxfp4_gemm
     dt = DTYPES[dtype]
