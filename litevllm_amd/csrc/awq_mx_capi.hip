@@ -74,6 +74,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   p.N = (int)N;
   p.M = (int)M;
   p.wrows = N;
+  p.a_rows = M;
   p.c = (uint16_t*)c;
   p.ldc = ldc;
   p.bias = bias;

@@ -77,7 +77,7 @@ struct MxArgs {
   const uint8_t *a, *as;  // codes [rows, K/2], scales [rows, K/32]
   const uint8_t *w, *ws;  // codes [experts][wrows, K/2], scales [experts][wrows, K/32]
   int K, N, M;            // N: output columns (gate_up: I)
-  int64_t wrows;          // rows of w per expert
+  int64_t wrows, a_rows;  // rows of w per expert; rows of a
   // dense
   uint16_t* c;
   int64_t ldc;

@@ -130,7 +130,7 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   MxArgs g{};
   g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);
   g.w = c.gate_up, g.ws = c.gate_up_scales;
-  g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I;
+  g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I, g.a_rows = c.T;
   g.tiles = tiles, g.tile_count = (const int*)ws, g.order = order;
   g.topk = c.topk, g.act = c.act_kind;
   g.h = (uint8_t*)(ws + w.h), g.hs = (uint8_t*)(ws + w.hs);
@@ -140,7 +140,7 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   MxArgs d = g;
   d.a = g.h, d.as = g.hs;
   d.w = c.down, d.ws = c.down_scales;
-  d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H;
+  d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H, d.a_rows = R;
   d.y = (float*)(ws + w.y);
   rc = launch_mx_grouped(d, false, rows, w.max_tiles, st);
   if (rc != AWQ_OK) return rc;

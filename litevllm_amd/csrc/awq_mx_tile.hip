@@ -5,31 +5,57 @@
 
 namespace awq {
 
-constexpr int kStageK = 256;  // K of a stage: 128 bytes of codes and 8 scale bytes per row
+// LDS of a block of `rows` rows (of both operands): two stages of 256 along K, two groups of 16 scale bytes a row
+// (a group serves two stages), and zeros to read as scales behind K's end.
+__host__ __device__ constexpr int mx_tile_lds(int rows, int tiles16) { return rows * (2 * 128 + 2 * 16) + tiles16 * 256; }
 
-// Loads 16 bytes per lane straight into LDS, lane l to base + 16 l.
-__device__ __forceinline__ void lds_load16(const uint8_t* src, void* base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+// Every direct load has landed and every LDS read is done, in every wave.
+__device__ __forceinline__ void wait_loads_and_sync() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// Block: BM rows of a by BN rows of w, WM x WN waves of (BM / WM) x (BN / WN); the stages along K are double
-// buffered, one barrier each.
+// acc[j] += b[j] . a^T for two neighbouring column tiles, as one piece of assembly: the compiler moves the builtin
+// behind the reads of whole stages, runs out of registers, and copies accumulators (M = 4096, N = 24576,
+// K = 4096: 404 us with it).  The wait states in front cover a copy of an operand by the VALU; the accumulators
+// may be used 18 wait states after the last of these (mfma_results).
+template <bool AGPR>
+__device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, const u32x4& b1, const u32x4& a, uint32_t s0, uint32_t s1,
+                                      uint32_t sa) {
+#define MX_MFMA(C, B, S) "v_mfma_scale_f32_16x16x128_f8f6f4 " C ", " B ", %4, " C ", " S ", %7 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+  if constexpr (AGPR)
+    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%2", "%5") "\n\t" MX_MFMA("%1", "%3", "%6")
+                 : "+a"(c0), "+a"(c1)
+                 : "v"(b0), "v"(b1), "v"(a), "v"(s0), "v"(s1), "v"(sa));
+  else
+    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%2", "%5") "\n\t" MX_MFMA("%1", "%3", "%6")
+                 : "+v"(c0), "+v"(c1)
+                 : "v"(b0), "v"(b1), "v"(a), "v"(s0), "v"(s1), "v"(sa));
+#undef MX_MFMA
+}
+
+// Block: BM rows of a by BN rows of w, WM x WN waves of (BM / WM) x (BN / WN).  A stage of 256 along K (one line
+// of codes a row) is loaded straight into LDS while the one before is used, in two halves of 128; a wave holds
+// the fragments of a half while it reads the next half's, so the buffer of a stage is free after its first
+// half: one barrier a stage, the loads under way for a whole stage's time.
 //
-// LDS: 16-byte chunk c of a tile's row sits at place c ^ (row & 7) of its 128 bytes, so that the 16 rows a
-// fragment reads lie in different banks; the direct loads write lanes in order, so it is their sources that are
-// permuted, inside the row's line.  Quarter q of a wave takes chunks 2 q and 2 q + 1 in its two steps of 128:
-// the order along K is free as long as both operands share it, and its two scale bytes are neighbours.
+// LDS: 16-byte chunk c (block c of the stage) of a row at place c ^ (row & 7) of its 128 bytes, so that the 16
+// rows of a fragment lie in different banks; the direct loads write lanes in order, so it is their sources that
+// are permuted, inside the row's line.  (Loads of half a line, in stages of 128, took 139 us where these take
+// 102: M = 4096, N = 24576, K = 4096, loads alone.)  The scale bytes come 16 a row, one load for two stages: a
+// row's bytes start anywhere in a word (K / 32 need not be a multiple of 4), so the loads start at the word and
+// the readers skip `sh` bytes, for the last ones into the next group.
 // The operands enter the MFMA swapped, so that a lane holds four consecutive columns of one row of c.
 //
-// K past the end: chunks repeat the row's last one (codes are finite) and both scales are 2^-127, which makes
-// their products 0 in fp32.
-template <int MODE, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
-  constexpr int THREADS = WM * WN * 64, WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int ROWS = BM + BN, STAGE = ROWS * 136;
-  static_assert(ROWS % (8 * WAVES) == 0, "whole loads");
-  extern __shared__ __align__(16) uint8_t lds[];  // per stage: codes [ROWS][128], scales [ROWS][8]
+// K past the end: the codes are whatever follows (any code is finite, and the loads stop at the operand's end),
+// both scales are 2^-127, and the products vanish in fp32.
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD>
+__global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
+  constexpr bool AGPR = TM * TN > 32;  // accumulators of more than half of the 256 VGPRs
+  static_assert(TN % 2 == 0, "");
+  extern __shared__ __align__(16) uint8_t lds[];  // codes [2][ROWS][128], scales [2][ROWS][16], zeros
 
   // blocks go to the 8 XCDs in turn: each takes a run of tiles, in groups of 8 row tiles, column by column, so
   // that the tiles it runs at once share rows of a and of w in its L2
@@ -46,54 +72,54 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(MxArgs p, int row
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
   const int KB = p.K / 32, stages = (KB + 7) / 8;
-  const uint8_t* w = p.w + (int64_t)t.expert * p.wrows * (p.K / 2);
-  const uint8_t* ws = p.ws + (int64_t)t.expert * p.wrows * KB;
-
-  // Row i of the stage (a's rows, then w's) times KB: its scales' offset in bytes, its codes' in 16 bytes.
-  // 32 bits hold it (checked on the host).
+  const int64_t a_base = MODE == kMxGateUp ? 0 : t.first, w_base = (int64_t)t.expert * p.wrows + n0;
+  const int last = p.N - 1 - n0;
+  // Row i of a stage (a's rows, then w's) behind the operand's base, times KB: the offset of its scales in bytes,
+  // of its codes in 16 bytes (in 32 bits: checked on the host)
   auto row_offset = [&](int i) -> uint32_t {
-    if (i < BM) return (uint32_t)mx_a_row<MODE>(p, t, i) * (uint32_t)KB;
+    if (i < BM) return (uint32_t)(mx_a_row<MODE>(p, t, i) - a_base) * (uint32_t)KB;
     const int j = i - BM;
-    uint32_t row;
-    if constexpr (MODE == kMxGateUp) row = (uint32_t)(min(n0 + (j < COLS ? j : j - COLS), p.N - 1) + (j < COLS ? 0 : p.N));
-    else row = (uint32_t)min(n0 + j, p.N - 1);
-    return row * (uint32_t)KB;
+    if constexpr (MODE == kMxGateUp) return (uint32_t)(min(j < COLS ? j : j - COLS, last) + (j < COLS ? 0 : p.N)) * (uint32_t)KB;
+    else return (uint32_t)min(j, last) * (uint32_t)KB;
   };
-  // this thread's loads: LOADS chunks of codes, A_LOADS of them a's, and the scales of SROWS rows
-  constexpr int LOADS = ROWS / (8 * WAVES), A_LOADS = BM / (8 * WAVES), SROWS = (ROWS + THREADS - 1) / THREADS;
-  static_assert(BM % (8 * WAVES) == 0, "whole loads");
-  uint32_t src[LOADS], ssrc[SROWS];
-  const int place = (lane & 7) ^ (lane >> 3);  // row & 7 is lane >> 3
+  auto rsrc = [&](const uint8_t* base, int64_t bytes) {
+    const uint64_t u = (uint64_t)(uintptr_t)base;
+    return u32x4{(uint32_t)u, (uint32_t)(u >> 32) & 0xFFFFu, (uint32_t)min(bytes, (int64_t)0xFFFFFFF0), 0x00020000u};
+  };
+  const int64_t a_blocks = (p.a_rows - a_base) * KB, w_blocks = (p.wrows - n0) * KB;
+  const u32x4 ars = rsrc(p.a + a_base * KB * 16, a_blocks * 16), wrs = rsrc(p.w + w_base * KB * 16, w_blocks * 16);
+  // scales from the word that holds the operand's first one, to the end of the word of its last
+  const uint8_t *as = p.as + a_base * KB, *ws = p.ws + w_base * KB;
+  const uint32_t a_in = (uint32_t)(uintptr_t)as & 3u, w_in = (uint32_t)(uintptr_t)ws & 3u;
+  const u32x4 asrs = rsrc(as - a_in, (a_blocks + a_in + 3) & ~(int64_t)3), wsrs = rsrc(ws - w_in, (w_blocks + w_in + 3) & ~(int64_t)3);
+
+  // this wave's loads of a stage: LOADS of 8 rows, the first A_LOADS of them a's; of a group of scales: those
+  // of 64 rows, in SLOADS loads (the last one not of every wave)
+  constexpr int LOADS = ROWS / (8 * WAVES), A_LOADS = BM / (8 * WAVES), SLOADS = (ROWS + 64 * WAVES - 1) / (64 * WAVES);
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0, "whole loads");
+  uint32_t src[LOADS], ssrc[SLOADS];
 #pragma unroll
-  for (int u = 0; u < LOADS; ++u) src[u] = row_offset((u * WAVES + wave) * 8 + (lane >> 3));
+  for (int u = 0; u < LOADS; ++u)
+    src[u] = (row_offset((u * WAVES + wave) * 8 + (lane >> 3)) + (uint32_t)((lane & 7) ^ (lane >> 3))) * 16u;
 #pragma unroll
-  for (int u = 0; u < SROWS; ++u) ssrc[u] = row_offset(min(tid + u * THREADS, ROWS - 1));
-  u32x2 sv[SROWS];
-  auto fetch = [&](int s) {
-    uint8_t* base = lds + (s & 1) * STAGE;
-    const int chunk = min(8 * s + place, KB - 1);
+  for (int u = 0; u < SLOADS; ++u) {
+    const int i = min((u * WAVES + wave) * 64 + lane, ROWS - 1);
+    ssrc[u] = (row_offset(i) + (i < BM ? a_in : w_in)) & ~3u;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  constexpr uint32_t SCALES = 2 * STAGE, ZEROS = SCALES + 2 * ROWS * 16;
+  auto load_codes = [&](int s) {
 #pragma unroll
     for (int u = 0; u < LOADS; ++u)
-      lds_load16((u < A_LOADS ? p.a : w) + (uint64_t)(src[u] + (uint32_t)chunk) * 16, base + (u * WAVES + wave) * 1024);
-    if (8 * s + 8 <= KB) {
-#pragma unroll
-      for (int u = 0; u < SROWS; ++u) __builtin_memcpy(&sv[u], (tid + u * THREADS < BM ? p.as : ws) + ssrc[u] + 8 * s, 8);
-    } else {
-#pragma unroll
-      for (int u = 0; u < SROWS; ++u) {
-        sv[u] = u32x2{0u, 0u};
-        const uint8_t* from = (tid + u * THREADS < BM ? p.as : ws) + ssrc[u] + 8 * s;
-#pragma unroll
-        for (int b = 0; b < 7; ++b)
-          if (b < KB - 8 * s) sv[u][b >> 2] |= (uint32_t)from[b] << (8 * (b & 3));
-      }
-    }
+      lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)s * 128u);
   };
-  auto put_scales = [&](int s) {
-    uint8_t* base = lds + (s & 1) * STAGE + ROWS * 128;
+  auto load_scales = [&](int g) {
 #pragma unroll
-    for (int u = 0; u < SROWS; ++u)
-      if (tid + u * THREADS < ROWS) *(u32x2*)(base + (tid + u * THREADS) * 8) = sv[u];
+    for (int u = 0; u < SLOADS; ++u) {
+      const int at = u * WAVES + wave;
+      if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
+      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)g * 16u);
+    }
   };
 
   f32x4 acc[TM][TN];
@@ -102,35 +128,94 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(MxArgs p, int row
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // where this lane reads its fragments (16 rows on: 2048 bytes) and their scales (256 bytes)
+  typedef const __attribute__((address_space(3))) u32x4* lds_u32x4;
+  typedef const __attribute__((address_space(3))) uint8_t* lds_u8;
   const int m0 = (wave / WN) * TM * 16, c0 = BM + (wave % WN) * TN * 16;
-  fetch(0);
-  put_scales(0);
-  __syncthreads();
-  for (int s = 0; s < stages; ++s) {
-    if (s + 1 < stages) fetch(s + 1);
-    const uint8_t* base = lds + (s & 1) * STAGE;
-    uint32_t sa[TM], sb[TN];
+  uint32_t rd_a[2], rd_b[2];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) sa[i] = *(const uint16_t*)(base + ROWS * 128 + (m0 + 16 * i + r) * 8 + 2 * q);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) sb[j] = *(const uint16_t*)(base + ROWS * 128 + (c0 + 16 * j + r) * 8 + 2 * q);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      u32x4 a[TM], b[TN];
-      const int at = ((2 * q + k) ^ (r & 7)) * 16;
-#pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = *(const u32x4*)(base + (m0 + 16 * i + r) * 128 + at);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = *(const u32x4*)(base + (c0 + 16 * j + r) * 128 + at);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = k == 0 ? mx_mfma<0, 0>(b[j], a[i], acc[i][j], sb[j], sa[i]) : mx_mfma<1, 1>(b[j], a[i], acc[i][j], sb[j], sa[i]);
-    }
-    if (s + 1 < stages) put_scales(s + 1);
-    __syncthreads();
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t chunk = (uint32_t)((4 * h + q) ^ (r & 7)) * 16u;
+    rd_a[h] = lds0 + (uint32_t)(m0 + r) * 128u + chunk;
+    rd_b[h] = lds0 + (uint32_t)(c0 + r) * 128u + chunk;
   }
+  // the 16 rows of a fragment are 16 KB bytes apart, so a lane's bytes start alike in all of them; a gathered
+  // row has a place of its own
+  uint32_t sh_a[TM], sh_b;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+    sh_a[i] = MODE == kMxGateUp ? ((row_offset(m0 + 16 * i + r) + a_in) & 3u) + (uint32_t)q : i == 0 ? (((uint32_t)r * (uint32_t)KB + a_in) & 3u) + (uint32_t)q : sh_a[0];
+  sh_b = (row_offset(c0 + r) + w_in & 3u) + (uint32_t)q;
+  // address of the scale of block q of half h of stage s
+  auto scale_at = [&](int s, int h, uint32_t row, uint32_t sh) -> uint32_t {
+    const uint32_t at = sh + (uint32_t)(8 * (s & 1) + 4 * h);  // byte in the group of 16
+    const uint32_t group = (uint32_t)(s >> 1) + (at >> 4);
+    return 8 * s + 4 * h + q < KB ? lds0 + SCALES + (group & 1u) * (ROWS * 16) + row * 16u + (at & 15u) : lds0 + ZEROS;
+  };
+  // the fragments of a half: a's row tile i, and all of w's, with their scales
+  u32x4 a[TM];
+  uint32_t sa[TM];
+  struct Cols {
+    u32x4 b[TN];
+    uint32_t s[TN];
+  };
+  auto read_a = [&](int s, int h, uint32_t scales, int i) {
+    a[i] = *(lds_u32x4)(rd_a[h] + (uint32_t)(s & 1) * STAGE + i * 2048);
+    sa[i] = MODE == kMxGateUp ? *(lds_u8)(scale_at(s, h, (uint32_t)(m0 + 16 * i + r), sh_a[i])) : *(lds_u8)(scales + i * 256);
+  };
+  auto read_cols = [&](int s, int h, Cols& c) {
+    const uint32_t at = scale_at(s, h, (uint32_t)(c0 + r), sh_b);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) c.b[j] = *(lds_u32x4)(rd_b[h] + (uint32_t)(s & 1) * STAGE + j * 2048);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) c.s[j] = *(lds_u8)(at + j * 256);
+  };
+  Cols first, second;
+  // The products of a half from its fragments: w's `now`, a's in place -- each is read again, for the next half
+  // (nh of stage ns), as soon as its products are under way.
+  auto multiply = [&](int ns, int nh, const Cols& now, Cols& next) {
+    const uint32_t at = scale_at(ns, nh, (uint32_t)(m0 + r), sh_a[0]);
+    read_cols(ns, nh, next);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; j += 2) mfma2<AGPR>(acc[i][j], acc[i][j + 1], now.b[j], now.b[j + 1], a[i], now.s[j], now.s[j + 1], sa[i]);
+      read_a(ns, nh, at, i);
+    }
+  };
+
+  load_scales(0);
+  load_codes(0);
+  for (int i = tid; i < (TM > TN ? TM : TN) * 64; i += WAVES * 64) ((uint32_t*)(lds + ZEROS))[i] = 0u;
+  wait_loads_and_sync();
+  if (stages > 1) load_codes(1);
+  if (stages > 1) load_scales(1);
+  {
+    const uint32_t at = scale_at(0, 0, (uint32_t)(m0 + r), sh_a[0]);
+    read_cols(0, 0, first);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) read_a(0, 0, at, i);
+  }
+  for (int s = 0; s < stages; ++s) {
+    multiply(s, 1, first, second);
+    wait_loads_and_sync();  // stage s + 1 is there, stage s has been read
+    if (s + 2 < stages) {
+      load_codes(s + 2);
+      if (s & 1) load_scales((s + 3) >> 1);
+    }
+    // after the last stage: fragments of nothing, which nobody uses
+    multiply(s + 1, 0, second, first);
+  }
+  // no use of an accumulator before the last product is through
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      if constexpr (AGPR) asm volatile("" : "+a"(acc[i][j]));
+      else asm volatile("" : "+v"(acc[i][j]));
+    }
+  __syncthreads();
 
   // lane: row m0 + 16 i + r, columns 16 j + 4 q .. + 3
   if constexpr (MODE == kMxGateUp) {
@@ -192,29 +277,37 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(MxArgs p, int row
       }
     }
   } else {
-    const bool whole = (p.ldc & 3) == 0 && ((uintptr_t)p.c & 7) == 0;
+    // through LDS, a region of each wave's own: rows of whole lines instead of 8 bytes in 16 rows at a time
+    // (M = 4096, N = 24576: 140 us of 412 before)
+    constexpr int LD = TN * 32 + 16;  // bytes of a row, and 16 so that the rows of a store lie in different banks
+    static_assert(WAVES * TM * 16 * LD <= mx_tile_lds(ROWS, TM > TN ? TM : TN), "the output tile");
+    uint8_t* mine = lds + wave * (TM * 16 * LD);
+    const int nw = n0 + c0 - BM;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = n0 + c0 - BM + 16 * j + 4 * q;
       float bias[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bias[e] = n + e < p.N ? load_bias(p.bias, p.bias_dtype, n + e) : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        const int n = nw + 16 * j + 4 * q + e;
+        bias[e] = n < p.N ? load_bias(p.bias, p.bias_dtype, n) : 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int m = m0 + 16 * i + r;
-        if (m >= t.rows) continue;
-        uint16_t* at = p.c + (int64_t)(t.first + m) * p.ldc + n;
-        uint16_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = p.out_bf16 ? f2bf_bits(acc[i][j][e] + bias[e]) : f2h_bits(acc[i][j][e] + bias[e]);
-        if (whole && n + 4 <= p.N) {
-          *(u32x2*)at = u32x2{(uint32_t)o[0] | ((uint32_t)o[1] << 16), (uint32_t)o[2] | ((uint32_t)o[3] << 16)};
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < p.N) at[e] = o[e];
-        }
+        const f32x4 v = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2], acc[i][j][3] + bias[3]};
+        *(u32x2*)(mine + (16 * i + r) * LD + 32 * j + 8 * q) =
+            p.out_bf16 ? u32x2{pack2<bf16>(v[0], v[1]), pack2<bf16>(v[2], v[3])} : u32x2{pack2<f16>(v[0], v[1]), pack2<f16>(v[2], v[3])};
       }
+    }
+    const int rows = min(TM * 16, t.rows - m0);
+    uint16_t* out = p.c + (int64_t)(t.first + m0) * p.ldc + nw;
+    if ((p.ldc & 7) == 0 && ((uintptr_t)p.c & 15) == 0 && nw + TN * 16 <= p.N) {
+      constexpr int LANES = TN * 2;  // of 16 bytes, to a row
+      for (int m = lane / LANES; m < rows; m += 64 / LANES)
+        *(u32x4*)(out + (int64_t)m * p.ldc + lane % LANES * 8) = *(const u32x4*)(mine + m * LD + lane % LANES * 16);
+    } else {
+      constexpr int LANES = TN * 16 < 64 ? TN * 16 : 64;
+      for (int m = lane / LANES; m < rows; m += 64 / LANES)
+        for (int n = lane % LANES; n < TN * 16 && nw + n < p.N; n += LANES) out[(int64_t)m * p.ldc + n] = *(const uint16_t*)(mine + m * LD + 2 * n);
     }
   }
 }
@@ -224,14 +317,14 @@ __global__ void __launch_bounds__(WM * WN * 64) mx_tile_kernel(MxArgs p, int row
 namespace awq_host {
 using namespace awq;
 
-template <int MODE, int BM, int BN, int WM, int WN>
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD>
 static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   constexpr int COLS = MODE == kMxGateUp ? BN / 2 : BN;
   const int64_t col_tiles = cdiv(p.N, COLS);
   if (row_tiles * col_tiles > 0x7FFFFFF0LL) return AWQ_ERR_UNSUPPORTED;
-  constexpr int lds = 2 * (BM + BN) * 136;
+  constexpr int lds = mx_tile_lds(BM + BN, BM / WM > BN / WN ? BM / WM / 16 : BN / WN / 16);
   static_assert(MODE != kMxGateUp || BM * (BN / 2 + 4) * 4 <= lds, "the up half");
-  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN>;
+  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN, PER_SIMD>;
   if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     (void)hipGetLastError();
     return AWQ_ERR_LAUNCH;
@@ -242,15 +335,15 @@ static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
 
 int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
   const int64_t big = cdiv(p.M, 256) * cdiv(p.N, 256), mid = cdiv(p.M, 128) * cdiv(p.N, 128);
-  if (big >= 256) return launch_tile<kMxDense, 256, 256, 2, 4>(p, cdiv(p.M, 256), st);
-  if (mid >= 256) return launch_tile<kMxDense, 128, 128, 2, 2>(p, cdiv(p.M, 128), st);
-  return launch_tile<kMxDense, 64, 64, 2, 2>(p, cdiv(p.M, 64), st);
+  if (big >= 256) return launch_tile<kMxDense, 256, 256, 4, 2, 2>(p, cdiv(p.M, 256), st);
+  if (mid >= 256) return launch_tile<kMxDense, 128, 128, 2, 2, 2>(p, cdiv(p.M, 128), st);
+  return launch_tile<kMxDense, 64, 64, 2, 2, 4>(p, cdiv(p.M, 64), st);
 }
 
 int launch_mx_tile_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
   if (rows == 128)
-    return gate_up ? launch_tile<kMxGateUp, 128, 128, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 128, 128, 2, 2>(p, row_tiles, st);
-  return gate_up ? launch_tile<kMxGateUp, 64, 128, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 64, 128, 2, 2>(p, row_tiles, st);
+    return gate_up ? launch_tile<kMxGateUp, 128, 128, 2, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 128, 128, 2, 2, 2>(p, row_tiles, st);
+  return gate_up ? launch_tile<kMxGateUp, 64, 128, 2, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 64, 128, 2, 2, 2>(p, row_tiles, st);
 }
 
 }  // namespace awq_host
