@@ -132,7 +132,9 @@ struct MoeCall {
 int launch_moe(const MoeCall& c, hipStream_t st);
 
 // ---- microscaled fp4 (awq_mx_*.hip) ----
-int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t M, int64_t K, int dtype, hipStream_t st);
+// lds: bytes between rows of scales
+int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, int64_t M, int64_t K, int dtype,
+                       hipStream_t st);
 int launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int64_t M, int64_t K, int dtype, hipStream_t st);
 
 // Workspace of one call over expert stacks (byte offsets): the number of row tiles, the routes sorted by

@@ -13,7 +13,8 @@ bool dtype_float(int d) { return dtype_16(d) || d == AWQ_DTYPE_F32; }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 constexpr int64_t kIntMax = 0x7FFFFFFFLL;
-constexpr int64_t kOffsets = 0xFFFFFFFFLL;  // blocks of 32 in an operand that the kernels count in 32 bits
+constexpr int64_t kMaxK = (int64_t)1 << 24;   // 256 rows of codes are addressed in 32 bits,
+constexpr int64_t kBytes = 0xFFFFFFF0LL;      // and so are all of the tokens' and all of an expert's gate and up
 }  // namespace
 
 extern "C" {
@@ -25,7 +26,7 @@ int awq_w4a16_mxfp4_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t
   if (!x || !codes || !scales) return AWQ_ERR_NULL;
   if (!dtype_float(dtype) || K > kIntMax) return AWQ_ERR_UNSUPPORTED;
   if ((M > 1 && (ldx < K || (ldx % 8) != 0)) || !aligned(x, 16) || !aligned(codes, 16)) return AWQ_ERR_STRIDE;
-  return launch_mx_quantize(x, ldx, codes, scales, M, K, dtype, (hipStream_t)stream);
+  return launch_mx_quantize(x, ldx, codes, scales, K / 32, M, K, dtype, (hipStream_t)stream);
 }
 
 int awq_w4a16_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int64_t M, int64_t K, int32_t out_dtype,
@@ -50,7 +51,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   if (M == 0 || N == 0) return AWQ_OK;
   if (!a || !w || !w_scales || !c) return AWQ_ERR_NULL;
   if (!dtype_16(act_dtype) || M > kIntMax || N > kIntMax || K > kIntMax) return AWQ_ERR_UNSUPPORTED;
-  if (M * (K / 32) > kOffsets || N * (K / 32) > kOffsets) return AWQ_ERR_UNSUPPORTED;
+  if (K > kMaxK) return AWQ_ERR_UNSUPPORTED;
   if (bias ? !dtype_float(bias_dtype) : bias_dtype != AWQ_DTYPE_NONE) return AWQ_ERR_UNSUPPORTED;
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(c, 2) || ldc < N) return AWQ_ERR_STRIDE;
   MxArgs p{};
@@ -63,7 +64,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
     if (!aligned(workspace, 256)) return AWQ_ERR_STRIDE;
     uint8_t* codes = (uint8_t*)workspace;
     uint8_t* scales = codes + align256((size_t)M * (size_t)(K / 2));
-    const int rc = launch_mx_quantize(a, lda, codes, scales, M, K, act_dtype, (hipStream_t)stream);
+    const int rc = launch_mx_quantize(a, lda, codes, scales, K / 32, M, K, act_dtype, (hipStream_t)stream);
     if (rc != AWQ_OK) return rc;
     p.a = codes;
     p.as = scales;
@@ -75,6 +76,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   p.M = (int)M;
   p.wrows = N;
   p.a_rows = M;
+  p.as_ld = (int)(K / 32);
   p.c = (uint16_t*)c;
   p.ldc = ldc;
   p.bias = bias;
@@ -98,7 +100,7 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
   if (!dtype_16(act_dtype) || !dtype_float(weights_dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
   if (activation != AWQ_MOE_ACT_SILU && activation != AWQ_MOE_ACT_GELU_TANH) return AWQ_ERR_UNSUPPORTED;
   if (E > 1024 || H > kIntMax || 2 * I > kIntMax || T > kIntMax || T * top_k > kIntMax) return AWQ_ERR_UNSUPPORTED;
-  if (T * (H / 32) > kOffsets || T * top_k * (I / 32) > kOffsets || 2 * I * (H / 32) > kOffsets) return AWQ_ERR_UNSUPPORTED;
+  if (H > kMaxK || I > kMaxK || T * (H / 2) > kBytes || I * H > kBytes) return AWQ_ERR_UNSUPPORTED;
   if ((T > 1 && (ldx < H || (ldx % 8) != 0 || ldo < H)) || !aligned(x, 16) || !aligned(out, 2)) return AWQ_ERR_STRIDE;
   if (!aligned(gate_up, 16) || !aligned(down, 16)) return AWQ_ERR_STRIDE;
   if (!workspace || workspace_bytes < awq_w4a16_mxfp4_moe_workspace_bytes(T, H, I, E, top_k)) return AWQ_ERR_WORKSPACE;

@@ -74,9 +74,10 @@ __device__ __forceinline__ void load8(const void* p, float* v) {
 enum MxMode { kMxDense = 0, kMxGateUp = 1, kMxDown = 2 };
 
 struct MxArgs {
-  const uint8_t *a, *as;  // codes [rows, K/2], scales [rows, K/32]
+  const uint8_t *a, *as;  // codes [rows, K/2], scales [rows, as_ld]
   const uint8_t *w, *ws;  // codes [experts][wrows, K/2], scales [experts][wrows, K/32]
   int K, N, M;            // N: output columns (gate_up: I)
+  int as_ld;              // bytes between rows of a's scales; a multiple of 4 for gate_up
   int64_t wrows, a_rows;  // rows of w per expert; rows of a
   // dense
   uint16_t* c;

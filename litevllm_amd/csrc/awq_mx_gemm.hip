@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kMxWaves * 64) mx_rows_kernel(MxArgs p) {
   for (int i = 0; i < MT; ++i) {
     const int64_t row = mx_a_row<MODE>(p, t, 16 * i + r);
     ac[i] = p.a + row * (p.K / 2) + q * 16;
-    asc[i] = p.as + row * KB + q;
+    asc[i] = p.as + row * p.as_ld + q;
   }
 
   f32x4 acc[MT][NT];

@@ -98,6 +98,9 @@ using namespace awq;
 // Rows of a row tile: what an expert gets on average, so that its weights are read about once.
 static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)16 * E ? 16 : (R <= (int64_t)128 * E ? 64 : 128); }
 
+// Bytes between rows of the tokens' scales: whole words, which the gathering kernel counts on.
+static int64_t scale_stride(int64_t K) { return cdiv(K / 32, 4) * 4; }
+
 MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk) {
   MxMoeWorkspace w{};
   const int64_t R = T * topk;
@@ -107,7 +110,7 @@ MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk
   w.tiles = al(w.order + R * 4);
   w.x = al(w.tiles + w.max_tiles * 12);
   w.xs = al(w.x + T * (H / 2));
-  w.h = al(w.xs + T * (H / 32));
+  w.h = al(w.xs + T * scale_stride(H));
   w.hs = al(w.h + R * (I / 2));
   w.y = al(w.hs + R * (I / 32));
   w.total = al(w.y + R * H * 4);
@@ -124,13 +127,13 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   const int rows = mx_moe_rows(R, c.E);
   mx_order_kernel<<<1, kOrderThreads, 2 * c.E * sizeof(int), st>>>(c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws);
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
-  int rc = launch_mx_quantize(c.x, c.ldx, (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), c.T, c.H, c.act_dtype, st);
+  int rc = launch_mx_quantize(c.x, c.ldx, (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), scale_stride(c.H), c.T, c.H, c.act_dtype, st);
   if (rc != AWQ_OK) return rc;
 
   MxArgs g{};
   g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);
   g.w = c.gate_up, g.ws = c.gate_up_scales;
-  g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I, g.a_rows = c.T;
+  g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I, g.a_rows = c.T, g.as_ld = (int)scale_stride(c.H);
   g.tiles = tiles, g.tile_count = (const int*)ws, g.order = order;
   g.topk = c.topk, g.act = c.act_kind;
   g.h = (uint8_t*)(ws + w.h), g.hs = (uint8_t*)(ws + w.hs);
@@ -140,7 +143,7 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   MxArgs d = g;
   d.a = g.h, d.as = g.hs;
   d.w = c.down, d.ws = c.down_scales;
-  d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H, d.a_rows = R;
+  d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H, d.a_rows = R, d.as_ld = (int)(c.I / 32);
   d.y = (float*)(ws + w.y);
   rc = launch_mx_grouped(d, false, rows, w.max_tiles, st);
   if (rc != AWQ_OK) return rc;

@@ -12,13 +12,15 @@ constexpr int kQuantThreads = 256;
 // inside their quad.  One pass: what it reads and writes bounds it.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t* __restrict__ codes,
-                                                                    uint8_t* __restrict__ scales, int64_t pieces, uint32_t per_row) {
+                                                                    uint8_t* __restrict__ scales, int64_t lds, int64_t pieces, uint32_t per_row) {
   const int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
   if (i >= pieces) return;  // whole blocks: pieces % 4 == 0
   const T* at = x + i * 8;
-  if (per_row) {  // rows apart
+  int64_t block = i >> 2;
+  if (per_row) {  // rows apart, here or there
     const int64_t row = i / per_row;
     at = x + row * ldx + (i - row * per_row) * 8;
+    block = row * lds + ((i - row * per_row) >> 2);
   }
   float v[8];
   if constexpr (std::is_same<T, float>::value) load8<float>(at, v);
@@ -30,7 +32,7 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __r
   top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
   const uint32_t byte = mx_scale_byte(top);
   codes[i] = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
-  if ((i & 3) == 0) scales[i >> 2] = (uint8_t)byte;
+  if ((i & 3) == 0) scales[block] = (uint8_t)byte;
 }
 
 // Eight values per lane.  An e2m1 value has two significant bits: times the scale it is exact in fp32
@@ -69,16 +71,17 @@ __global__ void __launch_bounds__(kQuantThreads) mx_dequantize_kernel(const uint
 namespace awq_host {
 using namespace awq;
 
-int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t M, int64_t K, int dtype, hipStream_t st) {
+int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, int64_t M, int64_t K, int dtype,
+                       hipStream_t st) {
   const int64_t pieces = M * (K / 8);
   if (pieces <= 0) return AWQ_OK;
   if (cdiv(pieces, kQuantThreads) > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)cdiv(pieces, kQuantThreads)), block(kQuantThreads);
-  const uint32_t per_row = (ldx == K || M == 1) ? 0u : (uint32_t)(K / 8);
+  const uint32_t per_row = ((ldx == K && lds == K / 32) || M == 1) ? 0u : (uint32_t)(K / 8);
   auto* o = (uint32_t*)codes;
-  if (dtype == AWQ_DTYPE_F16) mx_quantize_kernel<f16><<<grid, block, 0, st>>>((const f16*)x, ldx, o, scales, pieces, per_row);
-  else if (dtype == AWQ_DTYPE_BF16) mx_quantize_kernel<bf16><<<grid, block, 0, st>>>((const bf16*)x, ldx, o, scales, pieces, per_row);
-  else mx_quantize_kernel<float><<<grid, block, 0, st>>>((const float*)x, ldx, o, scales, pieces, per_row);
+  if (dtype == AWQ_DTYPE_F16) mx_quantize_kernel<f16><<<grid, block, 0, st>>>((const f16*)x, ldx, o, scales, lds, pieces, per_row);
+  else if (dtype == AWQ_DTYPE_BF16) mx_quantize_kernel<bf16><<<grid, block, 0, st>>>((const bf16*)x, ldx, o, scales, lds, pieces, per_row);
+  else mx_quantize_kernel<float><<<grid, block, 0, st>>>((const float*)x, ldx, o, scales, lds, pieces, per_row);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

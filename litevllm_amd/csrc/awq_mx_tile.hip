@@ -5,14 +5,22 @@
 
 namespace awq {
 
-// LDS of a block of `rows` rows (of both operands): two stages of 256 along K, two groups of 16 scale bytes a row
-// (a group serves two stages), and zeros to read as scales behind K's end.
-__host__ __device__ constexpr int mx_tile_lds(int rows, int tiles16) { return rows * (2 * 128 + 2 * 16) + tiles16 * 256; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) { return *(const __attribute__((address_space(3))) u32x4*)at; }
+__device__ __forceinline__ uint32_t lds_read1(uint32_t at) { return *(const __attribute__((address_space(3))) uint8_t*)at; }
+#pragma clang diagnostic pop
 
-// Every direct load has landed and every LDS read is done, in every wave.
+// LDS of a block of `rows` rows (of both operands): NBUF stages of 256 along K, NBUF groups of 16 scale bytes a row
+// (a group serves two stages; NBUF / 2 + 1 of them live), and zeros to read as scales behind K's end.
+__host__ __device__ constexpr int mx_tile_lds(int rows, int nbuf, int tiles16) { return rows * nbuf * (128 + 16) + tiles16 * 256; }
+
+// All but the N newest direct loads have landed and every LDS read is done, in every wave.
+template <int N>
 __device__ __forceinline__ void wait_loads_and_sync() {
+  static_assert(N < 64, "the counter's range");
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -36,7 +44,7 @@ __device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, con
 }
 
 // Block: BM rows of a by BN rows of w, WM x WN waves of (BM / WM) x (BN / WN).  A stage of 256 along K (one line
-// of codes a row) is loaded straight into LDS while the one before is used, in two halves of 128; a wave holds
+// of codes a row) is loaded straight into LDS while the NBUF - 1 before it are used, in two halves of 128; a wave holds
 // the fragments of a half while it reads the next half's, so the buffer of a stage is free after its first
 // half: one barrier a stage, the loads under way for a whole stage's time.
 //
@@ -50,22 +58,22 @@ __device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, con
 //
 // K past the end: the codes are whatever follows (any code is finite, and the loads stop at the operand's end),
 // both scales are 2^-127, and the products vanish in fp32.
-template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD>
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF>
 __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
   constexpr bool AGPR = TM * TN > 32;  // accumulators of more than half of the 256 VGPRs
   static_assert(TN % 2 == 0, "");
-  extern __shared__ __align__(16) uint8_t lds[];  // codes [2][ROWS][128], scales [2][ROWS][16], zeros
+  extern __shared__ __align__(16) uint8_t lds[];  // codes [NBUF][ROWS][128], scales [NBUF][ROWS][16], zeros
 
   // blocks go to the 8 XCDs in turn: each takes a run of tiles, in groups of 8 row tiles, column by column, so
   // that the tiles it runs at once share rows of a and of w in its L2
+  if (MODE != kMxDense) row_tiles = p.tile_count[0];
   const int tiles = row_tiles * col_tiles, per = (tiles + 7) / 8;
   const int id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
   if (((int)blockIdx.x >> 3) >= per || id >= tiles) return;
   const int group = id / (8 * col_tiles), in_group = id - group * 8 * col_tiles;
   const int group_rows = min(8, row_tiles - 8 * group);
   const int tm = 8 * group + in_group % group_rows, tn = in_group / group_rows;
-  if (MODE != kMxDense && tm >= p.tile_count[0]) return;
   const MxRows t = mx_rows<MODE, BM>(p, tm);
   constexpr int COLS = MODE == kMxGateUp ? BN / 2 : BN;
   const int n0 = tn * COLS;
@@ -74,24 +82,26 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
   const int KB = p.K / 32, stages = (KB + 7) / 8;
   const int64_t a_base = MODE == kMxGateUp ? 0 : t.first, w_base = (int64_t)t.expert * p.wrows + n0;
   const int last = p.N - 1 - n0;
-  // Row i of a stage (a's rows, then w's) behind the operand's base, times KB: the offset of its scales in bytes,
-  // of its codes in 16 bytes (in 32 bits: checked on the host)
-  auto row_offset = [&](int i) -> uint32_t {
-    if (i < BM) return (uint32_t)(mx_a_row<MODE>(p, t, i) - a_base) * (uint32_t)KB;
+  // Row i of a stage (a's rows, then w's) behind the operand's base, and the offsets of its codes (in 16 bytes) and
+  // of its scales (32 bits hold them: checked on the host)
+  auto row_of = [&](int i) -> uint32_t {
+    if (i < BM) return (uint32_t)(mx_a_row<MODE>(p, t, i) - a_base);
     const int j = i - BM;
-    if constexpr (MODE == kMxGateUp) return (uint32_t)(min(j < COLS ? j : j - COLS, last) + (j < COLS ? 0 : p.N)) * (uint32_t)KB;
-    else return (uint32_t)min(j, last) * (uint32_t)KB;
+    if constexpr (MODE == kMxGateUp) return (uint32_t)(min(j < COLS ? j : j - COLS, last) + (j < COLS ? 0 : p.N));
+    else return (uint32_t)min(j, last);
   };
+  auto code_offset = [&](int i) -> uint32_t { return row_of(i) * (uint32_t)KB; };
+  auto scale_offset = [&](int i) -> uint32_t { return row_of(i) * (uint32_t)(i < BM ? p.as_ld : KB); };
   auto rsrc = [&](const uint8_t* base, int64_t bytes) {
     const uint64_t u = (uint64_t)(uintptr_t)base;
-    return u32x4{(uint32_t)u, (uint32_t)(u >> 32) & 0xFFFFu, (uint32_t)min(bytes, (int64_t)0xFFFFFFF0), 0x00020000u};
+    return u32x4{(uint32_t)u, (uint32_t)(u >> 32) & 0xFFFFu, bytes < 0xFFFFFFF0LL ? (uint32_t)bytes : 0xFFFFFFF0u, 0x00020000u};
   };
-  const int64_t a_blocks = (p.a_rows - a_base) * KB, w_blocks = (p.wrows - n0) * KB;
-  const u32x4 ars = rsrc(p.a + a_base * KB * 16, a_blocks * 16), wrs = rsrc(p.w + w_base * KB * 16, w_blocks * 16);
+  const int64_t a_rows = p.a_rows - a_base, w_blocks = (p.wrows - n0) * KB;
+  const u32x4 ars = rsrc(p.a + a_base * KB * 16, a_rows * KB * 16), wrs = rsrc(p.w + w_base * KB * 16, w_blocks * 16);
   // scales from the word that holds the operand's first one, to the end of the word of its last
-  const uint8_t *as = p.as + a_base * KB, *ws = p.ws + w_base * KB;
+  const uint8_t *as = p.as + a_base * p.as_ld, *ws = p.ws + w_base * KB;
   const uint32_t a_in = (uint32_t)(uintptr_t)as & 3u, w_in = (uint32_t)(uintptr_t)ws & 3u;
-  const u32x4 asrs = rsrc(as - a_in, (a_blocks + a_in + 3) & ~(int64_t)3), wsrs = rsrc(ws - w_in, (w_blocks + w_in + 3) & ~(int64_t)3);
+  const u32x4 asrs = rsrc(as - a_in, ((a_rows - 1) * p.as_ld + KB + a_in + 3) & ~(int64_t)3), wsrs = rsrc(ws - w_in, (w_blocks + w_in + 3) & ~(int64_t)3);
 
   // this wave's loads of a stage: LOADS of 8 rows, the first A_LOADS of them a's; of a group of scales: those
   // of 64 rows, in SLOADS loads (the last one not of every wave)
@@ -100,25 +110,23 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
   uint32_t src[LOADS], ssrc[SLOADS];
 #pragma unroll
   for (int u = 0; u < LOADS; ++u)
-    src[u] = (row_offset((u * WAVES + wave) * 8 + (lane >> 3)) + (uint32_t)((lane & 7) ^ (lane >> 3))) * 16u;
+    src[u] = (code_offset((u * WAVES + wave) * 8 + (lane >> 3)) + (uint32_t)((lane & 7) ^ (lane >> 3))) * 16u;
 #pragma unroll
   for (int u = 0; u < SLOADS; ++u) {
     const int i = min((u * WAVES + wave) * 64 + lane, ROWS - 1);
-    ssrc[u] = (row_offset(i) + (i < BM ? a_in : w_in)) & ~3u;
+    ssrc[u] = (scale_offset(i) + (i < BM ? a_in : w_in)) & ~3u;
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  constexpr uint32_t SCALES = 2 * STAGE, ZEROS = SCALES + 2 * ROWS * 16;
-  auto load_codes = [&](int s) {
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u)
-      lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)s * 128u);
+  constexpr uint32_t SCALES = NBUF * STAGE, ZEROS = SCALES + NBUF * ROWS * 16;
+  auto load_code = [&](int s, int u) {
+    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & (NBUF - 1)) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)s * 128u);
   };
   auto load_scales = [&](int g) {
 #pragma unroll
     for (int u = 0; u < SLOADS; ++u) {
       const int at = u * WAVES + wave;
       if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
-      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)g * 16u);
+      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & (NBUF - 1)) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)g * 16u);
     }
   };
 
@@ -129,8 +137,6 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // where this lane reads its fragments (16 rows on: 2048 bytes) and their scales (256 bytes)
-  typedef const __attribute__((address_space(3))) u32x4* lds_u32x4;
-  typedef const __attribute__((address_space(3))) uint8_t* lds_u8;
   const int m0 = (wave / WN) * TM * 16, c0 = BM + (wave % WN) * TN * 16;
   uint32_t rd_a[2], rd_b[2];
 #pragma unroll
@@ -139,18 +145,17 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     rd_a[h] = lds0 + (uint32_t)(m0 + r) * 128u + chunk;
     rd_b[h] = lds0 + (uint32_t)(c0 + r) * 128u + chunk;
   }
-  // the 16 rows of a fragment are 16 KB bytes apart, so a lane's bytes start alike in all of them; a gathered
-  // row has a place of its own
-  uint32_t sh_a[TM], sh_b;
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-    sh_a[i] = MODE == kMxGateUp ? ((row_offset(m0 + 16 * i + r) + a_in) & 3u) + (uint32_t)q : i == 0 ? (((uint32_t)r * (uint32_t)KB + a_in) & 3u) + (uint32_t)q : sh_a[0];
-  sh_b = (row_offset(c0 + r) + w_in & 3u) + (uint32_t)q;
+  // the rows of a fragment's next 16 are a multiple of 16 bytes on, and those of a gathered operand whole words: a
+  // lane's scale bytes start alike in all its row tiles
+  const uint32_t sh_a = ((MODE == kMxGateUp ? 0u : (uint32_t)r * (uint32_t)p.as_ld) + a_in & 3u) + (uint32_t)q;
+  const uint32_t sh_b = (scale_offset(c0 + r) + w_in & 3u) + (uint32_t)q;
   // address of the scale of block q of half h of stage s
   auto scale_at = [&](int s, int h, uint32_t row, uint32_t sh) -> uint32_t {
     const uint32_t at = sh + (uint32_t)(8 * (s & 1) + 4 * h);  // byte in the group of 16
     const uint32_t group = (uint32_t)(s >> 1) + (at >> 4);
-    return 8 * s + 4 * h + q < KB ? lds0 + SCALES + (group & 1u) * (ROWS * 16) + row * 16u + (at & 15u) : lds0 + ZEROS;
+    uint32_t place = lds0 + SCALES + (group & (NBUF - 1)) * (ROWS * 16) + row * 16u + (at & 15u);
+    asm("" : "+v"(place));  // a select, no branch around it
+    return 8 * s + 4 * h + q < KB ? place : lds0 + ZEROS;
   };
   // the fragments of a half: a's row tile i, and all of w's, with their scales
   u32x4 a[TM];
@@ -160,51 +165,75 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     uint32_t s[TN];
   };
   auto read_a = [&](int s, int h, uint32_t scales, int i) {
-    a[i] = *(lds_u32x4)(rd_a[h] + (uint32_t)(s & 1) * STAGE + i * 2048);
-    sa[i] = MODE == kMxGateUp ? *(lds_u8)(scale_at(s, h, (uint32_t)(m0 + 16 * i + r), sh_a[i])) : *(lds_u8)(scales + i * 256);
+    a[i] = lds_read16(rd_a[h] + (uint32_t)(s & (NBUF - 1)) * STAGE + i * 2048);
+    sa[i] = lds_read1(scales + i * 256);
   };
   auto read_cols = [&](int s, int h, Cols& c) {
     const uint32_t at = scale_at(s, h, (uint32_t)(c0 + r), sh_b);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) c.b[j] = *(lds_u32x4)(rd_b[h] + (uint32_t)(s & 1) * STAGE + j * 2048);
+    for (int j = 0; j < TN; ++j) c.b[j] = lds_read16(rd_b[h] + (uint32_t)(s & (NBUF - 1)) * STAGE + j * 2048);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) c.s[j] = *(lds_u8)(at + j * 256);
+    for (int j = 0; j < TN; ++j) c.s[j] = lds_read1(at + j * 256);
   };
   Cols first, second;
-  // The products of a half from its fragments: w's `now`, a's in place -- each is read again, for the next half
-  // (nh of stage ns), as soon as its products are under way.
-  auto multiply = [&](int ns, int nh, const Cols& now, Cols& next) {
-    const uint32_t at = scale_at(ns, nh, (uint32_t)(m0 + r), sh_a[0]);
-    read_cols(ns, nh, next);
+  auto products = [&](int i, const Cols& now) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-      for (int j = 0; j < TN; j += 2) mfma2<AGPR>(acc[i][j], acc[i][j + 1], now.b[j], now.b[j + 1], a[i], now.s[j], now.s[j + 1], sa[i]);
-      read_a(ns, nh, at, i);
-    }
+    for (int j = 0; j < TN; j += 2) mfma2<AGPR>(acc[i][j], acc[i][j + 1], now.b[j], now.b[j + 1], a[i], now.s[j], now.s[j + 1], sa[i]);
   };
+  // a's fragments have one place: each is read again, for the next half, as soon as its products are under way
 
   load_scales(0);
-  load_codes(0);
+#pragma unroll
+  for (int s = 0; s < NBUF; ++s) {
+    if (s >= stages) break;
+    if (s & 1) load_scales((s + 1) >> 1);  // before the codes of the first stage that reads from it
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) load_code(s, u);
+  }
   for (int i = tid; i < (TM > TN ? TM : TN) * 64; i += WAVES * 64) ((uint32_t*)(lds + ZEROS))[i] = 0u;
-  wait_loads_and_sync();
-  if (stages > 1) load_codes(1);
-  if (stages > 1) load_scales(1);
+  if (stages >= NBUF) wait_loads_and_sync<(NBUF - 1) * LOADS>();
+  else wait_loads_and_sync<0>();
   {
-    const uint32_t at = scale_at(0, 0, (uint32_t)(m0 + r), sh_a[0]);
+    const uint32_t at = scale_at(0, 0, (uint32_t)(m0 + r), sh_a);
     read_cols(0, 0, first);
 #pragma unroll
     for (int i = 0; i < TM; ++i) read_a(0, 0, at, i);
   }
   for (int s = 0; s < stages; ++s) {
-    multiply(s, 1, first, second);
-    wait_loads_and_sync();  // stage s + 1 is there, stage s has been read
-    if (s + 2 < stages) {
-      load_codes(s + 2);
-      if (s & 1) load_scales((s + 3) >> 1);
+    {
+      const uint32_t at = scale_at(s, 1, (uint32_t)(m0 + r), sh_a);
+      read_cols(s, 1, second);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        products(i, first);
+        read_a(s, 1, at, i);
+      }
     }
-    // after the last stage: fragments of nothing, which nobody uses
-    multiply(s + 1, 0, second, first);
+    // The second half's reads are of the next stage, so they begin behind the barrier: with the first products
+    // before it, the reads that it waits for have come back.  The loads of stage s + NBUF go out between the
+    // products.  (After the last stage the fragments are of nothing, and nobody uses them.)
+    constexpr int AT = TM > 2 ? 1 : 0, SHARE = (LOADS + TM - AT - 1) / (TM - AT);
+    const uint32_t at = scale_at(s + 1, 0, (uint32_t)(m0 + r), sh_a);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      products(i, second);
+      if (i == AT) {
+        // stage s + 1 is there, stage s has been read
+        if (s + NBUF - 1 < stages) wait_loads_and_sync<(NBUF - 2) * LOADS>();
+        else wait_loads_and_sync<0>();
+        read_cols(s + 1, 0, first);
+#pragma unroll
+        for (int k = 0; k < AT; ++k) read_a(s + 1, 0, at, k);
+        if ((s & 1) && s + NBUF < stages) load_scales((s + NBUF + 1) >> 1);
+      }
+      if (i >= AT) {
+        read_a(s + 1, 0, at, i);
+        if (s + NBUF < stages) {
+#pragma unroll
+          for (int u = (i - AT) * SHARE; u < (i - AT + 1) * SHARE && u < LOADS; ++u) load_code(s + NBUF, u);
+        }
+      }
+    }
   }
   // no use of an accumulator before the last product is through
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
@@ -280,7 +309,7 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     // through LDS, a region of each wave's own: rows of whole lines instead of 8 bytes in 16 rows at a time
     // (M = 4096, N = 24576: 140 us of 412 before)
     constexpr int LD = TN * 32 + 16;  // bytes of a row, and 16 so that the rows of a store lie in different banks
-    static_assert(WAVES * TM * 16 * LD <= mx_tile_lds(ROWS, TM > TN ? TM : TN), "the output tile");
+    static_assert(WAVES * TM * 16 * LD <= mx_tile_lds(ROWS, NBUF, TM > TN ? TM : TN), "the output tile");
     uint8_t* mine = lds + wave * (TM * 16 * LD);
     const int nw = n0 + c0 - BM;
 #pragma unroll
@@ -317,14 +346,14 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
 namespace awq_host {
 using namespace awq;
 
-template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD>
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF>
 static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   constexpr int COLS = MODE == kMxGateUp ? BN / 2 : BN;
   const int64_t col_tiles = cdiv(p.N, COLS);
   if (row_tiles * col_tiles > 0x7FFFFFF0LL) return AWQ_ERR_UNSUPPORTED;
-  constexpr int lds = mx_tile_lds(BM + BN, BM / WM > BN / WN ? BM / WM / 16 : BN / WN / 16);
+  constexpr int lds = mx_tile_lds(BM + BN, NBUF, BM / WM > BN / WN ? BM / WM / 16 : BN / WN / 16);
   static_assert(MODE != kMxGateUp || BM * (BN / 2 + 4) * 4 <= lds, "the up half");
-  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN, PER_SIMD>;
+  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN, PER_SIMD, NBUF>;
   if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     (void)hipGetLastError();
     return AWQ_ERR_LAUNCH;
@@ -335,15 +364,15 @@ static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
 
 int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
   const int64_t big = cdiv(p.M, 256) * cdiv(p.N, 256), mid = cdiv(p.M, 128) * cdiv(p.N, 128);
-  if (big >= 256) return launch_tile<kMxDense, 256, 256, 4, 2, 2>(p, cdiv(p.M, 256), st);
-  if (mid >= 256) return launch_tile<kMxDense, 128, 128, 2, 2, 2>(p, cdiv(p.M, 128), st);
-  return launch_tile<kMxDense, 64, 64, 2, 2, 4>(p, cdiv(p.M, 64), st);
+  if (big >= 256) return launch_tile<kMxDense, 256, 256, 2, 4, 2, 2>(p, cdiv(p.M, 256), st);
+  if (mid >= 256) return launch_tile<kMxDense, 128, 128, 2, 4, 4, 2>(p, cdiv(p.M, 128), st);
+  return launch_tile<kMxDense, 64, 64, 2, 2, 2, 4>(p, cdiv(p.M, 64), st);
 }
 
 int launch_mx_tile_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
   if (rows == 128)
-    return gate_up ? launch_tile<kMxGateUp, 128, 128, 2, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 128, 128, 2, 2, 2>(p, row_tiles, st);
-  return gate_up ? launch_tile<kMxGateUp, 64, 128, 2, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 64, 128, 2, 2, 2>(p, row_tiles, st);
+    return gate_up ? launch_tile<kMxGateUp, 128, 128, 2, 4, 4, 2>(p, row_tiles, st) : launch_tile<kMxDown, 128, 128, 2, 4, 4, 2>(p, row_tiles, st);
+  return gate_up ? launch_tile<kMxGateUp, 64, 128, 2, 2, 2, 2>(p, row_tiles, st) : launch_tile<kMxDown, 64, 128, 2, 2, 2, 2>(p, row_tiles, st);
 }
 
 }  // namespace awq_host
