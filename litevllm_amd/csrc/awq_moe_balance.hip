@@ -12,16 +12,20 @@
 
 namespace awq {
 
-constexpr int kBalWaves = 4, kBalThreads = kBalWaves * 64;
+constexpr int kBalThreads = 1024, kBalWaves = kBalThreads / 64;
 
-__device__ __forceinline__ float wave_max_f32(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
-}
-__device__ __forceinline__ float wave_sum_f32(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+// Steps of a reduction over G = 16, 32 or 64 neighbouring lanes: DPP inside rows of 16, then across rows.
+template <int G, class Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // quad_perm [1, 0, 3, 2]
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // quad_perm [2, 3, 0, 1]
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  v = op(v, dpp(v, std::integral_constant<int, 0x140>{}));  // row_mirror
+  if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16));
+  if constexpr (G >= 64) v = op(v, __shfl_xor(v, 32));
   return v;
 }
 template <typename T>
@@ -30,17 +34,20 @@ __device__ __forceinline__ float logit(const void* z, int64_t i) {
   else return from_bits<T>(((const uint16_t*)z)[i]);
 }
 
-// Softmax of a row by the hardware's exp2 (a value below 2^-126 becomes 0); value v of a lane is expert 64 v + lane (0 past E).
-template <typename T, int V>
-__device__ __forceinline__ void row_softmax(const void* z, int64_t at, int E, int lane, float* p) {
-  float top = -__builtin_inff();
+// G lanes share a row, lane l of them the experts G v + l: a wave works on 64 / G rows at once, which keeps
+// the reductions short and the loads of several rows under way.
+template <typename T, int G, int V>
+__device__ __forceinline__ void load_row(const void* z, int64_t at, int E, int l, float* p) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = 64 * v + lane;
-    p[v] = e < E ? logit<T>(z, at + e) : -__builtin_inff();
-    top = fmaxf(top, p[v]);
-  }
-  top = wave_max_f32(top);
+  for (int v = 0; v < V; ++v) p[v] = G * v + l < E ? logit<T>(z, at + G * v + l) : -__builtin_inff();
+}
+// Softmax by the hardware's exp2 (a value below 2^-126 becomes 0); 0 past E.
+template <int G, int V>
+__device__ __forceinline__ void row_softmax(float* p) {
+  float top = p[0];
+#pragma unroll
+  for (int v = 1; v < V; ++v) top = fmaxf(top, p[v]);
+  top = group_reduce<G>(top, [](float a, float b) { return fmaxf(a, b); });
   if (top == -__builtin_inff()) top = 0.f;  // exp(-inf) = 0 for the whole row
   float s = 0.f;
 #pragma unroll
@@ -48,7 +55,7 @@ __device__ __forceinline__ void row_softmax(const void* z, int64_t at, int E, in
     p[v] = __expf(p[v] - top);
     s += p[v];
   }
-  s = wave_sum_f32(s);
+  s = group_reduce<G>(s, [](float a, float b) { return a + b; });
   const float inv = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
   for (int v = 0; v < V; ++v) p[v] *= inv;
@@ -59,105 +66,131 @@ struct BalanceArgs {
   int64_t ld;
   const uint8_t* mask;
   int T, E, topk, id64;
-  // partial sums of `blocks` blocks: probabilities [blocks][E] fp32, routes [blocks][E], kept [blocks]
+  // sums of each of `blocks` blocks, of `rows` rows: probabilities [blocks][E] fp32, routes [blocks][E], kept [blocks]
   float* part_p;
   int *part_c, *part_n;
   float *loss, *factor;
   int* counts;
-  int blocks;
+  int blocks, rows;
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kBalThreads) balance_rows_kernel(BalanceArgs a) {
-  extern __shared__ int hist[];  // [E], then the waves' sums [kBalWaves][64 V]
-  float* sums = (float*)(hist + a.E);
-  __shared__ int kept_all;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int e = t; e < a.E; e += kBalThreads) hist[e] = 0;
-  if (t == 0) kept_all = 0;
-  __syncthreads();
-  float acc[V] = {};
-  int kept = 0;
-  for (int row = blockIdx.x * kBalWaves + wave; row < a.T; row += a.blocks * kBalWaves) {
-    if (a.mask && !a.mask[row]) continue;
-    ++kept;
-    float p[V];
-    row_softmax<T, V>(a.logits, (int64_t)row * a.ld, a.E, lane, p);
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += p[v];
-    for (int j = lane; j < a.topk; j += 64) {
-      const int64_t r = (int64_t)row * a.topk + j;
-      const int64_t e = a.id64 ? ((const int64_t*)a.ids)[r] : (int64_t)((const int32_t*)a.ids)[r];
-      if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) sums[wave * 64 * V + 64 * v + lane] = acc[v];
-  if (lane == 0 && kept) atomicAdd(&kept_all, kept);
-  __syncthreads();
-  for (int e = t; e < a.E; e += kBalThreads) {
-    float s = sums[e];
-    for (int w = 1; w < kBalWaves; ++w) s += sums[w * 64 * V + e];
-    a.part_p[(int64_t)blockIdx.x * a.E + e] = s;
-    a.part_c[(int64_t)blockIdx.x * a.E + e] = hist[e];
-  }
-  if (t == 0) a.part_n[blockIdx.x] = kept_all;
-}
-
-// One block joins the blocks' sums, in block order, in fp64.
-__global__ void __launch_bounds__(1024) balance_join_kernel(BalanceArgs a) {
-  __shared__ double part[16];
-  __shared__ int kept_all;
+// Loss, counts and factors from every expert's sums (thread e has expert e's), by one block.
+__device__ __forceinline__ void balance_finish(const BalanceArgs& a, int kept, double p, int c) {
+  __shared__ double part[kBalWaves];
   const int t = threadIdx.x;
-  if (t == 0) kept_all = 0;
-  __syncthreads();
-  int kept = 0;
-  for (int b = t; b < a.blocks; b += 1024) kept += a.part_n[b];
-  if (kept) atomicAdd(&kept_all, kept);
-  __syncthreads();
-  const double n = kept_all > 0 ? (double)kept_all : 1.0;
+  const double n = kept > 0 ? (double)kept : 1.0;
   double mine = 0.0;
   if (t < a.E) {
-    double s = 0.0;
-    int c = 0;
-    for (int b = 0; b < a.blocks; ++b) {
-      s += (double)a.part_p[(int64_t)b * a.E + t];
-      c += a.part_c[(int64_t)b * a.E + t];
-    }
     const double f = (double)c / (n * a.topk);
     a.counts[t] = c;
     a.factor[t] = (float)(a.E * f / n);
-    mine = a.E * f * (s / n);
+    mine = a.E * f * (p / n);
   }
   mine = wave_sum_f64(mine);
   if ((t & 63) == 0) part[t >> 6] = mine;
   __syncthreads();
   if (t == 0) {
     double loss = 0.0;
-    for (int w = 0; w < 16; ++w) loss += part[w];
+    for (int w = 0; w < kBalWaves; ++w) loss += part[w];
     a.loss[0] = (float)loss;
   }
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(const void* __restrict__ logits, int64_t ld,
-                                                                   const uint8_t* __restrict__ mask, const float* __restrict__ factor,
-                                                                   const float* __restrict__ upstream, void* __restrict__ grad, int rows,
-                                                                   int E) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <typename T, int G, int V>
+__global__ void __launch_bounds__(kBalThreads) balance_rows_kernel(BalanceArgs a) {
+  constexpr int COLS = G * V, PER = 64 / G;
+  __shared__ float sums[kBalWaves][COLS];
+  __shared__ int hist[COLS], kept_all;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l = lane % G;
+  for (int e = t; e < COLS; e += kBalThreads) hist[e] = 0;
+  if (t == 0) kept_all = 0;
+  __syncthreads();
+  const int first = blockIdx.x * a.rows, end = min(first + a.rows, a.T);
+  for (int64_t i = (int64_t)first * a.topk + t; i < (int64_t)end * a.topk; i += kBalThreads) {
+    if (a.mask && !a.mask[i / a.topk]) continue;
+    const int64_t e = a.id64 ? ((const int64_t*)a.ids)[i] : (int64_t)((const int32_t*)a.ids)[i];
+    if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
+  }
+  float acc[V] = {};
+  int kept = 0;
+  for (int base = first + wave * PER; base < end; base += kBalWaves * PER) {
+    const int row = base + lane / G;
+    if (row >= end || (a.mask && !a.mask[row])) continue;
+    ++kept;
+    float p[V];
+    load_row<T, G, V>(a.logits, (int64_t)row * a.ld, a.E, l, p);
+    row_softmax<G, V>(p);
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] += p[v];
+  }
+  if (l == 0 && kept) atomicAdd(&kept_all, kept);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if constexpr (G <= 16) acc[v] += __shfl_xor(acc[v], 16);
+    if constexpr (G <= 32) acc[v] += __shfl_xor(acc[v], 32);
+    if (lane < G) sums[wave][G * v + l] = acc[v];
+  }
+  __syncthreads();
+  float s = 0.f;
+  if (t < a.E)
+    for (int w = 0; w < kBalWaves; ++w) s += sums[w][t];
+  if (a.blocks == 1) {
+    balance_finish(a, kept_all, s, t < a.E ? hist[t] : 0);
+    return;
+  }
+  if (t < a.E) {
+    a.part_p[(int64_t)blockIdx.x * a.E + t] = s;
+    a.part_c[(int64_t)blockIdx.x * a.E + t] = hist[t];
+  }
+  if (t == 0) a.part_n[blockIdx.x] = kept_all;
+}
+
+// One block joins the blocks' sums: threads of a column take shares of the blocks, added in order in fp64.
+__global__ void __launch_bounds__(kBalThreads) balance_join_kernel(BalanceArgs a) {
+  __shared__ double sp[kBalThreads];
+  __shared__ int sc[kBalThreads], kept_all;
+  const int t = threadIdx.x, shares = kBalThreads / a.E, share = t / a.E, e = t - share * a.E;
+  if (t == 0) kept_all = 0;
+  __syncthreads();
+  int kept = 0;
+  for (int b = t; b < a.blocks; b += kBalThreads) kept += a.part_n[b];
+  if (kept) atomicAdd(&kept_all, kept);
+  double s = 0.0;
+  int c = 0;
+  if (share < shares) {
+#pragma unroll 8
+    for (int b = share; b < a.blocks; b += shares) {
+      s += (double)a.part_p[(int64_t)b * a.E + e];
+      c += a.part_c[(int64_t)b * a.E + e];
+    }
+  }
+  sp[t] = s;
+  sc[t] = c;
+  __syncthreads();
+  if (t < a.E)
+    for (int i = 1; i < shares; ++i) s += sp[i * a.E + t], c += sc[i * a.E + t];
+  balance_finish(a, kept_all, s, c);
+}
+
+template <typename T, int G, int V>
+__global__ void __launch_bounds__(256) balance_grad_kernel(const void* __restrict__ logits, int64_t ld, const uint8_t* __restrict__ mask,
+                                                           const float* __restrict__ factor, const float* __restrict__ upstream,
+                                                           void* __restrict__ grad, int rows, int E) {
+  constexpr int PER = 64 / G;
+  const int lane = threadIdx.x & 63, l = lane % G;
   float f[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) f[v] = 64 * v + lane < E ? factor[64 * v + lane] : 0.f;
+  for (int v = 0; v < V; ++v) f[v] = G * v + l < E ? factor[G * v + l] : 0.f;
   const float g = upstream[0];
-  for (int row = blockIdx.x * kBalWaves + wave; row < rows; row += gridDim.x * kBalWaves) {
+  for (int64_t row = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * PER + lane / G; row < rows; row += (int64_t)gridDim.x * 4 * PER) {
     float p[V];
-    const bool in = !mask || mask[row];
-    if (in) {
-      row_softmax<T, V>(logits, (int64_t)row * ld, E, lane, p);
+    if (!mask || mask[row]) {
+      load_row<T, G, V>(logits, row * ld, E, l, p);
+      row_softmax<G, V>(p);
       float dot = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) dot = fmaf(f[v], p[v], dot);
-      dot = wave_sum_f32(dot);
+      dot = group_reduce<G>(dot, [](float a, float b) { return a + b; });
 #pragma unroll
       for (int v = 0; v < V; ++v) p[v] = g * (p[v] * (f[v] - dot));
     } else {
@@ -166,11 +199,10 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(const void* _
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int e = 64 * v + lane;
+      const int e = G * v + l;
       if (e >= E) continue;
-      const int64_t at = (int64_t)row * E + e;
-      if constexpr (std::is_same<T, float>::value) ((float*)grad)[at] = p[v];
-      else ((uint16_t*)grad)[at] = to_bits<T>(p[v]);
+      if constexpr (std::is_same<T, float>::value) ((float*)grad)[row * E + e] = p[v];
+      else ((uint16_t*)grad)[row * E + e] = to_bits<T>(p[v]);
     }
   }
 }
@@ -180,20 +212,29 @@ __global__ void __launch_bounds__(kBalThreads) balance_grad_kernel(const void* _
 namespace awq_host {
 using namespace awq;
 
-// Blocks of the forward pass: 16 rows for each of a block's waves, at most two blocks per CU.
-static int balance_blocks(int64_t T) { return (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(T, kBalWaves * 16), 512)); }
+// Up to 256 rows one block does everything; else at most a block per CU, so that the join stays small.
+static int balance_rows(int64_t T) { return T <= 256 ? 256 : (int)cdiv(T, std::min<int64_t>(256, cdiv(T, 64))); }
+static int balance_blocks(int64_t T) { return (int)std::max<int64_t>(1, cdiv(T, balance_rows(T))); }
 
 size_t balance_workspace_bytes(int64_t T, int E) { return (size_t)balance_blocks(T) * (size_t)(2 * E + 1) * 4; }
 
+// Lanes to a row and values to a lane by the number of experts.
+template <class F>
+static void by_width(int E, F f) {
+  using std::integral_constant;
+  if (E <= 64) f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  else if (E <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  else if (E <= 192) f(integral_constant<int, 16>{}, integral_constant<int, 12>{});
+  else if (E <= 256) f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  else if (E <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+  else f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+}
+
 template <typename T>
 static void rows_by_width(const BalanceArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.blocks), block(kBalThreads);
-  const auto lds = [&](int V) { return (size_t)(a.E + kBalWaves * 64 * V) * 4; };
-  if (a.E <= 64) balance_rows_kernel<T, 1><<<grid, block, lds(1), st>>>(a);
-  else if (a.E <= 128) balance_rows_kernel<T, 2><<<grid, block, lds(2), st>>>(a);
-  else if (a.E <= 256) balance_rows_kernel<T, 4><<<grid, block, lds(4), st>>>(a);
-  else if (a.E <= 512) balance_rows_kernel<T, 8><<<grid, block, lds(8), st>>>(a);
-  else balance_rows_kernel<T, 16><<<grid, block, lds(16), st>>>(a);
+  by_width(a.E, [&](auto g, auto v) {
+    balance_rows_kernel<T, decltype(g)::value, decltype(v)::value><<<dim3((unsigned)a.blocks), dim3(kBalThreads), 0, st>>>(a);
+  });
 }
 
 int launch_moe_balance(const void* logits, int64_t ld, int dtype, const void* ids, int id64, const uint8_t* mask, int64_t T, int E,
@@ -202,6 +243,7 @@ int launch_moe_balance(const void* logits, int64_t ld, int dtype, const void* id
   a.logits = logits, a.ids = ids, a.ld = ld, a.mask = mask;
   a.T = (int)T, a.E = E, a.topk = topk, a.id64 = id64;
   a.blocks = balance_blocks(T);
+  a.rows = balance_rows(T);
   a.part_p = (float*)workspace;
   a.part_c = (int*)(a.part_p + (size_t)a.blocks * E);
   a.part_n = a.part_c + (size_t)a.blocks * E;
@@ -210,19 +252,19 @@ int launch_moe_balance(const void* logits, int64_t ld, int dtype, const void* id
   else if (dtype == AWQ_DTYPE_BF16) rows_by_width<bf16>(a, st);
   else rows_by_width<float>(a, st);
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
-  balance_join_kernel<<<1, 1024, 0, st>>>(a);
+  if (a.blocks == 1) return AWQ_OK;
+  balance_join_kernel<<<1, kBalThreads, 0, st>>>(a);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
 template <typename T>
 static void grad_by_width(const void* logits, int64_t ld, const uint8_t* mask, const float* factor, const float* upstream, void* grad,
                           int T_, int E, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(cdiv(T_, kBalWaves), 2048)), block(kBalThreads);
-  if (E <= 64) balance_grad_kernel<T, 1><<<grid, block, 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
-  else if (E <= 128) balance_grad_kernel<T, 2><<<grid, block, 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
-  else if (E <= 256) balance_grad_kernel<T, 4><<<grid, block, 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
-  else if (E <= 512) balance_grad_kernel<T, 8><<<grid, block, 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
-  else balance_grad_kernel<T, 16><<<grid, block, 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
+  by_width(E, [&](auto g, auto v) {
+    constexpr int G = decltype(g)::value, V = decltype(v)::value;
+    const dim3 grid((unsigned)std::min<int64_t>(cdiv(T_, 4 * (64 / G)), 2048));
+    balance_grad_kernel<T, G, V><<<grid, dim3(256), 0, st>>>(logits, ld, mask, factor, upstream, grad, T_, E);
+  });
 }
 
 int launch_moe_balance_grad(const void* logits, int64_t ld, int dtype, const uint8_t* mask, const float* factor, const float* upstream,
