@@ -40,7 +40,7 @@ int awq_w4a16_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void
 }
 
 size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || mx_quantizes_itself(M, K)) return 0;
   return align256((size_t)M * (size_t)(K / 2)) + (size_t)M * (size_t)(K / 32);
 }
 
@@ -60,14 +60,20 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
     p.as = a_scales;
   } else {
     if (M > 1 && (lda < K || (lda % 8) != 0)) return AWQ_ERR_STRIDE;
-    if (!workspace || workspace_bytes < awq_w4a16_mxfp4_gemm_workspace_bytes(M, N, K)) return AWQ_ERR_WORKSPACE;
-    if (!aligned(workspace, 256)) return AWQ_ERR_STRIDE;
-    uint8_t* codes = (uint8_t*)workspace;
-    uint8_t* scales = codes + align256((size_t)M * (size_t)(K / 2));
-    const int rc = launch_mx_quantize(a, lda, codes, scales, K / 32, M, K, act_dtype, (hipStream_t)stream);
-    if (rc != AWQ_OK) return rc;
-    p.a = codes;
-    p.as = scales;
+    if (mx_quantizes_itself(M, K)) {
+      p.x = (const uint16_t*)a;
+      p.ldx = lda;
+      p.xrows = (int)M;
+    } else {
+      if (!workspace || workspace_bytes < awq_w4a16_mxfp4_gemm_workspace_bytes(M, N, K)) return AWQ_ERR_WORKSPACE;
+      if (!aligned(workspace, 256)) return AWQ_ERR_STRIDE;
+      uint8_t* codes = (uint8_t*)workspace;
+      uint8_t* scales = codes + align256((size_t)M * (size_t)(K / 2));
+      const int rc = launch_mx_quantize(a, lda, codes, scales, K / 32, M, K, act_dtype, (hipStream_t)stream);
+      if (rc != AWQ_OK) return rc;
+      p.a = codes;
+      p.as = scales;
+    }
   }
   p.w = w;
   p.ws = w_scales;

@@ -89,7 +89,24 @@ struct MxArgs {
   int topk, act;
   uint8_t *h, *hs;
   float* y;
+  // a in 16 bits, quantised by the blocks themselves: at most xrows rows a block
+  const uint16_t* x;
+  int64_t ldx;
+  int xrows;
+  // few routes, without a table
+  const void* ids;
+  int id64, routes, experts;
 };
+constexpr int kMxScanRoutes = 128;
+
+__device__ __forceinline__ int64_t mx_route_id(const void* ids, int id64, int64_t r) {
+  return id64 ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];
+}
+__device__ __forceinline__ float mx_route_weight(const void* w, int dtype, int64_t r) {
+  if (dtype == AWQ_DTYPE_F32) return ((const float*)w)[r];
+  const uint16_t b = ((const uint16_t*)w)[r];
+  return dtype == AWQ_DTYPE_F16 ? h_bits2f(b) : bf_bits2f(b);
+}
 
 // The rows that a block works on.
 struct MxRows {
@@ -104,7 +121,7 @@ __device__ __forceinline__ MxRows mx_rows(const MxArgs& p, int tile) {
     return {p.tiles[3 * tile], p.tiles[3 * tile + 1], p.tiles[3 * tile + 2]};
   }
 }
-// Row of a for row r of the block (rows past the end repeat the last: their results are dropped).
+// Row of a for row r of the block of a table's or a dense tile (rows past the end repeat the last: their results are dropped).
 template <int MODE>
 __device__ __forceinline__ int64_t mx_a_row(const MxArgs& p, const MxRows& t, int r) {
   const int at = t.first + (r < t.rows ? r : t.rows - 1);
@@ -116,6 +133,9 @@ __device__ __forceinline__ int64_t mx_a_row(const MxArgs& p, const MxRows& t, in
 
 namespace awq_host {
 int launch_mx_gemm(const awq::MxArgs& p, hipStream_t st);
+bool mx_quantizes_itself(int64_t M, int64_t K);  // whether launch_mx_gemm takes a in 16 bits (p.x)
+int launch_mx_scan_gate_up(const awq::MxArgs& p, hipStream_t st);
+int launch_mx_down_combine(const awq::MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st);
 int launch_mx_tile_gemm(const awq::MxArgs& p, hipStream_t st);
 int launch_mx_tile_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
 // gate_up or down product of the grouped routes in `row_tiles` (at most) row tiles of `rows` rows

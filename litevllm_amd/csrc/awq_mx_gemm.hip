@@ -1,119 +1,288 @@
-// Products of microscaled fp4 matrices on the scaled MFMA (format, modes and operand order:
-// awq_mx_common.h).
+// Products of microscaled fp4 matrices with few rows: operands straight from memory to registers (format,
+// modes and operand order: awq_mx_common.h).
+//
+// What bounds them is the read of the weights, once: a block has 16 columns (gate_up: 32 gate rows and the 32 up
+// rows of the same outputs), its waves share K, each asks for all that it will use before the first product, and
+// the waves' sums meet in LDS, in wave order.
+#include <algorithm>
+
 #include "awq_launch.h"
 #include "awq_mx_common.h"
 
 namespace awq {
-
-constexpr int kMxWaves = 4;
 
 // h of one value: act(gate) * up in fp32.
 __device__ __forceinline__ float mx_gated(float g, float u, int act) {
   return (act == AWQ_MOE_ACT_GELU_TANH ? gated_act_fast<1>(g) : gated_act_fast<0>(g)) * u;
 }
 
-// Block: 16 MT rows of a by 16 NT rows of w; its waves take the steps of 128 along K in turn and their
-// sums meet in LDS.  Operands go straight from memory to registers: each weight byte is used by one
-// block of the row tile only.
-// Grid x: column blocks, y: row tiles.  Gate_up blocks hold 32 gate rows and the same 32 up rows.
-template <int MODE, int MT, int NT>
-__global__ void __launch_bounds__(kMxWaves * 64) mx_rows_kernel(MxArgs p) {
-  __shared__ float red[kMxWaves][MT * NT][256];
-  const int tile = blockIdx.y;
-  if (MODE != kMxDense && tile >= p.tile_count[0]) return;
-  const MxRows t = mx_rows<MODE, 16 * MT>(p, tile);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
-  const int n0 = (int)blockIdx.x * COLS;
-  const int KB = p.K / 32, steps = (KB + 3) / 4;
+// The fragments of a pair of steps (256 along K, one line of a row): quarter q of the wave takes the pair's
+// blocks 2 q and 2 q + 1, one in each step -- the order along K is free as long as both operands share it -- so a
+// lane's codes are 32 neighbouring bytes and its two scales neighbours too.
+struct MxPair {
+  u32x4 c[2];
+  uint32_t s;
+};
+// `block`: 8 pair + 2 q.  Behind K's end codes 0 and the scale 2^-127.
+template <bool STREAM>
+__device__ __forceinline__ MxPair mx_load_pair(const uint8_t* codes, const uint8_t* scales, int block, int KB) {
+  MxPair f{{u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}}, 0u};
+  const u32x4* at = (const u32x4*)(codes + (int64_t)block * 16);
+  auto load = [](const u32x4* p) { return STREAM ? __builtin_nontemporal_load(p) : *p; };
+  if (block + 1 < KB) {
+    f.c[0] = load(at);
+    f.c[1] = load(at + 1);
+    uint16_t s;
+    __builtin_memcpy(&s, scales + block, 2);
+    f.s = s;
+  } else if (block < KB) {
+    f.c[0] = load(at);
+    f.s = scales[block];
+  }
+  return f;
+}
 
-  const uint8_t *wc[NT], *wsc[NT], *ac[MT], *asc[MT];
+// Eight values of a row to LDS codes, by a lane; the four lanes of a block share its largest magnitude.
+template <typename T>
+__device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, uint8_t* scales, int piece) {
+  float v[8];
+  load8<T>(x + piece * 8, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, mx_abs_bits(v[j]));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
+  const uint32_t byte = mx_scale_byte(top);
+  *(uint32_t*)(codes + piece * 4) = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
+  if ((piece & 3) == 0) scales[piece >> 2] = (uint8_t)byte;
+}
+
+// Grid x: column blocks, y: row tiles of 16 MT (with SCAN: routes).
+// X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one
+// launch less where the rows are few and short.
+// SCAN (gate_up): no table of tiles; block y takes all the routes of route y's expert, which it finds in the ids
+// itself, if y is the first of them.  A route's place is its own number.
+template <int MODE, int MT, int NT, int WAVES, bool X16, bool SCAN>
+__global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
+  constexpr int THREADS = WAVES * 64;
+  constexpr int U = MT == 1 && NT == 1 ? 4 : (MT * NT <= 4 ? 2 : 1);  // pairs of steps under way in a wave
+  __shared__ float red[WAVES][MT * NT][256];
+  __shared__ int list[SCAN ? kMxScanRoutes : 1], listed;
+  extern __shared__ __align__(16) uint8_t xq[];  // X16: codes [xrows][K/2 + 16], scales [xrows][K/32]
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  MxRows t;
+  if constexpr (SCAN) {
+    const int64_t e = mx_route_id(p.ids, p.id64, blockIdx.y);
+    if (e < 0 || e >= p.experts) return;
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    bool earlier = false;
+    for (int i = tid; i < p.routes; i += THREADS)
+      if (mx_route_id(p.ids, p.id64, i) == e) {
+        earlier = earlier || i < (int)blockIdx.y;
+        list[atomicAdd(&listed, 1)] = i;
+      }
+    if (__syncthreads_or(earlier)) return;
+    t = {(int)e, 0, listed};
+  } else {
+    if (MODE != kMxDense && (int)blockIdx.y >= p.tile_count[0]) return;
+    t = mx_rows<MODE, 16 * MT>(p, blockIdx.y);
+  }
+  constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
+  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = (KB + 7) / 8;
+
+  const uint8_t *wc[NT], *wsc[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     int64_t row;
     if constexpr (MODE == kMxGateUp) row = (j < NT / 2 ? n0 + 16 * j : p.N + n0 + 16 * (j - NT / 2)) + r;
-    else row = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
+    else row = min(n0 + 16 * j + r, p.N - 1);
     row += (int64_t)t.expert * p.wrows;
-    wc[j] = p.w + row * (p.K / 2) + q * 16;
-    wsc[j] = p.ws + row * KB + q;
+    wc[j] = p.w + row * (p.K / 2);
+    wsc[j] = p.ws + row * KB;
   }
+  const int ld = p.K / 2 + 16;
+  // a scanned expert may have more routes than a tile has rows (one that occurs twice in a token)
+  for (int base = 0; base < (SCAN ? t.rows : 1); base += 16 * MT) {
+    const int rows = SCAN ? min(t.rows - base, 16 * MT) : t.rows;
+    const uint8_t *ac[MT], *asc[MT];
+    if constexpr (!X16) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int64_t row = mx_a_row<MODE>(p, t, 16 * i + r);
-    ac[i] = p.a + row * (p.K / 2) + q * 16;
-    asc[i] = p.as + row * p.as_ld + q;
-  }
-
-  f32x4 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-#pragma unroll 2
-  for (int s = wave; s < steps; s += kMxWaves) {
-    const bool in = 4 * s + q < KB;  // the last step may end inside
-    u32x4 a[MT], b[NT];
-    uint32_t sa[MT], sb[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      b[j] = in ? *(const u32x4*)(wc[j] + (int64_t)s * 64) : u32x4{0u, 0u, 0u, 0u};
-      sb[j] = in ? wsc[j][s * 4] : 127u;
+      for (int i = 0; i < MT; ++i) {
+        const int64_t row = SCAN ? list[base + min(16 * i + r, rows - 1)] / p.topk : mx_a_row<MODE>(p, t, 16 * i + r);
+        ac[i] = p.a + row * (p.K / 2);
+        asc[i] = p.as + row * p.as_ld;
+      }
     }
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      a[i] = in ? *(const u32x4*)(ac[i] + (int64_t)s * 64) : u32x4{0u, 0u, 0u, 0u};
-      sa[i] = in ? asc[i][s * 4] : 127u;
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    MxPair b[U][NT];
+    auto load_w = [&](int first) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) b[u][j] = mx_load_pair<true>(wc[j], wsc[j], 8 * (first + u * WAVES) + 2 * q, KB);
+    };
+    load_w(wave);
+    if constexpr (X16) {
+      const int pieces = p.K / 8;
+      for (int m = 0; m < rows; ++m) {
+        const int64_t row = SCAN ? list[base + m] / p.topk : t.first + m;
+        const uint16_t* x = p.x + row * p.ldx;
+        uint8_t *codes = xq + m * ld, *scales = xq + p.xrows * ld + m * KB;
+        for (int i = tid; i < pieces; i += THREADS) {
+          if (p.out_bf16) mx_quantize8<bf16>(x, codes, scales, i);
+          else mx_quantize8<f16>(x, codes, scales, i);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const int m = min(16 * i + r, rows - 1);
+        ac[i] = xq + m * ld;
+        asc[i] = xq + p.xrows * ld + m * KB;
+      }
+    }
+    for (int first = wave; first < pairs; first += U * WAVES) {
+      if (first != wave) load_w(first);
+      MxPair a[U][MT];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[u][i] = mx_load_pair<false>(ac[i], asc[i], 8 * (first + u * WAVES) + 2 * q, KB);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            acc[i][j] = mx_mfma<0, 0>(a[u][i].c[0], b[u][j].c[0], acc[i][j], a[u][i].s, b[u][j].s);
+            acc[i][j] = mx_mfma<1, 1>(a[u][i].c[1], b[u][j].c[1], acc[i][j], a[u][i].s, b[u][j].s);
+          }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma<0, 0>(a[i], b[j], acc[i][j], sa[i], sb[j]);
-  }
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) red[wave][i * NT + j][(4 * q + u) * 16 + r] = acc[i][j][u];
-  __syncthreads();
+        for (int u = 0; u < 4; ++u) red[wave][i * NT + j][(4 * q + u) * 16 + r] = acc[i][j][u];
+    __syncthreads();
 
-  auto sum = [&](int tile16, int at) {
-    float v = red[0][tile16][at];
+    auto sum = [&](int tile16, int at) {
+      float v = red[0][tile16][at];
 #pragma unroll
-    for (int w = 1; w < kMxWaves; ++w) v += red[w][tile16][at];
-    return v;
-  };
-  if constexpr (MODE == kMxGateUp) {
-    // 32 lanes hold a row's 32 columns: their largest magnitude, then the codes, two to a byte
-    static_assert(NT == 4, "32 gate and 32 up rows");
-    const int n = threadIdx.x & 31;
-    for (int m = threadIdx.x >> 5; m < t.rows; m += kMxWaves * 2) {
-      const int at = (m & 15) * 16 + (n & 15), tg = (m >> 4) * NT + (n >> 4);
-      const float v = mx_gated(sum(tg, at), sum(tg + 2, at), p.act);
-      uint32_t top = mx_abs_bits(v);
+      for (int w = 1; w < WAVES; ++w) v += red[w][tile16][at];
+      return v;
+    };
+    if constexpr (MODE == kMxGateUp) {
+      // 32 lanes hold a row's 32 columns: their largest magnitude, then the codes, two to a byte
+      static_assert(NT == 4, "32 gate and 32 up rows");
+      const int n = tid & 31;
+      for (int m = tid >> 5; m < rows; m += THREADS / 32) {
+        const int at = (m & 15) * 16 + (n & 15), tg = (m >> 4) * NT + (n >> 4);
+        const float v = mx_gated(sum(tg, at), sum(tg + 2, at), p.act);
+        uint32_t top = mx_abs_bits(v);
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-      const uint32_t byte = mx_scale_byte(top);
-      const float other = __shfl_xor(v, 1);
-      if ((n & 1) == 0) {
-        const uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v, other, mx_scale_value(byte == 255u ? 0u : byte), 0);
-        p.h[(int64_t)(t.first + m) * (p.N / 2) + (n0 + n) / 2] = byte == 255u ? (uint8_t)0 : (uint8_t)code;
+        for (int d = 1; d < 32; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        const uint32_t byte = mx_scale_byte(top);
+        const float other = __shfl_xor(v, 1);
+        const int64_t place = SCAN ? list[base + m] : t.first + m;
+        if ((n & 1) == 0) {
+          const uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v, other, mx_scale_value(byte == 255u ? 0u : byte), 0);
+          p.h[place * (p.N / 2) + (n0 + n) / 2] = byte == 255u ? (uint8_t)0 : (uint8_t)code;
+        }
+        if (n == 0) p.hs[place * (p.N / 32) + n0 / 32] = (uint8_t)byte;
       }
-      if (n == 0) p.hs[(int64_t)(t.first + m) * (p.N / 32) + n0 / 32] = (uint8_t)byte;
-    }
-  } else {
-    for (int i = threadIdx.x; i < MT * NT * 256; i += kMxWaves * 64) {
-      const int t16 = i >> 8, at = i & 255, m = (t16 / NT) * 16 + (at >> 4), n = n0 + (t16 % NT) * 16 + (at & 15);
-      if (m >= t.rows || n >= p.N) continue;
-      float v = sum(t16, at);
-      if constexpr (MODE == kMxDense) {
-        v += load_bias(p.bias, p.bias_dtype, n);
-        p.c[(int64_t)(t.first + m) * p.ldc + n] = p.out_bf16 ? f2bf_bits(v) : f2h_bits(v);
-      } else {
-        p.y[(int64_t)p.order[t.first + m] * p.N + n] = v;
+    } else {
+      for (int i = tid; i < MT * NT * 256; i += THREADS) {
+        const int t16 = i >> 8, at = i & 255, m = (t16 / NT) * 16 + (at >> 4), n = n0 + (t16 % NT) * 16 + (at & 15);
+        if (m >= rows || n >= p.N) continue;
+        float v = sum(t16, at);
+        if constexpr (MODE == kMxDense) {
+          v += load_bias(p.bias, p.bias_dtype, n);
+          p.c[(int64_t)(t.first + m) * p.ldc + n] = p.out_bf16 ? f2bf_bits(v) : f2h_bits(v);
+        } else {
+          p.y[(int64_t)p.order[t.first + m] * p.N + n] = v;
+        }
       }
     }
+    if constexpr (SCAN) __syncthreads();
+  }
+}
+
+// The down product of at most kMxScanRoutes routes with the weighted sum over each token's slots, in one launch: a
+// block has 16 columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
+// place is its own number.
+constexpr int kDownWaves = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs p, const void* weights, int w_dtype,
+                                                                          uint16_t* out, int64_t ldo) {
+  constexpr int THREADS = kDownWaves * 64, U = 4;
+  __shared__ float y[kMxScanRoutes][16];
+  __shared__ int expert[kMxScanRoutes], todo[kMxScanRoutes], head[1024], todos, slot[kDownWaves][kMxScanRoutes];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
+  if (tid == 0) todos = 0;
+  for (int e = tid; e < p.experts; e += THREADS) head[e] = p.routes;
+  __syncthreads();
+  for (int i = tid; i < p.routes; i += THREADS) {
+    const int64_t e = mx_route_id(p.ids, p.id64, i);
+    expert[i] = e >= 0 && e < p.experts ? (int)e : -1;
+    if (expert[i] >= 0) atomicMin(&head[expert[i]], i);
+  }
+  __syncthreads();
+  for (int i = tid; i < p.routes; i += THREADS)
+    if (expert[i] >= 0 && head[expert[i]] == i) todo[atomicAdd(&todos, 1)] = i;
+  __syncthreads();
+  const int n0 = (int)blockIdx.x * 16, KB = p.K / 32, pairs = (KB + 7) / 8;
+  for (int k = wave; k < todos; k += kDownWaves) {
+    const int e = expert[todo[k]];
+    const int64_t row = (int64_t)e * p.wrows + min(n0 + r, p.N - 1);
+    const uint8_t *wc = p.w + row * (p.K / 2), *wsc = p.ws + row * KB;
+    // this expert's routes, to the wave's slots
+    int n = 0;
+    for (int i = 0; i < p.routes; i += 64) {
+      const bool its = i + lane < p.routes && expert[i + lane] == e;
+      const uint64_t m = __ballot(its);
+      if (its) slot[wave][n + __popcll(m & ((1ull << lane) - 1))] = i + lane;
+      n += __popcll(m);
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int at = 0; at < n; at += 16) {
+      const int mine = slot[wave][min(at + r, n - 1)];
+      const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2), *asc = p.as + (int64_t)mine * p.as_ld;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int first = 0; first < pairs; first += U) {
+        MxPair a[U], b[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) b[u] = mx_load_pair<true>(wc, wsc, 8 * (first + u) + 2 * q, KB);
+#pragma unroll
+        for (int u = 0; u < U; ++u) a[u] = mx_load_pair<false>(ac, asc, 8 * (first + u) + 2 * q, KB);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          // swapped: a lane holds four columns of the route in lane r
+          acc = mx_mfma<0, 0>(b[u].c[0], a[u].c[0], acc, b[u].s, a[u].s);
+          acc = mx_mfma<1, 1>(b[u].c[1], a[u].c[1], acc, b[u].s, a[u].s);
+        }
+      }
+      if (at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
+    }
+  }
+  __syncthreads();
+  const int tokens = p.routes / p.topk;
+  for (int i = tid; i < tokens * 16; i += THREADS) {
+    const int t = i >> 4, n = i & 15;
+    if (n0 + n >= p.N) continue;
+    float s = 0.f;
+    for (int j = 0; j < p.topk; ++j) {
+      const int route = t * p.topk + j;
+      if (expert[route] >= 0) s = fmaf(y[route][n], mx_route_weight(weights, w_dtype, route), s);
+    }
+    out[(int64_t)t * ldo + n0 + n] = to_bits<T>(s);
   }
 }
 
@@ -122,26 +291,52 @@ __global__ void __launch_bounds__(kMxWaves * 64) mx_rows_kernel(MxArgs p) {
 namespace awq_host {
 using namespace awq;
 
-template <int MODE, int MT, int NT>
-static void launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
+template <int MODE, int MT, int NT, int WAVES, bool X16, bool SCAN>
+static int launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
-  const dim3 grid((unsigned)cdiv(p.N, COLS), (unsigned)row_tiles);
-  mx_rows_kernel<MODE, MT, NT><<<grid, dim3(kMxWaves * 64), 0, st>>>(p);
+  auto kernel = mx_rows_kernel<MODE, MT, NT, WAVES, X16, SCAN>;
+  const size_t lds = X16 ? (size_t)p.xrows * (p.K / 2 + 16 + p.K / 32) : 0;
+  kernel<<<dim3((unsigned)cdiv(p.N, COLS), (unsigned)row_tiles), dim3(WAVES * 64), lds, st>>>(p);
+  return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
+
+// Waves of a block by the number of column blocks: 16 of them where there is a block to a CU, fewer where several
+// blocks share one.
+template <int MODE, int MT, int NT, bool X16, bool SCAN>
+static int launch_rows_by_waves(const MxArgs& p, int64_t row_tiles, int64_t blocks, hipStream_t st) {
+  if (MT * NT <= 2 && blocks <= 256) return launch_rows<MODE, MT, NT, MT * NT <= 2 ? 16 : 8, X16, SCAN>(p, row_tiles, st);
+  if (MT * NT <= 4 && blocks <= 512) return launch_rows<MODE, MT, NT, MT * NT <= 4 ? 8 : 4, X16, SCAN>(p, row_tiles, st);
+  return launch_rows<MODE, MT, NT, 4, X16, SCAN>(p, row_tiles, st);
+}
+
+// Up to here every block quantises a's rows for itself: 32768 values, a sweep or two of a block's threads.
+bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
 
 int launch_mx_gemm(const MxArgs& p, hipStream_t st) {
   if (p.M > 64) return launch_mx_tile_gemm(p, st);
-  if (p.M <= 16) launch_rows<kMxDense, 1, 1>(p, 1, st);
-  else if (p.M <= 32) launch_rows<kMxDense, 2, 1>(p, 1, st);
-  else launch_rows<kMxDense, 4, 2>(p, 1, st);
-  return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
+  const int64_t blocks = cdiv(p.N, 16);
+  if (p.x) return launch_rows_by_waves<kMxDense, 1, 1, true, false>(p, 1, blocks, st);
+  if (p.M <= 16) return launch_rows_by_waves<kMxDense, 1, 1, false, false>(p, 1, blocks, st);
+  if (p.M <= 32) return launch_rows_by_waves<kMxDense, 2, 1, false, false>(p, 1, blocks, st);
+  return launch_rows_by_waves<kMxDense, 4, 1, false, false>(p, 1, blocks, st);
 }
 
 int launch_mx_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
   if (rows > 16) return launch_mx_tile_grouped(p, gate_up, rows, row_tiles, st);
   if (row_tiles > 65535) return AWQ_ERR_UNSUPPORTED;
-  if (gate_up) launch_rows<kMxGateUp, 1, 4>(p, row_tiles, st);
-  else launch_rows<kMxDown, 1, 2>(p, row_tiles, st);
+  if (gate_up) return launch_rows<kMxGateUp, 1, 4, 4, false, false>(p, row_tiles, st);
+  return launch_rows<kMxDown, 1, 2, 4, false, false>(p, row_tiles, st);
+}
+
+int launch_mx_scan_gate_up(const MxArgs& p, hipStream_t st) {
+  if (p.x) return launch_rows<kMxGateUp, 1, 4, 4, true, true>(p, p.routes, st);
+  return launch_rows<kMxGateUp, 1, 4, 4, false, true>(p, p.routes, st);
+}
+
+int launch_mx_down_combine(const MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st) {
+  const dim3 grid((unsigned)cdiv(p.N, 16));
+  if (p.out_bf16) mx_down_combine_kernel<bf16><<<grid, dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  else mx_down_combine_kernel<f16><<<grid, dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

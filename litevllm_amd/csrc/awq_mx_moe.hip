@@ -9,10 +9,6 @@ namespace awq {
 
 constexpr int kOrderThreads = 1024;
 
-__device__ __forceinline__ int64_t route_id(const void* ids, int id64, int64_t r) {
-  return id64 ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];
-}
-
 // Sorts the routes by expert (one block): order[place] = route, and the table of row tiles, at most
 // `rows` places of one expert each.  The order inside an expert is that of the atomics; no result
 // depends on it, since every place's row is computed by itself and summed by its route.  Routes
@@ -27,7 +23,7 @@ __global__ void __launch_bounds__(kOrderThreads) mx_order_kernel(const void* __r
   for (int e = t; e < E; e += kOrderThreads) count[e] = 0;
   __syncthreads();
   for (int r = t; r < R; r += kOrderThreads) {
-    const int64_t e = route_id(ids, id64, r);
+    const int64_t e = mx_route_id(ids, id64, r);
     if (e >= 0 && e < E) atomicAdd(&count[e], 1);
   }
   __syncthreads();
@@ -50,15 +46,9 @@ __global__ void __launch_bounds__(kOrderThreads) mx_order_kernel(const void* __r
   if (t == kOrderThreads - 1) tile_count[0] = ft + nt;
   __syncthreads();
   for (int r = t; r < R; r += kOrderThreads) {
-    const int64_t e = route_id(ids, id64, r);
+    const int64_t e = mx_route_id(ids, id64, r);
     if (e >= 0 && e < E) order[atomicAdd(&cursor[e], 1)] = r;
   }
-}
-
-__device__ __forceinline__ float route_weight(const void* w, int dtype, int64_t r) {
-  if (dtype == AWQ_DTYPE_F32) return ((const float*)w)[r];
-  const uint16_t b = ((const uint16_t*)w)[r];
-  return dtype == AWQ_DTYPE_F16 ? h_bits2f(b) : bf_bits2f(b);
 }
 
 // out[t] = the sum over a token's slots, in slot order, of weight * y: fp32, one rounding.  A slot
@@ -73,10 +63,10 @@ __global__ void __launch_bounds__(256) mx_combine_kernel(const float* __restrict
   const int c = (int)(i - t * (H / 4)) * 4;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   for (int j = 0; j < topk; ++j) {
-    const int64_t r = t * topk + j, e = route_id(ids, id64, r);
+    const int64_t r = t * topk + j, e = mx_route_id(ids, id64, r);
     if (e < 0 || e >= E) continue;
     const f32x4 v = *(const f32x4*)(y + r * H + c);
-    const float g = route_weight(w, w_dtype, r);
+    const float g = mx_route_weight(w, w_dtype, r);
 #pragma unroll
     for (int u = 0; u < 4; ++u) s[u] = fmaf(v[u], g, s[u]);
   }
@@ -122,6 +112,29 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   if (R > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
   const MxMoeWorkspace w = mx_moe_workspace(c.T, c.H, c.I, c.E, c.topk);
   char* ws = (char*)c.workspace;
+  if (R <= kMxScanRoutes) {
+    // two launches: gate_up, which finds its routes and quantises its tokens itself, and down with the weighted sum
+    MxArgs g{};
+    if (c.H <= 4096) {
+      g.x = (const uint16_t*)c.x, g.ldx = c.ldx, g.xrows = 16;
+    } else {
+      const int rc = launch_mx_quantize(c.x, c.ldx, (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), c.H / 32, c.T, c.H, c.act_dtype, st);
+      if (rc != AWQ_OK) return rc;
+      g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);
+    }
+    g.w = c.gate_up, g.ws = c.gate_up_scales;
+    g.K = (int)c.H, g.N = (int)c.I, g.wrows = 2 * c.I, g.a_rows = c.T, g.as_ld = (int)(c.H / 32);
+    g.ids = c.ids, g.id64 = c.id64, g.routes = (int)R, g.experts = c.E, g.topk = c.topk;
+    g.act = c.act_kind, g.out_bf16 = c.act_dtype == AWQ_DTYPE_BF16;
+    g.h = (uint8_t*)(ws + w.h), g.hs = (uint8_t*)(ws + w.hs);
+    const int rc = launch_mx_scan_gate_up(g, st);
+    if (rc != AWQ_OK) return rc;
+    MxArgs d = g;
+    d.x = nullptr, d.a = g.h, d.as = g.hs;
+    d.w = c.down, d.ws = c.down_scales;
+    d.K = (int)c.I, d.N = (int)c.H, d.wrows = c.H, d.a_rows = R, d.as_ld = (int)(c.I / 32);
+    return launch_mx_down_combine(d, c.weights, c.weights_dtype, c.out, c.ldo, st);
+  }
   int* order = (int*)(ws + w.order);
   int* tiles = (int*)(ws + w.tiles);
   const int rows = mx_moe_rows(R, c.E);

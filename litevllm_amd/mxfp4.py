@@ -133,7 +133,8 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
     if a_scales is None:
         a, ld = _rows(a)
         ws_bytes = lib.awq_w4a16_mxfp4_gemm_workspace_bytes(m, n, k)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     else:
         a, a_scales = _dense(a), a_scales.contiguous()
     if bias is not None:
