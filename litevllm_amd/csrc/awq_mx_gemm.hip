@@ -23,27 +23,33 @@ struct MxPair {
   u32x4 c[2];
   uint32_t s[2];
 };
-// Behind K's end codes 0 and the scale 2^-127.
-__device__ __forceinline__ MxPair mx_load_pair(const uint8_t* codes, const uint8_t* scales, int pair, int q, int KB) {
-  MxPair f{{u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}}, {0u, 0u}};
+// A whole pair; its scales still as they lie in memory, all of a half's four in every lane: nothing here waits for a
+// load.
+__device__ __forceinline__ MxPair mx_load_pair(const uint8_t* codes, const uint8_t* scales, int pair, int q) {
+  MxPair f;
   const u32x4* at = (const u32x4*)(codes + (int64_t)pair * 128) + q;
-  const uint8_t* sat = scales + 8 * pair;
-  if (8 * pair + 8 <= KB) {
-    f.c[0] = at[0];
-    f.c[1] = at[4];
-    uint32_t s[2];
-    __builtin_memcpy(s, sat, 8);
-    f.s[0] = s[0] >> (8 * q);
-    f.s[1] = s[1] >> (8 * q);
-  } else {
+  f.c[0] = at[0];
+  f.c[1] = at[4];
+  __builtin_memcpy(f.s, scales + 8 * pair, 8);
+  return f;
+}
+// The pair that K ends in, in the same form: behind the end codes 0 and the scale 2^-127.
+__device__ __forceinline__ MxPair mx_load_last(const uint8_t* codes, const uint8_t* scales, int pair, int q, int KB) {
+  MxPair f{{u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}}, {0u, 0u}};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (8 * pair + 4 * h + q < KB) {
-        f.c[h] = at[4 * h];
-        f.s[h] = sat[4 * h + q];
-      }
+  for (int h = 0; h < 2; ++h) {
+    const int block = 8 * pair + 4 * h + q;
+    if (block < KB) {
+      f.c[h] = *(const u32x4*)(codes + (int64_t)block * 16);
+      f.s[h] = (uint32_t)scales[block] << (8 * q);
+    }
   }
   return f;
+}
+// c += a . b^T over the pair
+__device__ __forceinline__ f32x4 mx_mfma_pair(const MxPair& a, const MxPair& b, f32x4 c, int q) {
+  c = mx_mfma<0, 0>(a.c[0], b.c[0], c, a.s[0] >> (8 * q), b.s[0] >> (8 * q));
+  return mx_mfma<0, 0>(a.c[1], b.c[1], c, a.s[1] >> (8 * q), b.s[1] >> (8 * q));
 }
 
 // Eight values of a row to LDS codes, by a lane; the four lanes of a block share its largest magnitude.
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   __shared__ float red[WAVES][MT * NT][256];
   __shared__ int list[SCAN ? kMxScanRoutes : 1], listed;
   extern __shared__ __align__(16) uint8_t xq[];  // X16: codes [xrows][K/2 + 16], scales [xrows][K/32]
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
   MxRows t;
   if constexpr (SCAN) {
     const int64_t e = mx_route_id(p.ids, p.id64, blockIdx.y);
@@ -93,7 +99,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     t = mx_rows<MODE, 16 * MT>(p, blockIdx.y);
   }
   constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
-  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = (KB + 7) / 8;
+  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;  // whole ones
 
   const uint8_t *wc[NT], *wsc[NT];
 #pragma unroll
@@ -128,8 +134,10 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     auto load_w = [&](int first) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if (first + u * WAVES < pairs) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) b[u][j] = mx_load_pair(wc[j], wsc[j], first + u * WAVES, q, KB);
+          for (int j = 0; j < NT; ++j) b[u][j] = mx_load_pair(wc[j], wsc[j], first + u * WAVES, q);
+        }
     };
     load_w(wave);
     if constexpr (X16) {
@@ -156,17 +164,29 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
       MxPair a[U][MT];
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if (first + u * WAVES < pairs) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) a[u][i] = mx_load_pair(ac[i], asc[i], first + u * WAVES, q, KB);
+          for (int i = 0; i < MT; ++i) a[u][i] = mx_load_pair(ac[i], asc[i], first + u * WAVES, q);
+        }
 #pragma unroll
       for (int u = 0; u < U; ++u)
+        if (first + u * WAVES < pairs) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+          for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            acc[i][j] = mx_mfma<0, 0>(a[u][i].c[0], b[u][j].c[0], acc[i][j], a[u][i].s[0], b[u][j].s[0]);
-            acc[i][j] = mx_mfma<0, 0>(a[u][i].c[1], b[u][j].c[1], acc[i][j], a[u][i].s[1], b[u][j].s[1]);
-          }
+            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_pair(a[u][i], b[u][j], acc[i][j], q);
+        }
+    }
+    if ((KB & 7) != 0 && wave == pairs % WAVES) {
+      MxPair w[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w[j] = mx_load_last(wc[j], wsc[j], pairs, q, KB);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const MxPair x = mx_load_last(ac[i], asc[i], pairs, q, KB);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_pair(x, w[j], acc[i][j], q);
+      }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -242,7 +262,7 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
   for (int i = tid; i < p.routes; i += THREADS)
     if (expert[i] >= 0 && head[expert[i]] == i) todo[atomicAdd(&todos, 1)] = i;
   __syncthreads();
-  const int n0 = (int)blockIdx.x * 16, KB = p.K / 32, pairs = (KB + 7) / 8;
+  const int n0 = (int)blockIdx.x * 16, KB = p.K / 32, pairs = KB / 8;
   for (int k = wave; k < todos; k += kDownWaves) {
     const int e = expert[todo[k]];
     const int64_t row = (int64_t)e * p.wrows + min(n0 + r, p.N - 1);
@@ -260,19 +280,20 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
       const int mine = slot[wave][min(at + r, n - 1)];
       const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2), *asc = p.as + (int64_t)mine * p.as_ld;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      // the operands swapped: a lane holds four columns of the route in lane r
       for (int first = 0; first < pairs; first += U) {
         MxPair a[U], b[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) b[u] = mx_load_pair(wc, wsc, first + u, q, KB);
+        for (int u = 0; u < U; ++u)
+          if (first + u < pairs) b[u] = mx_load_pair(wc, wsc, first + u, q);
 #pragma unroll
-        for (int u = 0; u < U; ++u) a[u] = mx_load_pair(ac, asc, first + u, q, KB);
+        for (int u = 0; u < U; ++u)
+          if (first + u < pairs) a[u] = mx_load_pair(ac, asc, first + u, q);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          // swapped: a lane holds four columns of the route in lane r
-          acc = mx_mfma<0, 0>(b[u].c[0], a[u].c[0], acc, b[u].s[0], a[u].s[0]);
-          acc = mx_mfma<0, 0>(b[u].c[1], a[u].c[1], acc, b[u].s[1], a[u].s[1]);
-        }
+        for (int u = 0; u < U; ++u)
+          if (first + u < pairs) acc = mx_mfma_pair(b[u], a[u], acc, q);
       }
+      if ((KB & 7) != 0) acc = mx_mfma_pair(mx_load_last(wc, wsc, pairs, q, KB), mx_load_last(ac, asc, pairs, q, KB), acc, q);
       if (at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
     }
   }
