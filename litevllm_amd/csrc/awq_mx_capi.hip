@@ -60,12 +60,13 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
     p.as = a_scales;
   } else {
     if (M > 1 && (lda < K || (lda % 8) != 0)) return AWQ_ERR_STRIDE;
-    if (mx_quantizes_itself(M, K)) {
+    const size_t need = awq_w4a16_mxfp4_gemm_workspace_bytes(M, N, K);
+    if (need == 0) {
       p.x = (const uint16_t*)a;
       p.ldx = lda;
       p.xrows = (int)M;
     } else {
-      if (!workspace || workspace_bytes < awq_w4a16_mxfp4_gemm_workspace_bytes(M, N, K)) return AWQ_ERR_WORKSPACE;
+      if (!workspace || workspace_bytes < need) return AWQ_ERR_WORKSPACE;
       if (!aligned(workspace, 256)) return AWQ_ERR_STRIDE;
       uint8_t* codes = (uint8_t*)workspace;
       uint8_t* scales = codes + align256((size_t)M * (size_t)(K / 2));
@@ -88,7 +89,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   p.bias = bias;
   p.bias_dtype = bias_dtype;
   p.out_bf16 = act_dtype == AWQ_DTYPE_BF16;
-  return launch_mx_gemm(p, (hipStream_t)stream);
+  return M <= kMxRowsMax ? launch_mx_rows_gemm(p, (hipStream_t)stream) : launch_mx_tile_gemm(p, (hipStream_t)stream);
 }
 
 size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k) {

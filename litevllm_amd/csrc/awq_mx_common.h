@@ -132,12 +132,14 @@ __device__ __forceinline__ int64_t mx_a_row(const MxArgs& p, const MxRows& t, in
 }  // namespace awq
 
 namespace awq_host {
-int launch_mx_gemm(const awq::MxArgs& p, hipStream_t st);
-bool mx_quantizes_itself(int64_t M, int64_t K);  // whether launch_mx_gemm takes a in 16 bits (p.x)
-int launch_mx_scan_gate_up(const awq::MxArgs& p, hipStream_t st);
-int launch_mx_down_combine(const awq::MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st);
 int launch_mx_tile_gemm(const awq::MxArgs& p, hipStream_t st);
-int launch_mx_tile_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
+int launch_mx_rows_gemm(const awq::MxArgs& p, hipStream_t st);
+bool mx_quantizes_itself(int64_t M, int64_t K);  // whether launch_mx_rows_gemm takes a in 16 bits (p.x)
+constexpr int64_t kMxRowsMax = 16;               // rows that launch_mx_rows_gemm takes
 // gate_up or down product of the grouped routes in `row_tiles` (at most) row tiles of `rows` rows
 int launch_mx_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
+int launch_mx_tile_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
+// the same for at most kMxScanRoutes routes, without a table; down with the weighted sum
+int launch_mx_scan_gate_up(const awq::MxArgs& p, hipStream_t st);
+int launch_mx_down_combine(const awq::MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st);
 }  // namespace awq_host

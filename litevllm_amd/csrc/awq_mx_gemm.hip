@@ -67,6 +67,27 @@ __device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, 
   if ((piece & 3) == 0) scales[piece >> 2] = (uint8_t)byte;
 }
 
+// The routes of the expert of a route, found by a wave: two masks over the at most kMxScanRoutes routes.
+struct MxScan {
+  uint64_t lo, hi;
+  int expert, first;  // first: the lowest of them; -1 if the route has no expert
+  __device__ int count() const { return __popcll(lo) + __popcll(hi); }
+};
+__device__ __forceinline__ MxScan mx_scan(const MxArgs& p, int route, int lane) {
+  const int64_t e = mx_route_id(p.ids, p.id64, route);
+  const int64_t a = lane < p.routes ? mx_route_id(p.ids, p.id64, lane) : -1;
+  const int64_t b = lane + 64 < p.routes ? mx_route_id(p.ids, p.id64, lane + 64) : -1;
+  MxScan f{__ballot(a == e), __ballot(b == e), (int)e, -1};
+  if (e >= 0 && e < p.experts) f.first = f.lo ? __ffsll((unsigned long long)f.lo) - 1 : 63 + __ffsll((unsigned long long)f.hi);
+  return f;
+}
+__device__ __forceinline__ void mx_scan_list(const MxScan& f, int lane, int* list) {
+  const uint64_t below = (1ull << lane) - 1;
+  if (f.lo >> lane & 1) list[__popcll(f.lo & below)] = lane;
+  if (f.hi >> lane & 1) list[__popcll(f.lo) + __popcll(f.hi & below)] = lane + 64;
+}
+static_assert(kMxScanRoutes == 128, "two masks");
+
 // Grid x: column blocks, y: row tiles of 16 MT (with SCAN: routes).
 // X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one
 // launch less where the rows are few and short.
@@ -75,25 +96,18 @@ __device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, 
 template <int MODE, int MT, int NT, int WAVES, bool X16, bool SCAN>
 __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   constexpr int THREADS = WAVES * 64;
-  constexpr int U = MT == 1 && NT == 1 ? 4 : (MT * NT <= 4 ? 2 : 1);  // pairs of steps under way in a wave
+  constexpr int U = 1;  // pairs of steps under way in a wave; 2 or 4 measured the same: other waves fill in
   __shared__ float red[WAVES][MT * NT][256];
-  __shared__ int list[SCAN ? kMxScanRoutes : 1], listed;
+  __shared__ int list[SCAN ? kMxScanRoutes : 1];
   extern __shared__ __align__(16) uint8_t xq[];  // X16: codes [xrows][K/2 + 16], scales [xrows][K/32]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
   MxRows t;
   if constexpr (SCAN) {
-    const int64_t e = mx_route_id(p.ids, p.id64, blockIdx.y);
-    if (e < 0 || e >= p.experts) return;
-    if (tid == 0) listed = 0;
-    __syncthreads();
-    bool earlier = false;
-    for (int i = tid; i < p.routes; i += THREADS)
-      if (mx_route_id(p.ids, p.id64, i) == e) {
-        earlier = earlier || i < (int)blockIdx.y;
-        list[atomicAdd(&listed, 1)] = i;
-      }
-    if (__syncthreads_or(earlier)) return;
-    t = {(int)e, 0, listed};
+    // every wave looks for itself, so that its weights are asked for at once
+    const MxScan f = mx_scan(p, blockIdx.y, lane);
+    if (f.first != (int)blockIdx.y) return;
+    if (wave == 0) mx_scan_list(f, lane, list);
+    t = {f.expert, 0, f.count()};
   } else {
     if (MODE != kMxDense && (int)blockIdx.y >= p.tile_count[0]) return;
     t = mx_rows<MODE, 16 * MT>(p, blockIdx.y);
@@ -116,6 +130,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   for (int base = 0; base < (SCAN ? t.rows : 1); base += 16 * MT) {
     const int rows = SCAN ? min(t.rows - base, 16 * MT) : t.rows;
     const uint8_t *ac[MT], *asc[MT];
+    if constexpr (SCAN && !X16) __syncthreads();  // the list
     if constexpr (!X16) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -141,6 +156,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     };
     load_w(wave);
     if constexpr (X16) {
+      if constexpr (SCAN) __syncthreads();  // the list
       const int pieces = p.K / 8;
       for (int m = 0; m < rows; ++m) {
         const int64_t row = SCAN ? list[base + m] / p.topk : t.first + m;
@@ -239,43 +255,26 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
 }
 
 // The down product of at most kMxScanRoutes routes with the weighted sum over each token's slots, in one launch: a
-// block has 16 columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
-// place is its own number.
+// block has COLS columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
+// place is its own number.  8 columns (the fragments of w then hold each row twice) where 16 leave CUs without a block.
 constexpr int kDownWaves = 16;
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs p, const void* weights, int w_dtype,
                                                                           uint16_t* out, int64_t ldo) {
   constexpr int THREADS = kDownWaves * 64, U = 4;
-  __shared__ float y[kMxScanRoutes][16];
-  __shared__ int expert[kMxScanRoutes], todo[kMxScanRoutes], head[1024], todos, slot[kDownWaves][kMxScanRoutes];
+  __shared__ float y[kMxScanRoutes][COLS];
+  __shared__ int slot[kDownWaves][kMxScanRoutes];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
-  if (tid == 0) todos = 0;
-  for (int e = tid; e < p.experts; e += THREADS) head[e] = p.routes;
-  __syncthreads();
-  for (int i = tid; i < p.routes; i += THREADS) {
-    const int64_t e = mx_route_id(p.ids, p.id64, i);
-    expert[i] = e >= 0 && e < p.experts ? (int)e : -1;
-    if (expert[i] >= 0) atomicMin(&head[expert[i]], i);
-  }
-  __syncthreads();
-  for (int i = tid; i < p.routes; i += THREADS)
-    if (expert[i] >= 0 && head[expert[i]] == i) todo[atomicAdd(&todos, 1)] = i;
-  __syncthreads();
-  const int n0 = (int)blockIdx.x * 16, KB = p.K / 32, pairs = KB / 8;
-  for (int k = wave; k < todos; k += kDownWaves) {
-    const int e = expert[todo[k]];
-    const int64_t row = (int64_t)e * p.wrows + min(n0 + r, p.N - 1);
-    const uint8_t *wc = p.w + row * (p.K / 2), *wsc = p.ws + row * KB;
-    // this expert's routes, to the wave's slots
-    int n = 0;
-    for (int i = 0; i < p.routes; i += 64) {
-      const bool its = i + lane < p.routes && expert[i + lane] == e;
-      const uint64_t m = __ballot(its);
-      if (its) slot[wave][n + __popcll(m & ((1ull << lane) - 1))] = i + lane;
-      n += __popcll(m);
-    }
+  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;
+  for (int k = wave; k < p.routes; k += kDownWaves) {
+    const MxScan f = mx_scan(p, k, lane);
+    if (f.first != k) continue;  // another wave's, or nobody's
+    mx_scan_list(f, lane, slot[wave]);
     __builtin_amdgcn_wave_barrier();
+    const int64_t row = (int64_t)f.expert * p.wrows + min(n0 + (r & (COLS - 1)), p.N - 1);
+    const uint8_t *wc = p.w + row * (p.K / 2), *wsc = p.ws + row * KB;
+    const int n = f.count();
     for (int at = 0; at < n; at += 16) {
       const int mine = slot[wave][min(at + r, n - 1)];
       const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2), *asc = p.as + (int64_t)mine * p.as_ld;
@@ -294,18 +293,20 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
           if (first + u < pairs) acc = mx_mfma_pair(b[u], a[u], acc, q);
       }
       if ((KB & 7) != 0) acc = mx_mfma_pair(mx_load_last(wc, wsc, pairs, q, KB), mx_load_last(ac, asc, pairs, q, KB), acc, q);
-      if (at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
+      if (at + r < n && 4 * q < COLS) *(f32x4*)&y[mine][4 * q] = acc;
     }
+    __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
   const int tokens = p.routes / p.topk;
-  for (int i = tid; i < tokens * 16; i += THREADS) {
-    const int t = i >> 4, n = i & 15;
+  for (int i = tid; i < tokens * COLS; i += THREADS) {
+    const int t = i / COLS, n = i % COLS;
     if (n0 + n >= p.N) continue;
     float s = 0.f;
     for (int j = 0; j < p.topk; ++j) {
       const int route = t * p.topk + j;
-      if (expert[route] >= 0) s = fmaf(y[route][n], mx_route_weight(weights, w_dtype, route), s);
+      const int64_t e = mx_route_id(p.ids, p.id64, route);
+      if (e >= 0 && e < p.experts) s = fmaf(y[route][n], mx_route_weight(weights, w_dtype, route), s);
     }
     out[(int64_t)t * ldo + n0 + n] = to_bits<T>(s);
   }
@@ -325,25 +326,21 @@ static int launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
-// Waves of a block by the number of column blocks: 16 of them where there is a block to a CU, fewer where several
-// blocks share one.
-template <int MODE, int MT, int NT, bool X16, bool SCAN>
-static int launch_rows_by_waves(const MxArgs& p, int64_t row_tiles, int64_t blocks, hipStream_t st) {
-  if (MT * NT <= 2 && blocks <= 256) return launch_rows<MODE, MT, NT, MT * NT <= 2 ? 16 : 8, X16, SCAN>(p, row_tiles, st);
-  if (MT * NT <= 4 && blocks <= 512) return launch_rows<MODE, MT, NT, MT * NT <= 4 ? 8 : 4, X16, SCAN>(p, row_tiles, st);
-  return launch_rows<MODE, MT, NT, 4, X16, SCAN>(p, row_tiles, st);
+// Up to here every block quantises a's rows for itself (M = 8, K = 4096, N = 24576: 17.2 us against 13.4 and 1.6 for a
+// launch of its own; M = 2 12.4 against 12.0 and 1.6).
+bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= kMxRowsMax && M * K <= 16384; }
+
+// 16 columns a block where that gives a block per CU at most, else 32 (K = 4096, us, 16 and 32 columns: N = 4096, M = 1
+// 4.0, 5.2, M = 16 4.8, 6.4; N = 6144 5.7, 5.3 and 7.9, 6.5; N = 24576 12.0, 11.9 and 18.4, 14.9); 16 waves where a CU has
+// one block (K = 12288, N = 4096: 4 waves 10.1, 8 8.1, 16 7.7).
+template <bool X16>
+static int launch_rows_dense(const MxArgs& p, hipStream_t st) {
+  if (p.N <= 16 * 256) return launch_rows<kMxDense, 1, 1, 16, X16, false>(p, 1, st);
+  if (p.N <= 32 * 256) return launch_rows<kMxDense, 1, 2, 16, X16, false>(p, 1, st);
+  return launch_rows<kMxDense, 1, 2, 8, X16, false>(p, 1, st);
 }
-
-// Up to here every block quantises a's rows for itself: 32768 values, a sweep or two of a block's threads.
-bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= 16 && M * K <= 32768; }
-
-int launch_mx_gemm(const MxArgs& p, hipStream_t st) {
-  if (p.M > 64) return launch_mx_tile_gemm(p, st);
-  const int64_t blocks = cdiv(p.N, 16);
-  if (p.x) return launch_rows_by_waves<kMxDense, 1, 1, true, false>(p, 1, blocks, st);
-  if (p.M <= 16) return launch_rows_by_waves<kMxDense, 1, 1, false, false>(p, 1, blocks, st);
-  if (p.M <= 32) return launch_rows_by_waves<kMxDense, 2, 1, false, false>(p, 1, blocks, st);
-  return launch_rows_by_waves<kMxDense, 4, 1, false, false>(p, 1, blocks, st);
+int launch_mx_rows_gemm(const MxArgs& p, hipStream_t st) {
+  return p.x ? launch_rows_dense<true>(p, st) : launch_rows_dense<false>(p, st);
 }
 
 int launch_mx_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
@@ -359,9 +356,11 @@ int launch_mx_scan_gate_up(const MxArgs& p, hipStream_t st) {
 }
 
 int launch_mx_down_combine(const MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(p.N, 16));
-  if (p.out_bf16) mx_down_combine_kernel<bf16><<<grid, dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
-  else mx_down_combine_kernel<f16><<<grid, dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  auto go = [&](auto kernel, int cols) {
+    kernel<<<dim3((unsigned)cdiv(p.N, cols)), dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  };
+  if (p.N < 16 * 256) p.out_bf16 ? go(mx_down_combine_kernel<bf16, 8>, 8) : go(mx_down_combine_kernel<f16, 8>, 8);
+  else p.out_bf16 ? go(mx_down_combine_kernel<bf16, 16>, 16) : go(mx_down_combine_kernel<f16, 16>, 16);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

@@ -56,11 +56,14 @@ __device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, con
 // the readers skip `sh` bytes, for the last ones into the next group.
 // The operands enter the MFMA swapped, so that a lane holds four consecutive columns of one row of c.
 //
+// WK > 1 (few tiles, where the latency of a stage bounds a block): as many shares of K, each with waves and LDS of its
+// own, whose sums meet at the end (M = 64, K = N = 4096 9.8 us with one).
+//
 // K past the end: the codes are whatever follows (any code is finite, and the loads stop at the operand's end),
 // both scales are 2^-127, and the products vanish in fp32.
-template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF>
-__global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF, int WK>
+__global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
+  constexpr int WAVES = WM * WN /* of a share of K */, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
   constexpr bool AGPR = TM * TN > 32;  // accumulators of more than half of the 256 VGPRs
   static_assert(TN % 2 == 0, "");
   extern __shared__ __align__(16) uint8_t lds[];  // codes [NBUF][ROWS][128], scales [NBUF][ROWS][16], zeros
@@ -78,8 +81,12 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
   constexpr int COLS = MODE == kMxGateUp ? BN / 2 : BN;
   const int n0 = tn * COLS;
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
-  const int KB = p.K / 32, stages = (KB + 7) / 8;
+  // wave: of the WM x WN of share `part` of K
+  const int tid = threadIdx.x, wave_of_all = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave_of_all / WAVES, wave = wave_of_all % WAVES;
+  const int lane = tid & 63, r = lane & 15, q = lane >> 4, ptid = tid - part * (WAVES * 64);
+  const int KB = p.K / 32;
+  // the share's stages, as if the operands began and ended there (a share behind K's end: stages of nothing)
+  const int stages = ((KB + 7) / 8 + WK - 1) / WK, s0 = part * stages, blocks = KB - 8 * s0;
   const int64_t a_base = MODE == kMxGateUp ? 0 : t.first, w_base = (int64_t)t.expert * p.wrows + n0;
   const int last = p.N - 1 - n0;
   // Row i of a stage (a's rows, then w's) behind the operand's base, and the offsets of its codes (in 16 bytes) and
@@ -116,17 +123,18 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     const int i = min((u * WAVES + wave) * 64 + lane, ROWS - 1);
     ssrc[u] = (scale_offset(i) + (i < BM ? a_in : w_in)) & ~3u;
   }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  constexpr uint32_t SHARE_LDS = mx_tile_lds(ROWS, NBUF, TM > TN ? TM : TN);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + part * SHARE_LDS;
   constexpr uint32_t SCALES = NBUF * STAGE, ZEROS = SCALES + NBUF * ROWS * 16;
   auto load_code = [&](int s, int u) {
-    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & (NBUF - 1)) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)s * 128u);
+    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & (NBUF - 1)) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)(s0 + s) * 128u);
   };
   auto load_scales = [&](int g) {
 #pragma unroll
     for (int u = 0; u < SLOADS; ++u) {
       const int at = u * WAVES + wave;
       if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
-      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & (NBUF - 1)) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)g * 16u);
+      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & (NBUF - 1)) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)(s0 * 8 + g * 16));
     }
   };
 
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
     const uint32_t group = (uint32_t)(s >> 1) + (at >> 4);
     uint32_t place = lds0 + SCALES + (group & (NBUF - 1)) * (ROWS * 16) + row * 16u + (at & 15u);
     asm("" : "+v"(place));  // a select, no branch around it
-    return 8 * s + 4 * h + q < KB ? place : lds0 + ZEROS;
+    return 8 * s + 4 * h + q < blocks ? place : lds0 + ZEROS;
   };
   // the fragments of a half: a's row tile i, and all of w's, with their scales
   u32x4 a[TM];
@@ -190,7 +198,7 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) load_code(s, u);
   }
-  for (int i = tid; i < (TM > TN ? TM : TN) * 64; i += WAVES * 64) ((uint32_t*)(lds + ZEROS))[i] = 0u;
+  for (int i = ptid; i < (TM > TN ? TM : TN) * 64; i += WAVES * 64) ((uint32_t*)(lds + part * SHARE_LDS + ZEROS))[i] = 0u;
   if (stages >= NBUF) wait_loads_and_sync<(NBUF - 1) * LOADS>();
   else wait_loads_and_sync<0>();
   {
@@ -245,6 +253,31 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
       else asm volatile("" : "+v"(acc[i][j]));
     }
   __syncthreads();
+
+  if constexpr (WK > 1) {
+    // the shares' sums meet in LDS, in order: [share - 1][accumulator][thread]
+    constexpr int N4 = TM * TN, THREADS = WAVES * 64;
+    static_assert((WK - 1) * N4 * THREADS * 16 <= WK * SHARE_LDS, "the shares' sums");
+    f32x4* sums = (f32x4*)lds;
+    if (part > 0) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sums[((part - 1) * N4 + i * TN + j) * THREADS + ptid] = acc[i][j];
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int k = 0; k < WK - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] += sums[(k * N4 + i * TN + j) * THREADS + ptid];
+    }
+    __syncthreads();
+    if (part > 0) return;  // no barrier follows but the gated one, which has no shares
+    static_assert(MODE != kMxGateUp, "");
+  }
 
   // lane: row m0 + 16 i + r, columns 16 j + 4 q .. + 3
   if constexpr (MODE == kMxGateUp) {
@@ -346,27 +379,32 @@ __global__ void __launch_bounds__(WM * WN * 64, PER_SIMD) mx_tile_kernel(MxArgs 
 namespace awq_host {
 using namespace awq;
 
-template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF>
+template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF, int WK = 1>
 static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   constexpr int COLS = MODE == kMxGateUp ? BN / 2 : BN;
   const int64_t col_tiles = cdiv(p.N, COLS);
-  if (row_tiles * col_tiles > 0x7FFFFFF0LL) return AWQ_ERR_UNSUPPORTED;
-  constexpr int lds = mx_tile_lds(BM + BN, NBUF, BM / WM > BN / WN ? BM / WM / 16 : BN / WN / 16);
+  if (row_tiles * col_tiles > 0x7FFFFFFLL) return AWQ_ERR_UNSUPPORTED;
+  constexpr int lds = WK * mx_tile_lds(BM + BN, NBUF, BM / WM > BN / WN ? BM / WM / 16 : BN / WN / 16);
   static_assert(MODE != kMxGateUp || BM * (BN / 2 + 4) * 4 <= lds, "the up half");
-  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN, PER_SIMD, NBUF>;
+  auto kernel = mx_tile_kernel<MODE, BM, BN, WM, WN, PER_SIMD, NBUF, WK>;
   if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     (void)hipGetLastError();
     return AWQ_ERR_LAUNCH;
   }
-  kernel<<<dim3((unsigned)(cdiv(row_tiles * col_tiles, 8) * 8)), dim3(WM * WN * 64), lds, st>>>(p, (int)row_tiles, (int)col_tiles);
+  kernel<<<dim3((unsigned)(cdiv(row_tiles * col_tiles, 8) * 8)), dim3(WM * WN * WK * 64), lds, st>>>(p, (int)row_tiles, (int)col_tiles);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
+// Tiles of 256 x 256 where they give every CU one, of 128 x 128 where those do; else of 64 x 64.  Up to a tile per CU
+// K goes in shares: two from 8 stages on, four from 24 on (M = 64, N = 4096, us with 1, 2, 4: K = 1024 5.1, 5.2, 6.1;
+// K = 4096 9.4, 8.2, 8.6; K = 12288 22.7, 18.2, 15.6; with 316 tiles, M = 200, N = 5001, K = 4128 14.2, 15.3, 22.2).
 int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
-  const int64_t big = cdiv(p.M, 256) * cdiv(p.N, 256), mid = cdiv(p.M, 128) * cdiv(p.N, 128);
-  if (big >= 256) return launch_tile<kMxDense, 256, 256, 2, 4, 2, 2>(p, cdiv(p.M, 256), st);
-  if (mid >= 256) return launch_tile<kMxDense, 128, 128, 2, 4, 4, 2>(p, cdiv(p.M, 128), st);
-  return launch_tile<kMxDense, 64, 64, 2, 2, 2, 4>(p, cdiv(p.M, 64), st);
+  if (cdiv(p.M, 256) * cdiv(p.N, 256) >= 256) return launch_tile<kMxDense, 256, 256, 2, 4, 2, 2>(p, cdiv(p.M, 256), st);
+  if (cdiv(p.M, 128) * cdiv(p.N, 128) >= 256) return launch_tile<kMxDense, 128, 128, 2, 4, 4, 2>(p, cdiv(p.M, 128), st);
+  const int64_t rows = cdiv(p.M, 64), tiles = rows * cdiv(p.N, 64), stages = cdiv(p.K, 256);
+  if (tiles <= 256 && stages >= 24) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2, 4>(p, rows, st);
+  if (tiles <= 256 && stages >= 8) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2, 2>(p, rows, st);
+  return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2>(p, rows, st);
 }
 
 int launch_mx_tile_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {

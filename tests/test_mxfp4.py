@@ -49,7 +49,7 @@ def test_quantize_entries_refuse():
 def test_gemm_entry_refuses():
     lib, p = L.load(), _fake()
 
-    def call(a=p, lda=64, sa=None, w=p, sw=p, bias=None, c=p, ldc=16, m=2, n=16, k=64, dt=L.DTYPE_BF16, bdt=L.DTYPE_NONE, ws=p, wsb=4096):
+    def call(a=p, lda=64, sa=None, w=p, sw=p, bias=None, c=p, ldc=16, m=20, n=16, k=64, dt=L.DTYPE_BF16, bdt=L.DTYPE_NONE, ws=p, wsb=4096):
         return lib.awq_w4a16_mxfp4_gemm(a, lda, sa, w, sw, bias, c, ldc, m, n, k, dt, bdt, ws, wsb, None)
     assert call(a=None) == call(w=None) == call(sw=None) == call(c=None) == L.ERR_NULL
     assert call(k=48) == call(k=0) == call(m=-1) == L.ERR_SHAPE
@@ -185,7 +185,7 @@ def test_quantize_refuses():
     (1, 16, 32, None), (1, 1, 64, "f32"), (1, 4096, 4096, None), (2, 333, 1056, "f16"), (5, 48, 96, None), (13, 1000, 2048, "bf16"),
     (16, 256, 12288, None), (17, 128, 512, None), (33, 517, 160, "f32"), (57, 1024, 4096, None), (64, 256, 1024, None),
     (65, 130, 2080, "f16"), (128, 512, 384, None), (200, 5001, 288, "bf16"), (300, 256, 4128, None), (513, 771, 1024, None),
-    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None)])
+    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None), (64, 300, 4096, "f16"), (40, 5000, 12320, None), (15, 16500, 96, None), (12, 9000, 4128, "f32"), (600, 900, 2080, None)])
 def test_gemm(m, n, k, bias, dtype):
     from litevllm_amd import mxfp4_gemm
     dt = DTYPES[dtype]
@@ -315,7 +315,7 @@ def _experts(seed, e, i, h):
 @pytest.mark.parametrize("t,e,k,h,i,kind", [
     (1, 8, 2, 64, 32, "silu"), (1, 1, 1, 32, 32, "gelu"), (5, 8, 8, 160, 96, "silu"), (17, 4, 2, 256, 128, "gelu_pytorch_tanh"),
     (40, 64, 4, 512, 64, "silu"), (70, 3, 2, 96, 160, "silu"), (150, 2, 1, 128, 32, "silu"), (3, 5, 4, 4128, 64, "silu"), (16, 1, 8, 64, 64, "gelu"), (2, 300, 3, 96, 32, "silu"), (128, 7, 1, 64, 32, "silu"),
-    (43, 1000, 3, 64, 32, "silu"), (260, 5, 3, 64, 288, "gelu")])
+    (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (260, 5, 3, 64, 288, "gelu")])
 def test_moe(t, e, k, h, i, kind, dtype):
     from litevllm_amd import mxfp4_moe
     dt = DTYPES[dtype]
