@@ -64,6 +64,22 @@ __device__ __forceinline__ void load8(const void* p, float* v) {
   }
 }
 
+// Eight values of a row, number `piece`, by a lane; the four lanes of a block of 32 share its largest magnitude by two
+// DPP steps inside their quad.
+template <typename T>
+__device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, uint8_t* scales, int piece) {
+  float v[8];
+  load8<T>(x + piece * 8, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, mx_abs_bits(v[j]));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));
+  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
+  const uint32_t byte = mx_scale_byte(top);
+  *(uint32_t*)(codes + piece * 4) = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
+  if ((piece & 3) == 0) scales[piece >> 2] = (uint8_t)byte;
+}
+
 // One product of MXFP4 matrices: rows of `a` by rows of `w`.  Which rows, and where the sums go:
 //   kMxDense: c[m, n] = sum (+ bias), one rounding to 16 bits.
 //   kMxGateUp: a tile table row {expert, first, rows} names `rows` consecutive places of `order`; the
@@ -97,7 +113,7 @@ struct MxArgs {
   const void* ids;
   int id64, routes, experts;
 };
-constexpr int kMxScanRoutes = 128;
+constexpr int kMxScanRoutes = 64;
 
 __device__ __forceinline__ int64_t mx_route_id(const void* ids, int id64, int64_t r) {
   return id64 ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];

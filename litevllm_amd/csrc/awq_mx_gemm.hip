@@ -52,41 +52,22 @@ __device__ __forceinline__ f32x4 mx_mfma_pair(const MxPair& a, const MxPair& b, 
   return mx_mfma<0, 0>(a.c[1], b.c[1], c, a.s[1] >> (8 * q), b.s[1] >> (8 * q));
 }
 
-// Eight values of a row to LDS codes, by a lane; the four lanes of a block share its largest magnitude.
-template <typename T>
-__device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, uint8_t* scales, int piece) {
-  float v[8];
-  load8<T>(x + piece * 8, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, mx_abs_bits(v[j]));
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
-  const uint32_t byte = mx_scale_byte(top);
-  *(uint32_t*)(codes + piece * 4) = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
-  if ((piece & 3) == 0) scales[piece >> 2] = (uint8_t)byte;
-}
-
-// The routes of the expert of a route, found by a wave: two masks over the at most kMxScanRoutes routes.
+// The routes of the expert of a route, found by a wave: a mask over the at most kMxScanRoutes routes.
 struct MxScan {
-  uint64_t lo, hi;
+  uint64_t its;
   int expert, first;  // first: the lowest of them; -1 if the route has no expert
-  __device__ int count() const { return __popcll(lo) + __popcll(hi); }
 };
 __device__ __forceinline__ MxScan mx_scan(const MxArgs& p, int route, int lane) {
   const int64_t e = mx_route_id(p.ids, p.id64, route);
-  const int64_t a = lane < p.routes ? mx_route_id(p.ids, p.id64, lane) : -1;
-  const int64_t b = lane + 64 < p.routes ? mx_route_id(p.ids, p.id64, lane + 64) : -1;
-  MxScan f{__ballot(a == e), __ballot(b == e), (int)e, -1};
-  if (e >= 0 && e < p.experts) f.first = f.lo ? __ffsll((unsigned long long)f.lo) - 1 : 63 + __ffsll((unsigned long long)f.hi);
+  const int64_t mine = lane < p.routes ? mx_route_id(p.ids, p.id64, lane) : -1;
+  MxScan f{__ballot(mine == e), (int)e, -1};
+  if (e >= 0 && e < p.experts) f.first = __ffsll((unsigned long long)f.its) - 1;
   return f;
 }
 __device__ __forceinline__ void mx_scan_list(const MxScan& f, int lane, int* list) {
-  const uint64_t below = (1ull << lane) - 1;
-  if (f.lo >> lane & 1) list[__popcll(f.lo & below)] = lane;
-  if (f.hi >> lane & 1) list[__popcll(f.lo) + __popcll(f.hi & below)] = lane + 64;
+  if (f.its >> lane & 1) list[__popcll(f.its & ((1ull << lane) - 1))] = lane;
 }
-static_assert(kMxScanRoutes == 128, "two masks");
+static_assert(kMxScanRoutes == 64, "a lane each");
 
 // Grid x: column blocks, y: row tiles of 16 MT (with SCAN: routes).
 // X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one
@@ -107,7 +88,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     const MxScan f = mx_scan(p, blockIdx.y, lane);
     if (f.first != (int)blockIdx.y) return;
     if (wave == 0) mx_scan_list(f, lane, list);
-    t = {f.expert, 0, f.count()};
+    t = {f.expert, 0, (int)__popcll(f.its)};
   } else {
     if (MODE != kMxDense && (int)blockIdx.y >= p.tile_count[0]) return;
     t = mx_rows<MODE, 16 * MT>(p, blockIdx.y);
@@ -255,26 +236,32 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
 }
 
 // The down product of at most kMxScanRoutes routes with the weighted sum over each token's slots, in one launch: a
-// block has COLS columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
-// place is its own number.  8 columns (the fragments of w then hold each row twice) where 16 leave CUs without a block.
+// block has 16 columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
+// place is its own number.
 constexpr int kDownWaves = 16;
 
-template <typename T, int COLS>
+template <typename T>
 __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs p, const void* weights, int w_dtype,
                                                                           uint16_t* out, int64_t ldo) {
-  constexpr int THREADS = kDownWaves * 64, U = 4;
+  constexpr int THREADS = kDownWaves * 64, COLS = 16, U = 4;
   __shared__ float y[kMxScanRoutes][COLS];
-  __shared__ int slot[kDownWaves][kMxScanRoutes];
+  __shared__ int slot[kDownWaves][kMxScanRoutes], has[kMxScanRoutes];
+  __shared__ float weight[kMxScanRoutes];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
+  if (tid < p.routes) {
+    const int64_t e = mx_route_id(p.ids, p.id64, tid);
+    has[tid] = e >= 0 && e < p.experts;
+    weight[tid] = mx_route_weight(weights, w_dtype, tid);
+  }
   const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;
   for (int k = wave; k < p.routes; k += kDownWaves) {
     const MxScan f = mx_scan(p, k, lane);
     if (f.first != k) continue;  // another wave's, or nobody's
     mx_scan_list(f, lane, slot[wave]);
     __builtin_amdgcn_wave_barrier();
-    const int64_t row = (int64_t)f.expert * p.wrows + min(n0 + (r & (COLS - 1)), p.N - 1);
+    const int64_t row = (int64_t)f.expert * p.wrows + min(n0 + r, p.N - 1);
     const uint8_t *wc = p.w + row * (p.K / 2), *wsc = p.ws + row * KB;
-    const int n = f.count();
+    const int n = (int)__popcll(f.its);
     for (int at = 0; at < n; at += 16) {
       const int mine = slot[wave][min(at + r, n - 1)];
       const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2), *asc = p.as + (int64_t)mine * p.as_ld;
@@ -293,7 +280,7 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
           if (first + u < pairs) acc = mx_mfma_pair(b[u], a[u], acc, q);
       }
       if ((KB & 7) != 0) acc = mx_mfma_pair(mx_load_last(wc, wsc, pairs, q, KB), mx_load_last(ac, asc, pairs, q, KB), acc, q);
-      if (at + r < n && 4 * q < COLS) *(f32x4*)&y[mine][4 * q] = acc;
+      if (at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -305,8 +292,7 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
     float s = 0.f;
     for (int j = 0; j < p.topk; ++j) {
       const int route = t * p.topk + j;
-      const int64_t e = mx_route_id(p.ids, p.id64, route);
-      if (e >= 0 && e < p.experts) s = fmaf(y[route][n], mx_route_weight(weights, w_dtype, route), s);
+      if (has[route]) s = fmaf(y[route][n], weight[route], s);
     }
     out[(int64_t)t * ldo + n0 + n] = to_bits<T>(s);
   }
@@ -356,11 +342,9 @@ int launch_mx_scan_gate_up(const MxArgs& p, hipStream_t st) {
 }
 
 int launch_mx_down_combine(const MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st) {
-  auto go = [&](auto kernel, int cols) {
-    kernel<<<dim3((unsigned)cdiv(p.N, cols)), dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
-  };
-  if (p.N < 16 * 256) p.out_bf16 ? go(mx_down_combine_kernel<bf16, 8>, 8) : go(mx_down_combine_kernel<f16, 8>, 8);
-  else p.out_bf16 ? go(mx_down_combine_kernel<bf16, 16>, 16) : go(mx_down_combine_kernel<f16, 16>, 16);
+  const dim3 grid((unsigned)cdiv(p.N, 16)), block(kDownWaves * 64);
+  if (p.out_bf16) mx_down_combine_kernel<bf16><<<grid, block, 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  else mx_down_combine_kernel<f16><<<grid, block, 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

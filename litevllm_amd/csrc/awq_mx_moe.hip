@@ -9,46 +9,61 @@ namespace awq {
 
 constexpr int kOrderThreads = 1024;
 
-// Sorts the routes by expert (one block): order[place] = route, and the table of row tiles, at most
-// `rows` places of one expert each.  The order inside an expert is that of the atomics; no result
-// depends on it, since every place's row is computed by itself and summed by its route.  Routes
-// without an expert get no place.
-__global__ void __launch_bounds__(kOrderThreads) mx_order_kernel(const void* __restrict__ ids, int id64, int R, int E, int rows,
-                                                                 int* __restrict__ order, int* __restrict__ tiles,
-                                                                 int* __restrict__ tile_count) {
-  extern __shared__ int sh[];
-  int *count = sh, *cursor = sh + E;
-  __shared__ int tot[2][kOrderThreads / 64];
+// Block 0 sorts the routes by expert: order[place] = route, and the table of row tiles, at most `rows` places of one
+// expert each.  The order inside an expert is that of the atomics; no result depends on it, since every place's row
+// is computed by itself and summed by its route.  Routes without an expert get no place.
+// The other blocks quantise the tokens.
+template <typename T>
+__global__ void __launch_bounds__(kOrderThreads) mx_prepare_kernel(const void* __restrict__ ids, int id64, int R, int E, int rows,
+                                                                   int* __restrict__ order, int* __restrict__ tiles,
+                                                                   int* __restrict__ tile_count, const uint16_t* __restrict__ x,
+                                                                   int64_t ldx, int64_t pieces, int per_row, uint8_t* __restrict__ codes,
+                                                                   uint8_t* __restrict__ scales, int lds) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  for (int e = t; e < E; e += kOrderThreads) count[e] = 0;
-  __syncthreads();
-  for (int r = t; r < R; r += kOrderThreads) {
-    const int64_t e = mx_route_id(ids, id64, r);
-    if (e >= 0 && e < E) atomicAdd(&count[e], 1);
+  if (blockIdx.x > 0) {
+    const int64_t i = (int64_t)(blockIdx.x - 1) * kOrderThreads + t;
+    if (i >= pieces) return;  // whole blocks of 32: pieces % 4 == 0
+    const int64_t row = i / per_row;
+    const int piece = (int)(i - row * per_row);
+    mx_quantize8<T>(x + row * ldx, codes + row * per_row * 4, scales + row * lds, piece);
+    return;
   }
+  __shared__ int count[kOrderThreads], tot[2][kOrderThreads / 64];
+  constexpr int AT_ONCE = 16;  // ids of a thread under way
+  count[t] = 0;
+  __syncthreads();
+  auto for_routes = [&](auto f) {
+    for (int64_t base = t; base < R; base += kOrderThreads * AT_ONCE) {
+      int64_t e[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int64_t r = base + j * kOrderThreads;
+        e[j] = r < R ? mx_route_id(ids, id64, r) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (e[j] >= 0 && e[j] < E) f((int)(base + j * kOrderThreads), (int)e[j]);
+    }
+  };
+  for_routes([&](int, int e) { atomicAdd(&count[e], 1); });
   __syncthreads();
   // E <= kOrderThreads: one expert per thread; prefix sums of places and tiles
-  const int c = t < E ? count[t] : 0, nt = (c + rows - 1) / rows;
+  const int c = count[t], nt = (c + rows - 1) / rows;
   const int ic = wave_incl_scan_i32(c), it = wave_incl_scan_i32(nt);
   if (lane == 63) tot[0][wave] = ic, tot[1][wave] = it;
   __syncthreads();
   int first = ic - c, ft = it - nt;
   for (int w = 0; w < wave; ++w) first += tot[0][w], ft += tot[1][w];
-  if (t < E) {
-    cursor[t] = first;
-    for (int i = 0; i < nt; ++i) {
-      int* row = tiles + 3 * (ft + i);
-      row[0] = t;
-      row[1] = first + i * rows;
-      row[2] = min(rows, c - i * rows);
-    }
+  count[t] = first;  // from here on the expert's next place
+  for (int i = 0; i < nt; ++i) {
+    int* row = tiles + 3 * (ft + i);
+    row[0] = t;
+    row[1] = first + i * rows;
+    row[2] = min(rows, c - i * rows);
   }
   if (t == kOrderThreads - 1) tile_count[0] = ft + nt;
   __syncthreads();
-  for (int r = t; r < R; r += kOrderThreads) {
-    const int64_t e = mx_route_id(ids, id64, r);
-    if (e >= 0 && e < E) order[atomicAdd(&cursor[e], 1)] = r;
-  }
+  for_routes([&](int r, int e) { order[atomicAdd(&count[e], 1)] = r; });
 }
 
 // out[t] = the sum over a token's slots, in slot order, of weight * y: fp32, one rounding.  A slot
@@ -62,13 +77,25 @@ __global__ void __launch_bounds__(256) mx_combine_kernel(const float* __restrict
   if (t >= T_) return;
   const int c = (int)(i - t * (H / 4)) * 4;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < topk; ++j) {
-    const int64_t r = t * topk + j, e = mx_route_id(ids, id64, r);
-    if (e < 0 || e >= E) continue;
-    const f32x4 v = *(const f32x4*)(y + r * H + c);
-    const float g = mx_route_weight(w, w_dtype, r);
+  constexpr int AT_ONCE = 8;  // slots under way
+  for (int j = 0; j < topk; j += AT_ONCE) {
+    bool has[AT_ONCE];
+    float g[AT_ONCE];
+    f32x4 v[AT_ONCE];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) s[u] = fmaf(v[u], g, s[u]);
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const int64_t r = t * topk + j + k, e = j + k < topk ? mx_route_id(ids, id64, r) : -1;
+      has[k] = e >= 0 && e < E;
+      if (has[k]) g[k] = mx_route_weight(w, w_dtype, r);
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (has[k]) v[k] = *(const f32x4*)(y + (t * topk + j + k) * H + c);
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (has[k])
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] = fmaf(v[k][u], g[k], s[u]);
   }
   u32x2 o = {pack2<T>(s[0], s[1]), pack2<T>(s[2], s[3])};
   uint16_t* at = out + t * ldo + c;
@@ -86,7 +113,7 @@ namespace awq_host {
 using namespace awq;
 
 // Rows of a row tile: what an expert gets on average, so that its weights are read about once.
-static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)16 * E ? 16 : (R <= (int64_t)128 * E ? 64 : 128); }
+static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)4 * E ? 16 : (R <= (int64_t)128 * E ? 64 : 128); }
 
 // Bytes between rows of the tokens' scales: whole words, which the gathering kernel counts on.
 static int64_t scale_stride(int64_t K) { return cdiv(K / 32, 4) * 4; }
@@ -138,10 +165,15 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   int* order = (int*)(ws + w.order);
   int* tiles = (int*)(ws + w.tiles);
   const int rows = mx_moe_rows(R, c.E);
-  mx_order_kernel<<<1, kOrderThreads, 2 * c.E * sizeof(int), st>>>(c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws);
+  const int64_t pieces = c.T * (c.H / 8);
+  if (cdiv(pieces, kOrderThreads) >= 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
+  auto prepare = [&](auto kernel) {
+    kernel<<<dim3((unsigned)(1 + cdiv(pieces, kOrderThreads))), dim3(kOrderThreads), 0, st>>>(
+        c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws, (const uint16_t*)c.x, c.T > 1 ? c.ldx : c.H, pieces, (int)(c.H / 8),
+        (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), (int)scale_stride(c.H));
+  };
+  c.act_dtype == AWQ_DTYPE_BF16 ? prepare(mx_prepare_kernel<bf16>) : prepare(mx_prepare_kernel<f16>);
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
-  int rc = launch_mx_quantize(c.x, c.ldx, (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), scale_stride(c.H), c.T, c.H, c.act_dtype, st);
-  if (rc != AWQ_OK) return rc;
 
   MxArgs g{};
   g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);
@@ -150,7 +182,7 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   g.tiles = tiles, g.tile_count = (const int*)ws, g.order = order;
   g.topk = c.topk, g.act = c.act_kind;
   g.h = (uint8_t*)(ws + w.h), g.hs = (uint8_t*)(ws + w.hs);
-  rc = launch_mx_grouped(g, true, rows, w.max_tiles, st);
+  int rc = launch_mx_grouped(g, true, rows, w.max_tiles, st);
   if (rc != AWQ_OK) return rc;
 
   MxArgs d = g;
