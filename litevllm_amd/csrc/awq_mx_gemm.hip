@@ -52,17 +52,20 @@ __device__ __forceinline__ f32x4 mx_mfma_pair(const MxPair& a, const MxPair& b, 
   return mx_mfma<0, 0>(a.c[1], b.c[1], c, a.s[1] >> (8 * q), b.s[1] >> (8 * q));
 }
 
-// The routes of the expert of a route, found by a wave: a mask over the at most kMxScanRoutes routes.
+// The at most kMxScanRoutes routes in a wave's lanes: a lane holds the expert of the route with its number, or -1.
+__device__ __forceinline__ int mx_scan_ids(const MxArgs& p, int lane) {
+  const int64_t e = lane < p.routes ? mx_route_id(p.ids, p.id64, lane) : -1;
+  return e >= 0 && e < p.experts ? (int)e : -1;
+}
+// The routes that share a route's expert, as a mask; first: the lowest of them, -1 if the route has no expert.
 struct MxScan {
   uint64_t its;
-  int expert, first;  // first: the lowest of them; -1 if the route has no expert
+  int expert, first;
 };
-__device__ __forceinline__ MxScan mx_scan(const MxArgs& p, int route, int lane) {
-  const int64_t e = mx_route_id(p.ids, p.id64, route);
-  const int64_t mine = lane < p.routes ? mx_route_id(p.ids, p.id64, lane) : -1;
-  MxScan f{__ballot(mine == e), (int)e, -1};
-  if (e >= 0 && e < p.experts) f.first = __ffsll((unsigned long long)f.its) - 1;
-  return f;
+__device__ __forceinline__ MxScan mx_scan(int mine, int route) {
+  const int e = __builtin_amdgcn_readlane(mine, route);
+  const uint64_t its = __ballot(mine == e);
+  return {its, e, e < 0 ? -1 : __ffsll((unsigned long long)its) - 1};
 }
 __device__ __forceinline__ void mx_scan_list(const MxScan& f, int lane, int* list) {
   if (f.its >> lane & 1) list[__popcll(f.its & ((1ull << lane) - 1))] = lane;
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   MxRows t;
   if constexpr (SCAN) {
     // every wave looks for itself, so that its weights are asked for at once
-    const MxScan f = mx_scan(p, blockIdx.y, lane);
+    const MxScan f = mx_scan(mx_scan_ids(p, lane), blockIdx.y);
     if (f.first != (int)blockIdx.y) return;
     if (wave == 0) mx_scan_list(f, lane, list);
     t = {f.expert, 0, (int)__popcll(f.its)};
@@ -254,8 +257,9 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
     weight[tid] = mx_route_weight(weights, w_dtype, tid);
   }
   const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;
+  const int expert = mx_scan_ids(p, lane);
   for (int k = wave; k < p.routes; k += kDownWaves) {
-    const MxScan f = mx_scan(p, k, lane);
+    const MxScan f = mx_scan(expert, k);
     if (f.first != k) continue;  // another wave's, or nobody's
     mx_scan_list(f, lane, slot[wave]);
     __builtin_amdgcn_wave_barrier();
