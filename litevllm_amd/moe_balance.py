@@ -3,42 +3,46 @@ logits and ids it takes."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
 from .mxfp4 import _call
 
 
+def _forward(logits, ids, mask, experts):
+    """(loss, counts, buf): the gradient's factors are the first ``experts`` floats of ``buf``, scratch the rest."""
+    dev, t = logits.device, logits.shape[0]
+    ws_bytes = L.load().awq_w4a16_moe_balance_workspace_bytes(t, experts)
+    start = -(-experts // 4) * 4  # scratch on a 16-byte boundary
+    buf = torch.empty(start + ws_bytes // 4, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty(experts, dtype=torch.int32, device=dev)
+    at = buf.data_ptr()
+    _call(dev, "awq_w4a16_moe_balance", logits.data_ptr(), logits.stride(0) if t > 1 else experts, ops.dtype_code(logits.dtype),
+          ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, ops._ptr(mask), t, experts, ids.shape[1], loss.data_ptr(),
+          counts.data_ptr(), at, at + 4 * start, ws_bytes)
+    return loss, counts, buf
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, mask, experts):
-        dev, t = logits.device, logits.shape[0]
-        dt = ops.dtype_code(logits.dtype)
-        ld = logits.stride(0) if t > 1 else experts
-        ws_bytes = L.load().awq_w4a16_moe_balance_workspace_bytes(t, experts)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        factor = torch.empty(experts, dtype=torch.float32, device=dev)
-        counts = torch.empty(experts, dtype=torch.int32, device=dev)
-        _call(dev, "awq_w4a16_moe_balance", logits.data_ptr(), ld, dt, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32,
-              ops._ptr(mask), t, experts, ids.shape[1], loss.data_ptr(), counts.data_ptr(), factor.data_ptr(), ws.data_ptr(),
-              ws_bytes)
-        ctx.save_for_backward(logits, mask, factor)
+        loss, counts, buf = _forward(logits, ids, mask, experts)
+        ctx.save_for_backward(logits, mask, buf)
         ctx.mark_non_differentiable(counts)
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, upstream, _):
-        logits, mask, factor = ctx.saved_tensors
+        logits, mask, buf = ctx.saved_tensors
         t, experts = logits.shape
         grad = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
         if t:
             upstream = upstream.contiguous()
             _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
-                  ops.dtype_code(logits.dtype), ops._ptr(mask), factor.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t,
-                  experts)
+                  ops.dtype_code(logits.dtype), ops._ptr(mask), buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
+        if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
+            grad = torch._C._functions.DelayedError(b"moe_balance_loss is not differentiable twice", 1)(grad.requires_grad_())
         return grad, None, None, None
 
 
@@ -72,4 +76,7 @@ def moe_balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor,
     t = router_logits.shape[0]
     if (router_logits.stride(1) != 1 and experts > 1) or (t > 1 and router_logits.stride(0) < experts):
         router_logits = router_logits.contiguous()
-    return _BalanceLoss.apply(router_logits, topk_ids.contiguous(), mask, experts)
+    topk_ids = topk_ids.contiguous()
+    if router_logits.requires_grad and torch.is_grad_enabled():
+        return _BalanceLoss.apply(router_logits, topk_ids, mask, experts)
+    return _forward(router_logits, topk_ids, mask, experts)[:2]

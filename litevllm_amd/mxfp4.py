@@ -11,8 +11,6 @@ PyTorch's allocator for each call, so calls on different streams and captured gr
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from . import _lib as L
@@ -23,23 +21,24 @@ BLOCK = 32
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """One C call on ``dev``'s current stream; a launch needs its stream's device to be the current one."""
-    fn = getattr(L.load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch._C._cuda_getDevice() == dev.index:
-        rc = fn(*args, stream)
+    fn = getattr(L._lib or L.load(), name)
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, stream)
-    if rc != L.OK:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
         raise L.AWQKernelError(name, rc)
 
 
 def _check_codes(what: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
     """K of a quantised tensor, after its types and shapes."""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{what}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-    k = codes.shape[-1] * 2 if codes.dim() else -1
-    if k < 0 or k % BLOCK or codes.shape[:-1] != scales.shape[:-1] or scales.shape[-1] * BLOCK != k:
+    cs, ss = codes.shape, scales.shape
+    k = cs[-1] * 2 if cs else -1
+    if k < 0 or k % BLOCK or not ss or ss[-1] * BLOCK != k or cs[:-1] != ss[:-1]:
         raise ValueError(f"{what}: codes [..., K/2] and scales [..., K/{BLOCK}] do not match: "
                          f"{tuple(codes.shape)} and {tuple(scales.shape)}")
     return k
@@ -170,12 +169,13 @@ class MXFP4Weight:
         return y.view(x.shape[:-1] + (y.shape[-1],))
 
 
-@dataclass(frozen=True)
 class MXFP4Experts:
     """An MXFP4 expert stack ``[E, N, K]``: ``qweight`` uint8 ``[E, N, K/2]``, ``scales`` uint8 ``[E, N, K/32]``."""
 
-    qweight: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("qweight", "scales")
+
+    def __init__(self, qweight: torch.Tensor, scales: torch.Tensor):
+        self.qweight, self.scales = qweight, scales
 
     def dims(self) -> tuple[int, int, int]:
         """(E, K, N) of the stack."""
