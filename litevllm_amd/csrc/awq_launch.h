@@ -138,9 +138,10 @@ int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scal
 int launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int64_t M, int64_t K, int dtype, hipStream_t st);
 
 // Workspace of one call over expert stacks (byte offsets): the number of row tiles, the routes sorted by
-// expert, the tile table, the quantised tokens, the quantised intermediate and the per-route fp32 rows.
+// expert, the tile table, the sort's ranks and counts (of order_blocks > 1 blocks), the quantised tokens, the
+// quantised intermediate and the per-route fp32 rows.
 struct MxMoeWorkspace {
-  int64_t order, tiles, x, xs, h, hs, y, total, max_tiles;
+  int64_t order, tiles, rank, hist, x, xs, h, hs, y, total, max_tiles, order_blocks;
 };
 MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk);
 struct MxMoeCall {

@@ -7,63 +7,109 @@
 
 namespace awq {
 
-constexpr int kOrderThreads = 1024;
+constexpr int kOrderThreads = 1024, kOneBlockRoutes = 4096;
 
-// Block 0 sorts the routes by expert: order[place] = route, and the table of row tiles, at most `rows` places of one
-// expert each.  The order inside an expert is that of the atomics; no result depends on it, since every place's row
-// is computed by itself and summed by its route.  Routes without an expert get no place.
-// The other blocks quantise the tokens.
+// The places of the routes, sorted by expert: order[place] = route, and the table of row tiles, at most `rows` places of
+// one expert each.  The order inside an expert is that of atomics; no result depends on it, since every place's row is
+// computed by itself and summed by its route.  Routes without an expert get no place.
+//
+// Up to kOneBlockRoutes routes block 0 does it alone.  More: its LDS atomics, on few addresses, would take longer than
+// the rest (16384 routes to 64 experts: 19 us), so blocks of kOrderThreads routes count and rank theirs, and a second
+// launch adds up the counts (6 us for both).
+struct MxOrder {
+  const void* ids;
+  int id64, R, E, rows;
+  int *order, *tiles, *tile_count;
+  int blocks;         // of routes; 1: block 0 does everything
+  int *rank, *hist;   // rank[route] in its block and expert; hist[blocks][E]
+};
+
+// First place and first tile of every expert (thread e has expert e's) from its count, and its rows of the table if
+// `write`.
+__device__ __forceinline__ int mx_first_place(const MxOrder& o, int c, bool write) {
+  __shared__ int tot[2][kOrderThreads / 64];
+  const int t = threadIdx.x, wave = t >> 6, nt = (c + o.rows - 1) / o.rows;
+  const int ic = wave_incl_scan_i32(c), it = wave_incl_scan_i32(nt);
+  if ((t & 63) == 63) tot[0][wave] = ic, tot[1][wave] = it;
+  __syncthreads();
+  int first = ic - c, ft = it - nt;
+  for (int w = 0; w < wave; ++w) first += tot[0][w], ft += tot[1][w];
+  if (write) {
+    for (int i = 0; i < nt; ++i) {
+      int* row = o.tiles + 3 * (ft + i);
+      row[0] = t;
+      row[1] = first + i * o.rows;
+      row[2] = min(o.rows, c - i * o.rows);
+    }
+    if (t == kOrderThreads - 1) o.tile_count[0] = ft + nt;
+  }
+  return first;
+}
+
+// Blocks of routes first, then blocks that quantise the tokens.
 template <typename T>
-__global__ void __launch_bounds__(kOrderThreads) mx_prepare_kernel(const void* __restrict__ ids, int id64, int R, int E, int rows,
-                                                                   int* __restrict__ order, int* __restrict__ tiles,
-                                                                   int* __restrict__ tile_count, const uint16_t* __restrict__ x,
-                                                                   int64_t ldx, int64_t pieces, int per_row, uint8_t* __restrict__ codes,
-                                                                   uint8_t* __restrict__ scales, int lds) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (blockIdx.x > 0) {
-    const int64_t i = (int64_t)(blockIdx.x - 1) * kOrderThreads + t;
+__global__ void __launch_bounds__(kOrderThreads) mx_prepare_kernel(MxOrder o, const uint16_t* __restrict__ x, int64_t ldx, int64_t pieces,
+                                                                   int per_row, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                   int lds) {
+  __shared__ int count[kOrderThreads];
+  const int t = threadIdx.x;
+  if ((int)blockIdx.x >= o.blocks) {
+    const int64_t i = (int64_t)((int)blockIdx.x - o.blocks) * kOrderThreads + t;
     if (i >= pieces) return;  // whole blocks of 32: pieces % 4 == 0
     const int64_t row = i / per_row;
     const int piece = (int)(i - row * per_row);
     mx_quantize8<T>(x + row * ldx, codes + row * per_row * 4, scales + row * lds, piece);
     return;
   }
-  __shared__ int count[kOrderThreads], tot[2][kOrderThreads / 64];
-  constexpr int AT_ONCE = 16;  // ids of a thread under way
   count[t] = 0;
   __syncthreads();
-  auto for_routes = [&](auto f) {
-    for (int64_t base = t; base < R; base += kOrderThreads * AT_ONCE) {
-      int64_t e[AT_ONCE];
-#pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j) {
-        const int64_t r = base + j * kOrderThreads;
-        e[j] = r < R ? mx_route_id(ids, id64, r) : -1;
-      }
-#pragma unroll
-      for (int j = 0; j < AT_ONCE; ++j)
-        if (e[j] >= 0 && e[j] < E) f((int)(base + j * kOrderThreads), (int)e[j]);
-    }
-  };
-  for_routes([&](int, int e) { atomicAdd(&count[e], 1); });
-  __syncthreads();
-  // E <= kOrderThreads: one expert per thread; prefix sums of places and tiles
-  const int c = count[t], nt = (c + rows - 1) / rows;
-  const int ic = wave_incl_scan_i32(c), it = wave_incl_scan_i32(nt);
-  if (lane == 63) tot[0][wave] = ic, tot[1][wave] = it;
-  __syncthreads();
-  int first = ic - c, ft = it - nt;
-  for (int w = 0; w < wave; ++w) first += tot[0][w], ft += tot[1][w];
-  count[t] = first;  // from here on the expert's next place
-  for (int i = 0; i < nt; ++i) {
-    int* row = tiles + 3 * (ft + i);
-    row[0] = t;
-    row[1] = first + i * rows;
-    row[2] = min(rows, c - i * rows);
+  if (o.blocks > 1) {
+    const int64_t r = (int64_t)blockIdx.x * kOrderThreads + t;
+    const int64_t e = r < o.R ? mx_route_id(o.ids, o.id64, r) : -1;
+    if (e >= 0 && e < o.E) o.rank[r] = atomicAdd(&count[e], 1);
+    __syncthreads();
+    if (t < o.E) o.hist[(int64_t)blockIdx.x * o.E + t] = count[t];
+    return;
   }
-  if (t == kOrderThreads - 1) tile_count[0] = ft + nt;
+  constexpr int MOST = kOneBlockRoutes / kOrderThreads;
+  int64_t e[MOST];
+#pragma unroll
+  for (int j = 0; j < MOST; ++j) {
+    const int r = t + j * kOrderThreads;
+    e[j] = r < o.R ? mx_route_id(o.ids, o.id64, r) : -1;
+    if (e[j] >= o.E) e[j] = -1;
+  }
+#pragma unroll
+  for (int j = 0; j < MOST; ++j)
+    if (e[j] >= 0) atomicAdd(&count[e[j]], 1);
   __syncthreads();
-  for_routes([&](int r, int e) { order[atomicAdd(&count[e], 1)] = r; });
+  // E <= kOrderThreads: one expert per thread
+  const int first = mx_first_place(o, count[t], true);
+  count[t] = first;  // from here on the expert's next place
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < MOST; ++j)
+    if (e[j] >= 0) o.order[atomicAdd(&count[e[j]], 1)] = t + j * kOrderThreads;
+}
+
+// The second launch of many routes: block b places the routes of block b.
+__global__ void __launch_bounds__(kOrderThreads) mx_place_kernel(MxOrder o) {
+  __shared__ int base[kOrderThreads];
+  const int t = threadIdx.x;
+  int total = 0, before = 0;
+  if (t < o.E) {
+#pragma unroll 8
+    for (int b = 0; b < o.blocks; ++b) {
+      const int c = o.hist[(int64_t)b * o.E + t];
+      total += c;
+      before += b < (int)blockIdx.x ? c : 0;
+    }
+  }
+  base[t] = mx_first_place(o, total, blockIdx.x == 0) + before;
+  __syncthreads();
+  const int64_t r = (int64_t)blockIdx.x * kOrderThreads + t;
+  const int64_t e = r < o.R ? mx_route_id(o.ids, o.id64, r) : -1;
+  if (e >= 0 && e < o.E) o.order[base[e] + o.rank[r]] = (int)r;
 }
 
 // out[t] = the sum over a token's slots, in slot order, of weight * y: fp32, one rounding.  A slot
@@ -125,7 +171,10 @@ MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk
   w.max_tiles = R / mx_moe_rows(R, E) + std::min<int64_t>(R, E);
   w.order = 256;  // the tile count sits in front
   w.tiles = al(w.order + R * 4);
-  w.x = al(w.tiles + w.max_tiles * 12);
+  w.order_blocks = R <= kOneBlockRoutes ? 1 : cdiv(R, kOrderThreads);
+  w.rank = al(w.tiles + w.max_tiles * 12);
+  w.hist = al(w.rank + (w.order_blocks > 1 ? R * 4 : 0));
+  w.x = al(w.hist + (w.order_blocks > 1 ? w.order_blocks * E * 4 : 0));
   w.xs = al(w.x + T * (H / 2));
   w.h = al(w.xs + T * scale_stride(H));
   w.hs = al(w.h + R * (I / 2));
@@ -166,14 +215,19 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   int* tiles = (int*)(ws + w.tiles);
   const int rows = mx_moe_rows(R, c.E);
   const int64_t pieces = c.T * (c.H / 8);
-  if (cdiv(pieces, kOrderThreads) >= 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
+  if (cdiv(pieces, kOrderThreads) + w.order_blocks > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
+  MxOrder o{c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws, (int)w.order_blocks, (int*)(ws + w.rank), (int*)(ws + w.hist)};
   auto prepare = [&](auto kernel) {
-    kernel<<<dim3((unsigned)(1 + cdiv(pieces, kOrderThreads))), dim3(kOrderThreads), 0, st>>>(
-        c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws, (const uint16_t*)c.x, c.T > 1 ? c.ldx : c.H, pieces, (int)(c.H / 8),
-        (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs), (int)scale_stride(c.H));
+    kernel<<<dim3((unsigned)(w.order_blocks + cdiv(pieces, kOrderThreads))), dim3(kOrderThreads), 0, st>>>(
+        o, (const uint16_t*)c.x, c.T > 1 ? c.ldx : c.H, pieces, (int)(c.H / 8), (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs),
+        (int)scale_stride(c.H));
   };
   c.act_dtype == AWQ_DTYPE_BF16 ? prepare(mx_prepare_kernel<bf16>) : prepare(mx_prepare_kernel<f16>);
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
+  if (w.order_blocks > 1) {
+    mx_place_kernel<<<dim3((unsigned)w.order_blocks), dim3(kOrderThreads), 0, st>>>(o);
+    if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
+  }
 
   MxArgs g{};
   g.a = (const uint8_t*)(ws + w.x), g.as = (const uint8_t*)(ws + w.xs);

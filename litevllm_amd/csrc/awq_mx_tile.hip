@@ -207,7 +207,18 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
 #pragma unroll
     for (int i = 0; i < TM; ++i) read_a(0, 0, at, i);
   }
-  for (int s = 0; s < stages; ++s) {
+  // a wave whose rows all lie behind the tile's last only loads (an expert's last tile is half empty on average)
+  const bool idle = MODE != kMxDense && m0 >= t.rows;
+  for (int s = 0; idle && s < stages; ++s) {
+    if (s + NBUF - 1 < stages) wait_loads_and_sync<(NBUF - 2) * LOADS>();
+    else wait_loads_and_sync<0>();
+    if (s + NBUF < stages) {
+      if (s & 1) load_scales((s + NBUF + 1) >> 1);
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) load_code(s + NBUF, u);
+    }
+  }
+  for (int s = 0; !idle && s < stages; ++s) {
     {
       const uint32_t at = scale_at(s, 1, (uint32_t)(m0 + r), sh_a);
       read_cols(s, 1, second);
@@ -217,29 +228,25 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
         read_a(s, 1, at, i);
       }
     }
-    // The second half's reads are of the next stage, so they begin behind the barrier: with the first products
-    // before it, the reads that it waits for have come back.  The loads of stage s + NBUF go out between the
+    // The second half's reads are of the next stage, so they begin behind the barrier, which comes after its first
+    // products: by then the reads that it waits for have come back.  The loads of stage s + NBUF go out between the
     // products.  (After the last stage the fragments are of nothing, and nobody uses them.)
-    constexpr int AT = TM > 2 ? 1 : 0, SHARE = (LOADS + TM - AT - 1) / (TM - AT);
+    constexpr int SHARE = (LOADS + TM - 1) / TM;
     const uint32_t at = scale_at(s + 1, 0, (uint32_t)(m0 + r), sh_a);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       products(i, second);
-      if (i == AT) {
+      if (i == 0) {
         // stage s + 1 is there, stage s has been read
         if (s + NBUF - 1 < stages) wait_loads_and_sync<(NBUF - 2) * LOADS>();
         else wait_loads_and_sync<0>();
         read_cols(s + 1, 0, first);
-#pragma unroll
-        for (int k = 0; k < AT; ++k) read_a(s + 1, 0, at, k);
         if ((s & 1) && s + NBUF < stages) load_scales((s + NBUF + 1) >> 1);
       }
-      if (i >= AT) {
-        read_a(s + 1, 0, at, i);
-        if (s + NBUF < stages) {
+      read_a(s + 1, 0, at, i);
+      if (s + NBUF < stages) {
 #pragma unroll
-          for (int u = (i - AT) * SHARE; u < (i - AT + 1) * SHARE && u < LOADS; ++u) load_code(s + NBUF, u);
-        }
+        for (int u = i * SHARE; u < (i + 1) * SHARE && u < LOADS; ++u) load_code(s + NBUF, u);
       }
     }
   }
@@ -327,17 +334,19 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
       }
     }
   } else if constexpr (MODE == kMxDown) {
+    // through LDS, as below, in fp32
+    constexpr int LD = TN * 64 + 16, LANES = TN * 4;  // bytes of a row; lanes of 16 bytes to it
+    static_assert(WAVES * TM * 16 * LD <= mx_tile_lds(ROWS, NBUF, TM > TN ? TM : TN), "the output tile");
+    uint8_t* mine = lds + wave * (TM * 16 * LD);
+    const int nw = n0 + c0 - BM, n = nw + lane % LANES * 4;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int m = m0 + 16 * i + r;
-      if (m >= t.rows) continue;
-      float* y = p.y + (int64_t)p.order[t.first + m] * p.N;
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = n0 + c0 - BM + 16 * j + 4 * q;
-        if (n < p.N) *(f32x4*)(y + n) = acc[i][j];
-      }
-    }
+      for (int j = 0; j < TN; ++j) *(f32x4*)(mine + (16 * i + r) * LD + 64 * j + 16 * q) = acc[i][j];
+    const int rows = min(TM * 16, t.rows - m0);
+    if (n < p.N)
+      for (int m = lane / LANES; m < rows; m += 64 / LANES)
+        *(f32x4*)(p.y + (int64_t)p.order[t.first + m0 + m] * p.N + n) = *(const f32x4*)(mine + m * LD + lane % LANES * 16);
   } else {
     // through LDS, a region of each wave's own: rows of whole lines instead of 8 bytes in 16 rows at a time
     // (M = 4096, N = 24576: 140 us of 412 before)
