@@ -1,5 +1,7 @@
 // Products of microscaled fp4 matrices, many rows: tiles of both operands in LDS (format, modes and operand
 // order: awq_mx_common.h).
+#include <algorithm>
+
 #include "awq_launch.h"
 #include "awq_mx_common.h"
 
@@ -404,12 +406,16 @@ static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
-// Tiles of 256 x 256 where they give every CU one, of 128 x 128 where those do; else of 64 x 64.  Up to a tile per CU
+// Tiles of 256 x 256 run in rounds of one a CU, those of 128 x 128 two a CU, whose rounds run into each other: K = 4096, us
+// with one and the other: M = 2048, N = 24576 121, 146; M = 3000, N = 5000 44, 54; M = 2048, N = 6144 41, 43; M = 1000,
+// N = 24576 77, 78; M = 700, N = 4096 31, 17: about 38 a round against 26 for 512 tiles.  Fewer than 192 of them: tiles
+// of 64 x 64 (M = 512, N = 4096 13 against 15; M = 1024 22 against 19).  Up to a tile per CU of these
 // K goes in shares: two from 8 stages on, four from 24 on (M = 64, N = 4096, us with 1, 2, 4: K = 1024 5.1, 5.2, 6.1;
 // K = 4096 9.4, 8.2, 8.6; K = 12288 22.7, 18.2, 15.6; with 316 tiles, M = 200, N = 5001, K = 4128 14.2, 15.3, 22.2).
 int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
-  if (cdiv(p.M, 256) * cdiv(p.N, 256) >= 256) return launch_tile<kMxDense, 256, 256, 2, 4, 2, 2>(p, cdiv(p.M, 256), st);
-  if (cdiv(p.M, 128) * cdiv(p.N, 128) >= 256) return launch_tile<kMxDense, 128, 128, 2, 4, 4, 2>(p, cdiv(p.M, 128), st);
+  const int64_t big = cdiv(p.M, 256) * cdiv(p.N, 256), mid = cdiv(p.M, 128) * cdiv(p.N, 128);
+  if (512 * 38 * cdiv(big, 256) <= 26 * std::max<int64_t>(512, mid)) return launch_tile<kMxDense, 256, 256, 2, 4, 2, 2>(p, cdiv(p.M, 256), st);
+  if (mid >= 192) return launch_tile<kMxDense, 128, 128, 2, 4, 4, 2>(p, cdiv(p.M, 128), st);
   const int64_t rows = cdiv(p.M, 64), tiles = rows * cdiv(p.N, 64), stages = cdiv(p.K, 256);
   if (tiles <= 256 && stages >= 24) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2, 4>(p, rows, st);
   if (tiles <= 256 && stages >= 8) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2, 2>(p, rows, st);

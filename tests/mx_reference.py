@@ -73,29 +73,27 @@ def moe(x, weights, ids, w1, w2, kind):
     rounding border: the bound takes the codes at both ends of its error."""
     xq = rounded(x)
     out, off = torch.zeros_like(xq), torch.zeros_like(xq)
-    inter, experts = w2.shape[2], w1.shape[0]
-    for t in range(x.shape[0]):
-        for j in range(ids.shape[1]):
-            e = int(ids[t, j])
-            if not 0 <= e < experts:
-                continue
-            gu, dgu = gemm(xq[t:t + 1], w1[e])
-            g, u, dg, du = gu[:, :inter], gu[:, inter:], dgu[:, :inter], dgu[:, inter:]
-            h = act(g, kind) * u
-            # |act'| < 1.13; exp2 and reciprocal in hardware: a few 2^-23 of |act|, as |t| 2^-23 grows with g
-            dh = 1.13 * dg * (u.abs() + du) + act(g, kind).abs() * du + h.abs() * (16 + 4 * g.abs()) * 2.0 ** -23
-            size = h.abs()
-            lo, hi = rounded((size - dh).clamp(min=0)), rounded(size + dh)
-            e0, e1 = block_exponents((size - dh).clamp(min=0)), block_exponents(size + dh)
-            v0 = values_at(size, dh, e0)
-            v1 = values_at(size, dh, e1)
-            hq = rounded(h)
-            slack = torch.stack([lo, hi, *v0, *v1]).sub(hq.abs()).abs().amax(0)
-            y, dy = gemm(hq, w2[e])
-            dy = dy + slack @ w2[e].abs().t()
-            w = float(weights[t, j])
-            out[t] += w * y[0]
-            off[t] += abs(w) * (dy[0] + y[0].abs() * (ids.shape[1] + 1) * 2.0 ** -23)
+    inter, experts, slots = w2.shape[2], w1.shape[0], ids.shape[1]
+    weights = weights.to(xq.device).double()
+    for e in range(experts):
+        rows, slot = (ids.to(xq.device) == e).nonzero(as_tuple=True)
+        if not rows.numel():
+            continue
+        gu, dgu = gemm(xq[rows], w1[e])
+        g, u, dg, du = gu[:, :inter], gu[:, inter:], dgu[:, :inter], dgu[:, inter:]
+        h = act(g, kind) * u
+        # |act'| < 1.13; exp2 and reciprocal in hardware: a few 2^-23 of |act|, as |t| 2^-23 grows with g
+        dh = 1.13 * dg * (u.abs() + du) + act(g, kind).abs() * du + h.abs() * (16 + 4 * g.abs()) * 2.0 ** -23
+        size = h.abs()
+        ends = [(size - dh).clamp(min=0), size + dh]
+        hq = rounded(h)
+        near = [rounded(v) for v in ends] + [v for end in ends for v in values_at(size, dh, block_exponents(end))]
+        slack = torch.stack(near).sub(hq.abs()).abs().amax(0)
+        y, dy = gemm(hq, w2[e])
+        dy = dy + slack @ w2[e].abs().t()
+        w = weights[rows, slot].unsqueeze(1)
+        out.index_add_(0, rows, w * y)
+        off.index_add_(0, rows, w.abs() * (dy + y.abs() * (slots + 1) * 2.0 ** -23))
     return out, off
 
 
