@@ -14,7 +14,7 @@ bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 constexpr int64_t kIntMax = 0x7FFFFFFFLL;
 constexpr int64_t kMaxK = (int64_t)1 << 24;   // 256 rows of codes are addressed in 32 bits,
-constexpr int64_t kBytes = 0xFFFFFFF0LL;      // and so are all of the tokens' and all of an expert's gate and up
+constexpr int64_t kBytes = 0xFFFF0000LL;      // and so are all of the tokens' and all of an expert's gate and up
 }  // namespace
 
 extern "C" {

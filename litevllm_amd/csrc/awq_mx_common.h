@@ -18,12 +18,11 @@ namespace awq {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// c += a . b^T over 128 values of K.  sa / sb: scale bytes in bits 8 SEL .. 8 SEL + 7.
-template <int SELA, int SELB>
+// c += a . b^T over 128 values of K.  sa / sb: scale bytes in the low eight bits.
 __device__ __forceinline__ f32x4 mx_mfma(const u32x4& a, const u32x4& b, const f32x4& c, uint32_t sa, uint32_t sb) {
   const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, SELA, (int)sa, SELB, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
 // Scale byte of a block whose largest magnitude has these bits (sign clear; they order like the

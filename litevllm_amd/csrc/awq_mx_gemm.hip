@@ -4,8 +4,6 @@
 // What bounds them is the read of the weights, once: a block has 16 columns (gate_up: 32 gate rows and the 32 up
 // rows of the same outputs), its waves share K, each asks for all that it will use before the first product, and
 // the waves' sums meet in LDS, in wave order.
-#include <algorithm>
-
 #include "awq_launch.h"
 #include "awq_mx_common.h"
 
@@ -48,8 +46,8 @@ __device__ __forceinline__ MxPair mx_load_last(const uint8_t* codes, const uint8
 }
 // c += a . b^T over the pair
 __device__ __forceinline__ f32x4 mx_mfma_pair(const MxPair& a, const MxPair& b, f32x4 c, int q) {
-  c = mx_mfma<0, 0>(a.c[0], b.c[0], c, a.s[0] >> (8 * q), b.s[0] >> (8 * q));
-  return mx_mfma<0, 0>(a.c[1], b.c[1], c, a.s[1] >> (8 * q), b.s[1] >> (8 * q));
+  c = mx_mfma(a.c[0], b.c[0], c, a.s[0] >> (8 * q), b.s[0] >> (8 * q));
+  return mx_mfma(a.c[1], b.c[1], c, a.s[1] >> (8 * q), b.s[1] >> (8 * q));
 }
 
 // The at most kMxScanRoutes routes in a wave's lanes: a lane holds the expert of the route with its number, or -1.
@@ -72,16 +70,15 @@ __device__ __forceinline__ void mx_scan_list(const MxScan& f, int lane, int* lis
 }
 static_assert(kMxScanRoutes == 64, "a lane each");
 
-// Grid x: column blocks, y: row tiles of 16 MT (with SCAN: routes).
+// Grid x: column blocks, y: row tiles of 16 (with SCAN: routes).
 // X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one
 // launch less where the rows are few and short.
 // SCAN (gate_up): no table of tiles; block y takes all the routes of route y's expert, which it finds in the ids
 // itself, if y is the first of them.  A route's place is its own number.
-template <int MODE, int MT, int NT, int WAVES, bool X16, bool SCAN>
+template <int MODE, int NT, int WAVES, bool X16, bool SCAN>
 __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   constexpr int THREADS = WAVES * 64;
-  constexpr int U = 1;  // pairs of steps under way in a wave; 2 or 4 measured the same: other waves fill in
-  __shared__ float red[WAVES][MT * NT][256];
+  __shared__ float red[WAVES][NT][256];
   __shared__ int list[SCAN ? kMxScanRoutes : 1];
   extern __shared__ __align__(16) uint8_t xq[];  // X16: codes [xrows][K/2 + 16], scales [xrows][K/32]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
@@ -94,7 +91,7 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     t = {f.expert, 0, (int)__popcll(f.its)};
   } else {
     if (MODE != kMxDense && (int)blockIdx.y >= p.tile_count[0]) return;
-    t = mx_rows<MODE, 16 * MT>(p, blockIdx.y);
+    t = mx_rows<MODE, 16>(p, blockIdx.y);
   }
   constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
   const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;  // whole ones
@@ -111,34 +108,23 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   }
   const int ld = p.K / 2 + 16;
   // a scanned expert may have more routes than a tile has rows (one that occurs twice in a token)
-  for (int base = 0; base < (SCAN ? t.rows : 1); base += 16 * MT) {
-    const int rows = SCAN ? min(t.rows - base, 16 * MT) : t.rows;
-    const uint8_t *ac[MT], *asc[MT];
+  for (int base = 0; base < (SCAN ? t.rows : 1); base += 16) {
+    const int rows = SCAN ? min(t.rows - base, 16) : t.rows;
+    const uint8_t *ac, *asc;
     if constexpr (SCAN && !X16) __syncthreads();  // the list
     if constexpr (!X16) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int64_t row = SCAN ? list[base + min(16 * i + r, rows - 1)] / p.topk : mx_a_row<MODE>(p, t, 16 * i + r);
-        ac[i] = p.a + row * (p.K / 2);
-        asc[i] = p.as + row * p.as_ld;
-      }
+      const int64_t row = SCAN ? list[base + min(r, rows - 1)] / p.topk : mx_a_row<MODE>(p, t, r);
+      ac = p.a + row * (p.K / 2);
+      asc = p.as + row * p.as_ld;
     }
-    f32x4 acc[MT][NT];
+    f32x4 acc[NT];
+    MxPair b[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (wave < pairs) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    MxPair b[U][NT];
-    auto load_w = [&](int first) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (first + u * WAVES < pairs) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) b[u][j] = mx_load_pair(wc[j], wsc[j], first + u * WAVES, q);
-        }
-    };
-    load_w(wave);
+      for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], wave, q);
+    }
     if constexpr (X16) {
       if constexpr (SCAN) __syncthreads();  // the list
       const int pieces = p.K / 8;
@@ -152,54 +138,35 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
         }
       }
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int m = min(16 * i + r, rows - 1);
-        ac[i] = xq + m * ld;
-        asc[i] = xq + p.xrows * ld + m * KB;
-      }
+      const int m = min(r, rows - 1);
+      ac = xq + m * ld;
+      asc = xq + p.xrows * ld + m * KB;
     }
-    for (int first = wave; first < pairs; first += U * WAVES) {
-      if (first != wave) load_w(first);
-      MxPair a[U][MT];
+    // a pair at a time: two or four under way in a wave measured the same, other waves fill in
+    for (int pair = wave; pair < pairs; pair += WAVES) {
+      if (pair != wave) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (first + u * WAVES < pairs) {
+        for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], pair, q);
+      }
+      const MxPair a = mx_load_pair(ac, asc, pair, q);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) a[u][i] = mx_load_pair(ac[i], asc[i], first + u * WAVES, q);
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (first + u * WAVES < pairs) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_pair(a[u][i], b[u][j], acc[i][j], q);
-        }
+      for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, b[j], acc[j], q);
     }
     if ((KB & 7) != 0 && wave == pairs % WAVES) {
-      MxPair w[NT];
+      const MxPair a = mx_load_last(ac, asc, pairs, q, KB);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) w[j] = mx_load_last(wc[j], wsc[j], pairs, q, KB);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const MxPair x = mx_load_last(ac[i], asc[i], pairs, q, KB);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mx_mfma_pair(x, w[j], acc[i][j], q);
-      }
+      for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, mx_load_last(wc[j], wsc[j], pairs, q, KB), acc[j], q);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) red[wave][i * NT + j][(4 * q + u) * 16 + r] = acc[i][j][u];
+      for (int u = 0; u < 4; ++u) red[wave][j][(4 * q + u) * 16 + r] = acc[j][u];
     __syncthreads();
 
-    auto sum = [&](int tile16, int at) {
-      float v = red[0][tile16][at];
+    auto sum = [&](int j, int at) {
+      float v = red[0][j][at];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) v += red[w][tile16][at];
+      for (int w = 1; w < WAVES; ++w) v += red[w][j][at];
       return v;
     };
     if constexpr (MODE == kMxGateUp) {
@@ -207,8 +174,8 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
       static_assert(NT == 4, "32 gate and 32 up rows");
       const int n = tid & 31;
       for (int m = tid >> 5; m < rows; m += THREADS / 32) {
-        const int at = (m & 15) * 16 + (n & 15), tg = (m >> 4) * NT + (n >> 4);
-        const float v = mx_gated(sum(tg, at), sum(tg + 2, at), p.act);
+        const int at = m * 16 + (n & 15);
+        const float v = mx_gated(sum(n >> 4, at), sum((n >> 4) + 2, at), p.act);
         uint32_t top = mx_abs_bits(v);
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
@@ -222,10 +189,10 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
         if (n == 0) p.hs[place * (p.N / 32) + n0 / 32] = (uint8_t)byte;
       }
     } else {
-      for (int i = tid; i < MT * NT * 256; i += THREADS) {
-        const int t16 = i >> 8, at = i & 255, m = (t16 / NT) * 16 + (at >> 4), n = n0 + (t16 % NT) * 16 + (at & 15);
+      for (int i = tid; i < NT * 256; i += THREADS) {
+        const int j = i >> 8, at = i & 255, m = at >> 4, n = n0 + j * 16 + (at & 15);
         if (m >= rows || n >= p.N) continue;
-        float v = sum(t16, at);
+        float v = sum(j, at);
         if constexpr (MODE == kMxDense) {
           v += load_bias(p.bias, p.bias_dtype, n);
           p.c[(int64_t)(t.first + m) * p.ldc + n] = p.out_bf16 ? f2bf_bits(v) : f2h_bits(v);
@@ -307,10 +274,10 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
 namespace awq_host {
 using namespace awq;
 
-template <int MODE, int MT, int NT, int WAVES, bool X16, bool SCAN>
+template <int MODE, int NT, int WAVES, bool X16, bool SCAN>
 static int launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   constexpr int COLS = MODE == kMxGateUp ? 8 * NT : 16 * NT;
-  auto kernel = mx_rows_kernel<MODE, MT, NT, WAVES, X16, SCAN>;
+  auto kernel = mx_rows_kernel<MODE, NT, WAVES, X16, SCAN>;
   const size_t lds = X16 ? (size_t)p.xrows * (p.K / 2 + 16 + p.K / 32) : 0;
   kernel<<<dim3((unsigned)cdiv(p.N, COLS), (unsigned)row_tiles), dim3(WAVES * 64), lds, st>>>(p);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
@@ -325,9 +292,9 @@ bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= kMxRowsMax && M * K
 // one block (K = 12288, N = 4096: 4 waves 10.1, 8 8.1, 16 7.7).
 template <bool X16>
 static int launch_rows_dense(const MxArgs& p, hipStream_t st) {
-  if (p.N <= 16 * 256) return launch_rows<kMxDense, 1, 1, 16, X16, false>(p, 1, st);
-  if (p.N <= 32 * 256) return launch_rows<kMxDense, 1, 2, 16, X16, false>(p, 1, st);
-  return launch_rows<kMxDense, 1, 2, 8, X16, false>(p, 1, st);
+  if (p.N <= 16 * 256) return launch_rows<kMxDense, 1, 16, X16, false>(p, 1, st);
+  if (p.N <= 32 * 256) return launch_rows<kMxDense, 2, 16, X16, false>(p, 1, st);
+  return launch_rows<kMxDense, 2, 8, X16, false>(p, 1, st);
 }
 int launch_mx_rows_gemm(const MxArgs& p, hipStream_t st) {
   return p.x ? launch_rows_dense<true>(p, st) : launch_rows_dense<false>(p, st);
@@ -335,14 +302,13 @@ int launch_mx_rows_gemm(const MxArgs& p, hipStream_t st) {
 
 int launch_mx_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
   if (rows > 16) return launch_mx_tile_grouped(p, gate_up, rows, row_tiles, st);
-  if (row_tiles > 65535) return AWQ_ERR_UNSUPPORTED;
-  if (gate_up) return launch_rows<kMxGateUp, 1, 4, 4, false, false>(p, row_tiles, st);
-  return launch_rows<kMxDown, 1, 2, 4, false, false>(p, row_tiles, st);
+  if (gate_up) return launch_rows<kMxGateUp, 4, 4, false, false>(p, row_tiles, st);
+  return launch_rows<kMxDown, 2, 4, false, false>(p, row_tiles, st);
 }
 
 int launch_mx_scan_gate_up(const MxArgs& p, hipStream_t st) {
-  if (p.x) return launch_rows<kMxGateUp, 1, 4, 4, true, true>(p, p.routes, st);
-  return launch_rows<kMxGateUp, 1, 4, 4, false, true>(p, p.routes, st);
+  if (p.x) return launch_rows<kMxGateUp, 4, 4, true, true>(p, p.routes, st);
+  return launch_rows<kMxGateUp, 4, 4, false, true>(p, p.routes, st);
 }
 
 int launch_mx_down_combine(const MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st) {

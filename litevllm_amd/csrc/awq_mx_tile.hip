@@ -29,20 +29,15 @@ __device__ __forceinline__ void wait_loads_and_sync() {
 // acc[j] += b[j] . a^T for two neighbouring column tiles, as one piece of assembly: the compiler moves the builtin
 // behind the reads of whole stages, runs out of registers, and copies accumulators (M = 4096, N = 24576,
 // K = 4096: 404 us with it).  The wait states in front cover a copy of an operand by the VALU; the accumulators
-// may be used 18 wait states after the last of these (mfma_results).
-template <bool AGPR>
+// may be used 18 wait states after the last of these.
 __device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, const u32x4& b1, const u32x4& a, uint32_t s0, uint32_t s1,
                                       uint32_t sa) {
-#define MX_MFMA(C, B, S) "v_mfma_scale_f32_16x16x128_f8f6f4 " C ", " B ", %4, " C ", " S ", %7 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-  if constexpr (AGPR)
-    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%2", "%5") "\n\t" MX_MFMA("%1", "%3", "%6")
-                 : "+a"(c0), "+a"(c1)
-                 : "v"(b0), "v"(b1), "v"(a), "v"(s0), "v"(s1), "v"(sa));
-  else
-    asm volatile("s_nop 1\n\t" MX_MFMA("%0", "%2", "%5") "\n\t" MX_MFMA("%1", "%3", "%6")
-                 : "+v"(c0), "+v"(c1)
-                 : "v"(b0), "v"(b1), "v"(a), "v"(s0), "v"(s1), "v"(sa));
-#undef MX_MFMA
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %2, %4, %0, %5, %7 op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t"
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %1, %3, %4, %1, %6, %7 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+      : "+v"(c0), "+v"(c1)
+      : "v"(b0), "v"(b1), "v"(a), "v"(s0), "v"(s1), "v"(sa));
 }
 
 // Block: BM rows of a by BN rows of w, WM x WN waves of (BM / WM) x (BN / WN).  A stage of 256 along K (one line
@@ -66,7 +61,6 @@ __device__ __forceinline__ void mfma2(f32x4& c0, f32x4& c1, const u32x4& b0, con
 template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int NBUF, int WK>
 __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
   constexpr int WAVES = WM * WN /* of a share of K */, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
-  constexpr bool AGPR = TM * TN > 32;  // accumulators of more than half of the 256 VGPRs
   static_assert(TN % 2 == 0, "");
   extern __shared__ __align__(16) uint8_t lds[];  // codes [NBUF][ROWS][128], scales [NBUF][ROWS][16], zeros
 
@@ -188,7 +182,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   Cols first, second;
   auto products = [&](int i, const Cols& now) {
 #pragma unroll
-    for (int j = 0; j < TN; j += 2) mfma2<AGPR>(acc[i][j], acc[i][j + 1], now.b[j], now.b[j + 1], a[i], now.s[j], now.s[j + 1], sa[i]);
+    for (int j = 0; j < TN; j += 2) mfma2(acc[i][j], acc[i][j + 1], now.b[j], now.b[j + 1], a[i], now.s[j], now.s[j + 1], sa[i]);
   };
   // a's fragments have one place: each is read again, for the next half, as soon as its products are under way
 
@@ -257,10 +251,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      if constexpr (AGPR) asm volatile("" : "+a"(acc[i][j]));
-      else asm volatile("" : "+v"(acc[i][j]));
-    }
+    for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[i][j]));
   __syncthreads();
 
   if constexpr (WK > 1) {
