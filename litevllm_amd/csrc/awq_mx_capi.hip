@@ -13,6 +13,7 @@ bool dtype_float(int d) { return dtype_16(d) || d == AWQ_DTYPE_F32; }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 constexpr int64_t kIntMax = 0x7FFFFFFFLL;
+constexpr int64_t kMaxBalance = (int64_t)1 << 30;  // tokens and routes: 32 bits number them, a block's behind the last too
 constexpr int64_t kMaxK = (int64_t)1 << 24;   // 256 rows of codes are addressed in 32 bits,
 constexpr int64_t kBytes = 0xFFFF0000LL;      // and so are all of the tokens' and all of an expert's gate and up
 }  // namespace
@@ -130,7 +131,7 @@ int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, 
   if (T < 0 || E <= 0 || top_k <= 0) return AWQ_ERR_SHAPE;
   if (!loss || !counts || !factor || (T > 0 && (!logits || !topk_ids))) return AWQ_ERR_NULL;
   if (!dtype_float(logits_dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
-  if (E > 1024 || T > kIntMax || T * top_k > kIntMax) return AWQ_ERR_UNSUPPORTED;
+  if (E > 1024 || T > kMaxBalance || T * top_k > kMaxBalance) return AWQ_ERR_UNSUPPORTED;
   if (T > 1 && ld < E) return AWQ_ERR_STRIDE;
   if (!workspace || workspace_bytes < balance_workspace_bytes(T, E)) return AWQ_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return AWQ_ERR_STRIDE;
@@ -143,7 +144,7 @@ int awq_w4a16_moe_balance_grad(const void* logits, int64_t ld, int32_t logits_dt
   if (T < 0 || E <= 0) return AWQ_ERR_SHAPE;
   if (T == 0) return AWQ_OK;
   if (!logits || !factor || !upstream || !grad) return AWQ_ERR_NULL;
-  if (!dtype_float(logits_dtype) || E > 1024 || T > kIntMax) return AWQ_ERR_UNSUPPORTED;
+  if (!dtype_float(logits_dtype) || E > 1024 || T > kMaxBalance) return AWQ_ERR_UNSUPPORTED;
   if (T > 1 && ld < E) return AWQ_ERR_STRIDE;
   return launch_moe_balance_grad(logits, ld, logits_dtype, mask, factor, upstream, grad, T, E, (hipStream_t)stream);
 }

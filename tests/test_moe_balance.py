@@ -243,3 +243,13 @@ def test_entries_refuse():
     assert grad(dt=9) == grad(e=1025, ld=1025) == L.ERR_UNSUPPORTED
     assert grad(ld=3) == L.ERR_STRIDE
     assert grad(t=0) == L.OK
+
+
+def test_entries_refuse_more_tokens_than_they_number():
+    lib = L.load()
+    p = (ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p).value + 255) & ~255
+    for t, k in (((1 << 30) + 1, 1), ((1 << 31) - 1, 1), (1 << 29, 3)):
+        need = lib.awq_w4a16_moe_balance_workspace_bytes(t, 1)
+        assert lib.awq_w4a16_moe_balance(p, 1, L.DTYPE_F16, p, 32, None, t, 1, k, p, p, p, p, need, None) == L.ERR_UNSUPPORTED
+        if t > 1 << 30:
+            assert lib.awq_w4a16_moe_balance_grad(p, 1, L.DTYPE_F16, None, p, p, p, t, 1, None) == L.ERR_UNSUPPORTED
