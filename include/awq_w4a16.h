@@ -424,7 +424,8 @@ size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
  *   a: with a_scales NULL [M, K] of act_dtype, row stride lda (a multiple of 8), quantised in the call
  *      as awq_w4a16_mxfp4_quantize does; else codes [M, K/2] with a_scales [M, K/32] (lda and the workspace
  *      are not used).
- *   w: codes [N, K/2], w_scales [N, K/32];  bias: NULL or [N] of bias_dtype;  c: row stride ldc.
+ *   w: codes [N, K/2], w_scales [N, K/32];  bias: NULL or [N] of bias_dtype;  c: row stride ldc, apart from all that
+ *      the call reads (with few rows blocks read all of a while others write).
  *   Any M, N >= 0.  Results are bitwise reproducible.  A NaN block makes NaN of every output that reads it.
  *   workspace: 256-byte aligned; calls that may overlap must not share one. */
 int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, const uint8_t* w,
@@ -439,8 +440,8 @@ size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int3
  *   h = MXFP4(act(g) * u) of the fp32 sums g, u = MXFP4(x[t]) . W1_e^T (rows 0 .. I-1 gate, I .. 2I-1 up),
  *   out[t] = sum over j of w[t, j] * (h . W2_e^T), fp32 in slot order, one rounding.
  *   gate_up: codes [E, 2I, H/2], scales [E, 2I, H/32];  down: codes [E, H, I/2], scales [E, H, I/32].
- *   x: [T, H] act_dtype, row stride ldx (a multiple of 8);  out: row stride ldo.  Ids outside [0, E)
- *   contribute nothing; an expert may occur twice in a token.  E <= 1024, H % 32 == 0, I % 32 == 0.
+ *   x: [T, H] act_dtype, row stride ldx (a multiple of 8);  out: row stride ldo; it may lie over x, over nothing else
+ *   that the call reads.  Ids outside [0, E) contribute nothing; an expert may occur twice in a token.  E <= 1024, H % 32 == 0, I % 32 == 0.
  *   Results are bitwise reproducible.  workspace: 256-byte aligned. */
 int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_t ids_bits, const void* topk_weights,
                         int32_t weights_dtype, const uint8_t* gate_up, const uint8_t* gate_up_scales,
@@ -454,7 +455,8 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
  *   loss = E * sum_e (counts[e] / (n top_k)) * (sum over kept t of p[t, e] / n)      (1 when even)
  * No kept token: 0.  A row of nothing but -inf has p = 0.  What a masked row holds is not read.
  *   logits: [T, ld] of logits_dtype;  topk_ids: [T, top_k] int32 or int64, dense;  mask: NULL or [T] bytes;
- *   loss: 1 float;  counts: [E];  factor: [E] floats for awq_w4a16_moe_balance_grad.  E <= 1024.
+ *   loss: 1 float;  counts: [E];  factor: [E] floats for awq_w4a16_moe_balance_grad.  E <= 1024;
+ *   up to 2^30 tokens and routes.
  *   Results are bitwise reproducible.  workspace: 16-byte aligned, no zeroing needed. */
 size_t awq_w4a16_moe_balance_workspace_bytes(int64_t T, int32_t E);
 int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, const void* topk_ids,

@@ -4,7 +4,8 @@ two operands the matrix cores multiply in that format.
 The format (OCP Microscaling Formats 1.0): 32 consecutive values along the last dimension share a scale
 ``2 ** (byte - 127)``; a value is an e2m1 code.  A ``[..., K]`` tensor is ``codes`` uint8 ``[..., K/2]`` (the even
 index in the low four bits) and ``scales`` uint8 ``[..., K/32]``, as MXFP4 checkpoints hold weights; the kernels
-read that layout as it is, so no copy of a weight is built.  Activations are quantised on the way in.
+read that layout as it is, so no copy of a weight is built.  Activations are quantised on the way in.  None of these
+operators is differentiable.
 
 Every byte of the arithmetic runs in ``libawq_w4a16.so``; there is no CPU fallback.  Scratch memory comes from
 PyTorch's allocator for each call, so calls on different streams and captured graphs share none.
@@ -98,7 +99,8 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
     ``qweight`` uint8 ``[N, K/2]``, ``scales`` uint8 ``[N, K/32]``.  ``a``: fp16 or bf16 ``[M, K]``, quantised in the
     call, the result in its type; or, with ``a_scales``, codes that :func:`mxfp4_quantize` made (once for
     several projections of one input), the result in ``out_dtype`` (fp16 or bf16).  Other activations than
-    quantised ones are not provided.  Results are bitwise reproducible."""
+    quantised ones are not provided.  ``out`` may lie over a 16-bit ``a``, over no other operand.  Results are bitwise
+    reproducible."""
     dev = ops._require_device(a, qweight, scales, a_scales, bias, out)
     if a.dim() != 2 or qweight.dim() != 2:
         raise ValueError(f"a and qweight must be 2-D, got {tuple(a.shape)} and {tuple(qweight.shape)}")
@@ -124,6 +126,9 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
         raise ValueError(f"bad_output: out must be {dtype}, got {out.dtype}")
     else:
         ops.check_out(out, m, n, out)
+        if a_scales is None and m and a.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+            # few rows are read by every block, also while others write: a, which out may lie over, first
+            a, a_scales = mxfp4_quantize(a)
     if m == 0 or n == 0:
         return out
     lib = L.load()
@@ -189,7 +194,8 @@ def mxfp4_moe(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
 
     ``gate_up`` is the ``[E, 2I, H]`` stack (rows 0 .. I-1 gate, I .. 2I-1 up), ``down`` the ``[E, H, I]`` one; H and I
     are multiples of 32.  Sums are fp32 in slot order with one rounding; the routing weights enter in fp32.
-    Ids outside ``[0, E)`` contribute nothing.  Results are bitwise reproducible."""
+    Ids outside ``[0, E)`` contribute nothing.  ``out`` may lie over ``x``, over no other operand.  Results are bitwise
+    reproducible."""
     dev = ops._require_device(x, topk_weights, topk_ids, gate_up.qweight, gate_up.scales, down.qweight, down.scales, out)
     if x.dim() != 2 or gate_up.qweight.dim() != 3 or down.qweight.dim() != 3:
         raise ValueError("x must be [T, H] and the stacks [E, N, K/2]")

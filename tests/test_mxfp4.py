@@ -255,6 +255,75 @@ def test_gemm_strides_and_what_lies_around_the_output(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3, 16, 80])
+def test_gemm_over_its_own_input_and_beside_it(m):
+    from litevllm_amd import mxfp4_gemm, mxfp4_quantize
+    g = torch.Generator().manual_seed(11)
+    k = n = 1024
+    w, ws = mxfp4_quantize(torch.randn(n, k, generator=g).cuda())
+    x = torch.randn(m, k, generator=g).to(torch.bfloat16).cuda()
+    want = mxfp4_gemm(x, w, ws)
+    for _ in range(4):
+        a = x.clone()
+        assert mxfp4_gemm(a, w, ws, out=a) is a and torch.equal(a, want)
+        both = torch.cat([x, x], 1)
+        mxfp4_gemm(both[:, :k], w, ws, out=both[:, k:])
+        assert torch.equal(both[:, :k], x) and torch.equal(both[:, k:], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 8, 60])
+def test_moe_over_its_own_input(t):
+    from litevllm_amd import MXFP4Experts, mxfp4_moe, mxfp4_quantize
+    g = torch.Generator().manual_seed(12)
+    e, k, h, i = 4, 2, 512, 256
+    gu = MXFP4Experts(*mxfp4_quantize(torch.randn(e, 2 * i, h, generator=g).cuda()))
+    dn = MXFP4Experts(*mxfp4_quantize(torch.randn(e, h, i, generator=g).cuda()))
+    x = torch.randn(t, h, generator=g).to(torch.bfloat16).cuda()
+    ids = torch.randint(0, e, (t, k), generator=g).cuda()
+    w = torch.rand(t, k, generator=g).cuda()
+    want = mxfp4_moe(x, w, ids, gu, dn)
+    assert torch.equal(mxfp4_moe(x, w, ids, gu, dn, out=x), want) and torch.equal(x, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_gemm_with_a_weight_past_4_gib(m):
+    """The columns at the weight's end, whose codes lie past 2^32 bytes; the rest of it is zeros."""
+    from litevllm_amd import mxfp4_gemm
+    n, k, last = 530000, 16384, 70
+    w = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda")
+    ws = torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    assert w.numel() > 1 << 32
+    c, s, wv = _weight(31, last, k)
+    w[-last:], ws[-last:] = c, s
+    x = _made(32, m, k, dtype=torch.bfloat16).cuda()
+    y = mxfp4_gemm(x, w, ws)
+    ref, off = R.gemm(R.rounded(x), wv)
+    _close(y[:, -last:], ref, off, torch.bfloat16)
+    assert not bool(y[:, :-last].any())
+
+
+@pytest.mark.gpu
+def test_activations_past_4_gib():
+    """Rows at the end of an input whose codes pass 2^32 bytes: quantised, multiplied and brought back."""
+    from litevllm_amd import mxfp4_dequantize, mxfp4_gemm, mxfp4_quantize
+    m, n, k, last = 530000, 48, 16384, 300
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-last:] = _made(33, last, k, dtype=torch.bfloat16).cuda()
+    codes, scales = mxfp4_quantize(x)
+    c, s = R.quantize(x[-last:])
+    assert codes.numel() > 1 << 32 and torch.equal(codes[-last:], c) and torch.equal(scales[-last:], s)
+    wc, wsc, wv = _weight(34, n, k)
+    ref, off = R.gemm(R.values(c, s), wv)
+    for y in (mxfp4_gemm(x, wc, wsc), mxfp4_gemm(codes, wc, wsc, a_scales=scales, out_dtype=torch.bfloat16)):
+        _close(y[-last:], ref, off, torch.bfloat16)
+        assert not bool(y[:-last].any())
+    back = mxfp4_dequantize(codes, scales, torch.bfloat16)
+    assert torch.equal(back[-last:].double(), R.values(c, s)) and not bool(back[:-last].any())
+
+
+@pytest.mark.gpu
 def test_gemm_refuses_and_empty():
     from litevllm_amd import mxfp4_gemm, mxfp4_quantize
     c, s, _ = _weight(1, 32, 64)
