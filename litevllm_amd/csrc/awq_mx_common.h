@@ -65,10 +65,10 @@ __device__ __forceinline__ void load8(const void* p, float* v) {
 
 // Eight values of a row, number `piece`, by a lane; the four lanes of a block of 32 share its largest magnitude by two
 // DPP steps inside their quad.
-template <typename T>
-__device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, uint8_t* scales, int piece) {
+template <typename T, typename Piece>
+__device__ __forceinline__ void mx_quantize8(const void* x, uint8_t* codes, uint8_t* scales, Piece piece) {
   float v[8];
-  load8<T>(x + piece * 8, v);
+  load8<T>((const char*)x + piece * (Piece)(8 * sizeof(T)), v);
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = max(top, mx_abs_bits(v[j]));
@@ -77,6 +77,11 @@ __device__ __forceinline__ void mx_quantize8(const uint16_t* x, uint8_t* codes, 
   const uint32_t byte = mx_scale_byte(top);
   *(uint32_t*)(codes + piece * 4) = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
   if ((piece & 3) == 0) scales[piece >> 2] = (uint8_t)byte;
+}
+
+// h of one value: act(gate) * up in fp32.
+__device__ __forceinline__ float mx_gated(float g, float u, int act) {
+  return (act == AWQ_MOE_ACT_GELU_TANH ? gated_act_fast<1>(g) : gated_act_fast<0>(g)) * u;
 }
 
 // One product of MXFP4 matrices: rows of `a` by rows of `w`.  Which rows, and where the sums go:

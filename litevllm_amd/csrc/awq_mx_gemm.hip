@@ -9,11 +9,6 @@
 
 namespace awq {
 
-// h of one value: act(gate) * up in fp32.
-__device__ __forceinline__ float mx_gated(float g, float u, int act) {
-  return (act == AWQ_MOE_ACT_GELU_TANH ? gated_act_fast<1>(g) : gated_act_fast<0>(g)) * u;
-}
-
 // The fragments of a pair of steps (256 along K, one line of a row): a load of a wave takes half a line of each of
 // its 16 rows.  (Quarters of the wave with 32 neighbouring bytes each, whose scales are neighbours too: 12.6 us for
 // the reads of K = 4096, N = 24576 where these take 10.1; non-temporal loads 11.2, as weights in use stay in the MALL.)

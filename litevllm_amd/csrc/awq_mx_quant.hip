@@ -8,31 +8,14 @@ namespace awq {
 
 constexpr int kQuantThreads = 256;
 
-// Eight values per lane: the four lanes of a block of 32 share its largest magnitude by two DPP steps
-// inside their quad.  One pass: what it reads and writes bounds it.
+// Eight values per lane, consecutive lanes consecutive pieces.  One pass: what it reads and writes bounds it.
 template <typename T>
-__global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t* __restrict__ codes,
+__global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
                                                                     uint8_t* __restrict__ scales, int64_t lds, int64_t pieces, uint32_t per_row) {
   const int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
-  if (i >= pieces) return;  // whole blocks: pieces % 4 == 0
-  const T* at = x + i * 8;
-  int64_t block = i >> 2;
-  if (per_row) {  // rows apart, here or there
-    const int64_t row = i / per_row;
-    at = x + row * ldx + (i - row * per_row) * 8;
-    block = row * lds + ((i - row * per_row) >> 2);
-  }
-  float v[8];
-  if constexpr (std::is_same<T, float>::value) load8<float>(at, v);
-  else load8<T>(at, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, mx_abs_bits(v[j]));
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));
-  top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
-  const uint32_t byte = mx_scale_byte(top);
-  codes[i] = byte == 255u ? 0u : mx_codes8(v, mx_scale_value(byte));
-  if ((i & 3) == 0) scales[block] = (uint8_t)byte;
+  if (i >= pieces) return;  // whole blocks of 32: pieces % 4 == 0
+  const int64_t row = per_row ? i / per_row : 0;  // 0: all one row, as the rows follow each other here and there
+  mx_quantize8<T>(x + row * ldx, codes + row * per_row * 4, scales + row * lds, i - row * per_row);
 }
 
 // Eight values per lane.  An e2m1 value has two significant bits: times the scale it is exact in fp32
@@ -78,10 +61,9 @@ int launch_mx_quantize(const void* x, int64_t ldx, uint8_t* codes, uint8_t* scal
   if (cdiv(pieces, kQuantThreads) > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)cdiv(pieces, kQuantThreads)), block(kQuantThreads);
   const uint32_t per_row = ((ldx == K && lds == K / 32) || M == 1) ? 0u : (uint32_t)(K / 8);
-  auto* o = (uint32_t*)codes;
-  if (dtype == AWQ_DTYPE_F16) mx_quantize_kernel<f16><<<grid, block, 0, st>>>((const f16*)x, ldx, o, scales, lds, pieces, per_row);
-  else if (dtype == AWQ_DTYPE_BF16) mx_quantize_kernel<bf16><<<grid, block, 0, st>>>((const bf16*)x, ldx, o, scales, lds, pieces, per_row);
-  else mx_quantize_kernel<float><<<grid, block, 0, st>>>((const float*)x, ldx, o, scales, lds, pieces, per_row);
+  if (dtype == AWQ_DTYPE_F16) mx_quantize_kernel<f16><<<grid, block, 0, st>>>((const f16*)x, ldx, codes, scales, lds, pieces, per_row);
+  else if (dtype == AWQ_DTYPE_BF16) mx_quantize_kernel<bf16><<<grid, block, 0, st>>>((const bf16*)x, ldx, codes, scales, lds, pieces, per_row);
+  else mx_quantize_kernel<float><<<grid, block, 0, st>>>((const float*)x, ldx, codes, scales, lds, pieces, per_row);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

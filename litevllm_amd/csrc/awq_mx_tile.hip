@@ -307,8 +307,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
             const f32x4 u = *(const f32x4*)(up + m * LD + cw + 16 * (j + d) + 4 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float g = acc[i][j + d][e];
-              v[4 * d + e] = (p.act == AWQ_MOE_ACT_GELU_TANH ? gated_act_fast<1>(g) : gated_act_fast<0>(g)) * u[e];
+              v[4 * d + e] = mx_gated(acc[i][j + d][e], u[e], p.act);
               top = max(top, mx_abs_bits(v[4 * d + e]));
             }
           }
