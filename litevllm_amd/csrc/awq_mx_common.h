@@ -138,7 +138,8 @@ __device__ __forceinline__ MxRows mx_rows(const MxArgs& p, int tile) {
     const int first = tile * ROWS;
     return {0, first, p.M - first < ROWS ? p.M - first : ROWS};
   } else {
-    return {p.tiles[3 * tile], p.tiles[3 * tile + 1], p.tiles[3 * tile + 2]};
+    const auto* row = (const __attribute__((address_space(4))) int*)p.tiles + 3 * tile;  // constant here: scalar loads
+    return {row[0], row[1], row[2]};
   }
 }
 // Row of a for row r of the block of a table's or a dense tile (rows past the end repeat the last: their results are dropped).

@@ -185,7 +185,8 @@ def test_quantize_refuses():
     (1, 16, 32, None), (1, 1, 64, "f32"), (1, 4096, 4096, None), (2, 333, 1056, "f16"), (5, 48, 96, None), (13, 1000, 2048, "bf16"),
     (16, 256, 12288, None), (17, 128, 512, None), (33, 517, 160, "f32"), (57, 1024, 4096, None), (64, 256, 1024, None),
     (65, 130, 2080, "f16"), (128, 512, 384, None), (200, 5001, 288, "bf16"), (300, 256, 4128, None), (513, 771, 1024, None),
-    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None), (64, 300, 4096, "f16"), (40, 5000, 12320, None), (15, 16500, 96, None), (12, 9000, 4128, "f32"), (600, 900, 2080, None)])
+    (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None), (64, 300, 4096, "f16"), (40, 5000, 12320, None), (15, 16500, 96, None), (12, 9000, 4128, "f32"), (600, 900, 2080, None),
+    (700, 24010, 96, "bf16"), (690, 24000, 544, None), (2500, 20007, 64, "f32")])
 def test_gemm(m, n, k, bias, dtype):
     from litevllm_amd import mxfp4_gemm
     dt = DTYPES[dtype]
@@ -384,7 +385,8 @@ def _experts(seed, e, i, h):
 @pytest.mark.parametrize("t,e,k,h,i,kind", [
     (1, 8, 2, 64, 32, "silu"), (1, 1, 1, 32, 32, "gelu"), (5, 8, 8, 160, 96, "silu"), (17, 4, 2, 256, 128, "gelu_pytorch_tanh"),
     (40, 64, 4, 512, 64, "silu"), (70, 3, 2, 96, 160, "silu"), (150, 2, 1, 128, 32, "silu"), (3, 5, 4, 4128, 64, "silu"), (16, 1, 8, 64, 64, "gelu"), (2, 300, 3, 96, 32, "silu"), (128, 7, 1, 64, 32, "silu"),
-    (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (1400, 3, 3, 32, 32, "silu"), (260, 5, 3, 64, 288, "gelu")])
+    (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (1400, 3, 3, 32, 32, "silu"), (260, 5, 3, 64, 288, "gelu"),
+    (600, 64, 8, 1024, 320, "silu"), (1200, 40, 8, 544, 608, "silu"), (900, 5, 8, 1056, 96, "gelu")])
 def test_moe(t, e, k, h, i, kind, dtype):
     from litevllm_amd import mxfp4_moe
     dt = DTYPES[dtype]
