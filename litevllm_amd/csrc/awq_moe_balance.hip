@@ -4,7 +4,10 @@
 //   loss = E sum_e f_e P_e,  f_e = counts_e / (n top_k),  P_e = sum over kept t of p_te / n
 //   d loss / d logits_te = p_te (F_e - sum_j F_j p_tj),  F_e = E f_e / n  (f is piecewise constant)
 // A row of nothing but -inf has no probabilities: p = 0.  No kept token: loss 0, gradient 0.
-// Both passes read the logits once; the gradient computes the softmax again instead of keeping it.
+// Both passes read the logits once; the gradient computes the softmax again instead of keeping it (65536 tokens, 160
+// experts, fp32: 42 MB; forward 10.5 us and 3.4 for the join, gradient 13.6 us, which reads and writes at 6.2 TB/s, partly
+// from the caches).  Shorter calls are latencies and the launches; with a gradient the host is slower than the kernels
+// from a call of 16384 tokens, 64 experts on down (10.5 us of kernels).
 #include <algorithm>
 
 #include "awq_launch.h"
@@ -212,7 +215,8 @@ __global__ void __launch_bounds__(256) balance_grad_kernel(const void* __restric
 namespace awq_host {
 using namespace awq;
 
-// Up to 256 rows one block does everything; else at most a block per CU, so that the join stays small.
+// Up to 256 rows one block does everything (one launch); else at most a block per CU, so that the join, whose one block
+// reads every block's sums, stays small (256 blocks of 160 experts: 3.4 us).
 static int balance_rows(int64_t T) { return T <= 256 ? 256 : (int)cdiv(T, std::min<int64_t>(256, cdiv(T, 64))); }
 static int balance_blocks(int64_t T) { return (int)std::max<int64_t>(1, cdiv(T, balance_rows(T))); }
 

@@ -63,7 +63,7 @@ __device__ __forceinline__ MxScan mx_scan(int mine, int route) {
 __device__ __forceinline__ void mx_scan_list(const MxScan& f, int lane, int* list) {
   if (f.its >> lane & 1) list[__popcll(f.its & ((1ull << lane) - 1))] = lane;
 }
-static_assert(kMxScanRoutes == 64, "a lane each");
+static_assert(kMxScanRoutes <= 64, "a lane each");
 
 // Grid x: column blocks, y: row tiles of 16 (with SCAN: routes).
 // X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one

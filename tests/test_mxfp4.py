@@ -386,7 +386,8 @@ def _experts(seed, e, i, h):
     (1, 8, 2, 64, 32, "silu"), (1, 1, 1, 32, 32, "gelu"), (5, 8, 8, 160, 96, "silu"), (17, 4, 2, 256, 128, "gelu_pytorch_tanh"),
     (40, 64, 4, 512, 64, "silu"), (70, 3, 2, 96, 160, "silu"), (150, 2, 1, 128, 32, "silu"), (3, 5, 4, 4128, 64, "silu"), (16, 1, 8, 64, 64, "gelu"), (2, 300, 3, 96, 32, "silu"), (128, 7, 1, 64, 32, "silu"),
     (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (1400, 3, 3, 32, 32, "silu"), (260, 5, 3, 64, 288, "gelu"),
-    (600, 64, 8, 1024, 320, "silu"), (1200, 40, 8, 544, 608, "silu"), (900, 5, 8, 1056, 96, "gelu")])
+    (600, 64, 8, 1024, 320, "silu"), (1200, 40, 8, 544, 608, "silu"), (900, 5, 8, 1056, 96, "gelu"),
+    (32, 1, 1, 96, 64, "silu"), (30, 1, 1, 4128, 32, "silu"), (8, 2, 4, 288, 320, "gelu"), (33, 4, 1, 64, 96, "silu"), (700, 6, 8, 64, 32, "silu")])
 def test_moe(t, e, k, h, i, kind, dtype):
     from litevllm_amd import mxfp4_moe
     dt = DTYPES[dtype]
