@@ -58,7 +58,8 @@ def moe_balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor,
     which is 1 for an even load.  ``router_logits``: fp16, bf16 or fp32 ``[T, E]`` (E up to 1024); ``topk_ids``: int32 or
     int64 ``[T, top_k]``; ids outside ``[0, E)`` count nowhere.  What a masked row holds is not read and its
     gradient is 0; without a kept token loss and gradient are 0.  A row of nothing but ``-inf`` has no
-    probabilities.  The gradient takes the counts as constants; it is not differentiable again."""
+    probabilities.  The gradient takes the counts as constants; it is not differentiable again.  As for any operation, a backward is
+    captured into a graph only while no graph recorded outside the capture over the same leaves is alive."""
     ops._require_device(router_logits, topk_ids, mask)
     ops.dtype_code(router_logits.dtype)
     if router_logits.dim() != 2 or topk_ids.dim() != 2 or topk_ids.shape[0] != router_logits.shape[0]:
