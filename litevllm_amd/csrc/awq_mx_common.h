@@ -117,10 +117,7 @@ struct MxArgs {
   const void* ids;
   int id64, routes, experts;
 };
-// Up to here few routes take two launches, which find their experts in the ids, instead of four with a table (64 experts,
-// top 8, H = 2048, I = 1024, us: 2 tokens 18.5 against 22.9, 4 29.3 and 30.3, 5 31.9 and 31.0, 8 41.6 and 36.0; 8 experts,
-// top 2, H = 4096, I = 1536: 16 tokens 29.4 and 30.7, 32 35.6 and 30.0).
-constexpr int kMxScanRoutes = 32;
+constexpr int kMxScanRoutes = 64;  // of a call without a table
 
 __device__ __forceinline__ int64_t mx_route_id(const void* ids, int id64, int64_t r) {
   return id64 ? ((const int64_t*)ids)[r] : (int64_t)((const int32_t*)ids)[r];

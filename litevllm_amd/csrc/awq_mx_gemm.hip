@@ -68,8 +68,8 @@ static_assert(kMxScanRoutes <= 64, "a lane each");
 // Grid x: column blocks, y: row tiles of 16 (with SCAN: routes).
 // X16: a is 16-bit and quantised by every block for itself, into LDS, while its weights are on their way: one
 // launch less where the rows are few and short.
-// SCAN (gate_up): no table of tiles; block y takes all the routes of route y's expert, which it finds in the ids
-// itself, if y is the first of them.  A route's place is its own number.
+// SCAN (gate_up): no table of tiles; block y takes up to 16 routes of route y's expert from y on, which it finds in
+// the ids itself, if 16, 32, .. or none of the expert's lie in front of y.  A route's place is its own number.
 template <int MODE, int NT, int WAVES, bool X16, bool SCAN>
 __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   constexpr int THREADS = WAVES * 64;
@@ -80,10 +80,12 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
   MxRows t;
   if constexpr (SCAN) {
     // every wave looks for itself, so that its weights are asked for at once
-    const MxScan f = mx_scan(mx_scan_ids(p, lane), blockIdx.y);
-    if (f.first != (int)blockIdx.y) return;
+    MxScan f = mx_scan(mx_scan_ids(p, lane), blockIdx.y);
+    const uint64_t before = (1ull << blockIdx.y) - 1;
+    if (f.first < 0 || (__popcll(f.its & before) & 15) != 0) return;
+    f.its &= ~before;
     if (wave == 0) mx_scan_list(f, lane, list);
-    t = {f.expert, 0, (int)__popcll(f.its)};
+    t = {f.expert, 0, min((int)__popcll(f.its), 16)};
   } else {
     if (MODE != kMxDense && (int)blockIdx.y >= p.tile_count[0]) return;
     t = mx_rows<MODE, 16>(p, blockIdx.y);
@@ -102,123 +104,123 @@ __global__ void __launch_bounds__(WAVES * 64) mx_rows_kernel(MxArgs p) {
     wsc[j] = p.ws + row * KB;
   }
   const int ld = p.K / 2 + 16;
-  // a scanned expert may have more routes than a tile has rows (one that occurs twice in a token)
-  for (int base = 0; base < (SCAN ? t.rows : 1); base += 16) {
-    const int rows = SCAN ? min(t.rows - base, 16) : t.rows;
-    const uint8_t *ac, *asc;
-    if constexpr (SCAN && !X16) __syncthreads();  // the list
-    if constexpr (!X16) {
-      const int64_t row = SCAN ? list[base + min(r, rows - 1)] / p.topk : mx_a_row<MODE>(p, t, r);
-      ac = p.a + row * (p.K / 2);
-      asc = p.as + row * p.as_ld;
-    }
-    f32x4 acc[NT];
-    MxPair b[NT];
+  const uint8_t *ac, *asc;
+  if constexpr (SCAN && !X16) __syncthreads();  // the list
+  if constexpr (!X16) {
+    const int64_t row = SCAN ? list[min(r, t.rows - 1)] / p.topk : mx_a_row<MODE>(p, t, r);
+    ac = p.a + row * (p.K / 2);
+    asc = p.as + row * p.as_ld;
+  }
+  f32x4 acc[NT];
+  MxPair b[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (wave < pairs) {
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (wave < pairs) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], wave, q);
-    }
-    if constexpr (X16) {
-      if constexpr (SCAN) __syncthreads();  // the list
-      const int pieces = p.K / 8;
-      for (int m = 0; m < rows; ++m) {
-        const int64_t row = SCAN ? list[base + m] / p.topk : t.first + m;
-        const uint16_t* x = p.x + row * p.ldx;
-        uint8_t *codes = xq + m * ld, *scales = xq + p.xrows * ld + m * KB;
-        for (int i = tid; i < pieces; i += THREADS) {
-          if (p.out_bf16) mx_quantize8<bf16>(x, codes, scales, i);
-          else mx_quantize8<f16>(x, codes, scales, i);
-        }
+    for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], wave, q);
+  }
+  if constexpr (X16) {
+    if constexpr (SCAN) __syncthreads();  // the list
+    const int pieces = p.K / 8;
+    for (int m = 0; m < t.rows; ++m) {
+      const int64_t row = SCAN ? list[m] / p.topk : t.first + m;
+      const uint16_t* x = p.x + row * p.ldx;
+      uint8_t *codes = xq + m * ld, *scales = xq + p.xrows * ld + m * KB;
+      for (int i = tid; i < pieces; i += THREADS) {
+        if (p.out_bf16) mx_quantize8<bf16>(x, codes, scales, i);
+        else mx_quantize8<f16>(x, codes, scales, i);
       }
-      __syncthreads();
-      const int m = min(r, rows - 1);
-      ac = xq + m * ld;
-      asc = xq + p.xrows * ld + m * KB;
     }
-    // a pair at a time: two or four under way in a wave measured the same, other waves fill in
-    for (int pair = wave; pair < pairs; pair += WAVES) {
-      if (pair != wave) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], pair, q);
-      }
-      const MxPair a = mx_load_pair(ac, asc, pair, q);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, b[j], acc[j], q);
-    }
-    if ((KB & 7) != 0 && wave == pairs % WAVES) {
-      const MxPair a = mx_load_last(ac, asc, pairs, q, KB);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, mx_load_last(wc[j], wsc[j], pairs, q, KB), acc[j], q);
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) red[wave][j][(4 * q + u) * 16 + r] = acc[j][u];
     __syncthreads();
+    const int m = min(r, t.rows - 1);
+    ac = xq + m * ld;
+    asc = xq + p.xrows * ld + m * KB;
+  }
+  // a pair at a time: two or four under way in a wave measured the same, other waves fill in (unrolled: 3 tokens through
+  // 64 experts, H = 7168, I = 2048 127 us against 115, H = 2048, I = 1024 22.7 against 23.2)
+#pragma unroll 1
+  for (int pair = wave; pair < pairs; pair += WAVES) {
+    if (pair != wave) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) b[j] = mx_load_pair(wc[j], wsc[j], pair, q);
+    }
+    const MxPair a = mx_load_pair(ac, asc, pair, q);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, b[j], acc[j], q);
+  }
+  if ((KB & 7) != 0 && wave == pairs % WAVES) {
+    const MxPair a = mx_load_last(ac, asc, pairs, q, KB);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = mx_mfma_pair(a, mx_load_last(wc[j], wsc[j], pairs, q, KB), acc[j], q);
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) red[wave][j][(4 * q + u) * 16 + r] = acc[j][u];
+  __syncthreads();
 
-    auto sum = [&](int j, int at) {
-      float v = red[0][j][at];
+  auto sum = [&](int j, int at) {
+    float v = red[0][j][at];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) v += red[w][j][at];
-      return v;
-    };
-    if constexpr (MODE == kMxGateUp) {
-      // 32 lanes hold a row's 32 columns: their largest magnitude, then the codes, two to a byte
-      static_assert(NT == 4, "32 gate and 32 up rows");
-      const int n = tid & 31;
-      for (int m = tid >> 5; m < rows; m += THREADS / 32) {
-        const int at = m * 16 + (n & 15);
-        const float v = mx_gated(sum(n >> 4, at), sum((n >> 4) + 2, at), p.act);
-        uint32_t top = mx_abs_bits(v);
+    for (int w = 1; w < WAVES; ++w) v += red[w][j][at];
+    return v;
+  };
+  if constexpr (MODE == kMxGateUp) {
+    // 32 lanes hold a row's 32 columns: their largest magnitude, then the codes, two to a byte
+    static_assert(NT == 4, "32 gate and 32 up rows");
+    const int n = tid & 31;
+    for (int m = tid >> 5; m < t.rows; m += THREADS / 32) {
+      const int at = m * 16 + (n & 15);
+      const float v = mx_gated(sum(n >> 4, at), sum((n >> 4) + 2, at), p.act);
+      uint32_t top = mx_abs_bits(v);
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        const uint32_t byte = mx_scale_byte(top);
-        const float other = __shfl_xor(v, 1);
-        const int64_t place = SCAN ? list[base + m] : t.first + m;
-        if ((n & 1) == 0) {
-          const uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v, other, mx_scale_value(byte == 255u ? 0u : byte), 0);
-          p.h[place * (p.N / 2) + (n0 + n) / 2] = byte == 255u ? (uint8_t)0 : (uint8_t)code;
-        }
-        if (n == 0) p.hs[place * (p.N / 32) + n0 / 32] = (uint8_t)byte;
+      for (int d = 1; d < 32; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      const uint32_t byte = mx_scale_byte(top);
+      const float other = __shfl_xor(v, 1);
+      const int64_t place = SCAN ? list[m] : t.first + m;
+      if ((n & 1) == 0) {
+        const uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v, other, mx_scale_value(byte == 255u ? 0u : byte), 0);
+        p.h[place * (p.N / 2) + (n0 + n) / 2] = byte == 255u ? (uint8_t)0 : (uint8_t)code;
       }
-    } else {
-      for (int i = tid; i < NT * 256; i += THREADS) {
-        const int j = i >> 8, at = i & 255, m = at >> 4, n = n0 + j * 16 + (at & 15);
-        if (m >= rows || n >= p.N) continue;
-        float v = sum(j, at);
-        if constexpr (MODE == kMxDense) {
-          v += load_bias(p.bias, p.bias_dtype, n);
-          p.c[(int64_t)(t.first + m) * p.ldc + n] = p.out_bf16 ? f2bf_bits(v) : f2h_bits(v);
-        } else {
-          p.y[(int64_t)p.order[t.first + m] * p.N + n] = v;
-        }
+      if (n == 0) p.hs[place * (p.N / 32) + n0 / 32] = (uint8_t)byte;
+    }
+  } else {
+    for (int i = tid; i < NT * 256; i += THREADS) {
+      const int j = i >> 8, at = i & 255, m = at >> 4, n = n0 + j * 16 + (at & 15);
+      if (m >= t.rows || n >= p.N) continue;
+      float v = sum(j, at);
+      if constexpr (MODE == kMxDense) {
+        v += load_bias(p.bias, p.bias_dtype, n);
+        p.c[(int64_t)(t.first + m) * p.ldc + n] = p.out_bf16 ? f2bf_bits(v) : f2h_bits(v);
+      } else {
+        p.y[(int64_t)p.order[t.first + m] * p.N + n] = v;
       }
     }
-    if constexpr (SCAN) __syncthreads();
   }
 }
 
 // The down product of at most kMxScanRoutes routes with the weighted sum over each token's slots, in one launch: a
-// block has 16 columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
+// block has COLS columns of all experts, its waves an expert at a time, and the routes' sums meet in LDS.  A route's
 // place is its own number.
+// COLS = 8: rows 8 .. 15 of both operands of an MFMA are rows 0 .. 7 again, half of K on, so that a wave still loads 16 half
+// lines at once; two of the four quadrants of the product count, and are added up.
 constexpr int kDownWaves = 16;
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs p, const void* weights, int w_dtype,
                                                                           uint16_t* out, int64_t ldo) {
-  constexpr int THREADS = kDownWaves * 64, COLS = 16, U = 4;
+  constexpr int THREADS = kDownWaves * 64, U = 2 /* pairs under way; four do not fit the registers */, PARTS = 16 / COLS;
   __shared__ float y[kMxScanRoutes][COLS];
   __shared__ int slot[kDownWaves][kMxScanRoutes], has[kMxScanRoutes];
   __shared__ float weight[kMxScanRoutes];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane % COLS, q = lane >> 4;
   if (tid < p.routes) {
     const int64_t e = mx_route_id(p.ids, p.id64, tid);
     has[tid] = e >= 0 && e < p.experts;
     weight[tid] = mx_route_weight(weights, w_dtype, tid);
   }
-  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, pairs = KB / 8;
+  // a lane's part of K: pairs `from` .. `from` + share - 1; what is left behind the parts is part 0's
+  const int n0 = (int)blockIdx.x * COLS, KB = p.K / 32, share = KB / 8 / PARTS, part = (lane & 15) / COLS, from = part * share;
   const int expert = mx_scan_ids(p, lane);
   for (int k = wave; k < p.routes; k += kDownWaves) {
     const MxScan f = mx_scan(expert, k);
@@ -226,27 +228,34 @@ __global__ void __launch_bounds__(kDownWaves * 64) mx_down_combine_kernel(MxArgs
     mx_scan_list(f, lane, slot[wave]);
     __builtin_amdgcn_wave_barrier();
     const int64_t row = (int64_t)f.expert * p.wrows + min(n0 + r, p.N - 1);
-    const uint8_t *wc = p.w + row * (p.K / 2), *wsc = p.ws + row * KB;
+    const uint8_t *wc = p.w + row * (p.K / 2) + from * 128, *wsc = p.ws + row * KB + from * 8;
     const int n = (int)__popcll(f.its);
-    for (int at = 0; at < n; at += 16) {
+    for (int at = 0; at < n; at += COLS) {
       const int mine = slot[wave][min(at + r, n - 1)];
-      const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2), *asc = p.as + (int64_t)mine * p.as_ld;
+      const uint8_t *ac = p.a + (int64_t)mine * (p.K / 2) + from * 128, *asc = p.as + (int64_t)mine * p.as_ld + from * 8;
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
       // the operands swapped: a lane holds four columns of the route in lane r
-      for (int first = 0; first < pairs; first += U) {
+      for (int first = 0; first < share; first += U) {
         MxPair a[U], b[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (first + u < pairs) b[u] = mx_load_pair(wc, wsc, first + u, q);
+          if (first + u < share) b[u] = mx_load_pair(wc, wsc, first + u, q);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (first + u < pairs) a[u] = mx_load_pair(ac, asc, first + u, q);
+          if (first + u < share) a[u] = mx_load_pair(ac, asc, first + u, q);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (first + u < pairs) acc = mx_mfma_pair(b[u], a[u], acc, q);
+          if (first + u < share) acc = mx_mfma_pair(b[u], a[u], acc, q);
       }
-      if ((KB & 7) != 0) acc = mx_mfma_pair(mx_load_last(wc, wsc, pairs, q, KB), mx_load_last(ac, asc, pairs, q, KB), acc, q);
-      if (at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
+      for (int pair = PARTS * share; 8 * pair < KB; ++pair) {
+        const int end = part == 0 ? KB : 0;
+        acc = mx_mfma_pair(mx_load_last(wc, wsc, pair, q, end), mx_load_last(ac, asc, pair, q, end), acc, q);
+      }
+      if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] += __shfl(acc[u], (lane + 40) & 63);
+      }
+      if (lane < COLS * 4 && part == 0 && at + r < n) *(f32x4*)&y[mine][4 * q] = acc;
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -307,9 +316,14 @@ int launch_mx_scan_gate_up(const MxArgs& p, hipStream_t st) {
 }
 
 int launch_mx_down_combine(const MxArgs& p, const void* weights, int w_dtype, void* out, int64_t ldo, hipStream_t st) {
-  const dim3 grid((unsigned)cdiv(p.N, 16)), block(kDownWaves * 64);
-  if (p.out_bf16) mx_down_combine_kernel<bf16><<<grid, block, 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
-  else mx_down_combine_kernel<f16><<<grid, block, 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  auto go = [&](auto kernel, int cols) {
+    kernel<<<dim3((unsigned)cdiv(p.N, cols)), dim3(kDownWaves * 64), 0, st>>>(p, weights, w_dtype, (uint16_t*)out, ldo);
+  };
+  // 8 columns where that gives a block per CU at most (N = 2048: the whole call 23.1 us against 26.9 for 4 tokens through 64
+  // experts, I = 1024; N = 2880 41.0 against 38.1)
+  const bool narrow = p.N <= 8 * 256;
+  if (p.out_bf16) narrow ? go(mx_down_combine_kernel<bf16, 8>, 8) : go(mx_down_combine_kernel<bf16, 16>, 16);
+  else narrow ? go(mx_down_combine_kernel<f16, 8>, 8) : go(mx_down_combine_kernel<f16, 16>, 16);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 

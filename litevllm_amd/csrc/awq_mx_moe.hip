@@ -187,12 +187,22 @@ MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk
   return w;
 }
 
+// Few routes take two launches, which find their experts in the ids, instead of four with a table: 5 to 7 us less, against
+// slower streams (every block quantises its tokens, a wave of down has an expert to itself).  So it is for few routes an
+// expert and, if each route had an expert of its own, up to 320 MiB of weights.  us with two launches and with four, R routes to
+// E experts, H, I: R = 8, E = 64, 2048, 1024 11.3, 17.6; 32 23.0, 30.1; 64 32.3, 34.4; R = 16, E = 16, 2048, 5632 36.6, 43.0, 32
+// 59.1, 57.4; R = 16, E = 32, 2880, 2880 37.9, 40.7, 32 64.5, 59.5; R = 32, E = 32, 4096, 1536 54.4, 56.3, 64 70.4, 68.8;
+// R = 32, E = 256, 7168, 2048 149, 141; R = 16, E = 8, 4096, 1536 28.6, 29.8, 24 31.5, 29.8.
+static bool mx_scans(int64_t R, int64_t H, int64_t I, int E) {
+  return R <= kMxScanRoutes && R <= 2 * (int64_t)E && R * (3 * H * I / 32 * 17) <= (int64_t)320 << 20;
+}
+
 int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   const int64_t R = c.T * c.topk;
   if (R > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
   const MxMoeWorkspace w = mx_moe_workspace(c.T, c.H, c.I, c.E, c.topk);
   char* ws = (char*)c.workspace;
-  if (R <= kMxScanRoutes) {
+  if (mx_scans(R, c.H, c.I, c.E)) {
     // two launches: gate_up, which finds its routes and quantises its tokens itself, and down with the weighted sum
     MxArgs g{};
     if (c.H <= 4096) {

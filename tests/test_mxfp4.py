@@ -387,7 +387,8 @@ def _experts(seed, e, i, h):
     (40, 64, 4, 512, 64, "silu"), (70, 3, 2, 96, 160, "silu"), (150, 2, 1, 128, 32, "silu"), (3, 5, 4, 4128, 64, "silu"), (16, 1, 8, 64, 64, "gelu"), (2, 300, 3, 96, 32, "silu"), (128, 7, 1, 64, 32, "silu"),
     (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (1400, 3, 3, 32, 32, "silu"), (260, 5, 3, 64, 288, "gelu"),
     (600, 64, 8, 1024, 320, "silu"), (1200, 40, 8, 544, 608, "silu"), (900, 5, 8, 1056, 96, "gelu"),
-    (32, 1, 1, 96, 64, "silu"), (30, 1, 1, 4128, 32, "silu"), (8, 2, 4, 288, 320, "gelu"), (33, 4, 1, 64, 96, "silu"), (700, 6, 8, 64, 32, "silu")])
+    (32, 1, 1, 96, 64, "silu"), (30, 1, 1, 4128, 32, "silu"), (8, 2, 4, 288, 320, "gelu"), (33, 4, 1, 64, 96, "silu"), (700, 6, 8, 64, 32, "silu"),
+    (8, 64, 8, 2048, 544, "silu"), (5, 33, 11, 2112, 96, "gelu"), (9, 20, 4, 1056, 1824, "silu"), (40, 16, 11, 96, 64, "silu")])
 def test_moe(t, e, k, h, i, kind, dtype):
     from litevllm_amd import mxfp4_moe
     dt = DTYPES[dtype]
@@ -425,6 +426,24 @@ def test_moe_ids_without_an_expert_an_expert_twice_and_an_idle_token():
     assert torch.equal(torch.nan_to_num(room[1:7, 2:130]), torch.nan_to_num(want))
     room[1:7, 2:130] = -7.0
     assert bool((room == -7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,i", [(40, 64, 1, 96, 64), (20, 40, 3, 4128, 32), (7, 50, 9, 2080, 96), (300, 12, 2, 64, 64), (64, 32, 1, 288, 544)])
+def test_moe_all_routes_to_one_expert_and_none_to_any(t, e, k, h, i):
+    from litevllm_amd import mxfp4_moe
+    gu, dn, w1, w2 = _experts(61, e, i, h)
+    x = _made(62, t, h, dtype=torch.bfloat16).cuda()
+    weights = torch.rand(t, k, generator=torch.Generator().manual_seed(63)).cuda()
+    ids = torch.full((t, k), e - 2, dtype=torch.int32, device="cuda")
+    y = mxfp4_moe(x, weights, ids, gu, dn)
+    ref, off = R.moe(x, weights, ids, w1, w2, "silu")
+    _close(y, ref, off, torch.bfloat16)
+    assert torch.equal(y, mxfp4_moe(x, weights, ids.long(), gu, dn))
+    for none in (-1, e):
+        out = torch.full_like(x, 7.0)
+        mxfp4_moe(x, weights, torch.full_like(ids, none), gu, dn, out=out)
+        assert not bool(out.any())
 
 
 @pytest.mark.gpu
