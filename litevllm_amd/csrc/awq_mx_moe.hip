@@ -161,9 +161,9 @@ namespace awq_host {
 using namespace awq;
 
 // Rows of a row tile by what an expert gets on average, so that its weights are read about once.  64 experts, H = 2048,
-// I = 1024, us: 2 routes an expert 43 with 16 rows, 44 with 64, 4 49 and 47, 8 52 and 47; 64 70 with 64 rows, 71 with 128,
-// 100 103 and 89, 175 153 and 140, 256 211 and 179 (32 experts, H = 4096, I = 1536: 128 172 and 161).
-static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)2 * E ? 16 : (R <= (int64_t)64 * E ? 64 : 128); }
+// I = 1024, us: 2 routes an expert 41.9 with 16 rows, 42.7 with 64, 3 45.6 and 44.3, 8 51.9 and 46.4; 48 63 with 64 rows,
+// 64 with 128, 56 64 and 66, 64 74 and 71, 88 92 and 81 (32 experts, H = 4096, I = 1536: 45 94 and 99, 52 105 and 102).
+static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)2 * E ? 16 : (R <= (int64_t)56 * E ? 64 : 128); }
 
 // Bytes between rows of the tokens' scales: whole words, which the gathering kernel counts on.
 static int64_t scale_stride(int64_t K) { return cdiv(K / 32, 4) * 4; }

@@ -30,17 +30,20 @@ class _BalanceLoss(torch.autograd.Function):
         loss, counts, buf = _forward(logits, ids, mask, experts)
         ctx.save_for_backward(logits, mask, buf)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)  # no zeros in place of the counts' gradient
+        ctx.layout = (logits.stride(0) if logits.shape[0] > 1 else experts, ops.dtype_code(logits.dtype))
         return loss, counts
 
     @staticmethod
     def backward(ctx, upstream, _):
+        if upstream is None:
+            return None, None, None, None
         logits, mask, buf = ctx.saved_tensors
+        ld, dt = ctx.layout
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         t, experts = logits.shape
-        grad = torch.empty((t, experts), dtype=logits.dtype, device=logits.device)
-        if t:
-            upstream = upstream.contiguous()
-            _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
-                  ops.dtype_code(logits.dtype), ops._ptr(mask), buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
+        _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), ld, dt, None if mask is None else mask.data_ptr(),
+              buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
             grad = torch._C._functions.DelayedError(b"moe_balance_loss is not differentiable twice", 1)(grad.requires_grad_())
         return grad, None, None, None
