@@ -450,18 +450,18 @@ static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
 
 // Tiles of 256 x 256 run in rounds of one a CU, those of 128 x 128 two a CU; K = 4096, us with one and the other:
 // M = 2048, N = 24576 112, 148; M = 3000, N = 5000 39, 48; M = 2048, N = 6144 36.5, 37.7; M = 1000, N = 24576 72, 77;
-// M = 700, N = 24576 68, 59; M = 2048, N = 4096 36, 27: about 38 a round against 26 for 512 tiles.  Fewer than 192 of these:
-// tiles of 64 x 64 (M = 512, N = 4096 12.4 against 15.7; M = 1024 20.2 against 16.9).  Up to a tile per CU of these
-// K goes in shares: two from 4 stages on, four from 24 on (M = 64, N = 4096, us with 1, 2, 4: K = 512 4.0, 4.1, 5.5;
-// K = 1024 4.7, 4.5, 5.6; K = 4096 9.0, 7.3, 7.7; K = 6144 11.9, 9.1, 9.1; K = 12288 20.9, 15.2, 14.8; with 316 tiles,
-// M = 200, N = 5001, K = 4128 13.2, 13.6, 19.9).
+// M = 700, N = 24576 68, 59; M = 2048, N = 4096 36, 27: about 38 a round against 26 for 512 tiles.  Fewer than 160 of these:
+// tiles of 64 x 64 (M = 500, N = 4096 12.2 against 14.2; 640 16.1 and 14.4; 1000 19.3 and 16.9).  Up to a tile per CU of
+// these K goes in shares: two from 4 stages on, four from 24 on (M = 64, N = 4096, us with 1, 2, 4: K = 512 4.0, 4.1, 5.5;
+// K = 1024 4.7, 4.5, 5.6; K = 4096 9.0, 7.3, 7.7; K = 6144 11.9, 9.1, 9.1; K = 12288 20.9, 15.2, 14.8); up to two a CU two
+// from 20 on (M = 300: K = 2048 7.6, 7.7, K = 4128 12.1, 12.6, K = 8192 18.0, 16.7).
 int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
   const int64_t big = cdiv(p.M, 256) * cdiv(p.N, 256), mid = cdiv(p.M, 128) * cdiv(p.N, 128);
   if (512 * 38 * cdiv(big, 256) <= 26 * std::max<int64_t>(512, mid)) return launch_tile<kMxDense, 256, 256, 2, 4, 2>(p, cdiv(p.M, 256), st);
-  if (mid >= 192) return launch_tile<kMxDense, 128, 128, 2, 4, 4>(p, cdiv(p.M, 128), st);
+  if (mid >= 160) return launch_tile<kMxDense, 128, 128, 2, 4, 4>(p, cdiv(p.M, 128), st);
   const int64_t rows = cdiv(p.M, 64), tiles = rows * cdiv(p.N, 64), stages = cdiv(p.K, 256);
   if (tiles <= 256 && stages >= 24) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 4>(p, rows, st);
-  if (tiles <= 256 && stages >= 4) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2>(p, rows, st);
+  if (tiles <= 256 ? stages >= 4 : tiles <= 512 && stages >= 20) return launch_tile<kMxDense, 64, 64, 2, 2, 4, 2>(p, rows, st);
   return launch_tile<kMxDense, 64, 64, 2, 2, 4>(p, rows, st);
 }
 
