@@ -60,6 +60,13 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x, ld
 
 
+def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the addresses from first to last of two tensors (not empty) overlap."""
+    (x0, x1), (y0, y1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+                          for t in (x, y))
+    return x0 < y1 and y0 < x1
+
+
 def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` of ``x [..., K]`` (fp16, bf16 or fp32; K a multiple of 32).
 
@@ -126,7 +133,7 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
         raise ValueError(f"bad_output: out must be {dtype}, got {out.dtype}")
     else:
         ops.check_out(out, m, n, out)
-        if a_scales is None and m and a.untyped_storage().data_ptr() == out.untyped_storage().data_ptr():
+        if a_scales is None and m and n and _meet(a, out):
             # few rows are read by every block, also while others write: a, which out may lie over, first
             a, a_scales = mxfp4_quantize(a)
     if m == 0 or n == 0:

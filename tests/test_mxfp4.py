@@ -274,6 +274,20 @@ def test_gemm_over_its_own_input_and_beside_it(m):
 
 
 @pytest.mark.gpu
+def test_gemm_over_a_part_of_its_input_held_by_another_tensor():
+    from litevllm_amd import mxfp4_gemm, mxfp4_quantize
+    g = torch.Generator().manual_seed(13)
+    w, ws = mxfp4_quantize(torch.randn(1024, 1024, generator=g).cuda())
+    x = torch.randn(5, 1024, generator=g).to(torch.bfloat16).cuda()
+    want = mxfp4_gemm(x[1:], w, ws)
+    for _ in range(4):
+        buf = x.clone()
+        out = torch.from_dlpack(buf[:4])
+        mxfp4_gemm(buf[1:], w, ws, out=out)
+        assert torch.equal(buf[:4], want) and torch.equal(buf[4], x[4])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [1, 8, 60])
 def test_moe_over_its_own_input(t):
     from litevllm_amd import MXFP4Experts, mxfp4_moe, mxfp4_quantize
