@@ -141,7 +141,7 @@ int launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out,
 // expert, the tile table, the sort's ranks and counts (of order_blocks > 1 blocks), the quantised tokens, the
 // quantised intermediate and the per-route fp32 rows.
 struct MxMoeWorkspace {
-  int64_t order, tiles, rank, hist, x, xs, h, hs, y, total, max_tiles, order_blocks;
+  int64_t order, tiles, rank, hist, x, xs, h, hs, y, total, max_tiles, order_blocks, order_per;
 };
 MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk);
 struct MxMoeCall {

@@ -14,7 +14,8 @@ constexpr int kOrderThreads = 1024, kOneBlockRoutes = 6144;
 // computed by itself and summed by its route.  Routes without an expert get no place.
 //
 // Up to kOneBlockRoutes routes block 0 does it alone.  More: its LDS atomics, on few addresses, would take longer than
-// the rest (16384 routes to 64 experts: 19 us), so blocks of kOrderThreads routes count and rank theirs, and a second
+// the rest (16384 routes to 64 experts: 19 us), so at most 256 blocks of kOrderThreads routes, or of several times as many,
+// count and rank theirs, and a second
 // launch adds up the counts (6 us for both; the whole call with one block and with several: 4096 routes 70 and 78 us, 5600
 // 89 and 91, 8192 126 and 123).
 struct MxOrder {
@@ -22,6 +23,7 @@ struct MxOrder {
   int id64, R, E, rows;
   int *order, *tiles, *tile_count;
   int blocks;         // of routes; 1: block 0 does everything
+  int64_t per;        // routes of a block, a multiple of kOrderThreads
   int *rank, *hist;   // rank[route] in its block and expert; hist[blocks][E]
 };
 
@@ -65,9 +67,11 @@ __global__ void __launch_bounds__(kOrderThreads) mx_prepare_kernel(MxOrder o, co
   count[t] = 0;
   __syncthreads();
   if (o.blocks > 1) {
-    const int64_t r = (int64_t)blockIdx.x * kOrderThreads + t;
-    const int64_t e = r < o.R ? mx_route_id(o.ids, o.id64, r) : -1;
-    if (e >= 0 && e < o.E) o.rank[r] = atomicAdd(&count[e], 1);
+    const int64_t start = (int64_t)blockIdx.x * o.per, end = min(start + o.per, (int64_t)o.R);
+    for (int64_t r = start + t; r < end; r += kOrderThreads) {
+      const int64_t e = mx_route_id(o.ids, o.id64, r);
+      if (e >= 0 && e < o.E) o.rank[r] = atomicAdd(&count[e], 1);
+    }
     __syncthreads();
     if (t < o.E) o.hist[(int64_t)blockIdx.x * o.E + t] = count[t];
     return;
@@ -108,9 +112,11 @@ __global__ void __launch_bounds__(kOrderThreads) mx_place_kernel(MxOrder o) {
   }
   base[t] = mx_first_place(o, total, blockIdx.x == 0) + before;
   __syncthreads();
-  const int64_t r = (int64_t)blockIdx.x * kOrderThreads + t;
-  const int64_t e = r < o.R ? mx_route_id(o.ids, o.id64, r) : -1;
-  if (e >= 0 && e < o.E) o.order[base[e] + o.rank[r]] = (int)r;
+  const int64_t start = (int64_t)blockIdx.x * o.per, end = min(start + o.per, (int64_t)o.R);
+  for (int64_t r = start + t; r < end; r += kOrderThreads) {
+    const int64_t e = mx_route_id(o.ids, o.id64, r);
+    if (e >= 0 && e < o.E) o.order[base[e] + o.rank[r]] = (int)r;
+  }
 }
 
 // out[t] = the sum over a token's slots, in slot order, of weight * y: fp32, one rounding.  A slot
@@ -175,7 +181,8 @@ MxMoeWorkspace mx_moe_workspace(int64_t T, int64_t H, int64_t I, int E, int topk
   w.max_tiles = R / mx_moe_rows(R, E) + std::min<int64_t>(R, E);
   w.order = 256;  // the tile count sits in front
   w.tiles = al(w.order + R * 4);
-  w.order_blocks = R <= kOneBlockRoutes ? 1 : cdiv(R, kOrderThreads);
+  w.order_per = cdiv(R, (int64_t)256 * kOrderThreads) * kOrderThreads;
+  w.order_blocks = R <= kOneBlockRoutes ? 1 : cdiv(R, w.order_per);
   w.rank = al(w.tiles + w.max_tiles * 12);
   w.hist = al(w.rank + (w.order_blocks > 1 ? R * 4 : 0));
   w.x = al(w.hist + (w.order_blocks > 1 ? w.order_blocks * E * 4 : 0));
@@ -230,7 +237,7 @@ int launch_mx_moe(const MxMoeCall& c, hipStream_t st) {
   const int rows = mx_moe_rows(R, c.E);
   const int64_t pieces = c.T * (c.H / 8);
   if (cdiv(pieces, kOrderThreads) + w.order_blocks > 0x7FFFFFFFLL) return AWQ_ERR_UNSUPPORTED;
-  MxOrder o{c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws, (int)w.order_blocks, (int*)(ws + w.rank), (int*)(ws + w.hist)};
+  MxOrder o{c.ids, c.id64, (int)R, c.E, rows, order, tiles, (int*)ws, (int)w.order_blocks, w.order_per, (int*)(ws + w.rank), (int*)(ws + w.hist)};
   auto prepare = [&](auto kernel) {
     kernel<<<dim3((unsigned)(w.order_blocks + cdiv(pieces, kOrderThreads))), dim3(kOrderThreads), 0, st>>>(
         o, (const uint16_t*)c.x, c.T > 1 ? c.ldx : c.H, pieces, (int)(c.H / 8), (uint8_t*)(ws + w.x), (uint8_t*)(ws + w.xs),

@@ -403,7 +403,8 @@ def _experts(seed, e, i, h):
     (43, 1000, 3, 64, 32, "silu"), (6, 9, 3, 4096, 288, "silu"), (2, 4, 2, 4224, 32, "gelu"), (1400, 3, 3, 32, 32, "silu"), (260, 5, 3, 64, 288, "gelu"),
     (600, 64, 8, 1024, 320, "silu"), (1200, 40, 8, 544, 608, "silu"), (900, 5, 8, 1056, 96, "gelu"),
     (32, 1, 1, 96, 64, "silu"), (30, 1, 1, 4128, 32, "silu"), (8, 2, 4, 288, 320, "gelu"), (33, 4, 1, 64, 96, "silu"), (700, 6, 8, 64, 32, "silu"),
-    (8, 64, 8, 2048, 544, "silu"), (5, 33, 11, 2112, 96, "gelu"), (9, 20, 4, 1056, 1824, "silu"), (40, 16, 11, 96, 64, "silu")])
+    (8, 64, 8, 2048, 544, "silu"), (5, 33, 11, 2112, 96, "gelu"), (9, 20, 4, 1056, 1824, "silu"), (40, 16, 11, 96, 64, "silu"),
+    (70000, 20, 4, 64, 32, "silu")])
 def test_moe(t, e, k, h, i, kind, dtype):
     from litevllm_amd import mxfp4_moe
     dt = DTYPES[dtype]
