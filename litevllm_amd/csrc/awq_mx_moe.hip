@@ -167,9 +167,10 @@ namespace awq_host {
 using namespace awq;
 
 // Rows of a row tile by what an expert gets on average, so that its weights are read about once.  64 experts, H = 2048,
-// I = 1024, us: 2 routes an expert 41.9 with 16 rows, 42.7 with 64, 3 45.6 and 44.3, 8 51.9 and 46.4; 48 63 with 64 rows,
-// 64 with 128, 56 64 and 66, 64 74 and 71, 88 92 and 81 (32 experts, H = 4096, I = 1536: 45 94 and 99, 52 105 and 102).
-static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)2 * E ? 16 : (R <= (int64_t)56 * E ? 64 : 128); }
+// I = 1024, us: 2 routes an expert 42.9 with 16 rows, 42.7 with 64, 3 46.7 and 44.2, 4 47.8 and 45.2 (128 experts, H = 4096,
+// I = 1536: 1 156 and 162); 32 52.8 with 64 rows, 54.2 with 128, 37 54.6 and 55.4, 44 60.8 and 57.8, 62 74 and 63 (32 experts,
+// H = 4096, I = 1536: 32 88.6 and 89.0, 45 92.8 and 91.5, 62 124 and 102).
+static int mx_moe_rows(int64_t R, int E) { return R <= (int64_t)2 * E ? 16 : (R <= (int64_t)40 * E ? 64 : 128); }
 
 // Bytes between rows of the tokens' scales: whole words, which the gathering kernel counts on.
 static int64_t scale_stride(int64_t K) { return cdiv(K / 32, 4) * 4; }

@@ -56,7 +56,7 @@ __device__ __forceinline__ void swap_rows(u32x4& x, u32x4& y, bool low) {
 // wave holds the fragments of a half while it reads the next half's, so the buffer of a stage is free after its first
 // half: one barrier a stage, the loads under way for a whole stage's time.  A tile's first two stages are loaded while
 // the results of the tile before go out, which takes no LDS (M = 4096, N = 24576, K = 4096: 228 us with blocks of one tile
-// whose results go through LDS, 221 so; K = 1024 90 and 82; 100 to 1024 tokens through 64 experts 9 to 13 in 100 less).
+// whose results go through LDS, 221 so; K = 1024 90 and 82; 100 tokens through 64 experts 53 and 48).
 //
 // What bounds it (M = 4096, N = 24576, K = 4096, 221 us, 3.7 PFLOP/s): its products alone take 143, its LDS reads 98, its
 // loads 128, products and reads 168, all but the stores 204, scales that need not be read 212.
@@ -80,8 +80,11 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   static_assert(TN == 2 || TN == 4, "");
   extern __shared__ __align__(16) uint8_t lds[];  // codes [2][ROWS][128], scales [2][ROWS][16], zeros
 
-  // blocks go to the 8 XCDs in turn: each takes a run of tiles, in groups of 8 row tiles, column by column, so
-  // that the tiles it runs at once share rows of a and of w in its L2
+  // Blocks go to the 8 XCDs in turn: each takes a run of tiles, in groups of 8 row tiles, column by column, so
+  // that the tiles it runs at once share rows of a and of w in its L2.  Row tiles of a table share rows of w only where an
+  // expert has several: they run one after another (64 experts, 500 tokens 65.8 us against 70.1 in groups of 8, 2048 170
+  // against 176; 32 experts, H = 4096 391 and 401).
+  constexpr int GROUP = MODE == kMxDense ? 8 : 1;
   if (MODE != kMxDense) row_tiles = p.tile_count[0];
   const int tiles = row_tiles * col_tiles, per = (tiles + 7) / 8;
   const int first_id = ((int)blockIdx.x & 7) * per, ids = min(per, tiles - first_id);
@@ -110,9 +113,9 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   constexpr int PLACES = MODE == kMxDown ? 2 * TM : 1;
   int place[PLACES] = {};  // kMxDown: rows of y of this lane's stores
   auto set_tile = [&](int id) {
-    const int group = id / (8 * col_tiles), in_group = id - group * 8 * col_tiles;
-    const int group_rows = min(8, row_tiles - 8 * group);
-    t = mx_rows<MODE, BM>(p, 8 * group + in_group % group_rows);
+    const int group = id / (GROUP * col_tiles), in_group = id - group * GROUP * col_tiles;
+    const int group_rows = min(GROUP, row_tiles - GROUP * group);
+    t = mx_rows<MODE, BM>(p, GROUP * group + in_group % group_rows);
     n0 = in_group / group_rows * COLS;
     const int64_t a_base = MODE == kMxGateUp ? 0 : t.first, w_base = (int64_t)t.expert * p.wrows + n0;
     const int last = p.N - 1 - n0;
@@ -441,9 +444,9 @@ static int launch_tile(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
     (void)hipGetLastError();
     return AWQ_ERR_LAUNCH;
   }
-  // As many blocks as run at once, each with several tiles, or (grouped 128 x 128: tiles of differing work, better dealt
-  // out one by one: 2048 tokens through 64 experts 176 us against 184; 4096 through 32, H = 4096 402 against 428) one each.
-  constexpr int64_t AT_ONCE = WK > 1 || (MODE != kMxDense && BM == 128) ? 0x7FFFFFFF : 256 * (4 * PER_SIMD / (WM * WN));
+  // As many blocks as run at once, each with several tiles (a tile each: 500 tokens through 64 experts 66.7 us against 63.2,
+  // 100 49.4 and 47.1, 2048 170.5 and 169.5; 4096 through 32, H = 4096 391 and 397).
+  constexpr int64_t AT_ONCE = WK > 1 ? 0x7FFFFFFF : 256 * (4 * PER_SIMD / (WM * WN));
   kernel<<<dim3((unsigned)std::min(cdiv(row_tiles * col_tiles, 8) * 8, AT_ONCE)), dim3(WM * WN * WK * 64), lds, st>>>(p, (int)row_tiles, (int)col_tiles);
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
@@ -465,9 +468,9 @@ int launch_mx_tile_gemm(const MxArgs& p, hipStream_t st) {
   return launch_tile<kMxDense, 64, 64, 2, 2, 4>(p, rows, st);
 }
 
-// Waves of 16 or 32 rows x 64 columns (64 x 128 tiles, us with them and with 4 waves: 20 tokens through 64 experts 43.5, 44.9; 64 46.4, 47.5;
-// 200 51.6, 51.3; 500 72.6, 77.3), but for down's 128 x 128 64 x 64, fewer LDS reads a product: 2048 tokens 175.6 against
-// 178.1, of gate_up 180.7.
+// Waves of 16 or 32 rows x 64 columns (64 x 128 tiles, us with them and with 4 waves: 20 tokens through 64 experts 43.5, 44.9;
+// 64 46.4, 47.5; 200 51.6, 51.3), but for down's 128 x 128 64 x 64, fewer LDS reads a product: 2048 tokens 170.5 against
+// 172.5, with gate_up's so, too, 170.8, 1024 118.7 against 113.3.
 int launch_mx_tile_grouped(const MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st) {
   if (rows == 128)
     return gate_up ? launch_tile<kMxGateUp, 128, 128, 4, 2, 4>(p, row_tiles, st) : launch_tile<kMxDown, 128, 128, 2, 2, 2>(p, row_tiles, st);
