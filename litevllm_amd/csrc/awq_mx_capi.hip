@@ -90,7 +90,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   p.bias = bias;
   p.bias_dtype = bias_dtype;
   p.out_bf16 = act_dtype == AWQ_DTYPE_BF16;
-  return M <= kMxRowsMax ? launch_mx_rows_gemm(p, (hipStream_t)stream) : launch_mx_tile_gemm(p, (hipStream_t)stream);
+  return mx_takes_rows(M, N, K) ? launch_mx_rows_gemm(p, (hipStream_t)stream) : launch_mx_tile_gemm(p, (hipStream_t)stream);
 }
 
 size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k) {

@@ -156,7 +156,7 @@ namespace awq_host {
 int launch_mx_tile_gemm(const awq::MxArgs& p, hipStream_t st);
 int launch_mx_rows_gemm(const awq::MxArgs& p, hipStream_t st);
 bool mx_quantizes_itself(int64_t M, int64_t K);  // whether launch_mx_rows_gemm takes a in 16 bits (p.x)
-constexpr int64_t kMxRowsMax = 16;               // rows that launch_mx_rows_gemm takes
+bool mx_takes_rows(int64_t M, int64_t N, int64_t K);  // whether launch_mx_rows_gemm is the kernel of the size
 // gate_up or down product of the grouped routes in `row_tiles` (at most) row tiles of `rows` rows
 int launch_mx_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);
 int launch_mx_tile_grouped(const awq::MxArgs& p, bool gate_up, int rows, int64_t row_tiles, hipStream_t st);

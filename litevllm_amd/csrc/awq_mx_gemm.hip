@@ -287,18 +287,25 @@ static int launch_rows(const MxArgs& p, int64_t row_tiles, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
 
+// Up to 16 rows, and more, in row tiles that each read the weights, while these give a block per CU at most, or two for
+// short K (us with these kernels and with tiles: M = 20, N = 512, K = 2048 3.3, 5.2; M = 32, N = 2048, K = 4096 5.0, 7.1;
+// M = 64, N = 1024, K = 4096 4.9, 7.2; two: M = 64, N = 2048, K = 2048 4.5, 5.4, K = 4096 7.5, 7.2; M = 32, N = 4096, K = 2048
+// 4.5, 5.3, K = 4096 7.6, 7.2; more: M = 64, N = 4096, K = 2048 7.0, 5.4).
+bool mx_takes_rows(int64_t M, int64_t N, int64_t K) { return M <= 16 || cdiv(M, 16) * cdiv(N, 16) <= (K <= 2048 ? 512 : 256); }
+
 // Up to here every block quantises a's rows for itself (M = 8, K = 4096, N = 24576: 17.2 us against 13.4 and 1.6 for a
 // launch of its own; M = 2 12.4 against 12.0 and 1.6).
-bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= kMxRowsMax && M * K <= 16384; }
+bool mx_quantizes_itself(int64_t M, int64_t K) { return M <= 16 && M * K <= 16384; }
 
 // 16 columns a block where that gives a block per CU at most, else 32 (K = 4096, us, 16 and 32 columns: N = 4096, M = 1
 // 4.0, 5.2, M = 16 4.8, 6.4; N = 6144 5.7, 5.3 and 7.9, 6.5; N = 24576 12.0, 11.9 and 18.4, 14.9); 16 waves where a CU has
 // one block (K = 12288, N = 4096: 4 waves 10.1, 8 8.1, 16 7.7).
 template <bool X16>
 static int launch_rows_dense(const MxArgs& p, hipStream_t st) {
-  if (p.N <= 16 * 256) return launch_rows<kMxDense, 1, 16, X16, false>(p, 1, st);
-  if (p.N <= 32 * 256) return launch_rows<kMxDense, 2, 16, X16, false>(p, 1, st);
-  return launch_rows<kMxDense, 2, 8, X16, false>(p, 1, st);
+  const int64_t tiles = cdiv(p.M, 16);
+  if (p.N <= 16 * 256) return launch_rows<kMxDense, 1, 16, X16, false>(p, tiles, st);
+  if (p.N <= 32 * 256) return launch_rows<kMxDense, 2, 16, X16, false>(p, tiles, st);
+  return launch_rows<kMxDense, 2, 8, X16, false>(p, tiles, st);
 }
 int launch_mx_rows_gemm(const MxArgs& p, hipStream_t st) {
   return p.x ? launch_rows_dense<true>(p, st) : launch_rows_dense<false>(p, st);

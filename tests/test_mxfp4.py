@@ -187,7 +187,8 @@ def test_quantize_refuses():
     (65, 130, 2080, "f16"), (128, 512, 384, None), (200, 5001, 288, "bf16"), (300, 256, 4128, None), (513, 771, 1024, None),
     (1030, 2048, 512, "f32"), (2100, 1100, 256, None), (2100, 2111, 288, "f16"), (4100, 4203, 96, None), (4000, 4300, 800, "bf16"), (8, 20000, 256, None), (129, 1, 32, None), (64, 300, 4096, "f16"), (40, 5000, 12320, None), (15, 16500, 96, None), (12, 9000, 4128, "f32"), (600, 900, 2080, None),
     (700, 24010, 96, "bf16"), (690, 24000, 544, None), (2500, 20007, 64, "f32"),
-    (300, 4001, 5152, "f16"), (630, 4100, 1056, None)])
+    (300, 4001, 5152, "f16"), (630, 4100, 1056, None),
+    (17, 1, 32, None), (100, 500, 2080, "bf16"), (33, 4096, 992, None), (250, 257, 4128, "f32"), (1000, 64, 544, "f16"), (31, 2000, 8224, None)])
 def test_gemm(m, n, k, bias, dtype):
     from litevllm_amd import mxfp4_gemm
     dt = DTYPES[dtype]
