@@ -9,6 +9,14 @@ from . import ops
 from .mxfp4 import _call
 
 
+def _rows(logits: torch.Tensor) -> torch.Tensor:
+    """``logits``, or a copy, as rows that the kernels can read."""
+    t, e = logits.shape
+    if (logits.stride(1) != 1 and e > 1) or (t > 1 and logits.stride(0) < e):
+        return logits.contiguous()
+    return logits
+
+
 def _forward(logits, ids, mask, experts):
     """(loss, counts, buf): the gradient's factors are the first ``experts`` floats of ``buf``, scratch the rest."""
     dev, t = logits.device, logits.shape[0]
@@ -31,19 +39,26 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, mask, buf)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)  # no zeros in place of the counts' gradient
-        ctx.layout = (logits.stride(0) if logits.shape[0] > 1 else experts, ops.dtype_code(logits.dtype))
+        ctx.shape = logits.shape
         return loss, counts
 
     @staticmethod
     def backward(ctx, upstream, _):
         if upstream is None:
             return None, None, None, None
+        # saved-tensor hooks may give back copies with other strides
         logits, mask, buf = ctx.saved_tensors
-        ld, dt = ctx.layout
-        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
-        t, experts = logits.shape
-        _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), ld, dt, None if mask is None else mask.data_ptr(),
-              buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
+        dev, (t, experts) = ops._require_device(logits, mask, buf, upstream), ctx.shape
+        if logits.shape != ctx.shape or buf.dtype is not torch.float32 or buf.dim() != 1 or buf.shape[0] < experts or (
+                mask is not None and (mask.dtype is not torch.bool or mask.shape != (t,))):
+            raise RuntimeError("moe_balance_loss: saved tensors came back with other shapes or types")
+        logits = _rows(logits)
+        if mask is not None:
+            mask = mask.contiguous()
+        buf = buf.contiguous()
+        grad = torch.empty((t, experts), dtype=logits.dtype, device=dev)
+        _call(dev, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
+              ops.dtype_code(logits.dtype), ops._ptr(mask), buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
             grad = torch._C._functions.DelayedError(b"moe_balance_loss is not differentiable twice", 1)(grad.requires_grad_())
         return grad, None, None, None
@@ -77,10 +92,7 @@ def moe_balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor,
         if mask.dtype != torch.bool or mask.shape != router_logits.shape[:1]:
             raise ValueError(f"mask must be bool [{router_logits.shape[0]}], got {mask.dtype} {tuple(mask.shape)}")
         mask = mask.contiguous()
-    t = router_logits.shape[0]
-    if (router_logits.stride(1) != 1 and experts > 1) or (t > 1 and router_logits.stride(0) < experts):
-        router_logits = router_logits.contiguous()
-    topk_ids = topk_ids.contiguous()
+    router_logits, topk_ids = _rows(router_logits), topk_ids.contiguous()
     if router_logits.requires_grad and torch.is_grad_enabled():
         return _BalanceLoss.apply(router_logits, topk_ids, mask, experts)
     return _forward(router_logits, topk_ids, mask, experts)[:2]

@@ -253,3 +253,78 @@ def test_entries_refuse_more_tokens_than_they_number():
         assert lib.awq_w4a16_moe_balance(p, 1, L.DTYPE_F16, p, 32, None, t, 1, k, p, p, p, p, need, None) == L.ERR_UNSUPPORTED
         if t > 1 << 30:
             assert lib.awq_w4a16_moe_balance_grad(p, 1, L.DTYPE_F16, None, p, p, p, t, 1, None) == L.ERR_UNSUPPORTED
+
+
+class _Hooks(torch.autograd.graph.saved_tensors_hooks):
+    """Gives saved tensors back as copies made by `copy`."""
+
+    def __init__(self, copy):
+        super().__init__(lambda t: t, lambda t: copy(t) if t.dim() == 2 else t)
+
+
+def _every_second_column(t):
+    """A copy whose rows are not dense."""
+    wide = torch.zeros(t.shape[0], 2 * t.shape[1], dtype=t.dtype, device=t.device)
+    wide[:, ::2] = t
+    return wide[:, ::2]
+
+
+# copies of other strides than the original's
+COPIES = {"dense": lambda t: t.contiguous().clone(), "wide": lambda t: torch.cat([t, t, t], 1)[:, t.shape[1]:2 * t.shape[1]],
+          "transposed": lambda t: t.t().contiguous().t(), "apart": _every_second_column}
+
+
+@pytest.mark.parametrize("copy", list(COPIES))
+def test_the_backward_reads_saved_logits_by_their_own_strides(copy, monkeypatch):
+    """Without a GPU, the launches replaced: hooks may give the logits back with other strides than they had."""
+    from litevllm_amd import moe_balance as B
+    calls = []
+    monkeypatch.setattr(B, "_call", lambda dev, name, *args: calls.append((name, args)))
+    monkeypatch.setattr(B.ops, "_require_device", lambda *t: torch.device("cpu"))
+    seen = []
+
+    def back(t):
+        seen.append(COPIES[copy](t))
+        return seen[-1]
+    wide = torch.randn(6, 31, requires_grad=True)
+    ids = torch.zeros(6, 2, dtype=torch.int32)
+    with _Hooks(back):
+        loss, _ = B.moe_balance_loss(wide[:, 5:29], ids)
+    grad, = torch.autograd.grad(loss, wide)
+    assert grad.shape == (6, 31)
+    (first, forward), (second, backward) = calls
+    assert first == "awq_w4a16_moe_balance" and forward[1] == 31
+    assert second == "awq_w4a16_moe_balance_grad"
+    z, ld = backward[0], backward[1]
+    if copy in ("dense", "wide"):
+        assert z == seen[0].data_ptr() and ld == seen[0].stride(0)
+    else:
+        assert ld == 24  # a dense copy of what came back
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copy", [*COPIES, "save_on_cpu"])
+def test_gradient_under_saved_tensor_hooks(copy):
+    from litevllm_amd import moe_balance_loss
+    z, ids, mask = _case(15, 40, 24, 3, "f32", 0.2)
+    wide = torch.zeros(80, 31, device="cuda")
+    wide[::2, 5:29] = z
+    wide.requires_grad_(True)
+    kept = torch.stack([mask, ~mask], 1)[:, 0]  # every second byte
+    want, = torch.autograd.grad(moe_balance_loss(wide[::2, 5:29], ids, kept)[0], wide)
+    assert torch.equal(want[::2, 5:29], _check(z, ids, mask))
+    with torch.autograd.graph.save_on_cpu() if copy == "save_on_cpu" else _Hooks(COPIES[copy]):
+        loss, _ = moe_balance_loss(wide[::2, 5:29], ids, kept)
+    assert torch.equal(torch.autograd.grad(loss, wide)[0], want)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_come_back_elsewhere_or_as_others_are_refused():
+    from litevllm_amd import moe_balance_loss
+    z, ids, _ = _case(16, 6, 8, 2, "f32")
+    z.requires_grad_(True)
+    for back in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.half() if t.dim() == 1 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            loss, _ = moe_balance_loss(z, ids)
+        with pytest.raises((RuntimeError, ValueError)):
+            loss.backward()
