@@ -4,6 +4,7 @@
 
 #include "awq_launch.h"
 #include "awq_mx_common.h"
+#include "awq_mx_span.h"
 
 namespace awq {
 
@@ -72,8 +73,8 @@ __device__ __forceinline__ void swap_rows(u32x4& x, u32x4& y, bool low) {
 // WK > 1 (few tiles, where the latency of a stage bounds a block): as many shares of K, each with waves and LDS of its
 // own, whose sums meet at the end; such a block has one tile.
 //
-// K past the end: the codes are whatever follows (any code is finite, and the loads stop at the operand's end),
-// both scales are 2^-127, and the products vanish in fp32.
+// K past the end: the codes are the next row's, or zeros behind the operand's last (any code is finite; what may be read:
+// awq_mx_span.h), both scales are 2^-127, and the products vanish in fp32.
 template <int MODE, int BM, int BN, int WM, int WN, int PER_SIMD, int WK>
 __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(MxArgs p, int row_tiles, int col_tiles) {
   constexpr int WAVES = WM * WN /* of a share of K */, TM = BM / WM / 16, TN = BN / WN / 16, ROWS = BM + BN, STAGE = ROWS * 128;
@@ -119,39 +120,38 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
     n0 = in_group / group_rows * COLS;
     const int64_t a_base = MODE == kMxGateUp ? 0 : t.first, w_base = (int64_t)t.expert * p.wrows + n0;
     const int last = p.N - 1 - n0;
-    // Row i of a stage (a's rows, then w's: a wave's gate columns and then their up columns) behind the operand's base, and
-    // the offsets of its codes (in 16 bytes) and of its scales (32 bits hold them: checked on the host)
+    // row i of a stage (a's rows, then w's: a wave's gate columns and then their up columns) behind the operand's base
     auto row_of = [&](int i) -> uint32_t {
       if (i < BM) return (uint32_t)(mx_a_row<MODE>(p, t, i) - a_base);
-      const int j = i - BM;
-      if constexpr (MODE == kMxGateUp) return (uint32_t)(min(j / 64 * 32 + j % 32, last) + (j % 64 < 32 ? 0 : p.N));
-      else return (uint32_t)min(j, last);
+      return mx_w_row(MODE == kMxGateUp, i - BM, last, p.N);
     };
-    auto scale_offset = [&](int i) -> uint32_t { return row_of(i) * (uint32_t)(i < BM ? p.as_ld : KB); };
-    auto rsrc = [&](const uint8_t* base, int64_t bytes) {
-      const uint64_t u = (uint64_t)(uintptr_t)base;
-      return u32x4{(uint32_t)u, (uint32_t)(u >> 32) & 0xFFFFu, bytes < 0xFFFFFFF0LL ? (uint32_t)bytes : 0xFFFFFFF0u, 0x00020000u};
+    // what the tile's loads may read: gathered rows are all of a's; scales begin with the word that holds the first one
+    const uint32_t a_rows = MODE == kMxGateUp ? (uint32_t)p.a_rows : (uint32_t)t.rows, w_rows = mx_w_rows(MODE == kMxGateUp, BN, last, p.N);
+    const uint64_t as = (uint64_t)(uintptr_t)p.as + (uint64_t)(a_base * p.as_ld), ws = (uint64_t)(uintptr_t)p.ws + (uint64_t)(w_base * KB);
+    const uint32_t a_in = (uint32_t)as & 3u, w_in = (uint32_t)ws & 3u;
+    auto span = [&](u32x4& rs, uint64_t base, uint32_t bytes, uint32_t from) {
+      mx_span_set(rs, base, bytes);
+      rs[3] = 0x00020000u;
+      mx_span_advance(rs, from);
     };
-    const int64_t a_rows = p.a_rows - a_base, w_blocks = (p.wrows - n0) * KB;
-    ars = rsrc(p.a + a_base * KB * 16, a_rows * KB * 16), wrs = rsrc(p.w + w_base * KB * 16, w_blocks * 16);
-    // scales from the word that holds the operand's first one, to the end of the word of its last
-    const uint8_t *as = p.as + a_base * p.as_ld, *ws = p.ws + w_base * KB;
-    const uint32_t a_in = (uint32_t)(uintptr_t)as & 3u, w_in = (uint32_t)(uintptr_t)ws & 3u;
-    asrs = rsrc(as - a_in, ((a_rows - 1) * p.as_ld + KB + a_in + 3) & ~(int64_t)3), wsrs = rsrc(ws - w_in, (w_blocks + w_in + 3) & ~(int64_t)3);
+    span(ars, (uint64_t)(uintptr_t)p.a + (uint64_t)(a_base * KB * 16), mx_code_bytes(a_rows, KB), s0 * 128);
+    span(wrs, (uint64_t)(uintptr_t)p.w + (uint64_t)(w_base * KB * 16), mx_code_bytes(w_rows, KB), s0 * 128);
+    span(asrs, as - a_in, mx_scale_bytes(a_rows, p.as_ld, KB, a_in), s0 * 8);
+    span(wsrs, ws - w_in, mx_scale_bytes(w_rows, KB, KB, w_in), s0 * 8);
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int i = (u * WAVES + wave) * 8 + (lane >> 3);
-      src[u] = (row_of(i) * (uint32_t)KB + (uint32_t)((lane & 7) ^ (lane >> 3))) * 16u;
+      src[u] = mx_code_offset(row_of(i), KB, lane);
     }
 #pragma unroll
     for (int u = 0; u < SLOADS; ++u) {
       const int i = min((u * WAVES + wave) * 64 + lane, ROWS - 1);
-      ssrc[u] = (scale_offset(i) + (i < BM ? a_in : w_in)) & ~3u;
+      ssrc[u] = mx_scale_offset(row_of(i), i < BM ? p.as_ld : KB, i < BM ? a_in : w_in);
     }
     // the rows of a fragment's next 16 are a multiple of 16 bytes on, and those of a gathered operand whole words: a
     // lane's scale bytes start alike in all its row tiles
     sh_a = ((MODE == kMxGateUp ? 0u : (uint32_t)r * (uint32_t)p.as_ld) + a_in & 3u) + (uint32_t)q;
-    sh_b = (scale_offset(c0 + r) + w_in & 3u) + (uint32_t)q;
+    sh_b = (row_of(c0 + r) * (uint32_t)KB + w_in & 3u) + (uint32_t)q;
     if constexpr (MODE == kMxDown) {
 #pragma unroll
       for (int k = 0; k < PLACES; ++k) place[k] = p.order[t.first + min(m0 + 8 * k + (r & 7), t.rows - 1)];
@@ -160,16 +160,19 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   constexpr uint32_t SHARE_LDS = mx_tile_lds(ROWS, TM > TN ? TM : TN);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + part * SHARE_LDS;
   constexpr uint32_t SCALES = 2 * STAGE, ZEROS = SCALES + 2 * ROWS * 16;
+  // stages, and groups of scales, are loaded in order: each moves the descriptors on to the next
   auto load_code = [&](int s, int u) {
-    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u], (uint32_t)(s0 + s) * 128u);
+    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u], 0u);
+    if (u == LOADS - 1) mx_span_advance(ars, 128), mx_span_advance(wrs, 128);
   };
   auto load_scales = [&](int g) {
 #pragma unroll
     for (int u = 0; u < SLOADS; ++u) {
       const int at = u * WAVES + wave;
       if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
-      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u], (uint32_t)(s0 * 8 + g * 16));
+      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u], 0u);
     }
+    mx_span_advance(asrs, 16), mx_span_advance(wsrs, 16);
   };
 
   f32x4 acc[TM][TN];
