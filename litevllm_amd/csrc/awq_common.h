@@ -563,16 +563,20 @@ __device__ __forceinline__ u32x4 rsrc_words(const void* base, uint32_t nbytes) {
 // LDS reads (it cannot tell LDS buffers apart and would wait for every load in flight before
 // each of them); a kernel waits for these loads itself before its barrier.  M0 carries the
 // LDS address and nothing else in these kernels uses M0.
+// The waits in front of the load are in the assembly too, as the compiler does not see that it is one: a state behind
+// the write of M0, and five behind a vector instruction that wrote a scalar register of it (a spilled descriptor comes
+// back by v_readlane).  tests/test_isa_waits.py looks for them in the built library.
+#define AWQ_LDS_DMA_WAIT "s_nop 3\n\t"
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_dma16(const u32x4& rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\t" AWQ_LDS_DMA_WAIT "buffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4(const u32x4& rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\t" AWQ_LDS_DMA_WAIT "buffer_load_dword %1, %2, %3 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");
