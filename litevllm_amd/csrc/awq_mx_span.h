@@ -1,38 +1,23 @@
 // What the direct loads of the microscaled tile kernel read (awq_mx_tile.hip): plain C++, so that a host program can walk
 // every address (tests/mx_span_walk.cpp).
 //
-// A load's position along K is part of its descriptor's base, and what is left of the operand behind it is the
-// descriptor's size: the range check, per dword of a load, then ends every load at the operand's end, whether or not it
-// counts the SGPR offset (gfx950 does; it is documented as left out).
+// The range check covers the VGPR offset, per dword of a load; whether the SGPR offset counts is documented as no, and
+// measured as yes on gfx950.  So a stage's position along K is in the SGPR offset only where all of the stage lies inside K,
+// and no load of it leaves its row; the stages that pass K's end have it in the VGPR offset, and so have all scales, and
+// the check ends them with the operand.
 #pragma once
 
 #include <cstdint>
 
 namespace awq {
 
-// Words 0 .. 2 of a buffer descriptor: 48 bits of address, and the bytes behind it that may be read.
-template <typename Rsrc>
-constexpr void mx_span_set(Rsrc& rs, uint64_t base, uint32_t bytes) {
-  rs[0] = (uint32_t)base;
-  rs[1] = (uint32_t)(base >> 32) & 0xFFFFu;
-  rs[2] = bytes;
+// Of the `stages` stages of 8 blocks from block 8 s0 on, those that lie inside K.
+constexpr int mx_whole_stages(int KB, int s0, int stages) {
+  const int whole = KB / 8 - s0;
+  return whole < 0 ? 0 : (whole < stages ? whole : stages);
 }
-#ifdef __HIPCC__
-#define AWQ_SPAN_FN __host__ __device__ __forceinline__
-#else
-#define AWQ_SPAN_FN inline
-#endif
-template <typename Rsrc>
-AWQ_SPAN_FN void mx_span_advance(Rsrc& rs, uint32_t by) {
-  const uint32_t lo = rs[0] + by;
-  rs[1] += lo < by ? 1u : 0u;
-  rs[0] = lo;
-  uint32_t left = rs[2] > by ? rs[2] : by;
-#ifdef __HIP_DEVICE_COMPILE__
-  asm("" : "+s"(left));  // a maximum and a difference in scalar registers, no saturating subtraction, which only vectors have
-#endif
-  rs[2] = left - by;
-}
+constexpr uint32_t mx_code_position(int s) { return (uint32_t)s * 128u; }
+constexpr uint32_t mx_scale_position(int s0, int group) { return (uint32_t)(s0 * 8 + group * 16); }
 
 // Rows of w of a tile from its first on: the last one read, and how many that spans.  gate_up: row j of the tile's BN is a
 // gate column's (the first 32 of 64) or its up column's, N rows on.
@@ -44,7 +29,7 @@ constexpr uint32_t mx_w_row(bool gate_up, int j, int last, int N) {
 constexpr uint32_t mx_w_rows(bool gate_up, int BN, int last, int N) { return mx_w_row(gate_up, BN - 1, last, N) + 1u; }
 
 // Codes: KB blocks of 16 bytes a row.  Lane l of a wave's load of eight rows reads chunk (l & 7) ^ (l >> 3) of a line.
-// 32 bits hold them: checked on the host.
+// 32 bits hold them, and the positions behind K's end with them: checked on the host.
 constexpr uint32_t mx_code_bytes(uint32_t rows, uint32_t KB) { return rows * KB * 16u; }
 constexpr uint32_t mx_code_offset(uint32_t row, uint32_t KB, int lane) {
   return (row * KB + (uint32_t)((lane & 7) ^ (lane >> 3))) * 16u;

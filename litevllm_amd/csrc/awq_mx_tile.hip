@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   const int lane = tid & 63, r = lane & 15, q = lane >> 4, ptid = tid - part * (WAVES * 64);
   const int KB = p.K / 32;
   // the share's stages, as if the operands began and ended there (a share behind K's end: stages of nothing)
-  const int stages = ((KB + 7) / 8 + WK - 1) / WK, s0 = part * stages, blocks = KB - 8 * s0;
+  const int stages = ((KB + 7) / 8 + WK - 1) / WK, s0 = part * stages, blocks = KB - 8 * s0, whole = mx_whole_stages(KB, s0, stages);
   // the wave's rows and columns in the tile
   const int m0 = (wave / WN) * TM * 16, c0 = BM + (wave % WN) * TN * 16;
 
@@ -129,15 +129,11 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
     const uint32_t a_rows = MODE == kMxGateUp ? (uint32_t)p.a_rows : (uint32_t)t.rows, w_rows = mx_w_rows(MODE == kMxGateUp, BN, last, p.N);
     const uint64_t as = (uint64_t)(uintptr_t)p.as + (uint64_t)(a_base * p.as_ld), ws = (uint64_t)(uintptr_t)p.ws + (uint64_t)(w_base * KB);
     const uint32_t a_in = (uint32_t)as & 3u, w_in = (uint32_t)ws & 3u;
-    auto span = [&](u32x4& rs, uint64_t base, uint32_t bytes, uint32_t from) {
-      mx_span_set(rs, base, bytes);
-      rs[3] = 0x00020000u;
-      mx_span_advance(rs, from);
-    };
-    span(ars, (uint64_t)(uintptr_t)p.a + (uint64_t)(a_base * KB * 16), mx_code_bytes(a_rows, KB), s0 * 128);
-    span(wrs, (uint64_t)(uintptr_t)p.w + (uint64_t)(w_base * KB * 16), mx_code_bytes(w_rows, KB), s0 * 128);
-    span(asrs, as - a_in, mx_scale_bytes(a_rows, p.as_ld, KB, a_in), s0 * 8);
-    span(wsrs, ws - w_in, mx_scale_bytes(w_rows, KB, KB, w_in), s0 * 8);
+    auto rsrc = [](uint64_t base, uint32_t bytes) { return u32x4{(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, bytes, 0x00020000u}; };
+    ars = rsrc((uint64_t)(uintptr_t)p.a + (uint64_t)(a_base * KB * 16), mx_code_bytes(a_rows, KB));
+    wrs = rsrc((uint64_t)(uintptr_t)p.w + (uint64_t)(w_base * KB * 16), mx_code_bytes(w_rows, KB));
+    asrs = rsrc(as - a_in, mx_scale_bytes(a_rows, p.as_ld, KB, a_in));
+    wsrs = rsrc(ws - w_in, mx_scale_bytes(w_rows, KB, KB, w_in));
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
       const int i = (u * WAVES + wave) * 8 + (lane >> 3);
@@ -160,19 +156,23 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   constexpr uint32_t SHARE_LDS = mx_tile_lds(ROWS, TM > TN ? TM : TN);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + part * SHARE_LDS;
   constexpr uint32_t SCALES = 2 * STAGE, ZEROS = SCALES + 2 * ROWS * 16;
-  // stages, and groups of scales, are loaded in order: each moves the descriptors on to the next
-  auto load_code = [&](int s, int u) {
-    lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u], 0u);
-    if (u == LOADS - 1) mx_span_advance(ars, 128), mx_span_advance(wrs, 128);
+  // loads `from` .. `to` - 1 of stage s's LOADS
+  auto load_codes = [&](int s, int from, int to) {
+    auto all = [&](uint32_t voff, uint32_t soff) {
+#pragma unroll
+      for (int u = from; u < to && u < LOADS; ++u)
+        lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u] + voff, soff);
+    };
+    if (s < whole) all(0u, mx_code_position(s0 + s));
+    else all(mx_code_position(s0 + s), 0u);
   };
   auto load_scales = [&](int g) {
 #pragma unroll
     for (int u = 0; u < SLOADS; ++u) {
       const int at = u * WAVES + wave;
       if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
-      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u], 0u);
+      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u] + mx_scale_position(s0, g), 0u);
     }
-    mx_span_advance(asrs, 16), mx_span_advance(wsrs, 16);
   };
 
   f32x4 acc[TM][TN];
@@ -224,8 +224,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
     for (int s = 0; s < 2; ++s) {
       if (s >= stages) break;
       if (s & 1) load_scales(1);  // before the codes of the first stage that reads from it
-#pragma unroll
-      for (int u = 0; u < LOADS; ++u) load_code(s, u);
+      load_codes(s, 0, LOADS);
     }
   };
   // the results of a tile go out behind the next one's first loads, in at least STORES stores where this wave's part of
@@ -270,8 +269,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
       next_stage(s);
       if (s + 2 < stages) {
         if (s & 1) load_scales((s + 3) >> 1);
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) load_code(s + 2, u);
+        load_codes(s + 2, 0, LOADS);
       }
     }
     for (int s = 0; !idle && s < stages; ++s) {
@@ -298,10 +296,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
           if ((s & 1) && s + 2 < stages) load_scales((s + 3) >> 1);
         }
         read_a(s + 1, 0, at, i);
-        if (s + 2 < stages) {
-#pragma unroll
-          for (int u = i * SHARE; u < (i + 1) * SHARE && u < LOADS; ++u) load_code(s + 2, u);
-        }
+        if (s + 2 < stages) load_codes(s + 2, i * SHARE, (i + 1) * SHARE);
       }
     }
     // no use of an accumulator before the last product is through

@@ -10,13 +10,11 @@
 namespace {
 using namespace awq;
 
+// words of a descriptor: where an operand begins, and its bytes
 struct Rsrc {
-  uint32_t w[4];
-  uint32_t& operator[](int i) { return w[i]; }
-  uint32_t operator[](int i) const { return w[i]; }
-  uint64_t base() const { return (uint64_t)w[1] << 32 | w[0]; }
+  uint64_t base;
+  uint32_t bytes;
 };
-// rows of `ld` bytes from address lo on, each with `bytes` of its own
 struct Operand {
   uint64_t lo, hi;
 };
@@ -33,11 +31,12 @@ void fail(const Case& c, const char* what, int part, int stage, int row) {
               c.BM, c.BN, c.WK, c.KB, c.rows, c.a_rows, c.N, c.n0, c.in, part, stage, row);
   std::exit(1);
 }
-// a 16-byte load: every dword that the descriptor's size lets through is the operand's
-void touch(const Case& c, const Rsrc& rs, uint32_t off, const Operand& o, int part, int stage, int row) {
+// A 16-byte load: every dword that the range check lets through is the operand's, whether or not the check counts the SGPR
+// offset (leaving it out lets more through).
+void touch(const Case& c, const Rsrc& rs, uint32_t voff, uint32_t soff, const Operand& o, int part, int stage, int row) {
   for (uint32_t d = 0; d < 16; d += 4) {
-    if ((uint64_t)off + d + 4 > rs[2]) continue;
-    const uint64_t at = rs.base() + off + d;
+    if ((uint64_t)voff + d + 4 > rs.bytes) continue;
+    const uint64_t at = rs.base + voff + soff + d;
     if (at < (o.lo & ~(uint64_t)3) || at + 4 > ((o.hi + 3) & ~(uint64_t)3)) fail(c, "outside the operand", part, stage, row);
   }
   ++walked;
@@ -49,7 +48,6 @@ void walk(const Case& c) {
   const uint32_t a_ld = gate_up ? (uint32_t)(KB + 3) / 4 * 4 : (uint32_t)KB;
   const uint32_t a_rows = (uint32_t)(gate_up ? c.a_rows : c.rows), w_rows = mx_w_rows(gate_up, c.BN, last, c.N);
   const uint32_t w_left = (uint32_t)((gate_up ? 2 : 1) * c.N - c.n0);  // of the expert, from n0 on
-  // just below a multiple of 2^32, so that positions carry
   const uint64_t a0 = 0x3FFFFFFF0ull, w0 = 0x4FFFFFFE0ull, as0 = 0x1FFFFFFFCull + (gate_up ? 0 : c.in), ws0 = 0x2FFFFFFF8ull + c.in;
   const Operand oa{a0, a0 + (uint64_t)a_rows * KB * 16}, ow{w0, w0 + (uint64_t)w_left * KB * 16};
   const Operand osa{as0, as0 + (uint64_t)(a_rows - 1) * a_ld + KB}, osw{ws0, ws0 + (uint64_t)w_left * KB};
@@ -62,39 +60,36 @@ void walk(const Case& c) {
   for (int part = 0; part < c.WK; ++part) {
     const int s0 = part * stages;
     const uint32_t a_in = (uint32_t)as0 & 3u, w_in = (uint32_t)ws0 & 3u;
-    Rsrc ars{}, wrs{}, asrs{}, wsrs{};
-    mx_span_set(ars, a0, mx_code_bytes(a_rows, KB)), mx_span_advance(ars, s0 * 128);
-    mx_span_set(wrs, w0, mx_code_bytes(w_rows, KB)), mx_span_advance(wrs, s0 * 128);
-    mx_span_set(asrs, as0 - a_in, mx_scale_bytes(a_rows, a_ld, KB, a_in)), mx_span_advance(asrs, s0 * 8);
-    mx_span_set(wsrs, ws0 - w_in, mx_scale_bytes(w_rows, KB, KB, w_in)), mx_span_advance(wsrs, s0 * 8);
+    const int whole = mx_whole_stages(KB, s0, stages);
+    const Rsrc ars{a0, mx_code_bytes(a_rows, KB)}, wrs{w0, mx_code_bytes(w_rows, KB)};
+    const Rsrc asrs{as0 - a_in, mx_scale_bytes(a_rows, a_ld, KB, a_in)}, wsrs{ws0 - w_in, mx_scale_bytes(w_rows, KB, KB, w_in)};
     auto codes = [&](int s) {
       for (int i = 0; i < ROWS; ++i)
         for (int l = 8 * (i & 7); l < 8 * (i & 7) + 8; ++l) {
           const bool a = i < c.BM;
           const Rsrc& rs = a ? ars : wrs;
-          const uint32_t row = row_of(i), off = mx_code_offset(row, KB, l);
-          touch(c, rs, off, a ? oa : ow, part, s, i);
+          const uint32_t row = row_of(i), src = mx_code_offset(row, KB, l), position = mx_code_position(s0 + s);
+          const uint32_t voff = s < whole ? src : src + position, soff = s < whole ? position : 0u;
+          touch(c, rs, voff, soff, a ? oa : ow, part, s, i);
           const int block = 8 * (s0 + s) + ((l & 7) ^ (l >> 3));
-          if (block < KB && (off + 16 > rs[2] || rs.base() + off != (a ? a0 : w0) + ((uint64_t)row * KB + block) * 16))
+          if (block < KB && ((uint64_t)voff + soff + 16 > rs.bytes || rs.base + voff + soff != (a ? a0 : w0) + ((uint64_t)row * KB + block) * 16))
             fail(c, "not its codes", part, s, i);
         }
-      mx_span_advance(ars, 128), mx_span_advance(wrs, 128);
     };
     auto scales = [&](int g) {
       for (int i = 0; i < ROWS; ++i) {
         const bool a = i < c.BM;
         const Rsrc& rs = a ? asrs : wsrs;
-        const uint32_t row = row_of(i), off = mx_scale_offset(row, a ? a_ld : KB, a ? a_in : w_in);
-        touch(c, rs, off, a ? osa : osw, part, g, i);
+        const uint32_t row = row_of(i), off = mx_scale_offset(row, a ? a_ld : KB, a ? a_in : w_in) + mx_scale_position(s0, g);
+        touch(c, rs, off, 0, a ? osa : osw, part, g, i);
         // the row's bytes of this share that lie in the group
-        const uint64_t mine = (a ? as0 + (uint64_t)row * a_ld : ws0 + (uint64_t)row * KB) + 8 * s0, from = rs.base() + off;
+        const uint64_t mine = (a ? as0 + (uint64_t)row * a_ld : ws0 + (uint64_t)row * KB) + 8 * s0, from = rs.base + off;
         for (uint64_t b = mine; b < mine + 8 * stages && b < mine + (uint64_t)(KB - 8 * s0 > 0 ? KB - 8 * s0 : 0); ++b) {
           if (b < from || b >= from + 16) continue;
-          if ((uint64_t)off + ((b - from) & ~(uint64_t)3) + 4 > rs[2]) fail(c, "not its scales", part, g, i);
+          if ((uint64_t)off + ((b - from) & ~(uint64_t)3) + 4 > rs.bytes) fail(c, "not its scales", part, g, i);
         }
         if (from != (mine & ~(uint64_t)3) + 16 * (uint64_t)g) fail(c, "not its group", part, g, i);
       }
-      mx_span_advance(asrs, 16), mx_span_advance(wsrs, 16);
     };
     // as the kernel issues them
     scales(0);
