@@ -426,7 +426,7 @@ size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
  *      are not used).
  *   w: codes [N, K/2], w_scales [N, K/32];  bias: NULL or [N] of bias_dtype;  c: row stride ldc, apart from all that
  *      the call reads (with few rows blocks read all of a while others write).
- *   Any M, N >= 0.  Results are bitwise reproducible.  A NaN block makes NaN of every output that reads it.
+ *   M up to 2^31 - 1, N up to 2^31 - 256, K up to 2^24.  Results are bitwise reproducible.  A NaN block makes NaN of every output that reads it.
  *   workspace: 256-byte aligned; calls that may overlap must not share one. */
 int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, const uint8_t* w,
                          const uint8_t* w_scales, const void* bias, void* c, int64_t ldc, int64_t M, int64_t N,

@@ -14,6 +14,7 @@ bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0;
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 constexpr int64_t kIntMax = 0x7FFFFFFFLL;
 constexpr int64_t kMaxBalance = (int64_t)1 << 30;  // tokens and routes: 32 bits number them, a block's behind the last too
+constexpr int64_t kMaxN = kIntMax - 255;       // columns of a block, those behind the last too, in 32 bits
 constexpr int64_t kMaxK = (int64_t)1 << 24;   // 256 rows of codes are addressed in 32 bits,
 constexpr int64_t kBytes = 0xFFFF0000LL;      // and so are all of the tokens' and all of an expert's gate and up
 }  // namespace
@@ -51,8 +52,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   if (M < 0 || N < 0 || K <= 0 || (K % 32) != 0) return AWQ_ERR_SHAPE;
   if (M == 0 || N == 0) return AWQ_OK;
   if (!a || !w || !w_scales || !c) return AWQ_ERR_NULL;
-  if (!dtype_16(act_dtype) || M > kIntMax || N > kIntMax || K > kIntMax) return AWQ_ERR_UNSUPPORTED;
-  if (K > kMaxK) return AWQ_ERR_UNSUPPORTED;
+  if (!dtype_16(act_dtype) || M > kIntMax || N > kMaxN || K > kMaxK) return AWQ_ERR_UNSUPPORTED;
   if (bias ? !dtype_float(bias_dtype) : bias_dtype != AWQ_DTYPE_NONE) return AWQ_ERR_UNSUPPORTED;
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(c, 2) || ldc < N) return AWQ_ERR_STRIDE;
   MxArgs p{};

@@ -568,3 +568,16 @@ def test_a_layer_of_router_balance_experts_and_projection(t):
     assert float((logits.grad.double() - grad).abs().max()) <= 1e-5 * float(grad.abs().max())
     _close(y, *R.moe(x, w.cpu(), ids.cpu(), w1, w2, "silu"), torch.float16)
     _close(z, *R.gemm(R.rounded(y), R.rounded(dense)), torch.float16)
+
+
+def test_gemm_entry_refuses_columns_that_a_block_cannot_number():
+    """A block's columns, also those behind the last, are numbered in 32 bits: up to 2^31 - 256."""
+    lib, p = L.load(), _fake()
+
+    def call(n, m):
+        return lib.awq_w4a16_mxfp4_gemm(p, 64, None, p, p, None, p, n, m, n, 64, L.DTYPE_BF16, L.DTYPE_NONE, None, 0, None)
+    for m in (20, 300):
+        assert call((1 << 31) - 256, m) == L.ERR_WORKSPACE  # what it has to say next
+    for n in ((1 << 31) - 255, (1 << 31) - 8, (1 << 31) - 1, 1 << 31):
+        for m in (1, 20, 300):
+            assert call(n, m) == L.ERR_UNSUPPORTED
