@@ -1,7 +1,8 @@
 """Drop-in for ``vllm/model_executor/layers/quantization/awq.py``: ``AWQConfig`` builds and
 caches an ``AWQWeight`` (zero points present) or ``PackedInt4Weight`` (none) on the
 layer at the first ``apply`` and forwards ``weight.matmul(x, layer.bias, config=...)``
-(``awq.py:40-104``)."""
+(``awq.py:40-104``).  A layer whose ``qweight`` and ``scales`` are both uint8 holds MXFP4 and
+gets an ``MXFP4Weight``."""
 from __future__ import annotations
 
 from typing import Any
@@ -9,6 +10,7 @@ from typing import Any
 import torch
 import torch.nn as nn
 
+from .mxfp4 import MXFP4Weight, is_mxfp4
 from .tensor import AWQWeight, PackedInt4Weight
 
 
@@ -58,6 +60,9 @@ class AWQConfig(QuantizationConfig):
                 if w is not None and w.numel() > 1:
                     return torch.nn.functional.linear(x, w, getattr(layer, "bias", None))
                 raise RuntimeError(f"AWQ weight not ready for layer '{prefix}'")
+            if is_mxfp4(qweight, layer.scales):
+                layer._quant_weight = MXFP4Weight(qweight, layer.scales, prefix=getattr(layer, "prefix", ""))
+                return self.apply(layer, x, **kwargs)
             g = int(getattr(layer, "group_size", self.group_size))
             k = qweight.shape[1] * 8 if self.layout == "ref" else qweight.shape[0]
             if k % g != 0:

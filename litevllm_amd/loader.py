@@ -1,10 +1,13 @@
 """On-disk format adapter for AWQ linear layers: the loader step of
-``vllm/model_executor/model_loader/__init__.py:551-797``, for the two int4 checkpoint formats.
+``vllm/model_executor/model_loader/__init__.py:551-797``, for the two int4 checkpoint formats,
+and MXFP4 beside them.
 
 * compressed-tensors pack-quantized: ``weight_packed [N, K/8]`` (sequential nibbles along K),
   ``weight_scale [N, K/G]``, optional ``weight_zero_point`` -- the reference runtime layout;
 * AutoAWQ: ``qweight [K, N/8]`` (interleaved nibbles along N), ``scales [K/G, N]``,
-  ``qzeros [K/G, N/8]``.
+  ``qzeros [K/G, N/8]``;
+* MXFP4 (no counterpart in the reference): ``weight_packed`` or ``qweight`` uint8 ``[N, K/2]``,
+  ``weight_scale`` or ``scales`` uint8 ``[N, K/32]``.
 
 ``awq_components`` collects one module's tensors under the reference's alias list
 (``qweight`` <- ``weight_packed`` / ``qweight`` / ``weight``; ``scales`` <- ``weight_scale`` /
@@ -12,13 +15,14 @@
 ``weight_zero_point``, which the reference's list does not know.  ``make_awq_weight`` infers
 the layout and group size from the shapes, maps the zero point, and returns an ``AWQWeight``
 (or ``PackedInt4Weight`` without zeros), optionally converted once to the AutoAWQ layout the
-kernels read natively and with its decode copy prepared.
+kernels read natively and with its decode copy prepared; of MXFP4 tensors, an ``MXFP4Weight``.
 """
 from __future__ import annotations
 
 import torch
 
 from . import ops
+from .mxfp4 import MXFP4Weight, is_mxfp4
 from .tensor import AWQWeight, PackedInt4Weight
 
 ALIASES = {
@@ -107,12 +111,16 @@ def _zeros_for(qzeros: torch.Tensor | None, layout: str, K: int, N: int, G: int)
 
 def make_awq_weight(comps: dict, *, prefix: str = "", device: torch.device | str | None = None,
                     to_autoawq: bool = True, prepare_decode: bool = False):
-    """An ``AWQWeight`` (zeros present) or ``PackedInt4Weight`` (symmetric) from one module's
-    checkpoint tensors.  ``to_autoawq`` converts a reference-layout weight once on the device
+    """An ``AWQWeight`` (zeros present), ``PackedInt4Weight`` (symmetric) or ``MXFP4Weight`` from one
+    module's checkpoint tensors.  ``to_autoawq`` converts a reference-layout weight once on the device
     (lossless); ``prepare_decode`` also builds the decode stream copy up front."""
     qweight, scales = comps["qweight"], comps["scales"]
     if device is not None:
         qweight, scales = qweight.to(device), scales.to(device)
+    if is_mxfp4(qweight, scales):
+        if comps.get("qzeros") is not None:
+            raise ValueError(f"MXFP4 has no zero points, '{prefix}' has them")
+        return MXFP4Weight(qweight.contiguous(), scales.contiguous(), prefix=prefix)
     layout, K, N, G = detect_layout(qweight, scales)
     qzeros = comps.get("qzeros")
     if qzeros is not None and device is not None:

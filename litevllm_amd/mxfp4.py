@@ -13,9 +13,11 @@ PyTorch's allocator for each call, so calls on different streams and captured gr
 from __future__ import annotations
 
 import torch
+import torch.nn as nn
 
 from . import _lib as L
 from . import ops
+from .tensor import QuantizedLinearWeight
 
 BLOCK = 32
 
@@ -156,15 +158,23 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
     return out
 
 
-class MXFP4Weight:
-    """A linear layer's MXFP4 weight, beside :class:`AWQWeight`: ``qweight`` uint8 ``[N, K/2]``, ``scales`` uint8
-    ``[N, K/32]``."""
+def is_mxfp4(qweight: torch.Tensor, scales: torch.Tensor) -> bool:
+    """Whether a layer's tensors are MXFP4's: both uint8 (the scales of int4 weights are floating point)."""
+    return qweight.dtype is torch.uint8 and scales.dtype is torch.uint8
+
+
+class MXFP4Weight(QuantizedLinearWeight):
+    """A linear layer's MXFP4 weight, beside :class:`AWQWeight` and used as it is: ``qweight`` uint8 ``[N, K/2]``,
+    ``scales`` uint8 ``[N, K/32]``."""
 
     def __init__(self, qweight: torch.Tensor, scales: torch.Tensor, prefix: str = ""):
+        super().__init__()
         if qweight.dim() != 2:
             raise ValueError(f"qweight must be [N, K/2], got {tuple(qweight.shape)}")
         _check_codes("MXFP4Weight", qweight, scales)
-        self.qweight, self.scales, self.prefix = qweight, scales, prefix
+        self.qweight = nn.Parameter(qweight, requires_grad=False)
+        self.scales = nn.Parameter(scales, requires_grad=False)
+        self.prefix = prefix
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor, prefix: str = "") -> "MXFP4Weight":
@@ -175,8 +185,9 @@ class MXFP4Weight:
         """The ``[N, K]`` values."""
         return mxfp4_dequantize(self.qweight, self.scales, dtype)
 
-    def matmul(self, x: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
-        """``x [..., K] @ W^T (+ bias)``, in ``x``'s type (:func:`mxfp4_gemm`)."""
+    def matmul(self, x: torch.Tensor, bias: torch.Tensor | None = None, *, config: object | None = None) -> torch.Tensor:
+        """``x [..., K] @ W^T (+ bias)``, in ``x``'s type (:func:`mxfp4_gemm`).  Of the policies in ``config`` none applies:
+        there is one path."""
         y = mxfp4_gemm(x.reshape(-1, x.shape[-1]), self.qweight, self.scales, bias=bias)
         return y.view(x.shape[:-1] + (y.shape[-1],))
 

@@ -581,3 +581,66 @@ def test_gemm_entry_refuses_columns_that_a_block_cannot_number():
     for n in ((1 << 31) - 255, (1 << 31) - 8, (1 << 31) - 1, 1 << 31):
         for m in (1, 20, 300):
             assert call(n, m) == L.ERR_UNSUPPORTED
+
+
+# ------------------------------------------------------------------ the framework's linear method
+def _layer(**tensors):
+    from litevllm_amd.awq import AWQConfig
+    layer = torch.nn.Module()
+    cfg = AWQConfig.from_config({"config_groups": {"group_0": {"weights": {"num_bits": 4, "group_size": 32}}}})
+    cfg.init_layer(layer)
+    cfg.load_weights(layer, tensors.items())
+    return cfg, layer
+
+
+def test_the_linear_method_calls_the_product(monkeypatch):
+    """Without a GPU, the product replaced: what ``AWQConfig.apply`` hands it, for a weight that the layer holds and for
+    one that it builds of the layer's tensors."""
+    from litevllm_amd import MXFP4Weight, mxfp4
+    calls = []
+
+    def gemm(a, qweight, scales, a_scales=None, bias=None, **kw):
+        calls.append((a, qweight, scales, bias, kw))
+        return a.new_zeros(a.shape[0], qweight.shape[0])
+    monkeypatch.setattr(mxfp4, "mxfp4_gemm", gemm)
+    c, s = R.quantize(_made(110, 48, 64))
+    x, bias = torch.zeros(2, 3, 64, dtype=torch.bfloat16), torch.ones(48)
+    cfg, layer = _layer(qweight=c, scales=s, bias=bias)
+    held = torch.nn.Module()
+    held._quant_weight, held.bias = MXFP4Weight(c, s, prefix="p"), None
+    for on, b in ((layer, layer.bias), (held, None)):
+        for kw in ({}, {"config": {"kernel_policy": {}}}, {"inf_config": object()}):
+            assert cfg.apply(on, x, **kw).shape == (2, 3, 48)
+            a, qweight, scales, got, rest = calls.pop()
+            assert a.shape == (6, 64) and torch.equal(qweight, c) and torch.equal(scales, s) and got is b and not rest
+    assert isinstance(layer._quant_weight, MXFP4Weight)
+    # like the other weights a module, whose tensors move and are saved with the layer's
+    assert set(held.state_dict()) == {"_quant_weight.qweight", "_quant_weight.scales"}
+    assert not any(p.requires_grad for p in held.parameters())
+
+
+def test_the_loader_knows_the_format():
+    from litevllm_amd import MXFP4Weight, loader
+    c, s = R.quantize(_made(111, 48, 128))
+    w = loader.make_awq_weight(loader.awq_components({"m.weight_packed": c, "m.weight_scale": s}, "m"), prefix="m")
+    assert type(w) is MXFP4Weight and w.prefix == "m" and torch.equal(w.qweight, c) and torch.equal(w.scales, s)
+    with pytest.raises(ValueError):
+        loader.make_awq_weight({"qweight": c, "scales": s[:, :2]})
+    with pytest.raises(ValueError):  # the format has no zero points
+        loader.make_awq_weight({"qweight": c, "scales": s, "qzeros": torch.zeros(48, 4, dtype=torch.uint8)})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40])
+def test_the_linear_method_on_mxfp4_tensors(m):
+    from litevllm_amd import loader, mxfp4_gemm
+    from litevllm_amd.awq import AWQConfig
+    c, s = R.quantize(_made(112, 80, 128))
+    b = _made(113, 80)
+    x = _made(114, m, 1, 128, dtype=torch.bfloat16).cuda()
+    want = mxfp4_gemm(x.view(m, 128), c.cuda(), s.cuda(), bias=b.cuda()).view(m, 1, 80)
+    cfg, layer = _layer(weight_packed_qweight=c, scales=s, bias=b)
+    assert torch.equal(cfg.apply(layer.cuda(), x, inf_config=None), want)
+    held = torch.nn.Module()
+    held._quant_weight, held.bias = loader.make_awq_weight({"qweight": c, "scales": s}), b.cuda()
+    assert torch.equal(AWQConfig().apply(held.cuda(), x), want)
