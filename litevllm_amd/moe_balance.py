@@ -6,7 +6,7 @@ import torch
 
 from . import _lib as L
 from . import ops
-from .mxfp4 import _call
+from .mxfp4 import _call, _derivative_asked, _Refused
 
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
@@ -48,6 +48,7 @@ class _BalanceLoss(torch.autograd.Function):
             return None, None, None, None
         # saved-tensor hooks may give back copies with other strides
         logits, mask, buf = ctx.saved_tensors
+        inputs = logits, upstream
         dev, (t, experts) = ops._require_device(logits, mask, buf, upstream), ctx.shape
         if logits.shape != ctx.shape or buf.dtype is not torch.float32 or buf.dim() != 1 or buf.shape[0] < experts or (
                 mask is not None and (mask.dtype is not torch.bool or mask.shape != (t,))):
@@ -60,7 +61,7 @@ class _BalanceLoss(torch.autograd.Function):
         _call(dev, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
               ops.dtype_code(logits.dtype), ops._ptr(mask), buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
-            grad = torch._C._functions.DelayedError(b"moe_balance_loss is not differentiable twice", 1)(grad.requires_grad_())
+            grad = _Refused.apply("moe_balance_loss is not differentiable twice", grad, *inputs)
         return grad, None, None, None
 
 
@@ -93,6 +94,6 @@ def moe_balance_loss(router_logits: torch.Tensor, topk_ids: torch.Tensor,
             raise ValueError(f"mask must be bool [{router_logits.shape[0]}], got {mask.dtype} {tuple(mask.shape)}")
         mask = mask.contiguous()
     router_logits, topk_ids = _rows(router_logits), topk_ids.contiguous()
-    if router_logits.requires_grad and torch.is_grad_enabled():
+    if _derivative_asked("moe_balance_loss", None, router_logits):
         return _BalanceLoss.apply(router_logits, topk_ids, mask, experts)
     return _forward(router_logits, topk_ids, mask, experts)[:2]

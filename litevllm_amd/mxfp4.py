@@ -5,7 +5,8 @@ The format (OCP Microscaling Formats 1.0): 32 consecutive values along the last 
 ``2 ** (byte - 127)``; a value is an e2m1 code.  A ``[..., K]`` tensor is ``codes`` uint8 ``[..., K/2]`` (the even
 index in the low four bits) and ``scales`` uint8 ``[..., K/32]``, as MXFP4 checkpoints hold weights; the kernels
 read that layout as it is, so no copy of a weight is built.  Activations are quantised on the way in.  None of these
-operators is differentiable.
+operators is differentiable: where an input requires a gradient, a backward through the result raises, and so does the
+call where the result cannot carry that (codes, ``out``, forward-mode derivatives).
 
 Every byte of the arithmetic runs in ``libawq_w4a16.so``; there is no CPU fallback.  Scratch memory comes from
 PyTorch's allocator for each call, so calls on different streams and captured graphs share none.
@@ -14,6 +15,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import ops
@@ -33,6 +35,36 @@ def _call(dev: torch.device, name: str, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         raise L.AWQKernelError(name, rc)
+
+
+class _Refused(torch.autograd.Function):
+    """A result unchanged, whose derivative is refused: a backward that reaches it on its way to any of ``inputs`` raises."""
+
+    @staticmethod
+    def forward(ctx, why, result, *inputs):
+        ctx.why = why
+        return result
+
+    @staticmethod
+    def backward(ctx, *upstream):
+        raise RuntimeError(ctx.why)
+
+
+def _derivative_asked(name: str, out: torch.Tensor | None, *inputs: torch.Tensor | None) -> bool:
+    """Whether a backward may ask for a derivative in ``inputs``, which the result has to refuse.  Raises where it cannot: for
+    a caller's ``out``, and for an input with a tangent of forward mode."""
+    if forward_ad._current_level >= 0:
+        for t in inputs:
+            if t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative")
+    if not torch.is_grad_enabled():
+        return False
+    for t in inputs:
+        if t is not None and t.requires_grad:
+            if out is not None:
+                raise RuntimeError(f"{name} with out= takes no inputs that require a gradient")
+            return True
+    return False
 
 
 def _check_codes(what: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
@@ -77,6 +109,9 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     NaN or an infinity takes the NaN scale (byte 255): all of it stands for NaN."""
     dev = ops._require_device(x)
     dt = ops.dtype_code(x.dtype)
+    if _derivative_asked("mxfp4_quantize", None, x):
+        raise RuntimeError("mxfp4_quantize is not differentiable, and codes cannot carry that to a backward: detach the input or "
+                           "call it under torch.no_grad()")
     if x.dim() == 0 or x.shape[-1] % BLOCK:
         raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {tuple(x.shape)}")
     k = x.shape[-1]
@@ -129,6 +164,7 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
         raise TypeError(f"unsupported dtype {dtype}: fp16 or bf16")
     if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must be [{n}], got {tuple(bias.shape)}")
+    asked, inputs = _derivative_asked("mxfp4_gemm", out, a, bias), (a, bias)
     if out is None:
         out = torch.empty((m, n), dtype=dtype, device=dev)
     elif out.dtype != dtype:
@@ -155,7 +191,7 @@ def mxfp4_gemm(a: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, a_s
     _call(dev, "awq_w4a16_mxfp4_gemm", a.data_ptr(), ld, ops._ptr(a_scales), qweight.data_ptr(), scales.data_ptr(),
           ops._ptr(bias), out.data_ptr(), out.stride(0) if m > 1 else n, m, n, k, ops.dtype_code(dtype),
           L.DTYPE_NONE if bias is None else ops.dtype_code(bias.dtype), ops._ptr(ws), ws_bytes)
-    return out
+    return _Refused.apply("mxfp4_gemm is not differentiable", out, *inputs) if asked else out
 
 
 def is_mxfp4(qweight: torch.Tensor, scales: torch.Tensor) -> bool:
@@ -178,8 +214,8 @@ class MXFP4Weight(QuantizedLinearWeight):
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor, prefix: str = "") -> "MXFP4Weight":
-        """Quantises a dense ``[N, K]`` weight."""
-        return cls(*mxfp4_quantize(weight), prefix=prefix)
+        """Quantises the values of a dense ``[N, K]`` weight."""
+        return cls(*mxfp4_quantize(weight.detach()), prefix=prefix)
 
     def dense_weight(self, dtype: torch.dtype = torch.float16) -> torch.Tensor:
         """The ``[N, K]`` values."""
@@ -236,6 +272,7 @@ def mxfp4_moe(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     wdt, k = ops.dtype_code(topk_weights.dtype), topk_ids.shape[1]
+    asked, inputs = _derivative_asked("mxfp4_moe", out, x, topk_weights), (x, topk_weights)
     if out is None:
         out = torch.empty((t, h), dtype=x.dtype, device=dev)
     else:
@@ -253,4 +290,4 @@ def mxfp4_moe(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tenso
     _call(dev, "awq_w4a16_mxfp4_moe", x.data_ptr(), ld, topk_ids.data_ptr(), 64 if topk_ids.dtype == torch.int64 else 32,
           topk_weights.data_ptr(), wdt, w1.data_ptr(), s1.data_ptr(), w2.data_ptr(), s2.data_ptr(), out.data_ptr(),
           out.stride(0) if t > 1 else h, t, h, inter, e, k, act, ops.dtype_code(x.dtype), ws.data_ptr(), ws_bytes)
-    return out
+    return _Refused.apply("mxfp4_moe is not differentiable", out, *inputs) if asked else out

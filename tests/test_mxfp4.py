@@ -644,3 +644,106 @@ def test_the_linear_method_on_mxfp4_tensors(m):
     held = torch.nn.Module()
     held._quant_weight, held.bias = loader.make_awq_weight({"qweight": c, "scales": s}), b.cuda()
     assert torch.equal(AWQConfig().apply(held.cuda(), x), want)
+
+
+# ------------------------------------------------------------------ derivatives
+def _without_launches(monkeypatch):
+    """The operators on CPU tensors, nothing launched."""
+    from litevllm_amd import moe_balance, mxfp4
+    monkeypatch.setattr(mxfp4, "_call", lambda *a: None)
+    monkeypatch.setattr(moe_balance, "_call", lambda *a: None)
+    monkeypatch.setattr(mxfp4.ops, "_require_device", lambda *t: torch.device("cpu"))
+
+
+def _leaves():
+    return (torch.randn(3, 64, dtype=torch.bfloat16, requires_grad=True), torch.randn(48, requires_grad=True),
+            torch.rand(3, 2, requires_grad=True))
+
+
+def _calls(x, bias, weights):
+    """Name -> a call with a floating result, and the leaves that it depends on."""
+    from litevllm_amd import MXFP4Experts, MXFP4Weight, mxfp4_gemm, mxfp4_moe
+    dev = x.device
+    c, s = (t.to(dev) for t in R.quantize(_made(120, 48, 64)))
+    gu, dn = (MXFP4Experts(*(t.to(dev) for t in R.quantize(_made(121, 4, *shape)))) for shape in ((64, 64), (64, 32)))
+    ids = torch.zeros(3, 2, dtype=torch.int32, device=dev)
+    return {"gemm": (lambda: mxfp4_gemm(x, c, s), [x]), "bias": (lambda: mxfp4_gemm(x.detach(), c, s, bias=bias), [bias]),
+            "weight": (lambda: MXFP4Weight(c, s).matmul(x, bias), [x, bias]),
+            "moe": (lambda: mxfp4_moe(x, weights, ids, gu, dn), [x, weights]),
+            "routing": (lambda: mxfp4_moe(x.detach(), weights, ids, gu, dn), [weights])}
+
+
+@pytest.mark.parametrize("name", ["gemm", "bias", "weight", "moe", "routing"])
+def test_a_derivative_is_refused_and_not_dropped(name, monkeypatch):
+    _without_launches(monkeypatch)
+    x, bias, weights = _leaves()
+    call, leaves = _calls(x, bias, weights)[name]
+    y = call()
+    assert y.requires_grad and y.dtype == torch.bfloat16
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        y.float().sum().backward()
+    for leaf in leaves:  # also where the leaf has another way into the result
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(call().float().sum() + (2 * leaf.float()).sum(), leaf)
+    with torch.no_grad():
+        assert not call().requires_grad
+    for leaf in (x, bias, weights):
+        leaf.requires_grad_(False)
+    assert not call().requires_grad
+
+
+def test_where_a_result_cannot_carry_the_refusal_the_call_is_refused(monkeypatch):
+    import torch.autograd.forward_ad as fwd
+
+    from litevllm_amd import MXFP4Experts, MXFP4Weight, moe_balance_loss, mxfp4_gemm, mxfp4_moe, mxfp4_quantize
+    _without_launches(monkeypatch)
+    x, bias, weights = _leaves()
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        mxfp4_quantize(x)
+    with torch.no_grad():
+        mxfp4_quantize(x)
+    assert not MXFP4Weight.from_dense(x).scales.requires_grad  # a weight's conversion takes its values
+    c, s = R.quantize(_made(120, 48, 64))
+    gu, dn = (MXFP4Experts(*R.quantize(_made(121, 4, *shape))) for shape in ((64, 64), (64, 32)))
+    ids = torch.zeros(3, 2, dtype=torch.int32)
+    for call in (lambda out: mxfp4_gemm(x, c, s, out=out[:, :48]), lambda out: mxfp4_moe(x, weights, ids, gu, dn, out=out)):
+        out = torch.zeros(3, 64, dtype=torch.bfloat16)
+        with pytest.raises(RuntimeError, match="out="):
+            call(out)
+        with torch.no_grad():
+            call(out)
+    x, bias, weights = (t.detach() for t in (x, bias, weights))
+    logits = torch.randn(3, 4)
+    with fwd.dual_level():
+        dx, db, dw, dl = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, bias, weights, logits))
+        for call in (lambda: mxfp4_quantize(dx), lambda: mxfp4_gemm(dx, c, s), lambda: mxfp4_gemm(x, c, s, bias=db),
+                     lambda: mxfp4_moe(dx, weights, ids, gu, dn), lambda: mxfp4_moe(x, dw, ids, gu, dn), lambda: moe_balance_loss(dl, ids)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        mxfp4_gemm(x, c, s, bias=bias)
+        moe_balance_loss(logits, ids)
+
+
+def test_a_second_derivative_of_the_balance_loss_is_refused_and_not_dropped(monkeypatch):
+    from litevllm_amd import moe_balance_loss
+    _without_launches(monkeypatch)
+    z, up = torch.randn(3, 4, requires_grad=True), torch.tensor(2.0, requires_grad=True)
+    loss, _ = moe_balance_loss(z, torch.zeros(3, 2, dtype=torch.int32))
+    g, = torch.autograd.grad(loss, z, up, create_graph=True)
+    for leaf in (z, up):  # also where the leaf has another way into the result
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad(g.sum() + (2 * leaf).sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_results_that_refuse_a_derivative_are_the_same():
+    x, bias, weights = (t.detach().cuda().requires_grad_(True) for t in _leaves())
+    for call, _ in _calls(x, bias, weights).values():
+        y = call()
+        with torch.no_grad():
+            assert torch.equal(y, call())
+        assert y.requires_grad
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            y.float().sum().backward()
