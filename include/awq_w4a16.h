@@ -416,7 +416,7 @@ int awq_w4a16_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void
                                int32_t out_dtype, void* stream);
 
 /* Workspace bytes of awq_w4a16_mxfp4_gemm for an `a` that is not quantised yet (no zeroing needed; 0 for few
- * rows, which the kernel quantises itself). */
+ * rows, which the kernel quantises itself, and, like the queries below, for sizes that the call refuses). */
 size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /* C[M, N] = A . W^T (+ bias), both operands MXFP4, sums and bias in fp32, one rounding to act_dtype (F16 or

@@ -17,6 +17,13 @@ constexpr int64_t kMaxBalance = (int64_t)1 << 30;  // tokens and routes: 32 bits
 constexpr int64_t kMaxN = kIntMax - 255;       // columns of a block, those behind the last too, in 32 bits
 constexpr int64_t kMaxK = (int64_t)1 << 24;   // 256 rows of codes are addressed in 32 bits,
 constexpr int64_t kBytes = 0xFFFF0000LL;      // and so are all of the tokens' and all of an expert's gate and up
+
+// What the calls take; their workspace queries answer 0 for the rest.
+bool gemm_fits(int64_t M, int64_t N, int64_t K) { return M <= kIntMax && N <= kMaxN && K <= kMaxK; }
+bool moe_fits(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k) {
+  return E <= 1024 && H <= kMaxK && I <= kMaxK && T <= kIntMax && T * top_k <= kIntMax && T * (H / 2) <= kBytes && I * H <= kBytes;
+}
+bool balance_fits(int64_t T, int32_t E) { return E <= 1024 && T <= kMaxBalance; }
 }  // namespace
 
 extern "C" {
@@ -42,7 +49,7 @@ int awq_w4a16_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void
 }
 
 size_t awq_w4a16_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || mx_quantizes_itself(M, K)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !gemm_fits(M, N, K) || mx_quantizes_itself(M, K)) return 0;
   return align256((size_t)M * (size_t)(K / 2)) + (size_t)M * (size_t)(K / 32);
 }
 
@@ -52,7 +59,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
   if (M < 0 || N < 0 || K <= 0 || (K % 32) != 0) return AWQ_ERR_SHAPE;
   if (M == 0 || N == 0) return AWQ_OK;
   if (!a || !w || !w_scales || !c) return AWQ_ERR_NULL;
-  if (!dtype_16(act_dtype) || M > kIntMax || N > kMaxN || K > kMaxK) return AWQ_ERR_UNSUPPORTED;
+  if (!dtype_16(act_dtype) || !gemm_fits(M, N, K)) return AWQ_ERR_UNSUPPORTED;
   if (bias ? !dtype_float(bias_dtype) : bias_dtype != AWQ_DTYPE_NONE) return AWQ_ERR_UNSUPPORTED;
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(c, 2) || ldc < N) return AWQ_ERR_STRIDE;
   MxArgs p{};
@@ -94,7 +101,7 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
 }
 
 size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k) {
-  if (T <= 0 || H <= 0 || I <= 0 || E <= 0 || top_k <= 0) return 0;
+  if (T <= 0 || H <= 0 || I <= 0 || E <= 0 || top_k <= 0 || !moe_fits(T, H, I, E, top_k)) return 0;
   return (size_t)mx_moe_workspace(T, H, I, E, top_k).total;
 }
 
@@ -107,8 +114,7 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
   if (!x || !topk_ids || !topk_weights || !gate_up || !gate_up_scales || !down || !down_scales || !out) return AWQ_ERR_NULL;
   if (!dtype_16(act_dtype) || !dtype_float(weights_dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
   if (activation != AWQ_MOE_ACT_SILU && activation != AWQ_MOE_ACT_GELU_TANH) return AWQ_ERR_UNSUPPORTED;
-  if (E > 1024 || H > kIntMax || 2 * I > kIntMax || T > kIntMax || T * top_k > kIntMax) return AWQ_ERR_UNSUPPORTED;
-  if (H > kMaxK || I > kMaxK || T * (H / 2) > kBytes || I * H > kBytes) return AWQ_ERR_UNSUPPORTED;
+  if (!moe_fits(T, H, I, E, top_k)) return AWQ_ERR_UNSUPPORTED;
   if ((T > 1 && (ldx < H || (ldx % 8) != 0 || ldo < H)) || !aligned(x, 16) || !aligned(out, 2)) return AWQ_ERR_STRIDE;
   if (!aligned(gate_up, 16) || !aligned(down, 16)) return AWQ_ERR_STRIDE;
   if (!workspace || workspace_bytes < awq_w4a16_mxfp4_moe_workspace_bytes(T, H, I, E, top_k)) return AWQ_ERR_WORKSPACE;
@@ -122,7 +128,7 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
 }
 
 size_t awq_w4a16_moe_balance_workspace_bytes(int64_t T, int32_t E) {
-  return T < 0 || E <= 0 ? 0 : balance_workspace_bytes(T, E);
+  return T < 0 || E <= 0 || !balance_fits(T, E) ? 0 : balance_workspace_bytes(T, E);
 }
 
 int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, const void* topk_ids, int32_t ids_bits,
@@ -131,7 +137,7 @@ int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, 
   if (T < 0 || E <= 0 || top_k <= 0) return AWQ_ERR_SHAPE;
   if (!loss || !counts || !factor || (T > 0 && (!logits || !topk_ids))) return AWQ_ERR_NULL;
   if (!dtype_float(logits_dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
-  if (E > 1024 || T > kMaxBalance || T * top_k > kMaxBalance) return AWQ_ERR_UNSUPPORTED;
+  if (!balance_fits(T, E) || T * top_k > kMaxBalance) return AWQ_ERR_UNSUPPORTED;
   if (T > 1 && ld < E) return AWQ_ERR_STRIDE;
   if (!workspace || workspace_bytes < balance_workspace_bytes(T, E)) return AWQ_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return AWQ_ERR_STRIDE;
@@ -144,7 +150,7 @@ int awq_w4a16_moe_balance_grad(const void* logits, int64_t ld, int32_t logits_dt
   if (T < 0 || E <= 0) return AWQ_ERR_SHAPE;
   if (T == 0) return AWQ_OK;
   if (!logits || !factor || !upstream || !grad) return AWQ_ERR_NULL;
-  if (!dtype_float(logits_dtype) || E > 1024 || T > kMaxBalance) return AWQ_ERR_UNSUPPORTED;
+  if (!dtype_float(logits_dtype) || !balance_fits(T, E)) return AWQ_ERR_UNSUPPORTED;
   if (T > 1 && ld < E) return AWQ_ERR_STRIDE;
   return launch_moe_balance_grad(logits, ld, logits_dtype, mask, factor, upstream, grad, T, E, (hipStream_t)stream);
 }

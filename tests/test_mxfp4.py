@@ -747,3 +747,20 @@ def test_results_that_refuse_a_derivative_are_the_same():
         assert y.requires_grad
         with pytest.raises(RuntimeError, match="not differentiable"):
             y.float().sum().backward()
+
+
+def test_workspace_queries_answer_nothing_for_what_the_calls_refuse():
+    lib = L.load()
+    big = (1 << 31, 1 << 40, 1 << 62, (1 << 63) - 1)
+    for t in ((1 << 30) + 1, *big):
+        assert lib.awq_w4a16_moe_balance_workspace_bytes(t, 8) == 0
+    assert lib.awq_w4a16_moe_balance_workspace_bytes(1 << 30, 8) > 0 < lib.awq_w4a16_moe_balance_workspace_bytes(0, 8)
+    assert lib.awq_w4a16_moe_balance_workspace_bytes(4, 1025) == 0
+    for n in big:
+        assert lib.awq_w4a16_mxfp4_gemm_workspace_bytes(n, 64, 64) == 0 == lib.awq_w4a16_mxfp4_gemm_workspace_bytes(64, 64, n)
+        assert lib.awq_w4a16_mxfp4_gemm_workspace_bytes(64, n, 64) == 0
+        assert lib.awq_w4a16_mxfp4_moe_workspace_bytes(n, 64, 64, 8, 1) == 0 == lib.awq_w4a16_mxfp4_moe_workspace_bytes(2, n, 64, 8, 1)
+        assert lib.awq_w4a16_mxfp4_moe_workspace_bytes(2, 64, n, 8, 1) == 0
+    assert lib.awq_w4a16_mxfp4_moe_workspace_bytes(1 << 20, 64, 64, 8, 1 << 12) == 0 == lib.awq_w4a16_mxfp4_moe_workspace_bytes(2, 64, 64, 1025, 1)
+    # 2^31 - 1 rows, and their codes and scales
+    assert lib.awq_w4a16_mxfp4_gemm_workspace_bytes((1 << 31) - 1, 64, 1 << 24) >= ((1 << 31) - 1) * ((1 << 23) + (1 << 19))
