@@ -564,19 +564,20 @@ __device__ __forceinline__ u32x4 rsrc_words(const void* base, uint32_t nbytes) {
 // each of them); a kernel waits for these loads itself before its barrier.  M0 carries the
 // LDS address and nothing else in these kernels uses M0.
 // The waits in front of the load are in the assembly too, as the compiler does not see that it is one: a state behind
-// the write of M0, and five behind a vector instruction that wrote a scalar register of it (a spilled descriptor comes
-// back by v_readlane).  tests/test_isa_waits.py looks for them in the built library.
-#define AWQ_LDS_DMA_WAIT "s_nop 3\n\t"
+// the write of M0, and, SPILLS, five behind a vector instruction that wrote a scalar register of it, as v_readlane does that
+// brings a spilled one back.  (For every kernel these cost 1 % of a prefill of 512 to 2048 rows; tests/test_isa_waits.py
+// looks for missing waits in the built library.)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+template <bool SPILLS = false>
 __device__ __forceinline__ void lds_dma16(const u32x4& rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\t" AWQ_LDS_DMA_WAIT "buffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
+               : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff), "n"(SPILLS ? 3 : 0)
                : "memory", "m0");
 }
 __device__ __forceinline__ void lds_dma4(const u32x4& rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\t" AWQ_LDS_DMA_WAIT "buffer_load_dword %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");

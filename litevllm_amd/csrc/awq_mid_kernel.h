@@ -75,7 +75,7 @@ __host__ __device__ constexpr MidLds mid_lds(int mt, int gk) {
 template <bool NT>
 __device__ __forceinline__ void mid_dma_w(const u32x4& rsrc, uint32_t lds, uint32_t voff, uint32_t soff) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\t" AWQ_LDS_DMA_WAIT "buffer_load_dwordx4 %1, %2, %3 offen nt lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rsrc), "s"(soff)
                  : "memory", "m0");

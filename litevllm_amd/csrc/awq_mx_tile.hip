@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
     auto all = [&](uint32_t voff, uint32_t soff) {
 #pragma unroll
       for (int u = from; u < to && u < LOADS; ++u)
-        lds_dma16(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u] + voff, soff);
+        lds_dma16<true>(u < A_LOADS ? ars : wrs, lds0 + (uint32_t)((s & 1) * STAGE + (u * WAVES + wave) * 1024), src[u] + voff, soff);
     };
     if (s < whole) all(0u, mx_code_position(s0 + s));
     else all(mx_code_position(s0 + s), 0u);
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
     for (int u = 0; u < SLOADS; ++u) {
       const int at = u * WAVES + wave;
       if (ROWS % (64 * WAVES) != 0 && at * 64 >= ROWS) continue;
-      lds_dma16(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u] + mx_scale_position(s0, g), 0u);
+      lds_dma16<true>(at * 64 < BM ? asrs : wsrs, lds0 + SCALES + (uint32_t)((g & 1) * ROWS * 16 + at * 1024), ssrc[u] + mx_scale_position(s0, g), 0u);
     }
   };
 
