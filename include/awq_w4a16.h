@@ -457,6 +457,7 @@ int awq_w4a16_mxfp4_moe(const void* x, int64_t ldx, const void* topk_ids, int32_
  *   logits: [T, ld] of logits_dtype;  topk_ids: [T, top_k] int32 or int64, dense;  mask: NULL or [T] bytes;
  *   loss: 1 float;  counts: [E];  factor: [E] floats for awq_w4a16_moe_balance_grad.  E <= 1024;
  *   up to 2^30 tokens and routes.
+ *   Probabilities are summed in fp32 in chains of at most 512, blocks' sums and the loss in fp64.
  *   Results are bitwise reproducible.  workspace: 16-byte aligned, no zeroing needed. */
 size_t awq_w4a16_moe_balance_workspace_bytes(int64_t T, int32_t E);
 int awq_w4a16_moe_balance(const void* logits, int64_t ld, int32_t logits_dtype, const void* topk_ids,

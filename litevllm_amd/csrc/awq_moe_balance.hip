@@ -15,7 +15,7 @@
 
 namespace awq {
 
-constexpr int kBalThreads = 1024, kBalWaves = kBalThreads / 64;
+constexpr int kBalThreads = 1024, kBalWaves = kBalThreads / 64, kBalChain = 512;
 
 // Steps of a reduction over G = 16, 32 or 64 neighbouring lanes: DPP inside rows of 16, then across rows.
 template <int G, class Op>
@@ -114,24 +114,31 @@ __global__ void __launch_bounds__(kBalThreads) balance_rows_kernel(BalanceArgs a
     const int64_t e = a.id64 ? ((const int64_t*)a.ids)[i] : (int64_t)((const int32_t*)a.ids)[i];
     if (e >= 0 && e < a.E) atomicAdd(&hist[e], 1);
   }
-  float acc[V] = {};
+  // Sums in chains of at most kBalChain rows, and a chain of those, at most as many up to 2^30 tokens: 2 * 512 roundings, where
+  // one chain would have up to 262144 (2^27 equal rows of p = 0.25: off by 3e-6, by 1.2e-4 in one chain).
+  float acc[V] = {}, all[V] = {};
   int kept = 0;
-  for (int base = first + wave * PER; base < end; base += kBalWaves * PER) {
-    const int row = base + lane / G;
-    if (row >= end || (a.mask && !a.mask[row])) continue;
-    ++kept;
-    float p[V];
-    load_row<T, G, V>(a.logits, (int64_t)row * a.ld, a.E, l, p);
-    row_softmax<G, V>(p);
+  for (int base = first + wave * PER; base < end;) {
+    const int stop = min(base + kBalChain * kBalWaves * PER, end);
+    for (; base < stop; base += kBalWaves * PER) {
+      const int row = base + lane / G;
+      if (row >= end || (a.mask && !a.mask[row])) continue;
+      ++kept;
+      float p[V];
+      load_row<T, G, V>(a.logits, (int64_t)row * a.ld, a.E, l, p);
+      row_softmax<G, V>(p);
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += p[v];
+      for (int v = 0; v < V; ++v) acc[v] += p[v];
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) all[v] += acc[v], acc[v] = 0.f;
   }
   if (l == 0 && kept) atomicAdd(&kept_all, kept);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    if constexpr (G <= 16) acc[v] += __shfl_xor(acc[v], 16);
-    if constexpr (G <= 32) acc[v] += __shfl_xor(acc[v], 32);
-    if (lane < G) sums[wave][G * v + l] = acc[v];
+    if constexpr (G <= 16) all[v] += __shfl_xor(all[v], 16);
+    if constexpr (G <= 32) all[v] += __shfl_xor(all[v], 32);
+    if (lane < G) sums[wave][G * v + l] = all[v];
   }
   __syncthreads();
   float s = 0.f;

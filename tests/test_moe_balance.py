@@ -328,3 +328,22 @@ def test_saved_tensors_that_come_back_elsewhere_or_as_others_are_refused():
             loss, _ = moe_balance_loss(z, ids)
         with pytest.raises((RuntimeError, ValueError)):
             loss.backward()
+
+
+@pytest.mark.gpu
+def test_sums_over_many_tokens():
+    """2^27 equal rows.  Their probability, just below the middle between two fp32 numbers next to sums past 1024, is rounded
+    down in every addition to such a sum: one chain of a lane's 8192 rows is off by 1.2e-4.  The bound: chains of 512, the 16 of
+    them, the 16 waves, and the blocks' sums in fp64."""
+    import math
+
+    from litevllm_amd import moe_balance_loss
+    t = 1 << 27
+    p = 0.25 + 0.49 * 2.0 ** -13
+    row = torch.tensor([math.log(p / (1 - p)), 0.0], device="cuda")
+    z = row.expand(t, 2).contiguous()
+    loss, counts = moe_balance_loss(z, torch.zeros(t, 1, dtype=torch.int32, device="cuda"))
+    assert counts.tolist() == [t, 0]
+    want = 2 * float(torch.softmax(row.double(), 0)[0])
+    tol = float(_prob_error(row.unsqueeze(0)).max()) + (512 + 16 + 16 + 2) * 2.0 ** -24
+    assert abs(float(loss) - want) <= want * tol, (float(loss) / want - 1, tol)
