@@ -764,3 +764,56 @@ def test_workspace_queries_answer_nothing_for_what_the_calls_refuse():
     assert lib.awq_w4a16_mxfp4_moe_workspace_bytes(1 << 20, 64, 64, 8, 1 << 12) == 0 == lib.awq_w4a16_mxfp4_moe_workspace_bytes(2, 64, 64, 1025, 1)
     # 2^31 - 1 rows, and their codes and scales
     assert lib.awq_w4a16_mxfp4_gemm_workspace_bytes((1 << 31) - 1, 64, 1 << 24) >= ((1 << 31) - 1) * ((1 << 23) + (1 << 19))
+
+
+# ------------------------------------------------------------------ scales far apart inside one sum
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 70, 416), (9, 300, 1280), (48, 70, 2080), (260, 130, 4128), (700, 4100, 1056), (2100, 2100, 288)])
+def test_gemm_blocks_of_one_sum_far_apart(m, n, k):
+    """Blocks of both operands 2^-25 to 2^25: terms up to 2^100 apart meet in a sum."""
+    from litevllm_amd import mxfp4_gemm
+    g = torch.Generator().manual_seed(m)
+    a, w = (torch.randint(0, 256, (r, k // 2), generator=g).to(torch.uint8).cuda() for r in (m, n))
+    sa, sw = (torch.randint(102, 153, (r, k // 32), generator=g).to(torch.uint8).cuda() for r in (m, n))
+    y = mxfp4_gemm(a, w, sw, a_scales=sa, out_dtype=torch.bfloat16)
+    _close(y, *R.gemm(R.values(a, sa), R.values(w, sw)), torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 70, 416), (9, 300, 1280), (48, 70, 2080), (260, 130, 4128), (700, 4100, 1056), (2100, 2100, 288)])
+def test_gemm_smallest_and_largest_scales(m, n, k):
+    """Scale bytes 0 and 254 in both operands: the other one of a block is near 254 and 0, so the products are near 1."""
+    from litevllm_amd import mxfp4_gemm
+    g = torch.Generator().manual_seed(m + 1)
+    a, w = (torch.randint(0, 256, (r, k // 2), generator=g).to(torch.uint8).cuda() for r in (m, n))
+    ends = torch.randint(0, 2, (k // 32,), generator=g) * 254
+    ends[:2] = torch.tensor([0, 254])
+    near = torch.randint(0, 4, (n, k // 32), generator=g)
+    sa = ends.expand(m, -1).to(torch.uint8).cuda()
+    sw = torch.where(ends == 0, 254 - near, near).to(torch.uint8).cuda()
+    y = mxfp4_gemm(a, w, sw, a_scales=sa, out_dtype=torch.bfloat16)
+    ref = R.gemm(R.values(a, sa), R.values(w, sw))
+    _close(y, *ref, torch.bfloat16)
+    if n == m:  # the operands' places changed
+        z = mxfp4_gemm(w, a, sa, a_scales=sw, out_dtype=torch.bfloat16)
+        _close(z, ref[0].t(), ref[1].t(), torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,e,k,h,i", [(2, 9, 3, 160, 64), (9, 2, 2, 416, 96), (40, 16, 4, 256, 64), (500, 5, 4, 288, 96)])
+def test_moe_blocks_of_one_sum_far_apart(t, e, k, h, i):
+    """The gate and up stack's blocks 2^-20 to 2^20 times their size, the tokens' the other way round, block by block but for 2^3:
+    the sums stay in the range that the activation is tested in."""
+    from litevllm_amd import MXFP4Experts, mxfp4_moe
+    g = torch.Generator().manual_seed(t)
+    c1, s1, _ = _weight(t, e, 2 * i, h)
+    c2, s2, _ = _weight(t + 1, e, h, i)
+    by = torch.randint(-20, 21, (h // 32,), generator=g)
+    s1 = (s1.int() + by.cuda() + torch.randint(-1, 2, s1.shape, generator=g).cuda()).to(torch.uint8)
+    x = (_made(t, t, h) * torch.pow(2.0, -by.float()).repeat_interleave(32)).bfloat16().cuda()
+    ids, weights = torch.randint(0, e, (t, k), generator=g), torch.rand(t, k, generator=g)
+    y = mxfp4_moe(x, weights.cuda(), ids.cuda(), MXFP4Experts(c1, s1), MXFP4Experts(c2, s2))
+    # on the CPU: the GPU's powers of two are not exact at all of these exponents, and a tie is then none
+    whole = torch.arange(-127, 128, dtype=torch.float64)
+    assert torch.pow(2.0, whole).tolist() == [2.0 ** n for n in range(-127, 128)]
+    _close(y.cpu(), *R.moe(x.cpu(), weights, ids, R.values(c1.cpu(), s1.cpu()), R.values(c2.cpu(), s2.cpu()), "silu"), torch.bfloat16)
