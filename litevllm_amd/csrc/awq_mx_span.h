@@ -2,8 +2,8 @@
 // every address (tests/mx_span_walk.cpp).
 //
 // The range check covers the VGPR offset, per dword of a load; whether the SGPR offset counts is documented as no, and
-// measured as yes on gfx950.  So a stage's position along K is in the SGPR offset only where all of the stage lies inside K,
-// and no load of it leaves its row; the stages that pass K's end have it in the VGPR offset, and so have all scales, and
+// measured as yes on gfx950.  So a stage's position along K may be in the SGPR offset only where all of the stage lies inside
+// K, and no load of it leaves its row; the stages that pass K's end have it in the VGPR offset, and so have all scales, and
 // the check ends them with the operand.
 #pragma once
 

@@ -98,7 +98,11 @@ __global__ void __launch_bounds__(WM * WN * WK * 64, PER_SIMD) mx_tile_kernel(Mx
   const int lane = tid & 63, r = lane & 15, q = lane >> 4, ptid = tid - part * (WAVES * 64);
   const int KB = p.K / 32;
   // the share's stages, as if the operands began and ended there (a share behind K's end: stages of nothing)
-  const int stages = ((KB + 7) / 8 + WK - 1) / WK, s0 = part * stages, blocks = KB - 8 * s0, whole = mx_whole_stages(KB, s0, stages);
+  const int stages = ((KB + 7) / 8 + WK - 1) / WK, s0 = part * stages, blocks = KB - 8 * s0;
+  // Stages whose position is in the scalar offset: all that may have it (awq_mx_span.h) where no register is left for sums
+  // (256 x 256 243 us against 245) or K is in shares (M = 57, N = 6144 11.4 and 11.7), else none, for a branch less
+  // (M = 700, N = 4096 20.8 and 20.1; M = 200, N = 5001 17.2 and 16.8; 2048 tokens through 64 experts 171.5 and 170.8).
+  const int whole = BM == 256 || WK > 1 ? mx_whole_stages(KB, s0, stages) : 0;
   // the wave's rows and columns in the tile
   const int m0 = (wave / WN) * TM * 16, c0 = BM + (wave % WN) * TN * 16;
 
