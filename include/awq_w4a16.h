@@ -433,7 +433,9 @@ int awq_w4a16_mxfp4_gemm(const void* a, int64_t lda, const uint8_t* a_scales, co
                          int64_t K, int32_t act_dtype, int32_t bias_dtype, void* workspace,
                          size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of awq_w4a16_mxfp4_moe (no zeroing needed). */
+/* Workspace bytes of awq_w4a16_mxfp4_moe (no zeroing needed): they grow with T * top_k * (4 H + 17 I / 32), 7.8 GB for
+ * 32768 tokens, top 8, H = 7168, I = 2048.  Tokens may be cut into calls: a token's result does not depend on the others'
+ * but for the rounding of its sums, whose order goes by the number of routes. */
 size_t awq_w4a16_mxfp4_moe_workspace_bytes(int64_t T, int64_t H, int64_t I, int32_t E, int32_t top_k);
 
 /* awq_w4a16_moe over MXFP4 stacks: with e = ids[t, j],

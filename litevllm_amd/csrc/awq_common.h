@@ -603,8 +603,9 @@ __device__ __forceinline__ void pin_after_wait(V& v) {
 }
 
 // Buffer resource over a whole tensor (raw addressing, bounds = nbytes).  Range checks
-// cover the VGPR offset only (the SGPR offset is excluded), so anything that must read as
-// zero past the end has to carry its position in the VGPR offset.
+// cover the VGPR offset, per dword; the SGPR offset is documented as excluded (measured on gfx950: it
+// counts), so anything that must read as zero past the end has to carry its position in the
+// VGPR offset.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint32_t nbytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)nbytes, 0x00020000);
 }

@@ -5,7 +5,7 @@
 //   d loss / d logits_te = p_te (F_e - sum_j F_j p_tj),  F_e = E f_e / n  (f is piecewise constant)
 // A row of nothing but -inf has no probabilities: p = 0.  No kept token: loss 0, gradient 0.
 // Both passes read the logits once; the gradient computes the softmax again instead of keeping it (65536 tokens, 160
-// experts, fp32: 42 MB; forward 10.5 us and 3.4 for the join, gradient 13.6 us, which reads and writes at 6.2 TB/s, partly
+// experts, fp32: 42 MB; forward 10.6 us and 7.1 for the join, gradient 13.9 us, which reads and writes at 6.2 TB/s, partly
 // from the caches).  Shorter calls are latencies and the launches; with a gradient the host is slower than the kernels
 // from a call of 16384 tokens, 64 experts on down (10.5 us of kernels).
 #include <algorithm>
@@ -223,7 +223,7 @@ namespace awq_host {
 using namespace awq;
 
 // Up to 256 rows one block does everything (one launch); else at most a block per CU, so that the join, whose one block
-// reads every block's sums, stays small (256 blocks of 160 experts: 3.4 us).
+// reads every block's sums, stays small (256 blocks of 160 experts: 7.1 us, of 64: 5.8).
 static int balance_rows(int64_t T) { return T <= 256 ? 256 : (int)cdiv(T, std::min<int64_t>(256, cdiv(T, 64))); }
 static int balance_blocks(int64_t T) { return (int)std::max<int64_t>(1, cdiv(T, balance_rows(T))); }
 

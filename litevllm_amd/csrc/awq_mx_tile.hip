@@ -59,8 +59,9 @@ __device__ __forceinline__ void swap_rows(u32x4& x, u32x4& y, bool low) {
 // the results of the tile before go out, which takes no LDS (M = 4096, N = 24576, K = 4096: 228 us with blocks of one tile
 // whose results go through LDS, 221 so; K = 1024 90 and 82; 100 tokens through 64 experts 53 and 48).
 //
-// What bounds it (M = 4096, N = 24576, K = 4096, 221 us, 3.7 PFLOP/s): its products alone take 143, its LDS reads 98, its
-// loads 128, products and reads 168, all but the stores 204, scales that need not be read 212.
+// What bounds it (M = 4096, N = 24576, K = 4096, 221 to 235 us by card and run, 3.5 to 3.7 PFLOP/s): where it takes 221, its
+// products alone take 143, its LDS reads 98, its loads 128, products and reads 168, all but the stores 204, scales that need
+// not be read 212.
 //
 // LDS: 16-byte chunk c (block c of the stage) of a row at place c ^ (row & 7) of its 128 bytes, so that the 16
 // rows of a fragment lie in different banks; the direct loads write lanes in order, so it is their sources that

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(128 * NWN, 2) prefill_stream_kernel(const Gemm
     }
   };
   // stage s's weight piece, scales and zero word into slot s & 1 (NB loads).  The stage's run
-  // offset s * 4096 rides in soffset, which the buffer range check does not cover, so a piece
+  // offset s * 4096 rides in soffset, which the buffer range check need not cover, so a piece
   // whose k-step 2 s + pks lies past K (stages past the last one, and the upper half of a last
   // half stage when K % 64 == 32) reads through an empty descriptor instead: zeros, no traffic.
   // Its activations are zero, so the zero piece adds nothing.
