@@ -43,6 +43,7 @@ class _Refused(torch.autograd.Function):
     @staticmethod
     def forward(ctx, why, result, *inputs):
         ctx.why = why
+        ctx.mark_dirty(result)  # the result itself, no view of it
         return result
 
     @staticmethod

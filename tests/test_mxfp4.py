@@ -817,3 +817,18 @@ def test_moe_blocks_of_one_sum_far_apart(t, e, k, h, i):
     whole = torch.arange(-127, 128, dtype=torch.float64)
     assert torch.pow(2.0, whole).tolist() == [2.0 ** n for n in range(-127, 128)]
     _close(y.cpu(), *R.moe(x.cpu(), weights, ids, R.values(c1.cpu(), s1.cpu()), R.values(c2.cpu(), s2.cpu()), "silu"), torch.bfloat16)
+
+
+@pytest.mark.parametrize("name", ["gemm", "moe"])
+def test_a_result_that_refuses_a_derivative_can_be_written_to(name, monkeypatch):
+    _without_launches(monkeypatch)
+    call, (leaf, *_) = _calls(*_leaves())[name]
+    y = call()
+    assert not y._is_view()
+    y.zero_().add_(1.0)
+    y[0] = 3.0
+    assert y.detach().sum() == 2 * y.shape[1] + 3 * y.shape[1]
+    z = call()
+    z.add_(1.0)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(z.float().sum() + leaf.float().sum(), leaf)
