@@ -49,16 +49,18 @@ class _BalanceLoss(torch.autograd.Function):
         # saved-tensor hooks may give back copies with other strides
         logits, mask, buf = ctx.saved_tensors
         inputs = logits, upstream
-        dev, (t, experts) = ops._require_device(logits, mask, buf, upstream), ctx.shape
-        if logits.shape != ctx.shape or buf.dtype is not torch.float32 or buf.dim() != 1 or buf.shape[0] < experts or (
-                mask is not None and (mask.dtype is not torch.bool or mask.shape != (t,))):
-            raise RuntimeError("moe_balance_loss: saved tensors came back with other shapes or types")
-        logits = _rows(logits)
-        if mask is not None:
-            mask = mask.contiguous()
-        buf = buf.contiguous()
-        grad = torch.empty((t, experts), dtype=logits.dtype, device=dev)
-        _call(dev, "awq_w4a16_moe_balance_grad", logits.data_ptr(), logits.stride(0) if t > 1 else experts,
+        on, (t, experts) = upstream.get_device(), ctx.shape
+        if logits.get_device() != on or buf.get_device() != on or logits.shape != ctx.shape or (
+                buf.dtype is not torch.float32 or buf.numel() < experts) or (
+                mask is not None and (mask.get_device() != on or mask.dtype is not torch.bool or mask.shape != (t,))):
+            raise RuntimeError("moe_balance_loss: saved tensors came back elsewhere, or with other shapes or types")
+        ld = experts
+        if not logits.is_contiguous():
+            logits = _rows(logits)
+            ld = logits.stride(0)
+        mask, buf = None if mask is None else mask.contiguous(), buf.contiguous()
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        _call(logits.device, "awq_w4a16_moe_balance_grad", logits.data_ptr(), ld,
               ops.dtype_code(logits.dtype), ops._ptr(mask), buf.data_ptr(), upstream.data_ptr(), grad.data_ptr(), t, experts)
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
             grad = _Refused.apply("moe_balance_loss is not differentiable twice", grad, *inputs)
