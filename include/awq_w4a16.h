@@ -473,6 +473,49 @@ int awq_w4a16_moe_balance_grad(const void* logits, int64_t ld, int32_t logits_dt
                                const float* factor, const float* upstream, void* grad, int64_t T, int32_t E,
                                void* stream);
 
+/* ---- routes sorted by expert, and back ------------------------------------------------
+ * For experts whose products are not in this library: the tokens' rows in the order of the experts.  No counterpart in the
+ * reference, which sorts ids in its expert loop (fused_moe.py:17-56).  With R = T top_k routes r = t top_k + j in the order of
+ * (topk_ids[r], r), those with an id outside [0, E) left out:
+ *   offsets[e] .. offsets[e + 1] - 1 are the places of expert e;  experts[p]: the expert of place p, -1 behind the last;
+ *   places[t, j]: the place of a route, -1 for one that is left out;  rows[p] = x[t], 0 behind the last place.
+ *   x: [T, H] of dtype (F16, BF16 or F32), row stride ldx;  topk_ids: [T, top_k] int32 or int64, dense;  rows: [R, H] dense;
+ *   offsets: [E + 1];  experts: [R];  places: [T, top_k].  E <= 1024, R <= 2^30, H <= 2^24.  rows lie apart from x.
+ *   workspace: 16-byte aligned, no zeroing needed; calls that may overlap must not share one. */
+size_t awq_w4a16_moe_sort_workspace_bytes(int64_t T, int32_t E, int32_t top_k);
+int awq_w4a16_moe_sort(const void* x, int64_t ldx, const void* topk_ids, int32_t ids_bits, void* rows, int32_t* offsets,
+                       int32_t* experts, int32_t* places, int64_t T, int64_t H, int32_t E, int32_t top_k, int32_t dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[t] = sum over j of w[t, j] rows[places[t, j]] in slot order, fp32, one rounding; without topk_weights (NULL,
+ * weights_dtype NONE) w = 1: that is also the gradient of awq_w4a16_moe_sort in x.  Places outside [0, T top_k) add nothing.
+ *   rows: [T top_k, H] dense;  out: [T, H], row stride ldo, apart from rows;  topk_weights: [T, top_k] of weights_dtype. */
+int awq_w4a16_moe_unsort(const void* rows, const int32_t* places, const void* topk_weights, int32_t weights_dtype, void* out,
+                         int64_t ldo, int64_t T, int64_t H, int32_t top_k, int32_t dtype, void* stream);
+
+/* Its gradients, of which either may be left out (NULL): grad_rows[places[t, j]] = w[t, j] upstream[t], rows from total[0] on 0;
+ * grad_weights[t, j] = <upstream[t], rows[places[t, j]]>, 0 without a place.
+ *   upstream: [T, H], row stride ldu;  total: offsets + E of awq_w4a16_moe_sort;  grad_rows like rows, grad_weights like topk_weights
+ *   (which may be NULL for w = 1, with weights_dtype NONE, unless grad_weights is asked for). */
+int awq_w4a16_moe_unsort_grad(const void* upstream, int64_t ldu, const void* rows, const int32_t* places, const int32_t* total,
+                              const void* topk_weights, int32_t weights_dtype, void* grad_rows, void* grad_weights, int64_t T,
+                              int64_t H, int32_t top_k, int32_t dtype, void* stream);
+
+/* ---- low-rank adapters of many requests -------------------------------------------------
+ * What the reference adds behind a layer's quantised product (lite_linear.py:65-78), for all rows in one call:
+ *   out[m] = base[m] + s[l] (x[m] A_l^T) B_l^T,  l = ids[m];  out[m] = base[m] for an id outside [0, L).
+ * Sums in fp32; x A^T enters the second product with 16 bits of mantissa (bf16) or 21 (fp16); one rounding.
+ *   x: [M, K], base (NULL: zeros) and out: [M, N], all of dtype (F16 or BF16), row strides ldx, ldb, ldo;  lora_a: [L, R, K] and
+ *   lora_b: [L, N, R], dense but for the stride between adapters;  ids: [M] int32 or int64;  scales: [L] or NULL (1).
+ *   R <= 256; M <= 2^30, N and K <= 2^24.  Two bytes are alignment enough; 16 are faster.  out may be base (with its stride) and
+ *   lies apart from everything else.  Results are bitwise reproducible.
+ *   workspace: 16-byte aligned, no zeroing needed; calls that may overlap must not share one. */
+size_t awq_w4a16_lora_workspace_bytes(int64_t M, int64_t K, int64_t R);
+int awq_w4a16_lora_add(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* lora_a, int64_t a_stride,
+                       const void* lora_b, int64_t b_stride, const void* ids, int32_t ids_bits, const float* scales, void* out,
+                       int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t R, int32_t L, int32_t dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,7 @@ from .awq_triton import (  # noqa: F401
     packed_int4_fused_capability_check,
 )
 from .fused_pair import try_fused_awq_gate_up_activation, try_fused_awq_pair_matmul  # noqa: F401
+from .lora import LoRAAdapters, lora_add  # noqa: F401
 from .moe import (  # noqa: F401
     AWQExperts,
     awq_moe,
@@ -35,6 +36,7 @@ from .moe import (  # noqa: F401
     moe_route,
 )
 from .moe_balance import moe_balance_loss  # noqa: F401
+from .moe_sort import MoERoutes, moe_sort, moe_unsort  # noqa: F401
 from .mxfp4 import (  # noqa: F401
     MXFP4Experts,
     MXFP4Weight,

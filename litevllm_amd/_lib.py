@@ -101,6 +101,15 @@ SIGNATURES = {
                                              _c_p, _c_p, _c_p, _c_sz, _c_p]),
     "awq_w4a16_moe_balance_grad": (ctypes.c_int, [_c_p, _c_i64, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,
                                                   _c_p]),
+    "awq_w4a16_moe_sort_workspace_bytes": (_c_sz, [_c_i64, _c_i32, _c_i32]),
+    "awq_w4a16_moe_sort": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i32,
+                                          _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
+    "awq_w4a16_moe_unsort": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i32, _c_p, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_p]),
+    "awq_w4a16_moe_unsort_grad": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_i64, _c_i64,
+                                                 _c_i32, _c_i32, _c_p]),
+    "awq_w4a16_lora_workspace_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64]),
+    "awq_w4a16_lora_add": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_p, _c_p,
+                                          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_p, _c_sz, _c_p]),
 }
 
 MOE_ACT_SILU = 0

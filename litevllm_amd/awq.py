@@ -2,7 +2,8 @@
 caches an ``AWQWeight`` (zero points present) or ``PackedInt4Weight`` (none) on the
 layer at the first ``apply`` and forwards ``weight.matmul(x, layer.bias, config=...)``
 (``awq.py:40-104``).  A layer whose ``qweight`` and ``scales`` are both uint8 holds MXFP4 and
-gets an ``MXFP4Weight``."""
+gets an ``MXFP4Weight``.  With ``lora_ids`` the layer's ``lora_adapters`` are added to the product, where the
+reference adds its LoRA delta (``lite_linear.py:65-78``)."""
 from __future__ import annotations
 
 from typing import Any
@@ -28,6 +29,17 @@ class QuantizationConfig:
 
     def load_weights(self, layer: nn.Module, weights_iter):
         raise NotImplementedError
+
+
+def _with_lora(layer: nn.Module, y: torch.Tensor, x: torch.Tensor, ids: torch.Tensor | None) -> torch.Tensor:
+    """``y`` with the layer's adapters for the rows' ``ids`` (None: no request has one)."""
+    if ids is None:
+        return y
+    adapters = getattr(layer, "lora_adapters", None)
+    if adapters is None:
+        raise RuntimeError(f"lora_ids for layer '{getattr(layer, 'prefix', '<unknown>')}', which has no lora_adapters")
+    # y is this call's own: it takes the sum itself where no derivative can be asked for
+    return adapters.add(y, x, ids, out=None if torch.is_grad_enabled() else y)
 
 
 class AWQConfig(QuantizationConfig):
@@ -58,7 +70,8 @@ class AWQConfig(QuantizationConfig):
             if qweight is None or qweight.numel() <= 1:
                 w = getattr(layer, "weight", None)
                 if w is not None and w.numel() > 1:
-                    return torch.nn.functional.linear(x, w, getattr(layer, "bias", None))
+                    y = torch.nn.functional.linear(x, w, getattr(layer, "bias", None))
+                    return _with_lora(layer, y, x, kwargs.get("lora_ids"))
                 raise RuntimeError(f"AWQ weight not ready for layer '{prefix}'")
             if is_mxfp4(qweight, layer.scales):
                 layer._quant_weight = MXFP4Weight(qweight, layer.scales, prefix=getattr(layer, "prefix", ""))
@@ -80,7 +93,8 @@ class AWQConfig(QuantizationConfig):
                                           original_shape=getattr(layer, "weight_shape", None), **kw)
             layer._quant_weight = weight
         runtime_config = kwargs.get("inf_config", kwargs.get("config"))
-        return weight.matmul(x, getattr(layer, "bias", None), config=runtime_config)
+        y = weight.matmul(x, getattr(layer, "bias", None), config=runtime_config)
+        return _with_lora(layer, y, x, kwargs.get("lora_ids"))
 
     def load_weights(self, layer: nn.Module, weights_iter, expert_idx=None, part=None):
         for name, t in weights_iter:

@@ -166,4 +166,42 @@ int launch_moe_balance(const void* logits, int64_t ld, int dtype, const void* id
 int launch_moe_balance_grad(const void* logits, int64_t ld, int dtype, const uint8_t* mask, const float* factor, const float* upstream,
                             void* grad, int64_t T, int E, hipStream_t st);
 
+// ---- routes sorted by expert and back (awq_moe_sort.hip) ----
+size_t moe_sort_workspace_bytes(int64_t T, int E, int topk);
+struct MoeSortCall {
+  const void* x;
+  int64_t ldx;
+  const void* ids;
+  int id64;
+  void* rows;
+  int32_t *offsets, *experts, *places;
+  int64_t T, H;
+  int E, topk, elem_bytes;
+  void* workspace;
+};
+int launch_moe_sort(const MoeSortCall& c, hipStream_t st);
+// Forward: rows, weights (or NULL) to out.  Gradient: upstream, and what the wanted gradients take, to grad_rows and
+// grad_weights, either of which may be NULL; total: the number of places, on the device.
+struct MoeUnsortCall {
+  const void *rows, *weights, *upstream;
+  const int32_t *places, *total;
+  void *out, *grad_rows, *grad_weights;
+  int64_t T, H, ldo, ldu;
+  int topk, w_dtype, dtype;
+};
+int launch_moe_unsort(const MoeUnsortCall& c, hipStream_t st);
+int launch_moe_unsort_grad(const MoeUnsortCall& c, hipStream_t st);
+
+// ---- low-rank adapters (awq_lora.hip) ----
+size_t lora_workspace_bytes(int64_t M, int64_t K, int64_t R);
+struct LoraCall {
+  const void *base, *x, *a, *b, *ids;
+  const float* scales;
+  void* out;
+  int64_t ldb, ldx, ldo, a_stride, b_stride, M, N, K, R;
+  int L, id64, dtype;
+  void* workspace;
+};
+int launch_lora(const LoraCall& c, hipStream_t st);
+
 }  // namespace awq_host

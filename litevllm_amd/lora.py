@@ -1,0 +1,129 @@
+"""Low-rank adapters of many requests beside a shared projection: what the reference adds behind a layer's product
+(``lite_linear.py:65-78``), each row with its own adapter, in one call."""
+from __future__ import annotations
+
+from collections.abc import Sequence
+
+import torch
+import torch.nn as nn
+
+from . import _lib as L
+from . import ops
+from .mxfp4 import _call, _derivative_asked, _meet, _Refused
+from .moe_sort import _rows
+
+MAX_RANK = 256
+
+
+def _stack(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """An adapter stack, or a copy, dense but for the elements between adapters, and their number."""
+    count, rows, cols = t.shape
+    dense = rows * cols
+    if (cols > 1 and t.stride(2) != 1) or (rows > 1 and t.stride(1) != cols) or (count > 1 and t.stride(0) < dense):
+        t = t.contiguous()
+    return t, t.stride(0) if count > 1 else dense
+
+
+def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ids: torch.Tensor,
+             scales: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[m] = base[m] + scales[l] * (x[m] @ lora_a[l].T) @ lora_b[l].T`` with ``l = ids[m]``; ``base[m]`` where ``ids[m]`` is
+    outside ``[0, L)`` (a request without an adapter).
+
+    ``x [..., K]``, ``base [..., N]`` (None: zeros), fp16 or bf16; ``lora_a [L, R, K]`` and ``lora_b [L, N, R]`` in their type, R up
+    to 256 (adapters of lower ranks: zeros, :meth:`LoRAAdapters.stack`); ``ids [...]`` int32 or int64; ``scales`` fp32 ``[L]`` or
+    None (1).  Sums in fp32, ``x @ A^T`` enters the second product with 16 bits of mantissa (bf16) or 21 (fp16), one rounding.
+    ``out`` may be ``base`` itself, and lie over ``x`` or parts of ``base`` (which are copied first), over
+    no other operand.  Rows of the same adapter are cheapest next to each other, as a
+    request's tokens are.  Results are bitwise reproducible.  Not differentiable: a backward through the result
+    raises, and so does a call with ``out`` where an input requires a gradient."""
+    dev = ops._require_device(base, x, lora_a, lora_b, ids, scales, out)
+    if lora_a.dim() != 3 or lora_b.dim() != 3 or lora_a.shape[0] != lora_b.shape[0] or lora_a.shape[1] != lora_b.shape[2]:
+        raise ValueError(f"lora_a must be [L, R, K] and lora_b [L, N, R], got {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
+    adapters, rank, k = lora_a.shape
+    n = lora_b.shape[1]
+    if adapters < 1 or not 1 <= rank <= MAX_RANK or k < 1:
+        raise ValueError(f"at least one adapter and input, a rank of 1 to {MAX_RANK}, got lora_a {tuple(lora_a.shape)}")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"K mismatch: x is {tuple(x.shape)}, lora_a has {k}")
+    dtype, lead = x.dtype, x.shape[:-1]
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {dtype}: fp16 or bf16")
+    for what, t in (("base", base), ("lora_a", lora_a), ("lora_b", lora_b), ("out", out)):
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"{what} must be of x's type {dtype}, got {t.dtype}")
+    for what, t in (("base", base), ("out", out)):
+        if t is not None and t.shape != lead + (n,):
+            raise ValueError(f"{what} must be {tuple(lead + (n,))}, got {tuple(t.shape)}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if ids.shape != lead:
+        raise ValueError(f"ids must be {tuple(lead)}, got {tuple(ids.shape)}")
+    if scales is not None and (scales.dtype is not torch.float32 or scales.shape != (adapters,)):
+        raise ValueError(f"scales must be fp32 [{adapters}], got {scales.dtype} {tuple(scales.shape)}")
+    inputs = (base, x, lora_a, lora_b, scales)
+    asked = _derivative_asked("lora_add", out, *inputs)
+    m = ids.numel()
+    given, in_place = out is not None, out is not None and out is base
+    if out is None:
+        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+        to, ldo = out, n
+    else:
+        to = out if out.dim() == 2 else out.view(-1, n)  # raises where its rows are no matrix
+        ldo = to.stride(0) if m > 1 else n
+        if (n > 1 and to.stride(1) != 1) or ldo < n:
+            raise ValueError(f"bad_output: out must have dense rows apart from each other, got strides {out.stride()}")
+    if m == 0 or n == 0:
+        return out
+    x2, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+    at, ldb = None, n
+    if in_place:
+        at, ldb = to.data_ptr(), ldo
+    elif base is not None:
+        flat, ldb = _rows(base if base.dim() == 2 else base.reshape(-1, n))
+        if given and (flat.data_ptr() != to.data_ptr() or ldb != ldo) and _meet(flat, to):
+            flat, ldb = flat.clone(memory_format=torch.contiguous_format), n  # other elements of the same memory
+        at = flat.data_ptr()
+    if given and _meet(x2, to):
+        x2, ldx = x2.clone(memory_format=torch.contiguous_format), k  # read by blocks while others write
+    lora_a, a_stride = _stack(lora_a)
+    lora_b, b_stride = _stack(lora_b)
+    ids = ids.contiguous()
+    if scales is not None:
+        scales = scales.contiguous()
+    ws_bytes = L.load().awq_w4a16_lora_workspace_bytes(m, k, rank)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call(dev, "awq_w4a16_lora_add", at, ldb, x2.data_ptr(), ldx, lora_a.data_ptr(), a_stride, lora_b.data_ptr(), b_stride,
+          ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, ops._ptr(scales), to.data_ptr(), ldo, m, n, k, rank, adapters,
+          ops.dtype_code(dtype), ws.data_ptr(), ws_bytes)
+    return _Refused.apply("lora_add is not differentiable", out, *inputs) if asked else out
+
+
+class LoRAAdapters(nn.Module):
+    """The adapters of a linear layer: ``lora_a [L, R, K]``, ``lora_b [L, N, R]`` and ``scales`` fp32 ``[L]`` (alpha / rank; None:
+    1).  As ``layer.lora_adapters`` :meth:`AWQConfig.apply` adds them to the layer's product for the ids that a call names."""
+
+    def __init__(self, lora_a: torch.Tensor, lora_b: torch.Tensor, scales: torch.Tensor | None = None):
+        super().__init__()
+        self.lora_a = nn.Parameter(lora_a, requires_grad=False)
+        self.lora_b = nn.Parameter(lora_b, requires_grad=False)
+        self.scales = None if scales is None else nn.Parameter(scales, requires_grad=False)
+
+    @classmethod
+    def stack(cls, adapters: Sequence[tuple[torch.Tensor, torch.Tensor, float]]) -> "LoRAAdapters":
+        """Of ``(A [r, K], B [N, r], scale)`` of any ranks, zeros behind the lower ones."""
+        if not adapters:
+            raise ValueError("no adapters to stack")
+        first_a, first_b, _ = adapters[0]
+        rank = max(a.shape[0] for a, _, _ in adapters)
+        lora_a = first_a.new_zeros(len(adapters), rank, first_a.shape[1])
+        lora_b = first_b.new_zeros(len(adapters), first_b.shape[0], rank)
+        for i, (a, b, _) in enumerate(adapters):
+            if a.shape[0] != b.shape[1] or a.shape[1] != first_a.shape[1] or b.shape[0] != first_b.shape[0]:
+                raise ValueError(f"adapter {i}: A {tuple(a.shape)} and B {tuple(b.shape)} do not match or differ from the first's")
+            lora_a[i, :a.shape[0]] = a.detach()
+            lora_b[i, :, :a.shape[0]] = b.detach()
+        return cls(lora_a, lora_b, torch.tensor([float(s) for _, _, s in adapters], dtype=torch.float32, device=lora_a.device))
+
+    def add(self, base: torch.Tensor | None, x: torch.Tensor, ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """:func:`lora_add` with these adapters."""
+        return lora_add(base, x, self.lora_a, self.lora_b, ids, self.scales, out)

@@ -1,0 +1,162 @@
+"""The tokens' rows in the order of the experts that :func:`moe_route` chose, and back at the tokens with the routing's weights,
+for experts whose products the grouped kernels do not take (dense ones, ones that are trained, low-rank adapters of
+experts by :func:`lora_add`)."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+from . import ops
+from .mxfp4 import _call, _derivative_asked, _Refused
+
+
+class MoERoutes(NamedTuple):
+    """Where the routes went.  ``offsets`` int32 ``[E + 1]``: the places ``offsets[e] .. offsets[e + 1] - 1`` are expert ``e``'s;
+    ``experts`` int32 ``[T * top_k]``: the expert of a place, -1 behind the last; ``places`` int32 ``[T, top_k]``: the place of a
+    route, -1 for one without an expert."""
+
+    offsets: torch.Tensor
+    experts: torch.Tensor
+    places: torch.Tensor
+
+
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A 2-D ``x``, or a copy, whose rows are dense, and its row stride."""
+    n, h = x.shape
+    if (h > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < h):
+        x = x.contiguous()
+    return x, x.stride(0) if n > 1 else h
+
+
+def _back(name: str, on: int, *saved: tuple) -> None:
+    """Saved-tensor hooks may give back other tensors: each has to be on the device and of the type and shape that it had."""
+    for t, dtype, shape in saved:
+        if t is not None and (t.get_device() != on or t.dtype is not dtype or t.shape != shape):
+            raise RuntimeError(f"{name}: saved tensors came back elsewhere, or with other shapes or types")
+
+
+def _sorted(x, ids, experts):
+    (t, h), k, dev = x.shape, ids.shape[1], x.device
+    rows = torch.empty((t * k, h), dtype=x.dtype, device=dev)
+    # offsets, experts and places in one allocation
+    index = torch.empty(experts + 1 + 2 * t * k, dtype=torch.int32, device=dev)
+    offsets, of, places = index[:experts + 1], index[experts + 1:experts + 1 + t * k], index[experts + 1 + t * k:].view(t, k)
+    need = L.load().awq_w4a16_moe_sort_workspace_bytes(t, experts, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    x, ld = _rows(x)
+    _call(dev, "awq_w4a16_moe_sort", x.data_ptr(), ld, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, rows.data_ptr(),
+          offsets.data_ptr(), of.data_ptr(), places.data_ptr(), t, h, experts, k, ops.dtype_code(x.dtype), ops._ptr(ws), need)
+    return rows, offsets, of, places
+
+
+def _unsorted(rows, weights, places):
+    (t, k), h = places.shape, rows.shape[1]
+    out = torch.empty((t, h), dtype=rows.dtype, device=rows.device)
+    _call(rows.device, "awq_w4a16_moe_unsort", rows.data_ptr(), places.data_ptr(), ops._ptr(weights),
+          L.DTYPE_NONE if weights is None else ops.dtype_code(weights.dtype), out.data_ptr(), h, t, h, k, ops.dtype_code(rows.dtype))
+    return out
+
+
+class _Sort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ids, experts):
+        rows, offsets, of, places = _sorted(x, ids, experts)
+        ctx.save_for_backward(places)
+        ctx.mark_non_differentiable(offsets, of, places)
+        ctx.set_materialize_grads(False)
+        ctx.shape = ids.shape
+        return rows, offsets, of, places
+
+    @staticmethod
+    def backward(ctx, upstream, *_):
+        if upstream is None:
+            return None, None, None
+        places, = ctx.saved_tensors
+        _back("moe_sort", upstream.get_device(), (places, torch.int32, ctx.shape))
+        grad = _unsorted(upstream.contiguous(), None, places.contiguous())
+        if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
+            grad = _Refused.apply("moe_sort is not differentiable twice", grad, upstream)
+        return grad, None, None
+
+
+class _Unsort(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, places, offsets):
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, places, offsets)
+        ctx.of = (rows.dtype, rows.shape), None if weights is None else weights.dtype, places.shape, offsets.shape
+        return _unsorted(rows, weights, places)
+
+    @staticmethod
+    def backward(ctx, upstream):
+        rows, weights, places, offsets = ctx.saved_tensors
+        (dtype, shape), wdtype, routes, experts = ctx.of
+        _back("moe_unsort", upstream.get_device(), (rows, dtype, shape), (weights, wdtype, routes), (places, torch.int32, routes),
+              (offsets, torch.int32, experts))
+        (t, k), h, dev = routes, shape[1], upstream.device
+        flat, ld = _rows(upstream)
+        want_rows, want_weights = ctx.needs_input_grad[:2]
+        grad_rows = torch.empty(shape, dtype=dtype, device=dev) if want_rows else None
+        grad_weights = torch.empty(routes, dtype=wdtype, device=dev) if want_weights else None
+        dense = [None if a is None else a.contiguous() for a in (rows, weights, places, offsets)]
+        _call(dev, "awq_w4a16_moe_unsort_grad", flat.data_ptr(), ld, ops._ptr(dense[0]), dense[2].data_ptr(),
+              dense[3].data_ptr() + 4 * (experts[0] - 1), ops._ptr(dense[1]), L.DTYPE_NONE if wdtype is None else ops.dtype_code(wdtype),
+              ops._ptr(grad_rows), ops._ptr(grad_weights), t, h, k, ops.dtype_code(dtype))
+        if torch.is_grad_enabled():
+            inputs = upstream, rows, weights
+            grad_rows, grad_weights = (None if g is None else _Refused.apply("moe_unsort is not differentiable twice", g, *inputs)
+                                       for g in (grad_rows, grad_weights))
+        return grad_rows, grad_weights, None, None
+
+
+def moe_sort(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, MoERoutes]:
+    """``(rows, routes)``: the rows ``[T * top_k, H]`` of ``x [T, H]`` (fp16, bf16 or fp32), one for every route, expert after
+    expert and an expert's in the order of the tokens (:class:`MoERoutes`); differentiable in ``x``.
+
+    ``topk_ids``: int32 or int64 ``[T, top_k]``; routes whose id is outside ``[0, num_experts)`` (dropped ones, experts of other
+    devices) get no row, and as many rows behind the last are 0 (what a gradient holds there is not read).  1 to 1024 experts.
+    ``routes.offsets`` stays on the device; a loop over experts that needs it on the host reads it there itself.  The gradient
+    is not differentiable again.  As for any operation, a backward is captured into a graph only while no graph recorded
+    outside the capture over the same leaves is alive."""
+    ops._require_device(x, topk_ids)
+    ops.dtype_code(x.dtype)
+    if x.dim() != 2 or topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0]:
+        raise ValueError(f"x must be [T, H] and topk_ids [T, top_k], got {tuple(x.shape)} and {tuple(topk_ids.shape)}")
+    num_experts = int(num_experts)
+    if not 1 <= num_experts <= 1024 or topk_ids.shape[1] < 1:
+        raise ValueError(f"1 to 1024 experts and at least one route a token, got {num_experts} and {topk_ids.shape[1]}")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
+    topk_ids = topk_ids.contiguous()
+    run = _Sort.apply if _derivative_asked("moe_sort", None, x) else _sorted
+    rows, *routes = run(x, topk_ids, num_experts)
+    return rows, MoERoutes(*routes)
+
+
+def moe_unsort(rows: torch.Tensor, topk_weights: torch.Tensor | None, routes: MoERoutes) -> torch.Tensor:
+    """``out[t] = sum_j topk_weights[t, j] * rows[routes.places[t, j]]``, ``[T, H]`` in ``rows``' type: fp32 sums in slot order,
+    one rounding; differentiable in ``rows`` and ``topk_weights``.
+
+    ``rows [T * top_k, H]`` (fp16, bf16 or fp32) in the order of ``routes``, which :func:`moe_sort` gave; ``topk_weights``: fp16,
+    bf16 or fp32 ``[T, top_k]``, all 1 where it is None.  A route without a place adds nothing, its weight's gradient is 0;
+    what rows behind the last hold is not read, their gradient is 0.  The gradients are not differentiable again.  As for any
+    operation, a backward is captured into a graph only while no graph recorded outside the capture over the same leaves is alive."""
+    offsets, _, places = routes
+    ops._require_device(rows, topk_weights, offsets, places)
+    ops.dtype_code(rows.dtype)
+    if places.dtype != torch.int32 or offsets.dtype != torch.int32:
+        raise TypeError(f"routes must be int32, got {places.dtype} and {offsets.dtype}")
+    if places.dim() != 2 or places.shape[1] < 1 or offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError(f"routes must hold places [T, top_k] and offsets [E + 1], got {tuple(places.shape)} and {tuple(offsets.shape)}")
+    if rows.dim() != 2 or rows.shape[0] != places.numel():
+        raise ValueError(f"rows must be [{places.numel()}, H], got {tuple(rows.shape)}")
+    if topk_weights is not None:
+        ops.dtype_code(topk_weights.dtype)
+        if topk_weights.shape != places.shape:
+            raise ValueError(f"topk_weights must be {tuple(places.shape)}, got {tuple(topk_weights.shape)}")
+        topk_weights = topk_weights.contiguous()
+    rows, places = rows.contiguous(), places.contiguous()
+    if _derivative_asked("moe_unsort", None, rows, topk_weights):
+        return _Unsort.apply(rows, topk_weights, places, offsets)
+    return _unsorted(rows, topk_weights, places)
