@@ -8,9 +8,9 @@
 // rows, so the other rows of a tile only cost idle lanes.
 //
 // v enters the second product as two 16-bit numbers, v = high + low: 16 bits of mantissa at least for bf16, 21 for fp16, and
-// one rounding for the output.  Both halves meet the same B in one instruction of depth 32: 16 ranks, high parts then low
-// parts.  fp16 takes v / 2^e instead, with an e of its own for 16 ranks of a row that puts the largest of them at 2^13 .. 2^14:
-// v may pass fp16's range.
+// one rounding for the output.  Both halves meet the same B: ranks go in tiles of W = 32, an instruction for the high parts and
+// one for the low parts, or of 16 (rank 16 and less), high and low parts in one instruction of depth 32.  fp16 takes v / 2^e
+// instead, with an e of its own for a row's tile that puts the largest value at 2^13 .. 2^14: v may pass fp16's range.
 #include <algorithm>
 
 #include "awq_launch.h"
@@ -25,28 +25,23 @@ struct LoraArgs {
   const float* scales;
   uint16_t* out;
   float* partial;  // few rows: [splits][M][ranks], s_l not in it yet
-  uint16_t* v;     // many rows: [M][2 ranks], of each 16 ranks the high parts, then the low parts
-  float* powers;   // and [M][ranks / 16]: 2^e (fp16)
+  uint16_t* v;     // many rows: [M][2 ranks], of each W ranks the high parts, then the low parts
+  float* powers;   // and [M][ranks / W]: 2^e (fp16)
   int64_t ldb, ldx, ldo, a_stride, b_stride;
   int64_t M;
   int N, K, R, L, id64;
-  int ranks;  // R in whole tiles of 16
-  int slots;  // blocks that share a row tile's adapters
+  int ranks;  // R in whole tiles of W
+  int tiles;  // of 16 rows
+  int slots;  // blocks that share a row tile's adapters: block tile + tiles * slot, so that each slot's are on all XCDs
   int splits, per;  // shares of K, each of `per` units
   int cols;   // columns of a block
   int whole;  // columns that go by eight, see lora_whole
+  int ranges;   // many rows: blocks over the columns
 };
 
 __device__ __forceinline__ int lora_id(const LoraArgs& p, int64_t m) {
   const int64_t l = p.id64 ? ((const int64_t*)p.ids)[m] : (int64_t)((const int32_t*)p.ids)[m];
   return l >= 0 && l < p.L ? (int)l : -1;
-}
-// Eight elements of which the first n exist, zeros behind them.
-__device__ __forceinline__ u32x4 load8_to(const uint16_t* at, int n) {
-  if (n >= 8) return *(const u32x4_any*)at;
-  u32x4 v = {0, 0, 0, 0};
-  for (int i = 0; i < n; ++i) v[i >> 1] |= (uint32_t)at[i] << (16 * (i & 1));
-  return v;
 }
 // The neighbouring lane's value (lanes 0 and 1 swap, 2 and 3, ...), and the largest of 16 lanes.
 __device__ __forceinline__ u32x4 from_neighbour(u32x4 v) {
@@ -64,46 +59,60 @@ __device__ __forceinline__ float row_max16(float v) {
   return fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));
 }
 
-// v of a rank as its two parts, and 2^e; all 16 ranks of a row's tile in 16 neighbouring lanes.
+// v of a rank as its two parts.
 struct Halves {
   uint16_t high, low;
-  float power;
 };
 template <typename T>
 __device__ __forceinline__ Halves halves_of(float f) {
-  Halves h;
-  h.power = 1.f;
-  if constexpr (std::is_same<T, f16>::value) {
-    const int e = (int)(__builtin_bit_cast(uint32_t, row_max16(fabsf(f))) >> 23) - 127 - 13;
-    f = ldexpf(f, -e);
-    h.power = ldexpf(1.f, e);
-  }
-  h.high = to_bits<T>(f);
-  h.low = fabsf(f) < __builtin_inff() ? to_bits<T>(f - from_bits<T>(h.high)) : (uint16_t)0;  // no Inf - Inf
-  return h;
+  const uint16_t high = to_bits<T>(f);
+  return {high, fabsf(f) < __builtin_inff() ? to_bits<T>(f - from_bits<T>(high)) : (uint16_t)0};  // no Inf - Inf
 }
+// e of a row's tile from its largest value (0, Inf and NaN included).
+__device__ __forceinline__ int tile_exponent(float top) { return (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 13; }
 
 // ------------------------------------------------------------------ ranks
 constexpr int kUnit = 64;  // values of K that a wave takes at once: whole lines of both operands
 
-// RT tiles of 16 ranks by a tile of 16 rows and a share of K, whose units the waves take in turn, D of them at a time; the
-// waves' sums meet in LDS.  Loads cover whole lines, eight lanes each; a wave passes them through LDS of its own into the
-// matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and 32 + 8 q .. of rank i and of row i.  (Straight from
-// memory in that order a load's neighbouring lanes are in different lines: 4096 rows, K = 4096, rank 64 42 us.)
+// A rank's sum, or its parts of v, by W neighbouring lanes for a row's tile; rows that are not `mine` take part only.
+template <typename T, int W, bool FINAL>
+__device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank, float f, float scale, bool mine) {
+  if constexpr (FINAL) {
+    f = rank < p.R ? f * scale : 0.f;
+    if constexpr (std::is_same<T, f16>::value) {
+      float top = row_max16(fabsf(f));
+      if constexpr (W == 32) top = fmaxf(top, __shfl_xor(top, 16));
+      const int e = tile_exponent(top);
+      f = ldexpf(f, -e);
+      if (mine && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = ldexpf(1.f, e);
+    }
+    if (!mine) return;
+    const Halves h = halves_of<T>(f);
+    uint16_t* const to = p.v + m * 2 * p.ranks + 2 * (rank / W) * W + rank % W;
+    to[0] = h.high, to[W] = h.low;
+  } else if (mine) {
+    p.partial[((int64_t)blockIdx.z * p.M + m) * p.ranks + rank] = f;
+  }
+}
+
+// RT tiles of 16 ranks by a tile of 16 rows and a share of K, whose units the waves take in turn; the waves' sums meet in LDS.
+// D units of a wave are on their way in registers.  Loads cover whole lines, eight lanes each; a wave passes them through LDS
+// of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and 32 + 8 q .. of rank i and of row i.
+// (Straight from memory in that order a load's neighbouring lanes are in different lines: 4096 rows, K = 4096, rank 64 42 us.)
 // FINAL: the share is all of K, the parts of v go out; else the sums.
-template <typename T, int RT, int WAVES, int D, bool FINAL>
-__global__ void __launch_bounds__(64 * WAVES) lora_ranks_kernel(LoraArgs p) {
-  constexpr int TILES = 1 + RT, LD = kUnit + 8;  // rows 16 bytes apart from whole banks
+template <typename T, int RT, int W, int D, bool FINAL>
+__global__ void __launch_bounds__(256, 1) lora_ranks_kernel(LoraArgs p) {
+  constexpr int WAVES = 4, TILES = 1 + RT, LD = kUnit + 8;  // rows 16 bytes apart from whole banks
   union Lds {
-    uint16_t stage[WAVES][D][TILES * 16][LD];
+    uint16_t stage[WAVES][TILES * 16][LD];
     f32x4 part[WAVES][RT][64];
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, r8 = lane >> 3, c8 = 8 * (lane & 7);
-  const int tile = blockIdx.x / p.slots, slot = blockIdx.x - tile * p.slots, tile0 = blockIdx.y * RT;
+  const int tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
   const int64_t m0 = (int64_t)tile * 16;
   const int id = m0 + i < p.M ? lora_id(p, m0 + i) : -1;
-  const int begin = blockIdx.z * p.per, units = min(begin + p.per, (p.K + kUnit - 1) / kUnit);
+  const int begin = blockIdx.z * p.per + wave, units = min((int)(blockIdx.z + 1) * p.per, (p.K + kUnit - 1) / kUnit);
   uint32_t left = (uint32_t)(__ballot(id >= 0) & 0xFFFF);
   for (int n = 0; left; ++n) {
     const int first = __builtin_ctz(left), cur = __builtin_amdgcn_readlane(id, first);
@@ -119,44 +128,45 @@ __global__ void __launch_bounds__(64 * WAVES) lora_ranks_kernel(LoraArgs p) {
       for (int r = 0; r < RT; ++r) from[1 + r][h] = p.a + cur * p.a_stride + (int64_t)min(16 * (tile0 + r) + r8 + 8 * h, p.R - 1) * p.K + c8;
     }
     u32x4 piece[D][TILES][2];
-    auto load = [&](int u0) {
+    auto load = [&](int d, int u) {
+      if (u >= units) return;
+      // the last unit's pieces end with K: what lies past it, or belongs to the piece before, becomes 0 in both operands
+      const int k = u * kUnit + c8, at = min(k, p.K - 8) - c8, twice = k - c8 - at;
+#pragma unroll
+      for (int j = 0; j < TILES; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) piece[d][j][h] = *(const u32x4_any*)(from[j][h] + at);
+      if (u * kUnit + kUnit <= p.K) return;
+      u32x4 mask;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mask[j] = (2 * j >= twice ? 0xFFFFu : 0u) | (2 * j + 1 >= twice ? 0xFFFF0000u : 0u);
+#pragma unroll
+      for (int j = 0; j < TILES; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) piece[d][j][h] &= mask;
+    };
+    f32x4 acc[RT] = {};
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(d, begin + d * WAVES);
+    for (int u0 = begin; u0 < units; u0 += D * WAVES) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
         const int u = u0 + d * WAVES;
         if (u >= units) continue;
-        const bool whole = u * kUnit + kUnit <= p.K;
 #pragma unroll
         for (int j = 0; j < TILES; ++j)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint16_t* const at = from[j][h] + u * kUnit;
-            piece[d][j][h] = whole ? *(const u32x4_any*)at : load8_to(at, p.K - u * kUnit - c8);
-          }
-      }
-    };
-    f32x4 acc[RT] = {};
-    load(begin + wave);
-    for (int u0 = begin + wave; u0 < units; u0 += D * WAVES) {
-#pragma unroll
-      for (int d = 0; d < D; ++d)
-#pragma unroll
-        for (int j = 0; j < TILES; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) *(u32x4*)&lds.stage[wave][d][16 * j + r8 + 8 * h][c8] = piece[d][j][h];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      load(u0 + D * WAVES);
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        if (u0 + d * WAVES >= units) continue;
+          for (int h = 0; h < 2; ++h) *(u32x4*)&lds.stage[wave][16 * j + r8 + 8 * h][c8] = piece[d][j][h];
+        load(d, u + D * WAVES);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int k = 0; k < kUnit; k += 32) {
-          const u32x4 x = *(const u32x4*)&lds.stage[wave][d][i][k + 8 * q];
+          const u32x4 x = *(const u32x4*)&lds.stage[wave][i][k + 8 * q];
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            acc[r] = MfmaOp<T>::run(*(const u32x4*)&lds.stage[wave][d][16 * (1 + r) + i][k + 8 * q], x, acc[r]);
+          for (int r = 0; r < RT; ++r) acc[r] = MfmaOp<T>::run(*(const u32x4*)&lds.stage[wave][16 * (1 + r) + i][k + 8 * q], x, acc[r]);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __syncthreads();  // all waves are done with their stages
     // ranks 4 q .. 4 q + 3 of row i
@@ -164,30 +174,33 @@ __global__ void __launch_bounds__(64 * WAVES) lora_ranks_kernel(LoraArgs p) {
     for (int r = 0; r < RT; ++r) lds.part[wave][r][lane] = acc[r];
     __syncthreads();
     for (int at = t; at < RT * 256; at += 64 * WAVES) {
-      const int r = at >> 8, row = at >> 4 & 15, rank = 16 * (tile0 + r) + i;  // i == at % 16
+      const int row = at / W % 16, rank = at / (16 * W) * W + at % W, j = rank & 15;  // rank of the block's
       float f = 0.f;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) f += ((const float*)&lds.part[w][r][16 * (i >> 2) + row])[i & 3];
-      if (rank >= p.ranks) continue;  // for the whole row
-      const int64_t m = m0 + row;
-      if constexpr (FINAL) {
-        const Halves h = halves_of<T>(rank < p.R ? f * (p.scales ? p.scales[cur] : 1.f) : 0.f);
-        if (rows >> row & 1) {
-          uint16_t* const to = p.v + m * 2 * p.ranks + 32 * (tile0 + r) + i;
-          to[0] = h.high, to[16] = h.low;
-          if (std::is_same<T, f16>::value && i == 0) p.powers[m * (p.ranks / 16) + tile0 + r] = h.power;
-        }
-      } else if (rows >> row & 1) {
-        p.partial[((int64_t)blockIdx.z * p.M + m) * p.ranks + rank] = f;
-      }
+      for (int w = 0; w < WAVES; ++w) f += ((const float*)&lds.part[w][rank >> 4][16 * (j >> 2) + row])[j & 3];
+      const int all = 16 * tile0 + rank;
+      if (all < p.ranks) put_rank<T, W, FINAL>(p, m0 + row, all, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
     }
     __syncthreads();
   }
 }
 
+// Rows of fewer than eight values: a thread has a row and a rank.
+template <typename T, int W, bool FINAL>
+__global__ void __launch_bounds__(256) lora_ranks_short_kernel(LoraArgs p) {
+  const int64_t m = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const int rank = blockIdx.y * W + threadIdx.x % W;
+  const int id = m < p.M ? lora_id(p, m) : -1;
+  float f = 0.f;
+  if (id >= 0 && rank < p.R)
+    for (int k = 0; k < p.K; ++k)
+      f = fmaf(from_bits<T>(p.x[m * p.ldx + k]), from_bits<T>(p.a[id * p.a_stride + (int64_t)rank * p.K + k]), f);
+  put_rank<T, W, FINAL>(p, m, rank, f, p.scales ? p.scales[max(id, 0)] : 1.f, id >= 0);
+}
+
 // ------------------------------------------------------------------ columns
 // Columns behind p.whole, one by one, of the rows `rows` of `count`; parts(row) and power(row, tile) give a row's v.
-template <typename T, class Parts, class Power>
+template <typename T, int W, class Parts, class Power>
 __device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b, int64_t m0, int count, uint64_t rows, bool adapter,
                                             Parts parts, Power power) {
   const int odd = p.N - p.whole;
@@ -198,14 +211,14 @@ __device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b
     float s = 0.f;
     if (adapter) {
       const uint16_t* const v = parts(row);
-      for (int r0 = 0; r0 < p.R; r0 += 16) {
+      for (int r0 = 0; r0 < p.R; r0 += W) {
         float c = 0.f;
 #pragma unroll 4
-        for (int r = r0; r < min(r0 + 16, p.R); ++r) {
+        for (int r = r0; r < min(r0 + W, p.R); ++r) {
           const float f = from_bits<T>(b[(int64_t)col * p.R + r]);
-          c = fmaf(from_bits<T>(v[r0 + r + 16]), f, fmaf(from_bits<T>(v[r0 + r]), f, c));
+          c = fmaf(from_bits<T>(v[r0 + r + W]), f, fmaf(from_bits<T>(v[r0 + r]), f, c));
         }
-        s = fmaf(c, power(row, r0 >> 4), s);
+        s = fmaf(c, power(row, r0 / W), s);
       }
     }
     if (p.base) s += from_bits<T>(p.base[m * p.ldb + col]);
@@ -213,13 +226,15 @@ __device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b
   }
 }
 
-// Of the last tile's eight ranks 8 (q % 2) .. that a lane holds those that exist, as a mask of their bits.
-__device__ __forceinline__ u32x4 last_mask(const LoraArgs& p, int q) {
-  const int there = p.R - (p.ranks - 16) - 8 * (q & 1);
-  u32x4 mask;
+// A lane's eight ranks of a tile begin with this one, of either operand.
+template <int W>
+__device__ __forceinline__ int first_rank(int q) { return 8 * (W == 32 ? q : q & 1); }
+// What the two parts of v give with eight ranks of B, on top of c.
+template <typename T, int W>
+__device__ __forceinline__ f32x4 both_parts(const u32x4& b, const u32x4 (&v)[W / 16], f32x4 c) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) mask[j] = (2 * j < there ? 0xFFFFu : 0u) | (2 * j + 1 < there ? 0xFFFF0000u : 0u);
-  return mask;
+  for (int h = 0; h < W / 16; ++h) c = MfmaOp<T>::run(b, v[h], c);
+  return c;
 }
 template <typename T>
 __device__ __forceinline__ u32x4 added(const u32x4& base, const f32x4& d0, const f32x4& d1) {
@@ -233,19 +248,24 @@ __device__ __forceinline__ u32x4 added(const u32x4& base, const f32x4& d0, const
 }
 
 // Few rows: 16 by p.cols columns, B straight from memory.  A wave takes 32 columns at a time as two tiles of 16, tile c of them
-// the columns 8 (i / 4) + 4 c + i % 4, so that lane (q, i) ends with the eight columns 8 q .. 8 q + 7 of row i.  RT tiles of 16
+// the columns 8 (i / 4) + 4 c + i % 4, so that lane (q, i) ends with the eight columns 8 q .. 8 q + 7 of row i.  RT tiles of W
 // ranks at a time.  Base and B of the first columns are on their way while the shares of v are added up.
-template <typename T, int RT>
+template <typename T, int RT, int W>
 __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
-  extern __shared__ u32x4 dynamic_lds[];  // v: [16][ld], of each 16 ranks the high parts, then the low parts
+  constexpr int SUB = W / 16;
+  extern __shared__ u32x4 dynamic_lds[];  // v: [16][ld], of each W ranks the high parts, then the low parts
   __shared__ float power[16][16];
   uint16_t* const v = (uint16_t*)dynamic_lds;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / 16, ld = 2 * p.ranks + 8;
-  const int tile = blockIdx.x / p.slots, slot = blockIdx.x - tile * p.slots;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / W, ld = 2 * p.ranks + 8;
+  const int tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles;
   const int64_t m0 = (int64_t)tile * 16, m = m0 + i;
   const int id = m < p.M ? lora_id(p, m) : -2;
   const int begin = blockIdx.y * p.cols + wave * 32, end = min((int)(blockIdx.y + 1) * p.cols, p.whole);
-  const u32x4 mask = last_mask(p, q);
+  // of the last tile's eight ranks of this lane those that exist, as a mask of their bits
+  const int there = p.R - (p.ranks - W) - first_rank<W>(q);
+  u32x4 mask;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mask[j] = (2 * j < there ? 0xFFFFu : 0u) | (2 * j + 1 < there ? 0xFFFF0000u : 0u);
   uint32_t left = (uint32_t)(__ballot(id >= -1) & 0xFFFF);
   for (int n = 0; left; ++n) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
@@ -260,7 +280,7 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if (r0 + r >= tiles) continue;
-        const int at = 16 * (r0 + r) + 8 * (q & 1);
+        const int at = W * (r0 + r) + first_rank<W>(q);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           bv[c][r] = *(const u32x4_any*)(b + (int64_t)min(c0 + 8 * (i >> 2) + 4 * c + (i & 3), p.whole - 1) * p.R + (at < p.R ? at : 0));
@@ -277,21 +297,35 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
     if (cur >= 0) {
       const float scale = p.scales ? p.scales[cur] : 1.f;
       __syncthreads();  // v of the adapter before is read
-      // a wave has a row's 16 ranks, lane (q, i) the shares q, q + 4, ... of rank i
+      // a wave has a row's tile, lane (q, i) the shares q, q + 4, ... of ranks i and 16 + i
       for (int j = wave; j < 16 * tiles; j += 4) {
         const int row = j & 15, r = j >> 4;
         if (!(rows >> row & 1)) continue;
-        const float* const at = p.partial + (m0 + row) * p.ranks + 16 * r + i;
-        float f = 0.f, part[4];
+        const float* const at = p.partial + (m0 + row) * p.ranks + W * r + i;
+        float part[SUB][4], f[SUB];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) part[s] = q + 4 * s < p.splits ? at[(q + 4 * s) * p.M * p.ranks] : 0.f;
+        for (int h = 0; h < SUB; ++h)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) f += part[s];
-        f += __shfl_xor(f, 16);
-        f += __shfl_xor(f, 32);
-        const Halves h = halves_of<T>(16 * r + i < p.R ? f * scale : 0.f);
-        if (q < 2) v[row * ld + 32 * r + 16 * q + i] = q ? h.low : h.high;
-        if (lane == 0) power[row][r] = h.power;
+          for (int s = 0; s < 4; ++s) part[h][s] = q + 4 * s < p.splits ? at[(q + 4 * s) * p.M * p.ranks + 16 * h] : 0.f;
+        int e = 0;
+        float top = 0.f;
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+          f[h] = (part[h][0] + part[h][1]) + (part[h][2] + part[h][3]);
+          f[h] += __shfl_xor(f[h], 16);
+          f[h] += __shfl_xor(f[h], 32);
+          f[h] = W * r + 16 * h + i < p.R ? f[h] * scale : 0.f;
+          top = fmaxf(top, fabsf(f[h]));
+        }
+        if constexpr (std::is_same<T, f16>::value) {
+          e = tile_exponent(row_max16(top));
+          if (lane == 0) power[row][r] = ldexpf(1.f, e);
+        }
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+          const Halves two = halves_of<T>(std::is_same<T, f16>::value ? ldexpf(f[h], -e) : f[h]);
+          if (q < 2) v[row * ld + 2 * W * r + W * q + 16 * h + i] = q ? two.low : two.high;
+        }
       }
       __syncthreads();
     }
@@ -302,16 +336,18 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           if (r0 + r >= tiles) continue;
-          const u32x4 low = *(const u32x4*)(v + i * ld + 32 * (r0 + r) + 8 * q);
+          u32x4 low[SUB];
+#pragma unroll
+          for (int h = 0; h < SUB; ++h) low[h] = *(const u32x4*)(v + i * ld + 2 * W * (r0 + r) + W * h + 8 * q);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (r0 + r == tiles - 1) bv[c][r] &= mask;
             if constexpr (std::is_same<T, f16>::value) {
-              const f32x4 one = MfmaOp<T>::run(bv[c][r], low, f32x4{0.f, 0.f, 0.f, 0.f});
+              const f32x4 one = both_parts<T, W>(bv[c][r], low, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
               for (int j = 0; j < 4; ++j) sum[c][j] = fmaf(one[j], power[i][r0 + r], sum[c][j]);
             } else {
-              sum[c] = MfmaOp<T>::run(bv[c][r], low, sum[c]);
+              sum[c] = both_parts<T, W>(bv[c][r], low, sum[c]);
             }
           }
         }
@@ -324,142 +360,161 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
       if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
     }
     if (blockIdx.y + 1 == gridDim.y)
-      odd_columns<T>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; }, [&](int row, int r) { return power[row][r]; });
+      odd_columns<T, W>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; },
+                        [&](int row, int r) { return std::is_same<T, f16>::value ? power[row][r] : 1.f; });
   }
 }
 
-// Many rows: 128 by p.cols columns, 64 of them at a time: their B goes through LDS once for the four waves, which have 32 rows
+// Many rows: 64 by p.cols columns, 64 of them at a time: their B goes through LDS once for the four waves, which have 16 rows
 // each, and the next 64 columns' is on its way meanwhile.  Tile c of the four holds the columns 16 (i / 4) + 4 c + i % 4, so
 // that lane (q, i) ends with the sixteen columns 16 q .. 16 q + 15 of row i.  Neighbouring lanes swap halves of theirs, so that each
-// load and store of base and out covers whole lines of 128 bytes.
-template <typename T, int RT>
-__global__ void __launch_bounds__(256) lora_columns_kernel(LoraArgs p) {
-  constexpr int MT = 2, ROWS = 64 * MT, LD = 16 * RT + 8, PIECES = 64 * 2 * RT, EACH = (PIECES + 255) / 256;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][64][LD];  // [column][rank]
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / 16, chunks = (tiles + RT - 1) / RT;
-  // a row tile's blocks go to all XCDs, so that tiles of several adapters, which take longer, do not meet on one
-  const int64_t m0 = (int64_t)((blockIdx.x + blockIdx.y) % gridDim.x) * ROWS;
-  int id[2];
-  uint64_t left[2];
+// load and store of base and out covers whole lines of 128 bytes.  Two adapters at a time, so that a tile where one request ends
+// and the next begins takes no longer; the rows without an adapter go with the first two.
+// Neighbouring blocks have neighbouring columns, so that (in eights) an XCD reads the same columns' B for all row tiles.
+template <typename T, int RT, int W, bool THROUGH>
+__global__ void __launch_bounds__(256, 3) lora_columns_kernel(LoraArgs p) {
+  constexpr int ROWS = 64, SUB = W / 16, LD = W * RT + 8, ROW = W * RT / 8, PIECES = 64 * ROW, EACH = (PIECES + 255) / 256;
+  // [buffer][adapter][column][rank], the columns as the lanes take them: number 16 c + i of tile c and lane i
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][64][LD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, odd = i & 1;
+  const int tiles = p.ranks / W, chunks = (tiles + RT - 1) / RT, y = blockIdx.x % p.ranges;
+  const int64_t m0 = (int64_t)(blockIdx.x / p.ranges) * ROWS, mw = m0 + 16 * wave;
+  const int id = m0 + lane < p.M ? lora_id(p, m0 + lane) : -2;
+  const int begin = y * p.cols, end = min(begin + p.cols, p.whole);
+  const bool in_place = p.out == p.base && p.ldo == p.ldb;
+  uint64_t left = __ballot(id >= 0), none = __ballot(id == -1);
+  for (bool more = true; more; more = left != 0) {
+    // the two adapters' numbers and rows; a wave's own rows are bits 16 wave ..
+    int cur[2] = {-1, -1};
+    uint64_t rows[2] = {0, 0};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t m = m0 + 64 * h + lane;
-    id[h] = m < p.M ? lora_id(p, m) : -2;
-    left[h] = __ballot(id[h] >= -1);
-  }
-  const int begin = blockIdx.y * p.cols, end = min((int)(blockIdx.y + 1) * p.cols, p.whole), odd = i & 1;
-  while (left[0] | left[1]) {
-    const int cur = left[0] ? __builtin_amdgcn_readlane(id[0], __builtin_ctzll(left[0])) : __builtin_amdgcn_readlane(id[1], __builtin_ctzll(left[1]));
-    const uint64_t rows[2] = {__ballot(id[0] == cur), __ballot(id[1] == cur)};
-    left[0] &= ~rows[0], left[1] &= ~rows[1];
-    if (cur < 0 && p.out == p.base && p.ldo == p.ldb) continue;  // in place already
-    const uint16_t* const b = p.b + max(cur, 0) * p.b_stride;
-    const uint32_t mine = (uint32_t)(rows[wave >> 1] >> (32 * (wave & 1)));  // the wave's 32 rows
-    const int64_t mw = m0 + 32 * wave;
-    u32x4 stage[EACH], bs[MT][2];
+    for (int g = 0; g < 2; ++g)
+      if (left) {
+        cur[g] = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        rows[g] = __ballot(id == cur[g]);
+        left &= ~rows[g];
+      }
+    const uint64_t written = rows[0] | rows[1] | (in_place ? 0 : none);
+    const uint32_t mine[2] = {(uint32_t)(rows[0] >> 16 * wave) & 0xFFFF, (uint32_t)(rows[1] >> 16 * wave) & 0xFFFF};
+    const uint32_t touched = (uint32_t)(written >> 16 * wave) & 0xFFFF;
+    const bool second = mine[1] >> i & 1, neither = !((mine[0] | mine[1]) >> i & 1);
+    u32x4 stage[2][EACH], bs[2], low[RT][SUB];
+    float power[RT];
     auto load_b = [&](int c0, int chunk) {
 #pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        const int piece = t + 256 * e, col = piece / (2 * RT), at = 16 * RT * chunk + 8 * (piece % (2 * RT));
-        if (PIECES % 256 && piece >= PIECES) continue;
-        stage[e] = u32x4{0, 0, 0, 0};
-        if (at < p.R) stage[e] = *(const u32x4_any*)(b + (int64_t)min(c0 + col, p.whole - 1) * p.R + at);
-        if (at < p.R && at + 8 > p.R) {
+      for (int g = 0; g < 2; ++g) {
+        if (cur[g] < 0) continue;
+        const uint16_t* const b = p.b + cur[g] * p.b_stride;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          const int piece = t + 256 * e, col = piece / ROW, at = W * RT * chunk + 8 * (piece % ROW);
+          if (PIECES % 256 && piece >= PIECES) continue;
+          stage[g][e] = u32x4{0, 0, 0, 0};
+          if (at >= p.R) continue;
+          stage[g][e] = *(const u32x4_any*)(b + (int64_t)min(c0 + col, p.whole - 1) * p.R + at);
+          if (at + 8 <= p.R) continue;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            stage[e][j] &= (at + 2 * j < p.R ? 0xFFFFu : 0u) | (at + 2 * j + 1 < p.R ? 0xFFFF0000u : 0u);
+            stage[g][e][j] &= (at + 2 * j < p.R ? 0xFFFFu : 0u) | (at + 2 * j + 1 < p.R ? 0xFFFF0000u : 0u);
         }
       }
     };
-    // the rows and columns of a lane's loads and stores: both rows of a pair, the even or the odd half of their sixteen columns
-    auto row_of = [&](int mt, int k) { return 16 * mt + (i & ~1) + k; };
+    // a lane's loads and stores: both rows of a pair, the even or the odd half of their sixteen columns
     auto load_base = [&](int c0) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          bs[mt][k] = u32x4{0, 0, 0, 0};
-          if (p.base && (mine >> row_of(mt, k) & 1) && c0 + 16 * q + 8 * odd < end)
-            bs[mt][k] = *(const u32x4_any*)(p.base + (mw + row_of(mt, k)) * p.ldb + c0 + 16 * q + 8 * odd);
-        }
+      for (int k = 0; k < 2; ++k) {
+        bs[k] = u32x4{0, 0, 0, 0};
+        if (p.base && (touched >> ((i & ~1) + k) & 1) && c0 + 16 * q + 8 * odd < end)
+          bs[k] = *(const u32x4_any*)(p.base + (mw + (i & ~1) + k) * p.ldb + c0 + 16 * q + 8 * odd);
+      }
     };
-    u32x4 low[MT][RT];
-    float power[MT][RT];
     auto load_low = [&](int chunk) {
+      const int64_t m = min(mw + i, p.M - 1);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int r = 0; r < RT; ++r) {
+        if (chunk * RT + r >= tiles) continue;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int64_t m = min(mw + 16 * mt + i, p.M - 1);
-          if (chunk * RT + r >= tiles) continue;
-          low[mt][r] = *(const u32x4*)(p.v + m * 2 * p.ranks + 32 * (chunk * RT + r) + 8 * q);
-          if constexpr (std::is_same<T, f16>::value) power[mt][r] = p.powers[m * tiles + chunk * RT + r];
-        }
+        for (int h = 0; h < SUB; ++h) low[r][h] = *(const u32x4*)(p.v + m * 2 * p.ranks + 2 * W * (chunk * RT + r) + W * h + 8 * q);
+        if constexpr (std::is_same<T, f16>::value) power[r] = p.powers[m * tiles + chunk * RT + r];
+      }
     };
-    if (cur >= 0) {
-      load_b(begin, 0);
-      load_low(0);
-    }
+    load_b(begin, 0);
+    load_low(0);
     load_base(begin);
-    __syncthreads();  // the adapter before is done with the LDS
+    __syncthreads();  // the adapters before are done with the LDS
     int buf = 0;
     for (int c0 = begin; c0 < end; c0 += 64) {
-      f32x4 sum[MT][4] = {};
-      if (cur >= 0) {
+      f32x4 sum[4] = {};
+      if (cur[0] >= 0) {
         for (int chunk = 0; chunk < chunks; ++chunk, buf ^= 1) {
 #pragma unroll
-          for (int e = 0; e < EACH; ++e) {
-            const int piece = t + 256 * e;
-            if (PIECES % 256 && piece >= PIECES) continue;
-            *(u32x4*)&lds[buf][piece / (2 * RT)][8 * (piece % (2 * RT))] = stage[e];
+          for (int g = 0; g < 2; ++g) {
+            if (cur[g] < 0) continue;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+              const int piece = t + 256 * e;
+              if (PIECES % 256 && piece >= PIECES) continue;
+              const int col = piece / ROW;
+              *(u32x4*)&lds[buf][g][16 * (col >> 2 & 3) + 4 * (col >> 4) + (col & 3)][8 * (piece % ROW)] = stage[g][e];
+            }
           }
           __syncthreads();
           if (chunk + 1 < chunks) load_b(c0, chunk + 1);
           else if (c0 + 64 < end) load_b(c0 + 64, 0);
+          auto multiply = [&](int g, f32x4 (&to)[4]) {
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            if (chunk * RT + r >= tiles || !mine) continue;
+            for (int r = 0; r < RT; ++r) {
+              if (chunk * RT + r >= tiles) continue;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const u32x4 bv = *(const u32x4*)&lds[buf][16 * (i >> 2) + 4 * c + (i & 3)][16 * r + 8 * (q & 1)];
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
+              for (int c = 0; c < 4; ++c) {
+                const u32x4 bv = *(const u32x4*)&lds[buf][g][16 * c + i][W * r + first_rank<W>(q)];
                 if constexpr (std::is_same<T, f16>::value) {
-                  const f32x4 one = MfmaOp<T>::run(bv, low[mt][r], f32x4{0.f, 0.f, 0.f, 0.f});
+                  const f32x4 one = both_parts<T, W>(bv, low[r], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) sum[mt][c][j] = fmaf(one[j], power[mt][r], sum[mt][c][j]);
+                  for (int j = 0; j < 4; ++j) to[c][j] = fmaf(one[j], power[r], to[c][j]);
                 } else {
-                  sum[mt][c] = MfmaOp<T>::run(bv, low[mt][r], sum[mt][c]);
+                  to[c] = both_parts<T, W>(bv, low[r], to[c]);
                 }
               }
             }
+          };
+          if (mine[0] && mine[1]) {  // a wave where one request ends and the next begins
+            f32x4 with[4] = {sum[0], sum[1], sum[2], sum[3]};
+            multiply(0, sum);
+            multiply(1, with);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sum[c][j] = second ? with[c][j] : sum[c][j];
+          } else if (mine[0] | mine[1]) {
+            multiply(mine[0] ? 0 : 1, sum);
           }
           if (chunks > 1) load_low(chunk + 1 < chunks ? chunk + 1 : 0);
         }
       }
-      u32x4 now[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) now[mt][0] = bs[mt][0], now[mt][1] = bs[mt][1];
+      const u32x4 now[2] = {bs[0], bs[1]};
       if (c0 + 64 < end) load_base(c0 + 64);
+      if (neither) sum[0] = sum[1] = sum[2] = sum[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const u32x4 got = from_neighbour(odd ? now[0] : now[1]);
+      const u32x4 o0 = added<T>(odd ? got : now[0], sum[0], sum[1]), o1 = added<T>(odd ? now[1] : got, sum[2], sum[3]);
+      const u32x4 other = from_neighbour(odd ? o0 : o1);
+      const u32x4 o[2] = {odd ? other : o0, odd ? o1 : other};
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const u32x4 got = from_neighbour(odd ? now[mt][0] : now[mt][1]);
-        const u32x4 o0 = added<T>(odd ? got : now[mt][0], sum[mt][0], sum[mt][1]);
-        const u32x4 o1 = added<T>(odd ? now[mt][1] : got, sum[mt][2], sum[mt][3]);
-        const u32x4 other = from_neighbour(odd ? o0 : o1);
-        const u32x4 o[2] = {odd ? other : o0, odd ? o1 : other};
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if ((mine >> row_of(mt, k) & 1) && c0 + 16 * q + 8 * odd < end)
-            *(u32x4_any*)(p.out + (mw + row_of(mt, k)) * p.ldo + c0 + 16 * q + 8 * odd) = o[k];
-      }
+      for (int k = 0; k < 2; ++k)
+        if ((touched >> ((i & ~1) + k) & 1) && c0 + 16 * q + 8 * odd < end) {
+          u32x4_any* const to = (u32x4_any*)(p.out + (mw + (i & ~1) + k) * p.ldo + c0 + 16 * q + 8 * odd);
+          if constexpr (THROUGH) __builtin_nontemporal_store(o[k], to);
+          else *to = o[k];
+        }
     }
-    if (blockIdx.y + 1 == gridDim.y) {
+    if (y + 1 == p.ranges) {
+      auto parts = [&](int row) { return p.v + (m0 + row) * 2 * p.ranks; };
+      auto powers = [&](int row, int r) { return std::is_same<T, f16>::value ? p.powers[(m0 + row) * tiles + r] : 1.f; };
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        odd_columns<T>(p, b, m0 + 64 * h, 64, rows[h], cur >= 0, [&](int row) { return p.v + (m0 + 64 * h + row) * 2 * p.ranks; },
-                       [&](int row, int r) { return std::is_same<T, f16>::value ? p.powers[(m0 + 64 * h + row) * tiles + r] : 1.f; });
+      for (int g = 0; g < 2; ++g) odd_columns<T, W>(p, p.b + max(cur[g], 0) * p.b_stride, m0, 64, rows[g], true, parts, powers);
+      if (!in_place) odd_columns<T, W>(p, p.b, m0, 64, none, false, parts, powers);
     }
+    none = 0;
   }
 }
 
@@ -468,7 +523,8 @@ __global__ void __launch_bounds__(256) lora_columns_kernel(LoraArgs p) {
 namespace awq_host {
 using namespace awq;
 
-static int64_t lora_ranks(int64_t R) { return cdiv(R, 16) * 16; }
+static int64_t lora_tile(int64_t R) { return R <= 16 ? 16 : 32; }
+static int64_t lora_ranks(int64_t R) { return cdiv(R, lora_tile(R)) * lora_tile(R); }
 
 // Columns that go by eight: whole pieces of out, and B's pieces of eight ranks, of which a row's last may reach into the next
 // row, end with B.
@@ -479,18 +535,17 @@ static int64_t lora_whole(int64_t N, int64_t R) {
 
 struct LoraPlan {
   bool many;
-  int slots, rt, splits, per;  // rt: tiles of 16 ranks of a block of the first launch
+  int slots, splits, per;
 };
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
-  const int64_t tiles = cdiv(M, 16), ranks = lora_ranks(R) / 16, units = cdiv(K, kUnit);
+  const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit);
   l.many = M > 512;
   // a batch of single tokens has many adapters in a tile, prompts one or two
-  l.slots = M <= 128 ? (int)std::min<int64_t>(16, M) : 1;
-  l.rt = ranks >= 3 ? 4 : (int)ranks;
+  l.slots = M <= 128 ? (int)std::min<int64_t>(16, M) : l.many ? 2 : 1;
   l.splits = 1, l.per = (int)units;
   if (!l.many) {
-    const int64_t want = std::max<int64_t>(1, 256 / (tiles * l.slots * cdiv(ranks, l.rt)));
+    const int64_t want = std::max<int64_t>(1, 256 / (tiles * l.slots * cdiv(lora_ranks(R), 64)));
     l.per = (int)std::max<int64_t>(4, cdiv(units, std::min<int64_t>(want, 16)));
     l.splits = (int)cdiv(units, l.per);
   }
@@ -499,34 +554,44 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
 size_t lora_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   const LoraPlan l = lora_plan(M, K, R);
   const size_t values = (size_t)M * (size_t)lora_ranks(R);
-  return l.many ? values * 4 + values / 16 * 4 : (size_t)l.splits * values * 4;
+  return l.many ? values * 4 + values / (size_t)lora_tile(R) * 4 : (size_t)l.splits * values * 4;
 }
 
 template <typename T>
 static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
   using std::integral_constant;
-  const int tiles = p.ranks / 16;
+  // tiles of 16 ranks a block of the first launch, of W ranks at a time in the second, and W
   auto by_rank = [&](auto f) {
-    if (tiles == 1) f(integral_constant<int, 1>{});
-    else if (tiles == 2) f(integral_constant<int, 2>{});
-    else f(integral_constant<int, 4>{});
+    if (p.ranks == 16) f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<int, 16>{});
+    else if (p.ranks == 32) f(integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 32>{});
+    else f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 32>{});
   };
-  const int64_t row_tiles = cdiv(p.M, 16);
-  by_rank([&](auto n) {
-    constexpr int RT = decltype(n)::value, D = RT == 4 ? 1 : RT == 2 ? 2 : 4;
-    const dim3 grid((unsigned)(row_tiles * p.slots), (unsigned)cdiv(tiles, RT), (unsigned)l.splits);
-    if (l.many) lora_ranks_kernel<T, RT, 8, D == 4 ? 2 : D, true><<<grid, 512, 0, st>>>(p);
-    else lora_ranks_kernel<T, RT, 4, D, false><<<grid, 256, 0, st>>>(p);
+  by_rank([&](auto n, auto, auto w) {
+    constexpr int N = decltype(n)::value, W = decltype(w)::value, D = N == 4 ? 2 : 4;
+    if (p.K < 8) {
+      const dim3 grid((unsigned)cdiv(p.M, 256 / W), (unsigned)(p.ranks / W));
+      if (l.many) lora_ranks_short_kernel<T, W, true><<<grid, 256, 0, st>>>(p);
+      else lora_ranks_short_kernel<T, W, false><<<grid, 256, 0, st>>>(p);
+      return;
+    }
+    const dim3 grid((unsigned)(p.tiles * p.slots), (unsigned)cdiv(p.ranks, 16 * N), (unsigned)l.splits);
+    if (l.many) lora_ranks_kernel<T, N, W, D, true><<<grid, 256, 0, st>>>(p);
+    else lora_ranks_kernel<T, N, W, D, false><<<grid, 256, 0, st>>>(p);
   });
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
-  const int64_t x = l.many ? cdiv(p.M, 128) : row_tiles * p.slots, step = l.many ? 64 : 128;
+  const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 128;
   const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, 2048 / x);
   p.cols = (int)(cdiv(steps, std::min(want, steps)) * step);
-  const dim3 grid((unsigned)x, (unsigned)std::max<int64_t>(1, cdiv(p.whole, p.cols)));
-  by_rank([&](auto n) {
-    constexpr int RT = decltype(n)::value;
-    if (l.many) lora_columns_kernel<T, RT><<<grid, 256, 0, st>>>(p);
-    else lora_columns_few_kernel<T, RT><<<grid, 256, (size_t)16 * (2 * p.ranks + 8) * 2, st>>>(p);
+  p.ranges = (int)std::max<int64_t>(1, cdiv(p.whole, p.cols));
+  // results past the caches where they are many (and not in lines that base has brought there): N = 24576, rank 64, 4096 rows
+  // 112 us, 150 through them; 8192 columns of 2000 rows gain 3 us of 24, but the next reader may want those
+  const bool through = p.out != p.base && p.M * p.N >= (int64_t)32 << 20;
+  by_rank([&](auto, auto n, auto w) {
+    constexpr int RT = decltype(n)::value, W = decltype(w)::value;
+    const dim3 blocks((unsigned)(x * p.ranges));
+    if (l.many && through) lora_columns_kernel<T, RT, W, true><<<blocks, 256, 0, st>>>(p);
+    else if (l.many) lora_columns_kernel<T, RT, W, false><<<blocks, 256, 0, st>>>(p);
+    else lora_columns_few_kernel<T, RT, W><<<dim3((unsigned)x, (unsigned)p.ranges), 256, (size_t)16 * (2 * p.ranks + 8) * 2, st>>>(p);
   });
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }
@@ -539,7 +604,7 @@ int launch_lora(const LoraCall& c, hipStream_t st) {
   p.M = c.M, p.N = (int)c.N, p.K = (int)c.K, p.R = (int)c.R, p.L = c.L, p.id64 = c.id64;
   p.ranks = (int)lora_ranks(c.R), p.whole = (int)lora_whole(c.N, c.R);
   const LoraPlan l = lora_plan(c.M, c.K, c.R);
-  p.slots = l.slots, p.splits = l.splits, p.per = l.per;
+  p.tiles = (int)cdiv(c.M, 16), p.slots = l.slots, p.splits = l.splits, p.per = l.per;
   p.partial = (float*)c.workspace;
   p.v = (uint16_t*)c.workspace, p.powers = (float*)(p.v + (size_t)c.M * 2 * p.ranks);
   return c.dtype == AWQ_DTYPE_F16 ? lora_typed<f16>(p, l, st) : lora_typed<bf16>(p, l, st);
