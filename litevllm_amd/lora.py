@@ -13,6 +13,7 @@ from .mxfp4 import _call, _derivative_asked, _meet, _Refused
 from .moe_sort import _rows
 
 MAX_RANK = 256
+_DTYPES = {torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 
 
 def _stack(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -37,35 +38,38 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
     request's tokens are.  Results are bitwise reproducible.  Not differentiable: a backward through the result
     raises, and so does a call with ``out`` where an input requires a gradient."""
     dev = ops._require_device(base, x, lora_a, lora_b, ids, scales, out)
-    if lora_a.dim() != 3 or lora_b.dim() != 3 or lora_a.shape[0] != lora_b.shape[0] or lora_a.shape[1] != lora_b.shape[2]:
-        raise ValueError(f"lora_a must be [L, R, K] and lora_b [L, N, R], got {tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
-    adapters, rank, k = lora_a.shape
-    n = lora_b.shape[1]
+    a_shape, b_shape, x_shape, dtype = lora_a.shape, lora_b.shape, x.shape, x.dtype
+    if len(a_shape) != 3 or len(b_shape) != 3 or a_shape[0] != b_shape[0] or a_shape[1] != b_shape[2]:
+        raise ValueError(f"lora_a must be [L, R, K] and lora_b [L, N, R], got {tuple(a_shape)} and {tuple(b_shape)}")
+    adapters, rank, k = a_shape
+    n = b_shape[1]
     if adapters < 1 or not 1 <= rank <= MAX_RANK or k < 1:
-        raise ValueError(f"at least one adapter and input, a rank of 1 to {MAX_RANK}, got lora_a {tuple(lora_a.shape)}")
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"K mismatch: x is {tuple(x.shape)}, lora_a has {k}")
-    dtype, lead = x.dtype, x.shape[:-1]
-    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"at least one adapter and input, a rank of 1 to {MAX_RANK}, got lora_a {tuple(a_shape)}")
+    if not x_shape or x_shape[-1] != k:
+        raise ValueError(f"K mismatch: x is {tuple(x_shape)}, lora_a has {k}")
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise TypeError(f"unsupported dtype {dtype}: fp16 or bf16")
-    for what, t in (("base", base), ("lora_a", lora_a), ("lora_b", lora_b), ("out", out)):
-        if t is not None and t.dtype is not dtype:
-            raise TypeError(f"{what} must be of x's type {dtype}, got {t.dtype}")
-    for what, t in (("base", base), ("out", out)):
-        if t is not None and t.shape != lead + (n,):
-            raise ValueError(f"{what} must be {tuple(lead + (n,))}, got {tuple(t.shape)}")
-    if ids.dtype not in (torch.int32, torch.int64):
+    lead = x_shape[:-1]
+    shape = lead + (n,)
+    if lora_a.dtype is not dtype or lora_b.dtype is not dtype or (base is not None and base.dtype is not dtype) or (
+            out is not None and out.dtype is not dtype):
+        raise TypeError(f"base, lora_a, lora_b and out must be of x's type {dtype}, got "
+                        f"{[None if t is None else t.dtype for t in (base, lora_a, lora_b, out)]}")
+    if (base is not None and base.shape != shape) or (out is not None and out.shape != shape):
+        raise ValueError(f"base and out must be {tuple(shape)}, got {[None if t is None else tuple(t.shape) for t in (base, out)]}")
+    wide = ids.dtype is torch.int64
+    if not wide and ids.dtype is not torch.int32:
         raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
     if ids.shape != lead:
         raise ValueError(f"ids must be {tuple(lead)}, got {tuple(ids.shape)}")
     if scales is not None and (scales.dtype is not torch.float32 or scales.shape != (adapters,)):
         raise ValueError(f"scales must be fp32 [{adapters}], got {scales.dtype} {tuple(scales.shape)}")
-    inputs = (base, x, lora_a, lora_b, scales)
-    asked = _derivative_asked("lora_add", out, *inputs)
+    asked = _derivative_asked("lora_add", out, base, x, lora_a, lora_b, scales)
     m = ids.numel()
-    given, in_place = out is not None, out is not None and out is base
-    if out is None:
-        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+    given = out is not None
+    if not given:
+        out = torch.empty(shape, dtype=dtype, device=dev) if base is None or not base.is_contiguous() else torch.empty_like(base)
         to, ldo = out, n
     else:
         to = out if out.dim() == 2 else out.view(-1, n)  # raises where its rows are no matrix
@@ -74,28 +78,36 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
             raise ValueError(f"bad_output: out must have dense rows apart from each other, got strides {out.stride()}")
     if m == 0 or n == 0:
         return out
-    x2, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+    if x.is_contiguous():
+        ldx = k
+    else:
+        x, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
     at, ldb = None, n
-    if in_place:
+    if base is out:
         at, ldb = to.data_ptr(), ldo
     elif base is not None:
-        flat, ldb = _rows(base if base.dim() == 2 else base.reshape(-1, n))
+        flat = base
+        if not base.is_contiguous():
+            flat, ldb = _rows(base if base.dim() == 2 else base.reshape(-1, n))
         if given and (flat.data_ptr() != to.data_ptr() or ldb != ldo) and _meet(flat, to):
             flat, ldb = flat.clone(memory_format=torch.contiguous_format), n  # other elements of the same memory
         at = flat.data_ptr()
-    if given and _meet(x2, to):
-        x2, ldx = x2.clone(memory_format=torch.contiguous_format), k  # read by blocks while others write
-    lora_a, a_stride = _stack(lora_a)
-    lora_b, b_stride = _stack(lora_b)
+    if given and _meet(x, to):
+        x, ldx = x.clone(memory_format=torch.contiguous_format), k  # read by blocks while others write
+    a_stride, b_stride = rank * k, n * rank
+    if not lora_a.is_contiguous():
+        lora_a, a_stride = _stack(lora_a)
+    if not lora_b.is_contiguous():
+        lora_b, b_stride = _stack(lora_b)
     ids = ids.contiguous()
     if scales is not None:
         scales = scales.contiguous()
-    ws_bytes = L.load().awq_w4a16_lora_workspace_bytes(m, k, rank)
+    ws_bytes = (L._lib or L.load()).awq_w4a16_lora_workspace_bytes(m, k, rank)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call(dev, "awq_w4a16_lora_add", at, ldb, x2.data_ptr(), ldx, lora_a.data_ptr(), a_stride, lora_b.data_ptr(), b_stride,
-          ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, ops._ptr(scales), to.data_ptr(), ldo, m, n, k, rank, adapters,
-          ops.dtype_code(dtype), ws.data_ptr(), ws_bytes)
-    return _Refused.apply("lora_add is not differentiable", out, *inputs) if asked else out
+    _call(dev, "awq_w4a16_lora_add", at, ldb, x.data_ptr(), ldx, lora_a.data_ptr(), a_stride, lora_b.data_ptr(), b_stride,
+          ids.data_ptr(), 64 if wide else 32, None if scales is None else scales.data_ptr(), to.data_ptr(), ldo, m, n, k, rank,
+          adapters, code, ws.data_ptr(), ws_bytes)
+    return _Refused.apply("lora_add is not differentiable", out, base, x, lora_a, lora_b, scales) if asked else out
 
 
 class LoRAAdapters(nn.Module):

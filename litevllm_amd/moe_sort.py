@@ -25,8 +25,10 @@ class MoERoutes(NamedTuple):
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """A 2-D ``x``, or a copy, whose rows are dense, and its row stride."""
     n, h = x.shape
+    if x.is_contiguous():
+        return x, h
     if (h > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < h):
-        x = x.contiguous()
+        return x.contiguous(), h
     return x, x.stride(0) if n > 1 else h
 
 
@@ -37,48 +39,52 @@ def _back(name: str, on: int, *saved: tuple) -> None:
             raise RuntimeError(f"{name}: saved tensors came back elsewhere, or with other shapes or types")
 
 
-def _sorted(x, ids, experts):
-    (t, h), k, dev = x.shape, ids.shape[1], x.device
+def _index(x, ids, experts):
+    """(offsets, experts, places), one allocation, still to be written."""
+    t, k = ids.shape
+    r = t * k
+    offsets, of, places = torch.empty(experts + 1 + 2 * r, dtype=torch.int32, device=x.device).split_with_sizes((experts + 1, r, r))
+    return offsets, of, places.view(t, k)
+
+
+def _sorted(x, ids, experts, index):
+    (t, k), h, dev = ids.shape, x.shape[1], x.device
     rows = torch.empty((t * k, h), dtype=x.dtype, device=dev)
-    # offsets, experts and places in one allocation
-    index = torch.empty(experts + 1 + 2 * t * k, dtype=torch.int32, device=dev)
-    offsets, of, places = index[:experts + 1], index[experts + 1:experts + 1 + t * k], index[experts + 1 + t * k:].view(t, k)
-    need = L.load().awq_w4a16_moe_sort_workspace_bytes(t, experts, k)
+    need = (L._lib or L.load()).awq_w4a16_moe_sort_workspace_bytes(t, experts, k)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     x, ld = _rows(x)
-    _call(dev, "awq_w4a16_moe_sort", x.data_ptr(), ld, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, rows.data_ptr(),
+    offsets, of, places = index
+    _call(dev, "awq_w4a16_moe_sort", x.data_ptr(), ld, ids.data_ptr(), 64 if ids.dtype is torch.int64 else 32, rows.data_ptr(),
           offsets.data_ptr(), of.data_ptr(), places.data_ptr(), t, h, experts, k, ops.dtype_code(x.dtype), ops._ptr(ws), need)
-    return rows, offsets, of, places
+    return rows
 
 
 def _unsorted(rows, weights, places):
-    (t, k), h = places.shape, rows.shape[1]
-    out = torch.empty((t, h), dtype=rows.dtype, device=rows.device)
-    _call(rows.device, "awq_w4a16_moe_unsort", rows.data_ptr(), places.data_ptr(), ops._ptr(weights),
-          L.DTYPE_NONE if weights is None else ops.dtype_code(weights.dtype), out.data_ptr(), h, t, h, k, ops.dtype_code(rows.dtype))
+    (t, k), h, dtype = places.shape, rows.shape[1], rows.dtype
+    out = torch.empty((t, h), dtype=dtype, device=rows.device)
+    _call(rows.device, "awq_w4a16_moe_unsort", rows.data_ptr(), places.data_ptr(), None if weights is None else weights.data_ptr(),
+          L.DTYPE_NONE if weights is None else ops.dtype_code(weights.dtype), out.data_ptr(), h, t, h, k, ops.dtype_code(dtype))
     return out
 
 
 class _Sort(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, ids, experts):
-        rows, offsets, of, places = _sorted(x, ids, experts)
-        ctx.save_for_backward(places)
-        ctx.mark_non_differentiable(offsets, of, places)
-        ctx.set_materialize_grads(False)
-        ctx.shape = ids.shape
-        return rows, offsets, of, places
+    """The rows; the index, which is no function of x, is written on the way and comes from outside."""
 
     @staticmethod
-    def backward(ctx, upstream, *_):
-        if upstream is None:
-            return None, None, None
+    def forward(ctx, x, ids, experts, index):
+        places = index[2]
+        ctx.save_for_backward(places)
+        ctx.shape = ids.shape
+        return _sorted(x, ids, experts, index)
+
+    @staticmethod
+    def backward(ctx, upstream):
         places, = ctx.saved_tensors
         _back("moe_sort", upstream.get_device(), (places, torch.int32, ctx.shape))
         grad = _unsorted(upstream.contiguous(), None, places.contiguous())
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
             grad = _Refused.apply("moe_sort is not differentiable twice", grad, upstream)
-        return grad, None, None
+        return grad, None, None, None
 
 
 class _Unsort(torch.autograd.Function):
@@ -129,9 +135,9 @@ def moe_sort(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> tuple
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     topk_ids = topk_ids.contiguous()
+    index = _index(x, topk_ids, num_experts)
     run = _Sort.apply if _derivative_asked("moe_sort", None, x) else _sorted
-    rows, *routes = run(x, topk_ids, num_experts)
-    return rows, MoERoutes(*routes)
+    return run(x, topk_ids, num_experts, index), MoERoutes(*index)
 
 
 def moe_unsort(rows: torch.Tensor, topk_weights: torch.Tensor | None, routes: MoERoutes) -> torch.Tensor:
