@@ -22,7 +22,7 @@ bool lora_fits(int64_t M, int64_t N, int64_t K, int64_t R) {
 extern "C" {
 
 size_t awq_w4a16_moe_sort_workspace_bytes(int64_t T, int32_t E, int32_t top_k) {
-  return T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || !routes_fit(T, 0, top_k) ? 0 : moe_sort_workspace_bytes(T, E, top_k);
+  return T <= 0 || E <= 0 || E > 1024 || top_k <= 0 || top_k > 1024 || !routes_fit(T, 0, top_k) ? 0 : moe_sort_workspace_bytes(T, E, top_k);
 }
 
 int awq_w4a16_moe_sort(const void* x, int64_t ldx, const void* topk_ids, int32_t ids_bits, void* rows, int32_t* offsets,
@@ -31,7 +31,7 @@ int awq_w4a16_moe_sort(const void* x, int64_t ldx, const void* topk_ids, int32_t
   if (T < 0 || H < 0 || E <= 0 || top_k <= 0) return AWQ_ERR_SHAPE;
   if (!offsets || (T > 0 && (!topk_ids || !experts || !places || (H > 0 && (!x || !rows))))) return AWQ_ERR_NULL;
   if (!dtype_float(dtype) || (ids_bits != 32 && ids_bits != 64)) return AWQ_ERR_UNSUPPORTED;
-  if (E > 1024 || !routes_fit(T, H, top_k)) return AWQ_ERR_UNSUPPORTED;
+  if (E > 1024 || top_k > 1024 || !routes_fit(T, H, top_k)) return AWQ_ERR_UNSUPPORTED;
   const int size = dtype == AWQ_DTYPE_F32 ? 4 : 2;
   if ((T > 1 && ldx < H) || !aligned(x, size) || !aligned(rows, size)) return AWQ_ERR_STRIDE;
   const size_t need = awq_w4a16_moe_sort_workspace_bytes(T, E, top_k);

@@ -121,7 +121,8 @@ def moe_sort(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> tuple
     expert and an expert's in the order of the tokens (:class:`MoERoutes`); differentiable in ``x``.
 
     ``topk_ids``: int32 or int64 ``[T, top_k]``; routes whose id is outside ``[0, num_experts)`` (dropped ones, experts of other
-    devices) get no row, and as many rows behind the last are 0 (what a gradient holds there is not read).  1 to 1024 experts.
+    devices) get no row, and as many rows behind the last are 0 (what a gradient holds there is not read).  1 to 1024 experts and
+    routes a token.
     ``routes.offsets`` stays on the device; a loop over experts that needs it on the host reads it there itself.  The gradient
     is not differentiable again.  As for any operation, a backward is captured into a graph only while no graph recorded
     outside the capture over the same leaves is alive."""
@@ -130,8 +131,8 @@ def moe_sort(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> tuple
     if x.dim() != 2 or topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0]:
         raise ValueError(f"x must be [T, H] and topk_ids [T, top_k], got {tuple(x.shape)} and {tuple(topk_ids.shape)}")
     num_experts = int(num_experts)
-    if not 1 <= num_experts <= 1024 or topk_ids.shape[1] < 1:
-        raise ValueError(f"1 to 1024 experts and at least one route a token, got {num_experts} and {topk_ids.shape[1]}")
+    if not 1 <= num_experts <= 1024 or not 1 <= topk_ids.shape[1] <= 1024:
+        raise ValueError(f"1 to 1024 experts and 1 to 1024 routes a token, got {num_experts} and {topk_ids.shape[1]}")
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     topk_ids = topk_ids.contiguous()

@@ -41,7 +41,8 @@ def _whole(seed, *shape, size=4):
 # one launch and three, few and many experts, rows of one element, of odd widths, of several blocks
 CASES = [(1, 1, 1, 1, 0.0), (1, 8, 2, 7, 0.0), (4, 64, 8, 256, 0.0), (3, 5, 11, 33, 0.5), (37, 160, 6, 1001, 0.3), (511, 7, 8, 24, 0.0),
          (512, 1024, 8, 8, 0.1), (513, 64, 8, 130, 0.2), (4097, 33, 1, 5, 1.0), (9000, 200, 3, 40, 0.4), (20, 16, 2, 9000, 0.2),
-         (40000, 1024, 4, 12, 0.0), (700, 300, 9, 2056, 0.1)]
+         (40000, 1024, 4, 12, 0.0), (2048, 64, 8, 96, 0.0), (2049, 5, 4, 40, 0.2), (60, 40, 130, 20, 0.1), (9, 30, 700, 16, 0.1),
+         (70, 30, 600, 16, 0.1), (11, 1024, 1024, 3, 0.0), (4096, 513, 8, 10, 0.05), (4097, 512, 8, 9, 0.05), (700, 300, 9, 2056, 0.1)]
 
 
 def _check_sort(x, ids, experts):
@@ -288,7 +289,7 @@ def test_refusals():
     rows, routes = moe_sort(x, ids, 4)
     o, of, p = routes
     for bad in (lambda: moe_sort(x[0], ids, 4), lambda: moe_sort(x, ids[:5], 4), lambda: moe_sort(x, ids[0], 4), lambda: moe_sort(x, ids[:, :0], 4),
-                lambda: moe_sort(x, ids, 0), lambda: moe_sort(x, ids, 1025), lambda: moe_sort(x.cpu(), ids, 4), lambda: moe_sort(x.cpu(), ids.cpu(), 4),
+                lambda: moe_sort(x, ids, 0), lambda: moe_sort(x, ids.repeat(1, 513), 4), lambda: moe_sort(x, ids, 1025), lambda: moe_sort(x.cpu(), ids, 4), lambda: moe_sort(x.cpu(), ids.cpu(), 4),
                 lambda: moe_unsort(rows[:11], w, routes), lambda: moe_unsort(rows[0], w, routes), lambda: moe_unsort(rows, w[:5], routes),
                 lambda: moe_unsort(rows, w.cpu(), routes), lambda: moe_unsort(rows, w, MoERoutes(o, of, p[0])),
                 lambda: moe_unsort(rows, w, MoERoutes(o[:1], of, p)), lambda: moe_unsort(rows, w, MoERoutes(o, of, p[:, :0]))):
@@ -334,13 +335,13 @@ def test_entries_refuse():
         return lib.awq_w4a16_moe_sort(x, ld, ids, bits, rows, off, p, p, t, h, e, k, dt, ws, wsb, None)
     assert sort(x=None) == sort(ids=None) == sort(rows=None) == sort(off=None) == L.ERR_NULL
     assert sort(t=-1) == sort(h=-1) == sort(e=0) == sort(k=0) == L.ERR_SHAPE
-    assert sort(dt=0) == sort(bits=16) == sort(e=1025) == sort(t=(1 << 30) + 1) == sort(t=1 << 29, k=3) == L.ERR_UNSUPPORTED
+    assert sort(dt=0) == sort(bits=16) == sort(e=1025) == sort(k=1025) == sort(t=(1 << 30) + 1) == sort(t=1 << 29, k=3) == L.ERR_UNSUPPORTED
     assert sort(h=(1 << 24) + 1, ld=1 << 25) == L.ERR_UNSUPPORTED
     assert sort(ld=7) == sort(x=p + 1) == sort(rows=p + 2, dt=L.DTYPE_F32) == L.ERR_STRIDE
-    need = lib.awq_w4a16_moe_sort_workspace_bytes(5000, 8, 2)
-    assert need > 0 and sort(t=5000) == sort(t=5000, ws=p, wsb=need - 1) == L.ERR_WORKSPACE
-    assert sort(t=5000, ws=p + 4, wsb=need) == L.ERR_STRIDE
-    for t, e, k in ((0, 8, 2), (-1, 8, 2), (5, 0, 2), (5, 1025, 2), (5, 8, 0), ((1 << 30) + 1, 8, 1), (1 << 62, 8, 8)):
+    need = lib.awq_w4a16_moe_sort_workspace_bytes(50000, 8, 2)
+    assert need > 0 and sort(t=50000) == sort(t=50000, ws=p, wsb=need - 1) == L.ERR_WORKSPACE
+    assert sort(t=50000, ws=p + 4, wsb=need) == L.ERR_STRIDE
+    for t, e, k in ((0, 8, 2), (-1, 8, 2), (5, 0, 2), (5, 1025, 2), (5000, 8, 1025), (5, 8, 0), ((1 << 30) + 1, 8, 1), (1 << 62, 8, 8)):
         assert lib.awq_w4a16_moe_sort_workspace_bytes(t, e, k) == 0
 
     def unsort(rows=p, places=p, w=p, wdt=L.DTYPE_F32, out=p, ld=8, t=2, h=8, k=2, dt=L.DTYPE_F16):
