@@ -59,128 +59,140 @@ __device__ __forceinline__ float row_max16(float v) {
   return fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));
 }
 
-// v of a rank as its two parts.
-struct Halves {
+// v of a rank as its two parts, in units of `power`.
+struct Parts {
   uint16_t high, low;
+  float power;
 };
 template <typename T>
-__device__ __forceinline__ Halves halves_of(float f) {
+__device__ __forceinline__ Parts parts_of(float f, int e) {
+  if constexpr (std::is_same<T, f16>::value) f = ldexpf(f, -e);
   const uint16_t high = to_bits<T>(f);
-  return {high, fabsf(f) < __builtin_inff() ? to_bits<T>(f - from_bits<T>(high)) : (uint16_t)0};  // no Inf - Inf
+  return {high, fabsf(f) < __builtin_inff() ? to_bits<T>(f - from_bits<T>(high)) : (uint16_t)0,  // no Inf - Inf
+          std::is_same<T, f16>::value ? ldexpf(1.f, e) : 1.f};
 }
 // e of a row's tile from its largest value (0, Inf and NaN included).
 __device__ __forceinline__ int tile_exponent(float top) { return (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 13; }
+// The same for W neighbouring lanes that hold a row's tile.
+template <typename T, int W>
+__device__ __forceinline__ Parts tile_parts(float f) {
+  if constexpr (!std::is_same<T, f16>::value) return parts_of<T>(f, 0);
+  float top = row_max16(fabsf(f));
+  if constexpr (W == 32) top = fmaxf(top, __shfl_xor(top, 16));
+  return parts_of<T>(f, tile_exponent(top));
+}
 
 // ------------------------------------------------------------------ ranks
 constexpr int kUnit = 64;  // values of K that a wave takes at once: whole lines of both operands
 
-// A rank's sum, or its parts of v, by W neighbouring lanes for a row's tile; rows that are not `mine` take part only.
+template <int RT, int WAVES>
+union RankLds {
+  uint16_t stage[WAVES][(1 + RT) * 16][kUnit + 8];  // rows 16 bytes apart from whole banks
+  f32x4 part[WAVES][RT][64];
+};
+// RT tiles of 16 ranks, from tile0 on, of adapter `cur` by the rows `rows` of 16 and a share of K, whose units the waves take in
+// turn; the waves' sums come to lie in LDS.  A wave's next unit is on its way in registers (more of them made every size slower:
+// one row, K = N = 4096, rank 16 6.6 us with two, 7.3 with four, 6.3 as it is).  Loads cover whole lines, eight lanes each; a wave passes them through LDS of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and
+// 32 + 8 q .. of rank i and of row i.  (Straight from memory in that order a load's neighbouring lanes are in different lines:
+// 4096 rows, K = 4096, rank 64 42 us instead of 12.)
+template <typename T, int RT, int WAVES>
+__device__ __forceinline__ void tile_ranks(const LoraArgs& p, RankLds<RT, WAVES>& lds, int64_t m0, uint32_t rows, int cur, int tile0,
+                                           int begin, int units) {
+  constexpr int TILES = 1 + RT;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, r8 = lane >> 3, c8 = 8 * (lane & 7);
+  // two rows of each tile a lane; for rows of other adapters a row that is read anyway
+  const uint16_t* from[TILES][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    from[0][h] = p.x + (m0 + (rows >> (r8 + 8 * h) & 1 ? r8 + 8 * h : __builtin_ctz(rows))) * p.ldx + c8;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) from[1 + r][h] = p.a + cur * p.a_stride + (int64_t)min(16 * (tile0 + r) + r8 + 8 * h, p.R - 1) * p.K + c8;
+  }
+  u32x4 piece[TILES][2];
+  auto load = [&](int u) {
+    if (u >= units) return;
+    // the last unit's pieces end with K: what lies past it, or belongs to the piece before, becomes 0 in both operands
+    const int k = u * kUnit + c8, at = min(k, p.K - 8) - c8, twice = k - c8 - at;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) piece[j][h] = *(const u32x4_any*)(from[j][h] + at);
+    if (u * kUnit + kUnit <= p.K) return;
+    u32x4 mask;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mask[j] = (2 * j >= twice ? 0xFFFFu : 0u) | (2 * j + 1 >= twice ? 0xFFFF0000u : 0u);
+#pragma unroll
+    for (int j = 0; j < TILES; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) piece[j][h] &= mask;
+  };
+  f32x4 acc[RT] = {};
+  load(begin + wave);
+  for (int u = begin + wave; u < units; u += WAVES) {
+#pragma unroll
+    for (int j = 0; j < TILES; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *(u32x4*)&lds.stage[wave][16 * j + r8 + 8 * h][c8] = piece[j][h];
+    load(u + WAVES);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < kUnit; k += 32) {
+      const u32x4 x = *(const u32x4*)&lds.stage[wave][i][k + 8 * q];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) acc[r] = MfmaOp<T>::run(*(const u32x4*)&lds.stage[wave][16 * (1 + r) + i][k + 8 * q], x, acc[r]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();  // all waves are done with their stages
+  // ranks 4 q .. 4 q + 3 of row i
+#pragma unroll
+  for (int r = 0; r < RT; ++r) lds.part[wave][r][lane] = acc[r];
+  __syncthreads();
+}
+// f(row, rank of the block's, sum) of what lies there, a row's W ranks by W neighbouring lanes.
+template <int RT, int WAVES, int W, class F>
+__device__ __forceinline__ void for_ranks(const RankLds<RT, WAVES>& lds, F f) {
+  for (int at = threadIdx.x; at < RT * 256; at += 64 * WAVES) {
+    const int row = at / W % 16, rank = at / (16 * W) * W + at % W, j = rank & 15;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += ((const float*)&lds.part[w][rank >> 4][16 * (j >> 2) + row])[j & 3];
+    f(row, rank, s);
+  }
+}
+
+// A rank's sum (few rows), or with the whole of K its parts of v, by W neighbouring lanes; rows that are not `mine` take part only.
 template <typename T, int W, bool FINAL>
 __device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank, float f, float scale, bool mine) {
   if constexpr (FINAL) {
-    f = rank < p.R ? f * scale : 0.f;
-    if constexpr (std::is_same<T, f16>::value) {
-      float top = row_max16(fabsf(f));
-      if constexpr (W == 32) top = fmaxf(top, __shfl_xor(top, 16));
-      const int e = tile_exponent(top);
-      f = ldexpf(f, -e);
-      if (mine && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = ldexpf(1.f, e);
-    }
+    const Parts h = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
     if (!mine) return;
-    const Halves h = halves_of<T>(f);
     uint16_t* const to = p.v + m * 2 * p.ranks + 2 * (rank / W) * W + rank % W;
     to[0] = h.high, to[W] = h.low;
+    if (std::is_same<T, f16>::value && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = h.power;
   } else if (mine) {
     p.partial[((int64_t)blockIdx.z * p.M + m) * p.ranks + rank] = f;
   }
 }
 
-// RT tiles of 16 ranks by a tile of 16 rows and a share of K, whose units the waves take in turn; the waves' sums meet in LDS.
-// D units of a wave are on their way in registers.  Loads cover whole lines, eight lanes each; a wave passes them through LDS
-// of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and 32 + 8 q .. of rank i and of row i.
-// (Straight from memory in that order a load's neighbouring lanes are in different lines: 4096 rows, K = 4096, rank 64 42 us.)
-// FINAL: the share is all of K, the parts of v go out; else the sums.
-template <typename T, int RT, int W, int D, bool FINAL>
-__global__ void __launch_bounds__(256, 1) lora_ranks_kernel(LoraArgs p) {
-  constexpr int WAVES = 4, TILES = 1 + RT, LD = kUnit + 8;  // rows 16 bytes apart from whole banks
-  union Lds {
-    uint16_t stage[WAVES][TILES * 16][LD];
-    f32x4 part[WAVES][RT][64];
-  };
-  __shared__ __attribute__((aligned(16))) Lds lds;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, r8 = lane >> 3, c8 = 8 * (lane & 7);
-  const int tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
+template <typename T, int RT, int W, bool FINAL>
+__global__ void __launch_bounds__(256) lora_ranks_kernel(LoraArgs p) {
+  __shared__ __attribute__((aligned(16))) RankLds<RT, 4> lds;
+  const int lane = threadIdx.x & 63, tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
   const int64_t m0 = (int64_t)tile * 16;
-  const int id = m0 + i < p.M ? lora_id(p, m0 + i) : -1;
-  const int begin = blockIdx.z * p.per + wave, units = min((int)(blockIdx.z + 1) * p.per, (p.K + kUnit - 1) / kUnit);
+  const int id = m0 + (lane & 15) < p.M ? lora_id(p, m0 + (lane & 15)) : -1;
+  const int begin = blockIdx.z * p.per, units = min(begin + p.per, (p.K + kUnit - 1) / kUnit);
   uint32_t left = (uint32_t)(__ballot(id >= 0) & 0xFFFF);
   for (int n = 0; left; ++n) {
-    const int first = __builtin_ctz(left), cur = __builtin_amdgcn_readlane(id, first);
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
     const uint32_t rows = (uint32_t)(__ballot(id == cur) & 0xFFFF);
     left &= ~rows;
     if (n % p.slots != slot) continue;
-    // two rows of each tile a lane; for rows of other adapters a row that is read anyway
-    const uint16_t* from[TILES][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      from[0][h] = p.x + (m0 + (rows >> (r8 + 8 * h) & 1 ? r8 + 8 * h : first)) * p.ldx + c8;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) from[1 + r][h] = p.a + cur * p.a_stride + (int64_t)min(16 * (tile0 + r) + r8 + 8 * h, p.R - 1) * p.K + c8;
-    }
-    u32x4 piece[D][TILES][2];
-    auto load = [&](int d, int u) {
-      if (u >= units) return;
-      // the last unit's pieces end with K: what lies past it, or belongs to the piece before, becomes 0 in both operands
-      const int k = u * kUnit + c8, at = min(k, p.K - 8) - c8, twice = k - c8 - at;
-#pragma unroll
-      for (int j = 0; j < TILES; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) piece[d][j][h] = *(const u32x4_any*)(from[j][h] + at);
-      if (u * kUnit + kUnit <= p.K) return;
-      u32x4 mask;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) mask[j] = (2 * j >= twice ? 0xFFFFu : 0u) | (2 * j + 1 >= twice ? 0xFFFF0000u : 0u);
-#pragma unroll
-      for (int j = 0; j < TILES; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) piece[d][j][h] &= mask;
-    };
-    f32x4 acc[RT] = {};
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(d, begin + d * WAVES);
-    for (int u0 = begin; u0 < units; u0 += D * WAVES) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        const int u = u0 + d * WAVES;
-        if (u >= units) continue;
-#pragma unroll
-        for (int j = 0; j < TILES; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) *(u32x4*)&lds.stage[wave][16 * j + r8 + 8 * h][c8] = piece[d][j][h];
-        load(d, u + D * WAVES);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-        for (int k = 0; k < kUnit; k += 32) {
-          const u32x4 x = *(const u32x4*)&lds.stage[wave][i][k + 8 * q];
-#pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r] = MfmaOp<T>::run(*(const u32x4*)&lds.stage[wave][16 * (1 + r) + i][k + 8 * q], x, acc[r]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      }
-    }
-    __syncthreads();  // all waves are done with their stages
-    // ranks 4 q .. 4 q + 3 of row i
-#pragma unroll
-    for (int r = 0; r < RT; ++r) lds.part[wave][r][lane] = acc[r];
-    __syncthreads();
-    for (int at = t; at < RT * 256; at += 64 * WAVES) {
-      const int row = at / W % 16, rank = at / (16 * W) * W + at % W, j = rank & 15;  // rank of the block's
-      float f = 0.f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) f += ((const float*)&lds.part[w][rank >> 4][16 * (j >> 2) + row])[j & 3];
-      const int all = 16 * tile0 + rank;
-      if (all < p.ranks) put_rank<T, W, FINAL>(p, m0 + row, all, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
-    }
+    tile_ranks<T, RT, 4>(p, lds, m0, rows, cur, tile0, begin, units);
+    for_ranks<RT, 4, W>(lds, [&](int row, int rank, float f) {
+      rank += 16 * tile0;
+      if (rank < p.ranks) put_rank<T, W, FINAL>(p, m0 + row, rank, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
+    });
     __syncthreads();
   }
 }
@@ -204,7 +216,7 @@ template <typename T, int W, class Parts, class Power>
 __device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b, int64_t m0, int count, uint64_t rows, bool adapter,
                                             Parts parts, Power power) {
   const int odd = p.N - p.whole;
-  for (int at = threadIdx.x; at < count * odd; at += 256) {
+  for (int at = threadIdx.x; at < count * odd; at += blockDim.x) {
     const int row = at / odd, col = p.whole + at - row * odd;
     if (!(rows >> row & 1)) continue;
     const int64_t m = m0 + row;
@@ -249,10 +261,13 @@ __device__ __forceinline__ u32x4 added(const u32x4& base, const f32x4& d0, const
 
 // Few rows: 16 by p.cols columns, B straight from memory.  A wave takes 32 columns at a time as two tiles of 16, tile c of them
 // the columns 8 (i / 4) + 4 c + i % 4, so that lane (q, i) ends with the eight columns 8 q .. 8 q + 7 of row i.  RT tiles of W
-// ranks at a time.  Base and B of the first columns are on their way while the shares of v are added up.
-template <typename T, int RT, int W>
-__global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
-  constexpr int SUB = W / 16;
+// ranks at a time.  Base and B of the first columns are on their way while v is made ready: the shares of the first launch are
+// added up or, OWN > 0, all OWN tiles of 16 ranks computed by the block itself, for all of its columns.
+constexpr int few_waves(bool own) { return own ? 8 : 4; }
+template <typename T, int RT, int W, int OWN>
+__global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_columns_few_kernel(LoraArgs p) {
+  constexpr int SUB = W / 16, WAVES = few_waves(OWN > 0), STEP = WAVES * 32;
+  __shared__ __attribute__((aligned(16))) RankLds<OWN ? OWN : 1, OWN ? WAVES : 1> own;
   extern __shared__ u32x4 dynamic_lds[];  // v: [16][ld], of each W ranks the high parts, then the low parts
   __shared__ float power[16][16];
   uint16_t* const v = (uint16_t*)dynamic_lds;
@@ -297,8 +312,18 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
     if (cur >= 0) {
       const float scale = p.scales ? p.scales[cur] : 1.f;
       __syncthreads();  // v of the adapter before is read
+      if constexpr (OWN > 0) {
+        tile_ranks<T, OWN, WAVES>(p, own, m0, rows, cur, 0, 0, (p.K + kUnit - 1) / kUnit);
+        for_ranks<OWN, WAVES, W>(own, [&](int row, int rank, float f) {
+          if (rank >= p.ranks) return;
+          const Parts two = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
+          uint16_t* const to = v + row * ld + 2 * (rank / W) * W + rank % W;
+          to[0] = two.high, to[W] = two.low;
+          if (rank % W == 0) power[row][rank / W] = two.power;
+        });
+      }
       // a wave has a row's tile, lane (q, i) the shares q, q + 4, ... of ranks i and 16 + i
-      for (int j = wave; j < 16 * tiles; j += 4) {
+      for (int j = wave; j < 16 * tiles && !OWN; j += 4) {
         const int row = j & 15, r = j >> 4;
         if (!(rows >> row & 1)) continue;
         const float* const at = p.partial + (m0 + row) * p.ranks + W * r + i;
@@ -317,19 +342,17 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
           f[h] = W * r + 16 * h + i < p.R ? f[h] * scale : 0.f;
           top = fmaxf(top, fabsf(f[h]));
         }
-        if constexpr (std::is_same<T, f16>::value) {
-          e = tile_exponent(row_max16(top));
-          if (lane == 0) power[row][r] = ldexpf(1.f, e);
-        }
+        if constexpr (std::is_same<T, f16>::value) e = tile_exponent(row_max16(top));
 #pragma unroll
         for (int h = 0; h < SUB; ++h) {
-          const Halves two = halves_of<T>(std::is_same<T, f16>::value ? ldexpf(f[h], -e) : f[h]);
+          const Parts two = parts_of<T>(f[h], e);
           if (q < 2) v[row * ld + 2 * W * r + W * q + 16 * h + i] = q ? two.low : two.high;
+          if (lane == 0) power[row][r] = two.power;
         }
       }
       __syncthreads();
     }
-    for (int c0 = begin; c0 < end; c0 += 4 * 32) {
+    for (int c0 = begin; c0 < end; c0 += STEP) {
       f32x4 sum[2] = {};
       for (int r0 = 0; r0 < tiles && cur >= 0; r0 += RT) {
         if (r0) load_b(c0, r0);
@@ -353,15 +376,15 @@ __global__ void __launch_bounds__(256) lora_columns_few_kernel(LoraArgs p) {
         }
       }
       const u32x4 now = from;
-      if (c0 + 4 * 32 < end) {
-        load_base(c0 + 4 * 32);
-        if (cur >= 0) load_b(c0 + 4 * 32, 0);
+      if (c0 + STEP < end) {
+        load_base(c0 + STEP);
+        if (cur >= 0) load_b(c0 + STEP, 0);
       }
       if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
     }
     if (blockIdx.y + 1 == gridDim.y)
       odd_columns<T, W>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; },
-                        [&](int row, int r) { return std::is_same<T, f16>::value ? power[row][r] : 1.f; });
+                        [&](int row, int r) { return power[row][r]; });
   }
 }
 
@@ -534,7 +557,7 @@ static int64_t lora_whole(int64_t N, int64_t R) {
 }
 
 struct LoraPlan {
-  bool many;
+  bool many, own;  // own: the few rows' v by the blocks themselves
   int slots, splits, per;
 };
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
@@ -544,6 +567,10 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   // a batch of single tokens has many adapters in a tile, prompts one or two
   l.slots = M <= 128 ? (int)std::min<int64_t>(16, M) : l.many ? 2 : 1;
   l.splits = 1, l.per = (int)units;
+  // One launch where few rows' adapters are small enough to be read by all of a row's blocks.  us with one and with two, which
+  // cost the host 4 more (one row: A of 128 KB 6.3, 6.2, of 256 7.9, 6.7, of 384 11.2, 6.5; 64 rows of as many adapters: 128 KB
+  // 9.9, 12.9, 256 13.5, 16.1, 512 19.8, 25.0; 128 rows: 128 KB 12.7, 16.8, 256 KB and two adapters 21.4, 18.1).
+  l.own = lora_ranks(R) <= 64 && K >= 8 && lora_ranks(R) * K * 2 <= (M <= 32 ? 256 << 10 : M <= 64 ? 512 << 10 : M <= 128 ? 128 << 10 : 0);
   if (!l.many) {
     const int64_t want = std::max<int64_t>(1, 256 / (tiles * l.slots * cdiv(lora_ranks(R), 64)));
     l.per = (int)std::max<int64_t>(4, cdiv(units, std::min<int64_t>(want, 16)));
@@ -554,6 +581,7 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
 size_t lora_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   const LoraPlan l = lora_plan(M, K, R);
   const size_t values = (size_t)M * (size_t)lora_ranks(R);
+  if (l.own) return 0;
   return l.many ? values * 4 + values / (size_t)lora_tile(R) * 4 : (size_t)l.splits * values * 4;
 }
 
@@ -566,8 +594,8 @@ static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
     else if (p.ranks == 32) f(integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 32>{});
     else f(integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 32>{});
   };
-  by_rank([&](auto n, auto, auto w) {
-    constexpr int N = decltype(n)::value, W = decltype(w)::value, D = N == 4 ? 2 : 4;
+  if (!l.own) by_rank([&](auto n, auto, auto w) {
+    constexpr int N = decltype(n)::value, W = decltype(w)::value;
     if (p.K < 8) {
       const dim3 grid((unsigned)cdiv(p.M, 256 / W), (unsigned)(p.ranks / W));
       if (l.many) lora_ranks_short_kernel<T, W, true><<<grid, 256, 0, st>>>(p);
@@ -575,23 +603,25 @@ static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
       return;
     }
     const dim3 grid((unsigned)(p.tiles * p.slots), (unsigned)cdiv(p.ranks, 16 * N), (unsigned)l.splits);
-    if (l.many) lora_ranks_kernel<T, N, W, D, true><<<grid, 256, 0, st>>>(p);
-    else lora_ranks_kernel<T, N, W, D, false><<<grid, 256, 0, st>>>(p);
+    if (l.many) lora_ranks_kernel<T, N, W, true><<<grid, 256, 0, st>>>(p);
+    else lora_ranks_kernel<T, N, W, false><<<grid, 256, 0, st>>>(p);
   });
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
-  const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 128;
-  const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, 2048 / x);
+  const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 32 * few_waves(l.own);
+  const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, (l.own ? 256 : 2048) / x);
   p.cols = (int)(cdiv(steps, std::min(want, steps)) * step);
   p.ranges = (int)std::max<int64_t>(1, cdiv(p.whole, p.cols));
   // results past the caches where they are many (and not in lines that base has brought there): N = 24576, rank 64, 4096 rows
   // 112 us, 150 through them; 8192 columns of 2000 rows gain 3 us of 24, but the next reader may want those
   const bool through = p.out != p.base && p.M * p.N >= (int64_t)32 << 20;
-  by_rank([&](auto, auto n, auto w) {
+  by_rank([&](auto o, auto n, auto w) {
     constexpr int RT = decltype(n)::value, W = decltype(w)::value;
+    const size_t lds = (size_t)16 * (2 * p.ranks + 8) * 2;
     const dim3 blocks((unsigned)(x * p.ranges));
     if (l.many && through) lora_columns_kernel<T, RT, W, true><<<blocks, 256, 0, st>>>(p);
     else if (l.many) lora_columns_kernel<T, RT, W, false><<<blocks, 256, 0, st>>>(p);
-    else lora_columns_few_kernel<T, RT, W><<<dim3((unsigned)x, (unsigned)p.ranges), 256, (size_t)16 * (2 * p.ranks + 8) * 2, st>>>(p);
+    else if (l.own) lora_columns_few_kernel<T, RT, W, decltype(o)::value><<<dim3((unsigned)x, (unsigned)p.ranges), 64 * few_waves(true), lds, st>>>(p);
+    else lora_columns_few_kernel<T, RT, W, 0><<<dim3((unsigned)x, (unsigned)p.ranges), 256, lds, st>>>(p);
   });
   return hipGetLastError() == hipSuccess ? AWQ_OK : AWQ_ERR_LAUNCH;
 }

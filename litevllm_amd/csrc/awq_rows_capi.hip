@@ -91,8 +91,9 @@ int awq_w4a16_lora_add(const void* base, int64_t ldb, const void* x, int64_t ldx
   if (M > 1 && (ldx < K || ldo < N || (base && ldb < N))) return AWQ_ERR_STRIDE;
   if (L > 1 && (a_stride < R * K || b_stride < N * R)) return AWQ_ERR_STRIDE;
   if (!aligned(x, 2) || !aligned(lora_a, 2) || !aligned(lora_b, 2) || !aligned(base, 2) || !aligned(out, 2)) return AWQ_ERR_STRIDE;
-  if (!workspace || workspace_bytes < lora_workspace_bytes(M, K, R)) return AWQ_ERR_WORKSPACE;
-  if (!aligned(workspace, 16)) return AWQ_ERR_STRIDE;
+  const size_t need = lora_workspace_bytes(M, K, R);
+  if (need && (!workspace || workspace_bytes < need)) return AWQ_ERR_WORKSPACE;
+  if (need && !aligned(workspace, 16)) return AWQ_ERR_STRIDE;
   LoraCall c{};
   c.base = base, c.ldb = ldb, c.x = x, c.ldx = ldx, c.a = lora_a, c.a_stride = a_stride, c.b = lora_b, c.b_stride = b_stride;
   c.ids = ids, c.id64 = ids_bits == 64, c.scales = scales, c.out = out, c.ldo = ldo;

@@ -103,10 +103,10 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
     if scales is not None:
         scales = scales.contiguous()
     ws_bytes = (L._lib or L.load()).awq_w4a16_lora_workspace_bytes(m, k, rank)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _call(dev, "awq_w4a16_lora_add", at, ldb, x.data_ptr(), ldx, lora_a.data_ptr(), a_stride, lora_b.data_ptr(), b_stride,
           ids.data_ptr(), 64 if wide else 32, None if scales is None else scales.data_ptr(), to.data_ptr(), ldo, m, n, k, rank,
-          adapters, code, ws.data_ptr(), ws_bytes)
+          adapters, code, None if ws is None else ws.data_ptr(), ws_bytes)
     return _Refused.apply("lora_add is not differentiable", out, base, x, lora_a, lora_b, scales) if asked else out
 
 

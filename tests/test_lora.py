@@ -336,9 +336,9 @@ def test_entry_refuses():
     assert call(dt=L.DTYPE_F32) == call(bits=8) == call(r=257, sa=1 << 20, sb=1 << 20) == L.ERR_UNSUPPORTED
     assert call(m=(1 << 30) + 1) == call(n=(1 << 24) + 1, ldo=1 << 25, ldb=1 << 25, sb=1 << 40) == L.ERR_UNSUPPORTED
     assert call(ldx=7) == call(ldo=7) == call(ldb=7) == call(sa=31) == call(sb=31) == call(x=p + 1) == call(out=p + 1) == L.ERR_STRIDE
-    need = lib.awq_w4a16_lora_workspace_bytes(2, 8, 4)
-    assert need > 0 and call(ws=None) == call(wsb=need - 1) == L.ERR_WORKSPACE
-    assert call(ws=p + 4) == L.ERR_STRIDE
+    need = lib.awq_w4a16_lora_workspace_bytes(600, 8, 4)
+    assert need > 0 and call(m=600, ws=None) == call(m=600, wsb=need - 1) == L.ERR_WORKSPACE
+    assert call(m=600, ws=p + 4) == L.ERR_STRIDE
     assert call(m=0) == call(n=0) == L.OK
     for m, k, r in ((0, 8, 4), (-1, 8, 4), (2, 0, 4), (2, 8, 0), (2, 8, 257), ((1 << 30) + 1, 8, 4), (2, (1 << 24) + 1, 4)):
         assert lib.awq_w4a16_lora_workspace_bytes(m, k, r) == 0
