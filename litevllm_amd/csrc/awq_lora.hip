@@ -3,9 +3,9 @@
 //   l = ids[m];  v[m] = s_l x[m] A_l^T  (rank values);  out[m] = base[m] + v[m] B_l^T;  out[m] = base[m] without an adapter
 //
 // Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once).  Rows go in tiles that the matrix cores
-// take; a tile looks up which adapters its rows have and runs once for each: once where the rows of a request lie together,
-// as in prompts, up to 16 times in a batch of single tokens, where blocks (`slots`) share these.  The matrix cores do not mix
-// rows, so the other rows of a tile only cost idle lanes.
+// take; a tile looks up which adapters its rows have and is worked on once for each: once where the rows of a request lie
+// together, as in prompts, up to 16 times in a batch of single tokens.  Its blocks (`slots`) share these and, where it has fewer
+// adapters than blocks, an adapter's columns or K.  The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
 //
 // v enters the second product as two 16-bit numbers, v = high + low: 16 bits of mantissa at least for bf16, 21 for fp16, and
 // one rounding for the output.  Both halves meet the same B: ranks go in tiles of W = 32, an instruction for the high parts and
@@ -24,7 +24,7 @@ struct LoraArgs {
   const void* ids;
   const float* scales;
   uint16_t* out;
-  float* partial;  // few rows: [splits][M][ranks], s_l not in it yet
+  float* partial;  // few rows: [shares][M][ranks], s_l not in it yet
   uint16_t* v;     // many rows: [M][2 ranks], of each W ranks the high parts, then the low parts
   float* powers;   // and [M][ranks / W]: 2^e (fp16)
   int64_t ldb, ldx, ldo, a_stride, b_stride;
@@ -32,9 +32,10 @@ struct LoraArgs {
   int N, K, R, L, id64;
   int ranks;  // R in whole tiles of W
   int tiles;  // of 16 rows
-  int slots;  // blocks that share a row tile's adapters: block tile + tiles * slot, so that each slot's are on all XCDs
-  int splits, per;  // shares of K, each of `per` units
-  int cols;   // columns of a block
+  int slots;  // blocks that share a tile's adapters, for few rows as many as it may have: block tile + tiles * slot, so that
+              // each slot's are on all XCDs
+  int splits, shares;  // few rows: shares of K, and how many there may be with sub-shares
+  int cols;   // many rows: columns of a block
   int whole;  // columns that go by eight, see lora_whole
   int ranges;   // many rows: blocks over the columns
 };
@@ -42,6 +43,28 @@ struct LoraArgs {
 __device__ __forceinline__ int lora_id(const LoraArgs& p, int64_t m) {
   const int64_t l = p.id64 ? ((const int64_t*)p.ids)[m] : (int64_t)((const int32_t*)p.ids)[m];
   return l >= 0 && l < p.L ? (int)l : -1;
+}
+// An adapter of a tile of 16 rows and its rows, for a block of `slots`: the only one or, where the tile has fewer adapters than
+// blocks, one that the block shares with others, as number `part` of `parts`.  id: a row's adapter (lanes 0 .. 15), -1 for none,
+// which counts as an adapter, -2: no row.
+struct Group {
+  int adapter;
+  uint32_t rows;
+  int part, parts;
+};
+__device__ __forceinline__ Group group_of(int id, int slot, int slots) {
+  const uint32_t all = (uint32_t)(__ballot(id >= -1) & 0xFFFF);
+  int count = 0;
+  for (uint32_t left = all; left; ++count) left &= ~(uint32_t)__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctz(left)));
+  Group g{};
+  int mine = slot % count;
+  g.part = slot / count, g.parts = (slots - 1 - mine) / count + 1;
+  for (uint32_t left = all; mine >= 0; --mine) {
+    g.adapter = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+    g.rows = (uint32_t)__ballot(id == g.adapter) & left;
+    left &= ~g.rows;
+  }
+  return g;
 }
 // The neighbouring lane's value (lanes 0 and 1 swap, 2 and 3, ...), and the largest of 16 lanes.
 __device__ __forceinline__ u32x4 from_neighbour(u32x4 v) {
@@ -161,43 +184,58 @@ __device__ __forceinline__ void for_ranks(const RankLds<RT, WAVES>& lds, F f) {
   }
 }
 
-// A rank's sum (few rows), or with the whole of K its parts of v, by W neighbouring lanes; rows that are not `mine` take part only.
-template <typename T, int W, bool FINAL>
+// A rank's parts of v, by W neighbouring lanes; rows that are not `mine` take part only.
+template <typename T, int W>
 __device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank, float f, float scale, bool mine) {
-  if constexpr (FINAL) {
-    const Parts h = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
-    if (!mine) return;
-    uint16_t* const to = p.v + m * 2 * p.ranks + 2 * (rank / W) * W + rank % W;
-    to[0] = h.high, to[W] = h.low;
-    if (std::is_same<T, f16>::value && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = h.power;
-  } else if (mine) {
-    p.partial[((int64_t)blockIdx.z * p.M + m) * p.ranks + rank] = f;
-  }
+  const Parts h = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
+  if (!mine) return;
+  uint16_t* const to = p.v + m * 2 * p.ranks + 2 * (rank / W) * W + rank % W;
+  to[0] = h.high, to[W] = h.low;
+  if (std::is_same<T, f16>::value && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = h.power;
 }
 
-template <typename T, int RT, int W, bool FINAL>
+// Few rows: a block has an adapter of the tile and a share of K; those that share the adapter cut the share further, into
+// sub-shares (lora_shares).
+__device__ __forceinline__ int lora_shares(const LoraArgs& p, int parts) { return min(parts, p.shares / p.splits); }
+template <typename T, int RT, int W>
+__global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {
+  __shared__ __attribute__((aligned(16))) RankLds<RT, 4> lds;
+  const int i = threadIdx.x & 15, tile0 = blockIdx.y * RT;
+  const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16;
+  const Group g = group_of(m0 + i < p.M ? lora_id(p, m0 + i) : -2, blockIdx.x / p.tiles, p.slots);
+  const int shares = lora_shares(p, g.parts), share = blockIdx.z * shares + g.part;
+  if (g.adapter < 0 || g.part >= shares) return;
+  const int units = (p.K + kUnit - 1) / kUnit, per = (units + p.splits * shares - 1) / (p.splits * shares);
+  tile_ranks<T, RT, 4>(p, lds, m0, g.rows, g.adapter, tile0, share * per, min((share + 1) * per, units));
+  for_ranks<RT, 4, W>(lds, [&](int row, int rank, float f) {
+    rank += 16 * tile0;
+    if (rank < p.ranks && (g.rows >> row & 1)) p.partial[((int64_t)share * p.M + m0 + row) * p.ranks + rank] = f;
+  });
+}
+
+// Many rows: a block has every slots-th adapter of the tile and all of K.
+template <typename T, int RT, int W>
 __global__ void __launch_bounds__(256) lora_ranks_kernel(LoraArgs p) {
   __shared__ __attribute__((aligned(16))) RankLds<RT, 4> lds;
-  const int lane = threadIdx.x & 63, tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
-  const int64_t m0 = (int64_t)tile * 16;
-  const int id = m0 + (lane & 15) < p.M ? lora_id(p, m0 + (lane & 15)) : -1;
-  const int begin = blockIdx.z * p.per, units = min(begin + p.per, (p.K + kUnit - 1) / kUnit);
+  const int i = threadIdx.x & 15, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
+  const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16;
+  const int id = m0 + i < p.M ? lora_id(p, m0 + i) : -1;
   uint32_t left = (uint32_t)(__ballot(id >= 0) & 0xFFFF);
   for (int n = 0; left; ++n) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
     const uint32_t rows = (uint32_t)(__ballot(id == cur) & 0xFFFF);
     left &= ~rows;
     if (n % p.slots != slot) continue;
-    tile_ranks<T, RT, 4>(p, lds, m0, rows, cur, tile0, begin, units);
+    tile_ranks<T, RT, 4>(p, lds, m0, rows, cur, tile0, 0, (p.K + kUnit - 1) / kUnit);
     for_ranks<RT, 4, W>(lds, [&](int row, int rank, float f) {
       rank += 16 * tile0;
-      if (rank < p.ranks) put_rank<T, W, FINAL>(p, m0 + row, rank, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
+      if (rank < p.ranks) put_rank<T, W>(p, m0 + row, rank, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
     });
     __syncthreads();
   }
 }
 
-// Rows of fewer than eight values: a thread has a row and a rank.
+// Rows of fewer than eight values, one share: a thread has a row and a rank.
 template <typename T, int W, bool FINAL>
 __global__ void __launch_bounds__(256) lora_ranks_short_kernel(LoraArgs p) {
   const int64_t m = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
@@ -207,7 +245,8 @@ __global__ void __launch_bounds__(256) lora_ranks_short_kernel(LoraArgs p) {
   if (id >= 0 && rank < p.R)
     for (int k = 0; k < p.K; ++k)
       f = fmaf(from_bits<T>(p.x[m * p.ldx + k]), from_bits<T>(p.a[id * p.a_stride + (int64_t)rank * p.K + k]), f);
-  put_rank<T, W, FINAL>(p, m, rank, f, p.scales ? p.scales[max(id, 0)] : 1.f, id >= 0);
+  if constexpr (FINAL) put_rank<T, W>(p, m, rank, f, p.scales ? p.scales[max(id, 0)] : 1.f, id >= 0);
+  else if (id >= 0) p.partial[m * p.ranks + rank] = f;
 }
 
 // ------------------------------------------------------------------ columns
@@ -272,120 +311,117 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
   __shared__ float power[16][16];
   uint16_t* const v = (uint16_t*)dynamic_lds;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / W, ld = 2 * p.ranks + 8;
-  const int tile = blockIdx.x % p.tiles, slot = blockIdx.x / p.tiles;
-  const int64_t m0 = (int64_t)tile * 16, m = m0 + i;
+  const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16, m = m0 + i;
   const int id = m < p.M ? lora_id(p, m) : -2;
-  const int begin = blockIdx.y * p.cols + wave * 32, end = min((int)(blockIdx.y + 1) * p.cols, p.whole);
+  const Group g = group_of(id, blockIdx.x / p.tiles, p.slots);
+  if (g.adapter < 0 && p.out == p.base && p.ldo == p.ldb) return;  // in place already
+  const int cur = g.adapter, part = blockIdx.y * g.parts + g.part, parts = gridDim.y * g.parts;
+  const int steps = (p.whole + STEP - 1) / STEP, cols = (steps + parts - 1) / parts * STEP;
+  const int begin = min(part * cols, p.whole) + wave * 32, end = min((part + 1) * cols, p.whole);
+  if (part * cols >= p.whole && part + 1 < parts) return;  // nothing left
+  const uint32_t rows = g.rows;
+  const bool mine = id == cur;
+  const uint16_t* const b = p.b + max(cur, 0) * p.b_stride;
   // of the last tile's eight ranks of this lane those that exist, as a mask of their bits
   const int there = p.R - (p.ranks - W) - first_rank<W>(q);
   u32x4 mask;
 #pragma unroll
   for (int j = 0; j < 4; ++j) mask[j] = (2 * j < there ? 0xFFFFu : 0u) | (2 * j + 1 < there ? 0xFFFF0000u : 0u);
-  uint32_t left = (uint32_t)(__ballot(id >= -1) & 0xFFFF);
-  for (int n = 0; left; ++n) {
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
-    const uint32_t rows = (uint32_t)(__ballot(id == cur) & 0xFFFF);
-    left &= ~rows;
-    if (n % p.slots != slot) continue;
-    if (cur < 0 && p.out == p.base && p.ldo == p.ldb) continue;  // in place already
-    const uint16_t* const b = p.b + max(cur, 0) * p.b_stride;
-    const bool mine = id == cur;
-    u32x4 bv[2][RT], from;
-    auto load_b = [&](int c0, int r0) {
+  u32x4 bv[2][RT], from;
+  auto load_b = [&](int c0, int r0) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      if (r0 + r >= tiles) continue;
+      const int at = W * (r0 + r) + first_rank<W>(q);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        bv[c][r] = *(const u32x4_any*)(b + (int64_t)min(c0 + 8 * (i >> 2) + 4 * c + (i & 3), p.whole - 1) * p.R + (at < p.R ? at : 0));
+    }
+  };
+  auto load_base = [&](int c0) {
+    from = u32x4{0, 0, 0, 0};
+    if (p.base && mine && c0 + 8 * q < end) from = *(const u32x4_any*)(p.base + m * p.ldb + c0 + 8 * q);
+  };
+  if (begin < end) {
+    load_base(begin);
+    if (cur >= 0) load_b(begin, 0);
+  }
+  if (cur >= 0) {
+    const float scale = p.scales ? p.scales[cur] : 1.f;
+    const int shares = p.splits * lora_shares(p, g.parts);
+    if constexpr (OWN > 0) {
+      tile_ranks<T, OWN, WAVES>(p, own, m0, rows, cur, 0, 0, (p.K + kUnit - 1) / kUnit);
+      for_ranks<OWN, WAVES, W>(own, [&](int row, int rank, float f) {
+        if (rank >= p.ranks) return;
+        const Parts two = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
+        uint16_t* const to = v + row * ld + 2 * (rank / W) * W + rank % W;
+        to[0] = two.high, to[W] = two.low;
+        if (rank % W == 0) power[row][rank / W] = two.power;
+      });
+    }
+    // a wave has a row's tile, lane (q, i) the shares q, q + 4, ... of ranks i and 16 + i
+    for (int j = wave; j < 16 * tiles && !OWN; j += 4) {
+      const int row = j & 15, r = j >> 4;
+      if (!(rows >> row & 1)) continue;
+      const float* const at = p.partial + (m0 + row) * p.ranks + W * r + i;
+      float part[SUB][4], f[SUB];
+#pragma unroll
+      for (int h = 0; h < SUB; ++h)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) part[h][s] = q + 4 * s < shares ? at[(q + 4 * s) * p.M * p.ranks + 16 * h] : 0.f;
+      int e = 0;
+      float top = 0.f;
+#pragma unroll
+      for (int h = 0; h < SUB; ++h) {
+        f[h] = (part[h][0] + part[h][1]) + (part[h][2] + part[h][3]);
+        f[h] += __shfl_xor(f[h], 16);
+        f[h] += __shfl_xor(f[h], 32);
+        f[h] = W * r + 16 * h + i < p.R ? f[h] * scale : 0.f;
+        top = fmaxf(top, fabsf(f[h]));
+      }
+      if constexpr (std::is_same<T, f16>::value) e = tile_exponent(row_max16(top));
+#pragma unroll
+      for (int h = 0; h < SUB; ++h) {
+        const Parts two = parts_of<T>(f[h], e);
+        if (q < 2) v[row * ld + 2 * W * r + W * q + 16 * h + i] = q ? two.low : two.high;
+        if (lane == 0) power[row][r] = two.power;
+      }
+    }
+    __syncthreads();
+  }
+  for (int c0 = begin; c0 < end; c0 += STEP) {
+    f32x4 sum[2] = {};
+    for (int r0 = 0; r0 < tiles && cur >= 0; r0 += RT) {
+      if (r0) load_b(c0, r0);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if (r0 + r >= tiles) continue;
-        const int at = W * (r0 + r) + first_rank<W>(q);
+        u32x4 low[SUB];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          bv[c][r] = *(const u32x4_any*)(b + (int64_t)min(c0 + 8 * (i >> 2) + 4 * c + (i & 3), p.whole - 1) * p.R + (at < p.R ? at : 0));
-      }
-    };
-    auto load_base = [&](int c0) {
-      from = u32x4{0, 0, 0, 0};
-      if (p.base && mine && c0 + 8 * q < end) from = *(const u32x4_any*)(p.base + m * p.ldb + c0 + 8 * q);
-    };
-    if (begin < end) {
-      load_base(begin);
-      if (cur >= 0) load_b(begin, 0);
-    }
-    if (cur >= 0) {
-      const float scale = p.scales ? p.scales[cur] : 1.f;
-      __syncthreads();  // v of the adapter before is read
-      if constexpr (OWN > 0) {
-        tile_ranks<T, OWN, WAVES>(p, own, m0, rows, cur, 0, 0, (p.K + kUnit - 1) / kUnit);
-        for_ranks<OWN, WAVES, W>(own, [&](int row, int rank, float f) {
-          if (rank >= p.ranks) return;
-          const Parts two = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
-          uint16_t* const to = v + row * ld + 2 * (rank / W) * W + rank % W;
-          to[0] = two.high, to[W] = two.low;
-          if (rank % W == 0) power[row][rank / W] = two.power;
-        });
-      }
-      // a wave has a row's tile, lane (q, i) the shares q, q + 4, ... of ranks i and 16 + i
-      for (int j = wave; j < 16 * tiles && !OWN; j += 4) {
-        const int row = j & 15, r = j >> 4;
-        if (!(rows >> row & 1)) continue;
-        const float* const at = p.partial + (m0 + row) * p.ranks + W * r + i;
-        float part[SUB][4], f[SUB];
+        for (int h = 0; h < SUB; ++h) low[h] = *(const u32x4*)(v + i * ld + 2 * W * (r0 + r) + W * h + 8 * q);
 #pragma unroll
-        for (int h = 0; h < SUB; ++h)
+        for (int c = 0; c < 2; ++c) {
+          if (r0 + r == tiles - 1) bv[c][r] &= mask;
+          if constexpr (std::is_same<T, f16>::value) {
+            const f32x4 one = both_parts<T, W>(bv[c][r], low, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int s = 0; s < 4; ++s) part[h][s] = q + 4 * s < p.splits ? at[(q + 4 * s) * p.M * p.ranks + 16 * h] : 0.f;
-        int e = 0;
-        float top = 0.f;
-#pragma unroll
-        for (int h = 0; h < SUB; ++h) {
-          f[h] = (part[h][0] + part[h][1]) + (part[h][2] + part[h][3]);
-          f[h] += __shfl_xor(f[h], 16);
-          f[h] += __shfl_xor(f[h], 32);
-          f[h] = W * r + 16 * h + i < p.R ? f[h] * scale : 0.f;
-          top = fmaxf(top, fabsf(f[h]));
-        }
-        if constexpr (std::is_same<T, f16>::value) e = tile_exponent(row_max16(top));
-#pragma unroll
-        for (int h = 0; h < SUB; ++h) {
-          const Parts two = parts_of<T>(f[h], e);
-          if (q < 2) v[row * ld + 2 * W * r + W * q + 16 * h + i] = q ? two.low : two.high;
-          if (lane == 0) power[row][r] = two.power;
-        }
-      }
-      __syncthreads();
-    }
-    for (int c0 = begin; c0 < end; c0 += STEP) {
-      f32x4 sum[2] = {};
-      for (int r0 = 0; r0 < tiles && cur >= 0; r0 += RT) {
-        if (r0) load_b(c0, r0);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          if (r0 + r >= tiles) continue;
-          u32x4 low[SUB];
-#pragma unroll
-          for (int h = 0; h < SUB; ++h) low[h] = *(const u32x4*)(v + i * ld + 2 * W * (r0 + r) + W * h + 8 * q);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (r0 + r == tiles - 1) bv[c][r] &= mask;
-            if constexpr (std::is_same<T, f16>::value) {
-              const f32x4 one = both_parts<T, W>(bv[c][r], low, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sum[c][j] = fmaf(one[j], power[i][r0 + r], sum[c][j]);
-            } else {
-              sum[c] = both_parts<T, W>(bv[c][r], low, sum[c]);
-            }
+            for (int j = 0; j < 4; ++j) sum[c][j] = fmaf(one[j], power[i][r0 + r], sum[c][j]);
+          } else {
+            sum[c] = both_parts<T, W>(bv[c][r], low, sum[c]);
           }
         }
       }
-      const u32x4 now = from;
-      if (c0 + STEP < end) {
-        load_base(c0 + STEP);
-        if (cur >= 0) load_b(c0 + STEP, 0);
-      }
-      if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
     }
-    if (blockIdx.y + 1 == gridDim.y)
-      odd_columns<T, W>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; },
-                        [&](int row, int r) { return power[row][r]; });
+    const u32x4 now = from;
+    if (c0 + STEP < end) {
+      load_base(c0 + STEP);
+      if (cur >= 0) load_b(c0 + STEP, 0);
+    }
+    if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
   }
+  if (part + 1 == parts)
+    odd_columns<T, W>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; },
+                      [&](int row, int r) { return power[row][r]; });
 }
 
 // Many rows: 64 by p.cols columns, 64 of them at a time: their B goes through LDS once for the four waves, which have 16 rows
@@ -558,31 +594,28 @@ static int64_t lora_whole(int64_t N, int64_t R) {
 
 struct LoraPlan {
   bool many, own;  // own: the few rows' v by the blocks themselves
-  int slots, splits, per;
+  int slots, splits, shares;
 };
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
-  const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit);
-  l.many = M > 512;
-  // a batch of single tokens has many adapters in a tile, prompts one or two
-  l.slots = M <= 128 ? (int)std::min<int64_t>(16, M) : l.many ? 2 : 1;
-  l.splits = 1, l.per = (int)units;
+  const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit), ranks = lora_ranks(R);
+  l.many = M > 128;
+  // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little.
+  l.slots = (int)(l.many ? std::max<int64_t>(2, std::min<int64_t>(16, 65536 / M)) : std::min<int64_t>(16, M));
   // One launch where few rows' adapters are small enough to be read by all of a row's blocks.  us with one and with two, which
   // cost the host 4 more (one row: A of 128 KB 6.3, 6.2, of 256 7.9, 6.7, of 384 11.2, 6.5; 64 rows of as many adapters: 128 KB
   // 9.9, 12.9, 256 13.5, 16.1, 512 19.8, 25.0; 128 rows: 128 KB 12.7, 16.8, 256 KB and two adapters 21.4, 18.1).
-  l.own = lora_ranks(R) <= 64 && K >= 8 && lora_ranks(R) * K * 2 <= (M <= 32 ? 256 << 10 : M <= 64 ? 512 << 10 : M <= 128 ? 128 << 10 : 0);
-  if (!l.many) {
-    const int64_t want = std::max<int64_t>(1, 256 / (tiles * l.slots * cdiv(lora_ranks(R), 64)));
-    l.per = (int)std::max<int64_t>(4, cdiv(units, std::min<int64_t>(want, 16)));
-    l.splits = (int)cdiv(units, l.per);
-  }
+  l.own = !l.many && ranks <= 64 && K >= 8 && ranks * K * 2 <= (M <= 32 ? 256 << 10 : M <= 64 ? 512 << 10 : 128 << 10);
+  // at least four units a share, at most 16 shares
+  l.splits = (int)std::max<int64_t>(1, std::min(cdiv(units, 4), std::min<int64_t>(16, 256 / (tiles * l.slots * cdiv(ranks, 64)))));
+  l.shares = K < 8 ? 1 : std::min(16, l.splits * l.slots);
   return l;
 }
 size_t lora_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   const LoraPlan l = lora_plan(M, K, R);
   const size_t values = (size_t)M * (size_t)lora_ranks(R);
   if (l.own) return 0;
-  return l.many ? values * 4 + values / (size_t)lora_tile(R) * 4 : (size_t)l.splits * values * 4;
+  return l.many ? values * 4 + values / (size_t)lora_tile(R) * 4 : (size_t)l.shares * values * 4;
 }
 
 template <typename T>
@@ -602,9 +635,10 @@ static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
       else lora_ranks_short_kernel<T, W, false><<<grid, 256, 0, st>>>(p);
       return;
     }
-    const dim3 grid((unsigned)(p.tiles * p.slots), (unsigned)cdiv(p.ranks, 16 * N), (unsigned)l.splits);
-    if (l.many) lora_ranks_kernel<T, N, W, true><<<grid, 256, 0, st>>>(p);
-    else lora_ranks_kernel<T, N, W, false><<<grid, 256, 0, st>>>(p);
+    const unsigned x = (unsigned)(p.tiles * p.slots), y = (unsigned)cdiv(p.ranks, 16 * N);
+    if (!l.many) lora_ranks_few_kernel<T, N, W><<<dim3(x, y, (unsigned)l.splits), 256, 0, st>>>(p);
+    else if (N == 4 && p.tiles < 64) lora_ranks_kernel<T, 2, W><<<dim3(x, (unsigned)cdiv(p.ranks, 32)), 256, 0, st>>>(p);
+    else lora_ranks_kernel<T, N, W><<<dim3(x, y), 256, 0, st>>>(p);
   });
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
   const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 32 * few_waves(l.own);
@@ -634,7 +668,7 @@ int launch_lora(const LoraCall& c, hipStream_t st) {
   p.M = c.M, p.N = (int)c.N, p.K = (int)c.K, p.R = (int)c.R, p.L = c.L, p.id64 = c.id64;
   p.ranks = (int)lora_ranks(c.R), p.whole = (int)lora_whole(c.N, c.R);
   const LoraPlan l = lora_plan(c.M, c.K, c.R);
-  p.tiles = (int)cdiv(c.M, 16), p.slots = l.slots, p.splits = l.splits, p.per = l.per;
+  p.tiles = (int)cdiv(c.M, 16), p.slots = l.slots, p.splits = l.splits, p.shares = l.shares;
   p.partial = (float*)c.workspace;
   p.v = (uint16_t*)c.workspace, p.powers = (float*)(p.v + (size_t)c.M * 2 * p.ranks);
   return c.dtype == AWQ_DTYPE_F16 ? lora_typed<f16>(p, l, st) : lora_typed<bf16>(p, l, st);

@@ -52,7 +52,10 @@ CASES = [  # rows, requests, K, N, rank, adapters, without
     (7, 7, 72, 520, 16, 9, 0.3), (16, 16, 1024, 255, 32, 16, 0.0), (17, 3, 257, 300, 12, 5, 0.4), (29, 29, 2001, 501, 12, 16, 0.2),
     (64, 64, 512, 640, 32, 64, 0.1), (128, 20, 200, 96, 100, 7, 0.2), (129, 129, 130, 70, 24, 40, 0.2), (300, 5, 640, 333, 8, 20, 0.2),
     (513, 4, 96, 1100, 16, 3, 0.3), (600, 9, 128, 256, 256, 4, 0.2), (700, 700, 64, 48, 20, 30, 0.3), (1500, 6, 328, 700, 64, 4, 0.2),
-    (2049, 3, 1000, 80, 130, 2, 0.4), (40, 40, 12288, 64, 16, 3, 0.0), (5, 5, 64, 24580, 16, 6, 0.2)]
+    (2049, 3, 1000, 80, 130, 2, 0.4), (40, 40, 12288, 64, 16, 3, 0.0), (5, 5, 64, 24580, 16, 6, 0.2),
+    (100, 2, 4096, 520, 64, 4, 0.3), (96, 1, 12288, 300, 16, 1, 0.0), (33, 2, 9000, 1030, 40, 2, 0.0), (128, 128, 5000, 40, 24, 5, 0.2),
+    (16, 1, 12288, 4100, 128, 1, 0.0), (100, 3, 7, 90, 5, 2, 0.2), (20, 2, 6, 300, 200, 2, 0.2), (200, 200, 300, 200, 64, 30, 0.1),
+    (1100, 1100, 64, 72, 64, 50, 0.1), (64, 1, 600, 24600, 16, 1, 0.0)]
 
 
 @pytest.mark.gpu
