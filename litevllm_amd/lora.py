@@ -72,9 +72,14 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
         out = torch.empty(shape, dtype=dtype, device=dev) if base is None or not base.is_contiguous() else torch.empty_like(base)
         to, ldo = out, n
     else:
-        to = out if out.dim() == 2 else out.view(-1, n)  # raises where its rows are no matrix
+        to = out
+        if out.dim() != 2:
+            try:
+                to = out.view(-1, n) if n else out
+            except RuntimeError:
+                raise ValueError(f"bad_output: out's rows must be those of a matrix, got strides {out.stride()}") from None
         ldo = to.stride(0) if m > 1 else n
-        if (n > 1 and to.stride(1) != 1) or ldo < n:
+        if m and n and ((n > 1 and to.stride(-1) != 1) or ldo < n):
             raise ValueError(f"bad_output: out must have dense rows apart from each other, got strides {out.stride()}")
     if m == 0 or n == 0:
         return out
@@ -107,6 +112,8 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
     _call(dev, "awq_w4a16_lora_add", at, ldb, x.data_ptr(), ldx, lora_a.data_ptr(), a_stride, lora_b.data_ptr(), b_stride,
           ids.data_ptr(), 64 if wide else 32, None if scales is None else scales.data_ptr(), to.data_ptr(), ldo, m, n, k, rank,
           adapters, code, None if ws is None else ws.data_ptr(), ws_bytes)
+    if given:
+        torch.autograd.graph.increment_version(out)  # a backward that has saved it would take other values
     return _Refused.apply("lora_add is not differentiable", out, base, x, lora_a, lora_b, scales) if asked else out
 
 
@@ -138,4 +145,7 @@ class LoRAAdapters(nn.Module):
 
     def add(self, base: torch.Tensor | None, x: torch.Tensor, ids: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """:func:`lora_add` with these adapters."""
-        return lora_add(base, x, self.lora_a, self.lora_b, ids, self.scales, out)
+        scales = self.scales
+        if scales is not None and scales.dtype is not torch.float32:
+            scales = scales.float()  # the module was cast as a whole
+        return lora_add(base, x, self.lora_a, self.lora_b, ids, scales, out)

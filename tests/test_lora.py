@@ -278,9 +278,10 @@ def test_layers_with_adapters(kind):
         assert got.shape == plain.shape
         assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -11 + terms * ((k + 24) * 2.0 ** -23 + 2.0 ** -22) + 2.0 ** -25).all())
         assert torch.equal(got[(ids < 0) | (ids >= adapters)], plain[(ids < 0) | (ids >= adapters)])
-    del layer.lora_adapters
-    with pytest.raises(RuntimeError, match="no lora_adapters"):
-        cfg.apply(layer, x, lora_ids=ids)
+    layer.lora_adapters = layer.lora_adapters.half()  # scales as well: these are the same numbers in fp16
+    assert torch.equal(cfg.apply(layer, x, lora_ids=ids), got)
+    layer.lora_adapters = None
+    assert torch.equal(cfg.apply(layer, x, lora_ids=ids), plain)
 
 
 @pytest.mark.gpu
@@ -303,6 +304,21 @@ def test_derivatives_are_refused():
 
 
 @pytest.mark.gpu
+def test_a_backward_notices_what_out_overwrote():
+    from litevllm_amd import lora_add
+    g = torch.Generator().manual_seed(10)
+    x, y, a, b = _whole(g, 6, 32).half(), _whole(g, 6, 40).half(), _whole(g, 2, 4, 32).half(), _whole(g, 2, 40, 4).half()
+    w = torch.ones(6, 40, dtype=torch.float16, device="cuda", requires_grad=True)
+    loss = (w * y).sum()
+    lora_add(y, x, a, b, torch.zeros(6, dtype=torch.int32, device="cuda"), out=y)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        z = y.clone()
+        assert lora_add(z, x, a, b, torch.zeros(6, dtype=torch.int32, device="cuda"), out=z) is z
+
+
+@pytest.mark.gpu
 def test_refusals():
     from litevllm_amd import LoRAAdapters, lora_add
     g = torch.Generator().manual_seed(9)
@@ -318,6 +334,7 @@ def test_refusals():
                 lambda: lora_add(base, x.cpu(), a, b, ids), lambda: lora_add(base, x, a, b, ids.cpu()),
                 lambda: lora_add(base, x, a, b, ids, out=base[:5]), lambda: lora_add(base, x, a, b, ids, out=torch.empty(40, 6, dtype=torch.float16, device="cuda").t()),
                 lambda: lora_add(base, x, a, b, ids, out=torch.empty(1, 40, dtype=torch.float16, device="cuda").expand(6, 40)),
+                lambda: lora_add(base.view(2, 3, 40), x.view(2, 3, 32), a, b, ids.view(2, 3), out=torch.empty(3, 2, 40, dtype=torch.float16, device="cuda").transpose(0, 1)),
                 lambda: LoRAAdapters.stack([]), lambda: LoRAAdapters.stack([(a[0], b[0], 1.0), (a[0, :, :8], b[0], 1.0)])):
         with pytest.raises(ValueError):
             bad()
