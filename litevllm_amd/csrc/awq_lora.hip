@@ -213,10 +213,14 @@ __global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {
   });
 }
 
-// Many rows: a block has every slots-th adapter of the tile and all of K.
+// Many rows: a block has every slots-th adapter of the tile and all of K.  Of four tiles of ranks it is bound by the lines that
+// a CU's four waves load (0.7 MB of x and A for 16 rows, K = 4096) and pass through LDS, more waves made it slower (4096 rows,
+// rank 64, N = 4096: 45 us, with eight 49; rank 16, 2000 rows, N = 8192 28 and 24).
+constexpr int many_waves(int rt) { return rt == 4 ? 4 : 8; }
 template <typename T, int RT, int W>
-__global__ void __launch_bounds__(256) lora_ranks_kernel(LoraArgs p) {
-  __shared__ __attribute__((aligned(16))) RankLds<RT, 4> lds;
+__global__ void __launch_bounds__(64 * many_waves(RT)) lora_ranks_kernel(LoraArgs p) {
+  constexpr int WAVES = many_waves(RT);
+  __shared__ __attribute__((aligned(16))) RankLds<RT, WAVES> lds;
   const int i = threadIdx.x & 15, slot = blockIdx.x / p.tiles, tile0 = blockIdx.y * RT;
   const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16;
   const int id = m0 + i < p.M ? lora_id(p, m0 + i) : -1;
@@ -226,8 +230,8 @@ __global__ void __launch_bounds__(256) lora_ranks_kernel(LoraArgs p) {
     const uint32_t rows = (uint32_t)(__ballot(id == cur) & 0xFFFF);
     left &= ~rows;
     if (n % p.slots != slot) continue;
-    tile_ranks<T, RT, 4>(p, lds, m0, rows, cur, tile0, 0, (p.K + kUnit - 1) / kUnit);
-    for_ranks<RT, 4, W>(lds, [&](int row, int rank, float f) {
+    tile_ranks<T, RT, WAVES>(p, lds, m0, rows, cur, tile0, 0, (p.K + kUnit - 1) / kUnit);
+    for_ranks<RT, WAVES, W>(lds, [&](int row, int rank, float f) {
       rank += 16 * tile0;
       if (rank < p.ranks) put_rank<T, W>(p, m0 + row, rank, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
     });
@@ -600,8 +604,9 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
   const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit), ranks = lora_ranks(R);
   l.many = M > 128;
-  // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little.
-  l.slots = (int)(l.many ? std::max<int64_t>(2, std::min<int64_t>(16, 65536 / M)) : std::min<int64_t>(16, M));
+  // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little but wait
+  // for LDS (8192 rows of 6 requests 48 us with 4, 54 with 16; 500 rows of as many requests 43 and 35).
+  l.slots = (int)(l.many ? (M <= 512 ? 16 : 4) : std::min<int64_t>(16, M));
   // One launch where few rows' adapters are small enough to be read by all of a row's blocks.  us with one and with two, which
   // cost the host 4 more (one row: A of 128 KB 6.3, 6.2, of 256 7.9, 6.7, of 384 11.2, 6.5; 64 rows of as many adapters: 128 KB
   // 9.9, 12.9, 256 13.5, 16.1, 512 19.8, 25.0; 128 rows: 128 KB 12.7, 16.8, 256 KB and two adapters 21.4, 18.1).
@@ -637,13 +642,16 @@ static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
     }
     const unsigned x = (unsigned)(p.tiles * p.slots), y = (unsigned)cdiv(p.ranks, 16 * N);
     if (!l.many) lora_ranks_few_kernel<T, N, W><<<dim3(x, y, (unsigned)l.splits), 256, 0, st>>>(p);
-    else if (N == 4 && p.tiles < 64) lora_ranks_kernel<T, 2, W><<<dim3(x, (unsigned)cdiv(p.ranks, 32)), 256, 0, st>>>(p);
-    else lora_ranks_kernel<T, N, W><<<dim3(x, y), 256, 0, st>>>(p);
+    else if (N == 4 && p.tiles < 64) lora_ranks_kernel<T, 2, W><<<dim3(x, (unsigned)cdiv(p.ranks, 32)), 64 * many_waves(2), 0, st>>>(p);
+    else lora_ranks_kernel<T, N, W><<<dim3(x, y), 64 * many_waves(N), 0, st>>>(p);
   });
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
   const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 32 * few_waves(l.own);
   const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, (l.own ? 256 : 2048) / x);
   p.cols = (int)(cdiv(steps, std::min(want, steps)) * step);
+  // many rows: not so many columns that the last blocks' work shows (4096 rows, N = 24576: rank 16 99 us with 768 columns a
+  // block, 92 with 256, rank 64 127 and, with 512, 123)
+  if (l.many) p.cols = std::min(p.cols, p.ranks <= 32 ? 256 : 512);
   p.ranges = (int)std::max<int64_t>(1, cdiv(p.whole, p.cols));
   // results past the caches where they are many (and not in lines that base has brought there): N = 24576, rank 64, 4096 rows
   // 112 us, 150 through them; 8192 columns of 2000 rows gain 3 us of 24, but the next reader may want those
