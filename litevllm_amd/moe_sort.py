@@ -32,11 +32,8 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x, x.stride(0) if n > 1 else h
 
 
-def _back(name: str, on: int, *saved: tuple) -> None:
-    """Saved-tensor hooks may give back other tensors: each has to be on the device and of the type and shape that it had."""
-    for t, dtype, shape in saved:
-        if t is not None and (t.get_device() != on or t.dtype is not dtype or t.shape != shape):
-            raise RuntimeError(f"{name}: saved tensors came back elsewhere, or with other shapes or types")
+def _elsewhere(name: str):
+    return RuntimeError(f"{name}: saved tensors came back elsewhere, or with other shapes or types")
 
 
 def _index(x, ids, experts):
@@ -67,21 +64,28 @@ def _unsorted(rows, weights, places):
     return out
 
 
+# The backward passes run on a thread of the engine's, where each object that they touch comes from another core: they keep to
+# few.  Saved-tensor hooks may give back other tensors, so each is checked again.
 class _Sort(torch.autograd.Function):
     """The rows; the index, which is no function of x, is written on the way and comes from outside."""
 
     @staticmethod
     def forward(ctx, x, ids, experts, index):
-        places = index[2]
-        ctx.save_for_backward(places)
-        ctx.shape = ids.shape
+        ctx.save_for_backward(index[2])
+        ctx.of = x.shape, ids.shape, ops.dtype_code(x.dtype)
         return _sorted(x, ids, experts, index)
 
     @staticmethod
     def backward(ctx, upstream):
         places, = ctx.saved_tensors
-        _back("moe_sort", upstream.get_device(), (places, torch.int32, ctx.shape))
-        grad = _unsorted(upstream.contiguous(), None, places.contiguous())
+        shape, routes, code = ctx.of
+        if places.shape != routes or places.dtype is not torch.int32 or places.get_device() != upstream.get_device():
+            raise _elsewhere("moe_sort")
+        upstream, places = upstream.contiguous(), places.contiguous()
+        grad = upstream.new_empty(shape)
+        h = shape[1]
+        _call(upstream.device, "awq_w4a16_moe_unsort", upstream.data_ptr(), places.data_ptr(), None, L.DTYPE_NONE, grad.data_ptr(), h,
+              shape[0], h, routes[1], code)
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not taken as zero
             grad = _Refused.apply("moe_sort is not differentiable twice", grad, upstream)
         return grad, None, None, None
@@ -91,24 +95,28 @@ class _Unsort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, places, offsets):
         ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, places, offsets)
-        ctx.of = (rows.dtype, rows.shape), None if weights is None else weights.dtype, places.shape, offsets.shape
+        ctx.of = (rows.shape, rows.dtype, places.shape, None if weights is None else weights.dtype, offsets.shape,
+                  ops.dtype_code(rows.dtype), L.DTYPE_NONE if weights is None else ops.dtype_code(weights.dtype))
         return _unsorted(rows, weights, places)
 
     @staticmethod
     def backward(ctx, upstream):
         rows, weights, places, offsets = ctx.saved_tensors
-        (dtype, shape), wdtype, routes, experts = ctx.of
-        _back("moe_unsort", upstream.get_device(), (rows, dtype, shape), (weights, wdtype, routes), (places, torch.int32, routes),
-              (offsets, torch.int32, experts))
-        (t, k), h, dev = routes, shape[1], upstream.device
-        flat, ld = _rows(upstream)
-        want_rows, want_weights = ctx.needs_input_grad[:2]
-        grad_rows = torch.empty(shape, dtype=dtype, device=dev) if want_rows else None
-        grad_weights = torch.empty(routes, dtype=wdtype, device=dev) if want_weights else None
-        dense = [None if a is None else a.contiguous() for a in (rows, weights, places, offsets)]
-        _call(dev, "awq_w4a16_moe_unsort_grad", flat.data_ptr(), ld, ops._ptr(dense[0]), dense[2].data_ptr(),
-              dense[3].data_ptr() + 4 * (experts[0] - 1), ops._ptr(dense[1]), L.DTYPE_NONE if wdtype is None else ops.dtype_code(wdtype),
-              ops._ptr(grad_rows), ops._ptr(grad_weights), t, h, k, ops.dtype_code(dtype))
+        shape, dtype, routes, wdtype, experts, code, wcode = ctx.of
+        on = upstream.get_device()
+        if places.shape != routes or places.dtype is not torch.int32 or places.get_device() != on or (
+                offsets.shape != experts or offsets.dtype is not torch.int32 or offsets.get_device() != on) or (
+                rows is not None and (rows.shape != shape or rows.dtype is not dtype or rows.get_device() != on)) or (
+                weights is not None and (weights.shape != routes or weights.dtype is not wdtype or weights.get_device() != on)):
+            raise _elsewhere("moe_unsort")
+        want_rows, want_weights, _, _ = ctx.needs_input_grad
+        flat, ld = (upstream, shape[1]) if upstream.is_contiguous() else _rows(upstream)
+        grad_rows = upstream.new_empty(shape) if want_rows else None
+        grad_weights = upstream.new_empty(routes, dtype=wdtype) if want_weights else None
+        read, w, places, offsets = (None if t is None else t.contiguous() for t in (rows, weights, places, offsets))
+        _call(upstream.device, "awq_w4a16_moe_unsort_grad", flat.data_ptr(), ld, ops._ptr(read), places.data_ptr(),
+              offsets.data_ptr() + 4 * (experts[0] - 1), ops._ptr(w), wcode, ops._ptr(grad_rows), ops._ptr(grad_weights), routes[0],
+              shape[1], routes[1], code)
         if torch.is_grad_enabled():
             inputs = upstream, rows, weights
             grad_rows, grad_weights = (None if g is None else _Refused.apply("moe_unsort is not differentiable twice", g, *inputs)
