@@ -501,9 +501,11 @@ __global__ void __launch_bounds__(256, 3) lora_columns_kernel(LoraArgs p) {
         if constexpr (std::is_same<T, f16>::value) power[r] = p.powers[m * tiles + chunk * RT + r];
       }
     };
-    load_b(begin, 0);
-    load_low(0);
-    load_base(begin);
+    if (begin < end) {  // with few columns none goes by eight
+      load_b(begin, 0);
+      load_low(0);
+      load_base(begin);
+    }
     __syncthreads();  // the adapters before are done with the LDS
     int buf = 0;
     for (int c0 = begin; c0 < end; c0 += 64) {

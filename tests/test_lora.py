@@ -178,6 +178,18 @@ def test_in_place_slices_and_strides(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 100, 200, 1000])
+@pytest.mark.parametrize("n,r", [(1, 1), (1, 256), (7, 16), (8, 9), (8, 1), (15, 1), (16, 40)])
+def test_few_columns(m, n, r):
+    """Fewer columns than a piece has, or than B's last piece reaches over."""
+    g = torch.Generator().manual_seed(20 + m + n + r)
+    x, a, b, base = _whole(g, m, 40).half(), _whole(g, 3, r, 40, size=1).half(), _whole(g, 3, n, r, size=1).half(), _whole(g, m, n).half()
+    ids = _ids(g, m, 3, min(m, 5), 0.2)
+    _check_exact(base, x, a, b, ids, None)
+    _check_exact(None, x, a, b, ids, None)
+
+
+@pytest.mark.gpu
 def test_no_rows_no_columns():
     from litevllm_amd import lora_add
     z = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")
