@@ -90,7 +90,8 @@ struct Parts {
 template <typename T>
 __device__ __forceinline__ Parts parts_of(float f, int e) {
   if constexpr (std::is_same<T, f16>::value) f = ldexpf(f, -e);
-  const uint16_t high = to_bits<T>(f);
+  uint16_t high = to_bits<T>(f);
+  if (std::is_same<T, bf16>::value && fabsf(f) < __builtin_inff() && (high & 0x7FFF) == 0x7F80) --high;  // the rest fits into low
   return {high, fabsf(f) < __builtin_inff() ? to_bits<T>(f - from_bits<T>(high)) : (uint16_t)0,  // no Inf - Inf
           std::is_same<T, f16>::value ? ldexpf(1.f, e) : 1.f};
 }

@@ -118,6 +118,21 @@ def test_ranges_of_the_low_rank_values(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [4, 64])
+@pytest.mark.parametrize("m", [2, 100, 200])
+def test_low_rank_values_above_the_largest_bf16(m, k):
+    """1.9996 * 2^127 rounds to infinity in bf16 but not in fp32; B takes it down again."""
+    from litevllm_amd import lora_add
+    x, a, b = torch.zeros(m, k), torch.zeros(1, 2, k), torch.zeros(1, 24, 2)
+    x[:, 0], a[0, 0, 0], a[0, 1, 0], b[:, :, 0], b[:, ::2, 1] = 1.4140625 * 2.0 ** 63, 1.4140625 * 2.0 ** 64, -2.0 ** -60, 2.0 ** -100, 8.0
+    x, a, b = (t.bfloat16().cuda() for t in (x, a, b))
+    for sign in (1, -1):
+        got = lora_add(None, x * sign, a, b, torch.zeros(m, dtype=torch.int32, device="cuda"))
+        low = x.double() * sign @ a[0].double().t().contiguous()
+        assert torch.equal(got, (low @ b[0].double().t().contiguous()).bfloat16())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [30, 700])
 def test_infinities_and_nan_stay_in_their_rows(m):
     from litevllm_amd import lora_add
