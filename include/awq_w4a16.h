@@ -480,8 +480,8 @@ int awq_w4a16_moe_balance_grad(const void* logits, int64_t ld, int32_t logits_dt
  *   offsets[e] .. offsets[e + 1] - 1 are the places of expert e;  experts[p]: the expert of place p, -1 behind the last;
  *   places[t, j]: the place of a route, -1 for one that is left out;  rows[p] = x[t], 0 behind the last place.
  *   x: [T, H] of dtype (F16, BF16 or F32), row stride ldx;  topk_ids: [T, top_k] int32 or int64, dense;  rows: [R, H] dense;
- *   offsets: [E + 1];  experts: [R];  places: [T, top_k].  E and top_k <= 1024, R <= 2^30,
- *   H <= 2^24.  rows lie apart from x.
+ *   offsets: [E + 1];  experts: [R];  places: [T, top_k].  E and top_k <= 1024, T <= 2^23,
+ *   R <= 2^30, H <= 2^24, here and in the two below.  rows lie apart from x.
  *   workspace: 16-byte aligned, no zeroing needed; calls that may overlap must not share one. */
 size_t awq_w4a16_moe_sort_workspace_bytes(int64_t T, int32_t E, int32_t top_k);
 int awq_w4a16_moe_sort(const void* x, int64_t ldx, const void* topk_ids, int32_t ids_bits, void* rows, int32_t* offsets,
@@ -508,7 +508,7 @@ int awq_w4a16_moe_unsort_grad(const void* upstream, int64_t ldu, const void* row
  * Sums in fp32; x A^T enters the second product with 16 bits of mantissa (bf16) or 21 (fp16); one rounding.
  *   x: [M, K], base (NULL: zeros) and out: [M, N], all of dtype (F16 or BF16), row strides ldx, ldb, ldo;  lora_a: [L, R, K] and
  *   lora_b: [L, N, R], dense but for the stride between adapters;  ids: [M] int32 or int64;  scales: [L] or NULL (1).
- *   R <= 256; M <= 2^30, N and K <= 2^24.  Two bytes are alignment enough; 16 are faster.  out may be base (with its stride) and
+ *   R <= 256; M, N and K <= 2^24.  Two bytes are alignment enough; 16 are faster.  out may be base (with its stride) and
  *   lies apart from everything else.  Results are bitwise reproducible.
  *   workspace: 16-byte aligned, no zeroing needed; calls that may overlap must not share one. */
 size_t awq_w4a16_lora_workspace_bytes(int64_t M, int64_t K, int64_t R);

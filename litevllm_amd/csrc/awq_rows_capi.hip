@@ -10,12 +10,14 @@ bool dtype_16(int d) { return d == AWQ_DTYPE_F16 || d == AWQ_DTYPE_BF16; }
 bool dtype_float(int d) { return dtype_16(d) || d == AWQ_DTYPE_F32; }
 bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 constexpr int64_t kMaxRoutes = (int64_t)1 << 30;  // 32 bits number them, a block's behind the last too
+constexpr int64_t kMaxTokens = (int64_t)1 << 23;  // a launch's threads in 32 bits, with 256 a token,
+constexpr int64_t kMaxRows = (int64_t)1 << 24;    // or 128 a row
 constexpr int64_t kMaxWidth = (int64_t)1 << 24;   // a row's pieces, and blocks over them, in 32 and 16 bits
 constexpr int64_t kMaxRank = 256;
 
-bool routes_fit(int64_t T, int64_t H, int32_t top_k) { return T <= kMaxRoutes && T * top_k <= kMaxRoutes && H <= kMaxWidth; }
+bool routes_fit(int64_t T, int64_t H, int32_t top_k) { return T <= kMaxTokens && T * top_k <= kMaxRoutes && H <= kMaxWidth; }
 bool lora_fits(int64_t M, int64_t N, int64_t K, int64_t R) {
-  return M <= kMaxRoutes && N <= kMaxWidth && K <= kMaxWidth && R <= kMaxRank;
+  return M <= kMaxRows && N <= kMaxWidth && K <= kMaxWidth && R <= kMaxRank;
 }
 }  // namespace
 

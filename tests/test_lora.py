@@ -382,6 +382,7 @@ def test_entry_refuses():
     assert call(m=-1) == call(n=-1) == call(k=0) == call(r=0) == call(l=0) == L.ERR_SHAPE
     assert call(dt=L.DTYPE_F32) == call(bits=8) == call(r=257, sa=1 << 20, sb=1 << 20) == L.ERR_UNSUPPORTED
     assert call(m=(1 << 30) + 1) == call(n=(1 << 24) + 1, ldo=1 << 25, ldb=1 << 25, sb=1 << 40) == L.ERR_UNSUPPORTED
+    assert call(m=(1 << 24) + 1) == L.ERR_UNSUPPORTED and lib.awq_w4a16_lora_workspace_bytes((1 << 24) + 1, 8, 4) == 0
     assert call(ldx=7) == call(ldo=7) == call(ldb=7) == call(sa=31) == call(sb=31) == call(x=p + 1) == call(out=p + 1) == L.ERR_STRIDE
     need = lib.awq_w4a16_lora_workspace_bytes(600, 8, 4)
     assert need > 0 and call(m=600, ws=None) == call(m=600, wsb=need - 1) == L.ERR_WORKSPACE

@@ -225,6 +225,22 @@ def test_rows_past_4_gib():
 
 
 @pytest.mark.gpu
+def test_the_most_tokens():
+    from litevllm_amd import moe_sort, moe_unsort
+    t, h = 1 << 23, 2
+    x = (torch.arange(t, device="cuda") % 97).half().unsqueeze(1).repeat(1, h).requires_grad_(True)
+    ids = (torch.arange(t, device="cuda") % 5).unsqueeze(1) - 1
+    rows, routes = moe_sort(x, ids, 4)
+    assert torch.equal(routes.offsets.cpu(), torch.tensor([0, *(int((ids <= e).sum() - (ids < 0).sum()) for e in range(4))], dtype=torch.int32))
+    w = (torch.arange(t, device="cuda") % 3).float().unsqueeze(1).requires_grad_(True)
+    out = moe_unsort(rows, w, routes)
+    kept = (ids >= 0).float()
+    assert torch.equal(out, (x * w * kept).half())
+    dx, dw = torch.autograd.grad(out, (x, w), torch.ones_like(out))
+    assert torch.equal(dx, (w * kept).half().expand(t, h)) and torch.equal(dw, x.float().sum(1, keepdim=True) * kept)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [30, 3000])
 def test_replays_and_another_stream(t):
     from litevllm_amd import moe_sort, moe_unsort
@@ -337,6 +353,7 @@ def test_entries_refuse():
     assert sort(t=-1) == sort(h=-1) == sort(e=0) == sort(k=0) == L.ERR_SHAPE
     assert sort(dt=0) == sort(bits=16) == sort(e=1025) == sort(k=1025) == sort(t=(1 << 30) + 1) == sort(t=1 << 29, k=3) == L.ERR_UNSUPPORTED
     assert sort(h=(1 << 24) + 1, ld=1 << 25) == L.ERR_UNSUPPORTED
+    assert sort(t=(1 << 23) + 1, k=1) == L.ERR_UNSUPPORTED and lib.awq_w4a16_moe_sort_workspace_bytes((1 << 23) + 1, 8, 1) == 0
     assert sort(ld=7) == sort(x=p + 1) == sort(rows=p + 2, dt=L.DTYPE_F32) == L.ERR_STRIDE
     need = lib.awq_w4a16_moe_sort_workspace_bytes(50000, 8, 2)
     assert need > 0 and sort(t=50000) == sort(t=50000, ws=p, wsb=need - 1) == L.ERR_WORKSPACE
@@ -349,6 +366,7 @@ def test_entries_refuse():
     assert unsort(rows=None) == unsort(places=None) == unsort(out=None) == L.ERR_NULL
     assert unsort(t=-1) == unsort(h=-1) == unsort(k=0) == L.ERR_SHAPE
     assert unsort(dt=0) == unsort(wdt=0) == unsort(w=None) == unsort(t=1 << 30) == L.ERR_UNSUPPORTED
+    assert unsort(t=(1 << 23) + 1, k=1) == L.ERR_UNSUPPORTED
     assert unsort(ld=7) == unsort(rows=p + 1) == unsort(out=p + 1) == L.ERR_STRIDE
     assert unsort(t=0) == unsort(h=0) == L.OK
 
@@ -357,6 +375,7 @@ def test_entries_refuse():
     assert grad(up=None) == grad(rows=None) == grad(places=None) == grad(total=None) == L.ERR_NULL
     assert grad(t=-1) == grad(h=-1) == grad(k=0) == L.ERR_SHAPE
     assert grad(dt=0) == grad(wdt=0) == grad(w=None, wdt=0) == grad(w=None, gw=None) == grad(t=1 << 30) == L.ERR_UNSUPPORTED
+    assert grad(t=(1 << 23) + 1, k=1) == L.ERR_UNSUPPORTED
     assert grad(ld=7) == grad(up=p + 1) == grad(gr=p + 1) == L.ERR_STRIDE
     assert grad(t=0) == grad(gr=None, gw=None) == L.OK
 
