@@ -37,11 +37,12 @@ def _elsewhere(name: str):
 
 
 def _index(x, ids, experts):
-    """(offsets, experts, places), one allocation, still to be written."""
+    """(offsets, experts, places), one allocation, still to be written.  Each has a version of its own (``.data``): what a user
+    writes over one of them is no change of those that a backward has saved."""
     t, k = ids.shape
     r = t * k
     offsets, of, places = torch.empty(experts + 1 + 2 * r, dtype=torch.int32, device=x.device).split_with_sizes((experts + 1, r, r))
-    return offsets, of, places.view(t, k)
+    return offsets.data, of.data, places.view(t, k)
 
 
 def _sorted(x, ids, experts, index):

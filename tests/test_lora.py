@@ -265,6 +265,38 @@ def test_the_same_bits_replays_and_another_stream(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 100, 600])
+def test_two_calls_at_once_and_replays_in_place(m):
+    from litevllm_amd import LoRAAdapters
+    g = torch.Generator().manual_seed(30)
+    x, a, b, base = _whole(g, m, 5000, size=1).half(), _whole(g, 4, 80, 5000, size=1).half(), _whole(g, 4, 600, 80, size=1).half(), _whole(g, m, 600).half()
+    x[:, torch.rand(5000, generator=g).cuda() > 0.02] = 0
+    layer, ids = LoRAAdapters(a, b), _ids(g, m, 4, m, 0.2)
+    others = (ids + 1).clamp(-1, 3)
+    want = [_check_exact(base, x, a, b, i, None) for i in (ids, others)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    with torch.inference_mode():
+        for _ in range(8):
+            for s, i, to in zip(streams, (ids, others), got):
+                with torch.cuda.stream(s):
+                    to.append(layer.add(base, x, i))
+    torch.cuda.synchronize()
+    for to, w in zip(got, want):
+        assert all(torch.equal(t, w) for t in to)
+    y, graph = base.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.add(y, x, ids, out=y)
+    for _ in range(3):
+        again = layer.add(y, x, ids)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, again)
+
+
+@pytest.mark.gpu
 def test_a_row_does_not_depend_on_its_neighbours_adapters():
     from litevllm_amd import lora_add
     g = torch.Generator().manual_seed(6)

@@ -225,6 +225,55 @@ def test_rows_past_4_gib():
 
 
 @pytest.mark.gpu
+def test_routes_that_are_written_over():
+    """The adapters' ids may be made of routes.experts in place; places that a backward needs may not change unnoticed."""
+    from litevllm_amd import moe_sort, moe_unsort
+    x, w, ids = _whole(60, 6, 8).requires_grad_(True), _whole(61, 6, 2).requires_grad_(True), _ids(62, 6, 4, 2)
+    want = None
+    for touch in (lambda r: None, lambda r: r.experts.clamp_(min=0), lambda r: r.offsets.zero_(), lambda r: r.places.zero_()):
+        rows, routes = moe_sort(x, ids, 4)
+        touch(routes)
+        grad = lambda: torch.autograd.grad(rows, x, torch.ones_like(rows))[0]
+        if int(routes.places.max()) == 0:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                grad()
+        else:
+            got = grad()
+            want = got if want is None else want
+            assert torch.equal(got, want)
+    rows, routes = moe_sort(x, ids, 4)
+    out = moe_unsort(rows, w, routes)
+    routes.experts.zero_()
+    torch.autograd.grad(out, w, torch.ones_like(out), retain_graph=True)
+    routes.offsets.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, w, torch.ones_like(out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [30, 3000, 9000])
+def test_two_calls_at_once(t):
+    from litevllm_amd import moe_sort, moe_unsort
+    h, e, k = 264, 40, 4
+    x, w = _whole(70, t, h).bfloat16(), _whole(71, t, k)
+    ids = [_ids(72, t, e, k, 0.1), _ids(73, t, e, k, 0.3)]
+
+    def step(ids):
+        rows, routes = moe_sort(x, ids, e)
+        return [rows, *routes, moe_unsort(rows, w, routes)]
+    want, got, streams = [step(i) for i in ids], [[], []], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for s, i, to in zip(streams, ids, got):
+            with torch.cuda.stream(s):
+                to.append(step(i))
+    torch.cuda.synchronize()
+    for to, ref in zip(got, want):
+        assert all(torch.equal(a, b) for outs in to for a, b in zip(outs, ref))
+
+
+@pytest.mark.gpu
 def test_the_most_tokens():
     from litevllm_amd import moe_sort, moe_unsort
     t, h = 1 << 23, 2
