@@ -36,13 +36,11 @@ def _elsewhere(name: str):
     return RuntimeError(f"{name}: saved tensors came back elsewhere, or with other shapes or types")
 
 
-def _index(x, ids, experts):
-    """(offsets, experts, places), one allocation, still to be written.  Each has a version of its own (``.data``): what a user
-    writes over one of them is no change of those that a backward has saved."""
-    t, k = ids.shape
-    r = t * k
-    offsets, of, places = torch.empty(experts + 1 + 2 * r, dtype=torch.int32, device=x.device).split_with_sizes((experts + 1, r, r))
-    return offsets.data, of.data, places.view(t, k)
+def _index(ids, experts):
+    """(offsets, experts, places), still to be written; no views of one tensor, since a backward would take what a user writes
+    over one of them for a change of those that it has saved."""
+    places = torch.empty_like(ids, dtype=torch.int32)
+    return places.new_empty(experts + 1), places.new_empty(ids.numel()), places
 
 
 def _sorted(x, ids, experts, index):
@@ -145,7 +143,7 @@ def moe_sort(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int) -> tuple
     if topk_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"topk_ids must be int32 or int64, got {topk_ids.dtype}")
     topk_ids = topk_ids.contiguous()
-    index = _index(x, topk_ids, num_experts)
+    index = _index(topk_ids, num_experts)
     run = _Sort.apply if _derivative_asked("moe_sort", None, x) else _sorted
     return run(x, topk_ids, num_experts, index), MoERoutes(*index)
 

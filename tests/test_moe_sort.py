@@ -208,6 +208,18 @@ def test_no_tokens_and_empty_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,k,h", [(1023, 8, 16), (1025, 8, 16), (13000, 8, 1100), (26000, 8, 1100), (9000, 2, 8200)])
+def test_many_rows(t, k, h):
+    """Around the numbers of routes and bytes from which on other launches do the work."""
+    from litevllm_amd import moe_unsort
+    x = _whole(50 + k, t, h).half().requires_grad_(True)
+    rows, routes = _check_sort(x, _ids(51 + k, t, 37, k, 0.2), 37)
+    kept = (routes.places >= 0).sum(1, keepdim=True)
+    assert torch.equal(moe_unsort(rows, None, routes), (x * kept).half())
+    assert torch.equal(torch.autograd.grad(rows, x, torch.ones_like(rows))[0], kept.half().expand(t, h))
+
+
+@pytest.mark.gpu
 def test_rows_past_4_gib():
     from litevllm_amd import moe_sort, moe_unsort
     t, e, k, h = 66000, 16, 8, 4104
