@@ -606,13 +606,17 @@ struct LoraPlan {
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
   const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit), ranks = lora_ranks(R);
-  l.many = M > 128;
+  // Up to here rows may be single tokens of as many requests: 256 rows, N = 6144, rank 16, 64 adapters 22 us, by the kernels for many
+  // rows 44, rank 64 51 and 82, 500 rows, N = 4096, rank 32 36 and 59.  Prompts of so many rows gain less or lose some: 256 of four
+  // requests 8.9 and 11.3, rank 64 17.3 and 19.2, 500 of three, rank 32 12.7 and 12.1, N = 24576 25 and 21, 300, rank 128 28 and 19;
+  // 600 rows 14 and 11.
+  l.many = M > 512;
   // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little but wait
-  // for LDS (8192 rows of 6 requests 48 us with 4, 54 with 16; 500 rows of as many requests 43 and 35).
-  l.slots = (int)(l.many ? (M <= 512 ? 16 : 4) : std::min<int64_t>(16, M));
+  // for LDS (8192 rows of 6 requests 48 us with 4, 54 with 16).
+  l.slots = (int)(l.many ? 4 : std::min<int64_t>(16, M));
   // One launch where few rows' adapters are small enough to be read by all of a row's blocks.  us with one and with two, which
   // cost the host 4 more (one row: A of 128 KB 6.3, 6.2, of 256 7.9, 6.7, of 384 11.2, 6.5; 64 rows of as many adapters: 128 KB
-  // 9.9, 12.9, 256 13.5, 16.1, 512 19.8, 25.0; 128 rows: 128 KB 12.7, 16.8, 256 KB and two adapters 21.4, 18.1).
+  // 9.9, 12.9, 256 13.5, 16.1, 512 19.8, 25.0; 128 rows: 128 KB 12.7, 16.8, 256 KB and two adapters 21.4, 18.1; 500 rows: 64 KB 21, 27).
   l.own = !l.many && ranks <= 64 && K >= 8 && ranks * K * 2 <= (M <= 32 ? 256 << 10 : M <= 64 ? 512 << 10 : 128 << 10);
   // at least four units a share, at most 16 shares
   l.splits = (int)std::max<int64_t>(1, std::min(cdiv(units, 4), std::min<int64_t>(16, 256 / (tiles * l.slots * cdiv(ranks, 64)))));
@@ -650,7 +654,8 @@ static int lora_typed(LoraArgs p, const LoraPlan& l, hipStream_t st) {
   });
   if (hipGetLastError() != hipSuccess) return AWQ_ERR_LAUNCH;
   const int64_t x = l.many ? cdiv(p.M, 64) : p.tiles * p.slots, step = l.many ? 64 : 32 * few_waves(l.own);
-  const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, (l.own ? 256 : 2048) / x);
+  const int64_t steps = std::max<int64_t>(1, cdiv(p.whole, step)), want = std::max<int64_t>(1, (l.own ? 256 : l.many || p.M <= 128 ? 2048 : 1024) / x);
+  // (256 rows of four requests, rank 64: 17.3 us with 1024 blocks, 21.1 with 2048)
   p.cols = (int)(cdiv(steps, std::min(want, steps)) * step);
   // many rows: not so many columns that the last blocks' work shows (4096 rows, N = 24576: rank 16 99 us with 768 columns a
   // block, 92 with 256, rank 64 127 and, with 512, 123)

@@ -55,7 +55,9 @@ CASES = [  # rows, requests, K, N, rank, adapters, without
     (2049, 3, 1000, 80, 130, 2, 0.4), (40, 40, 12288, 64, 16, 3, 0.0), (5, 5, 64, 24580, 16, 6, 0.2),
     (100, 2, 4096, 520, 64, 4, 0.3), (96, 1, 12288, 300, 16, 1, 0.0), (33, 2, 9000, 1030, 40, 2, 0.0), (128, 128, 5000, 40, 24, 5, 0.2),
     (16, 1, 12288, 4100, 128, 1, 0.0), (100, 3, 7, 90, 5, 2, 0.2), (20, 2, 6, 300, 200, 2, 0.2), (200, 200, 300, 200, 64, 30, 0.1),
-    (1100, 1100, 64, 72, 64, 50, 0.1), (64, 1, 600, 24600, 16, 1, 0.0)]
+    (1100, 1100, 64, 72, 64, 50, 0.1), (64, 1, 600, 24600, 16, 1, 0.0),
+    (512, 512, 128, 256, 256, 9, 0.1), (511, 2, 5000, 70, 40, 3, 0.1), (520, 520, 300, 200, 64, 30, 0.1), (600, 3, 7, 90, 5, 2, 0.2),
+    (700, 3, 6, 50, 200, 2, 0.2), (514, 3, 1025, 65, 64, 3, 0.2)]
 
 
 @pytest.mark.gpu
@@ -119,7 +121,7 @@ def test_ranges_of_the_low_rank_values(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [4, 64])
-@pytest.mark.parametrize("m", [2, 100, 200])
+@pytest.mark.parametrize("m", [2, 100, 200, 600])
 def test_low_rank_values_above_the_largest_bf16(m, k):
     """1.9996 * 2^127 rounds to infinity in bf16 but not in fp32; B takes it down again."""
     from litevllm_amd import lora_add
