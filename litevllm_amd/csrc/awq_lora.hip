@@ -2,9 +2,10 @@
 //
 //   l = ids[m];  v[m] = s_l x[m] A_l^T  (rank values);  out[m] = base[m] + v[m] B_l^T;  out[m] = base[m] without an adapter
 //
-// Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once).  Rows go in tiles that the matrix cores
+// Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once).  Rows go in tiles of 16 that the matrix cores
 // take; a tile looks up which adapters its rows have and is worked on once for each: once where the rows of a request lie
-// together, as in prompts, up to 16 times in a batch of single tokens.  Its blocks (`slots`) share these and, where it has fewer
+// together, as in prompts, up to 16 times in a batch of single tokens, whose rows are put together by adapter where there are some
+// hundred of them.  Its blocks (`slots`) share these and, where it has fewer
 // adapters than blocks, an adapter's columns or K.  The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
 //
 // v enters the second product as two 16-bit numbers, v = high + low: 16 bits of mantissa at least for bf16, 21 for fp16, and
@@ -44,26 +45,112 @@ __device__ __forceinline__ int lora_id(const LoraArgs& p, int64_t m) {
   const int64_t l = p.id64 ? ((const int64_t*)p.ids)[m] : (int64_t)((const int32_t*)p.ids)[m];
   return l >= 0 && l < p.L ? (int)l : -1;
 }
-// An adapter of a tile of 16 rows and its rows, for a block of `slots`: the only one or, where the tile has fewer adapters than
-// blocks, one that the block shares with others, as number `part` of `parts`.  id: a row's adapter (lanes 0 .. 15), -1 for none,
-// which counts as an adapter, -2: no row.
+// Few rows go in groups of up to 16 of the same adapter, the rows without one as if they had the same.  A block has the group of its
+// number or, where there are fewer groups than blocks, shares one with others as number `part` of `parts`.
+constexpr int kFewRows = 512, kTogether = 128, kMostCounted = 1024;
 struct Group {
-  int adapter;
-  uint32_t rows;
+  int adapter;     // -1: none
+  uint32_t rows;   // which of the 16 exist
   int part, parts;
+  int row;         // that of lanes i, i + 16, ..., or one that exists
 };
-__device__ __forceinline__ Group group_of(int id, int slot, int slots) {
+struct GroupLds {
+  int seen[kMostCounted + 1];  // an adapter's rows so far
+  int key[kFewRows], rank[kFewRows];  // a row's adapter (-1), and its number among the adapter's rows
+  int row[16];
+  int adapter, rows, part, parts;
+};
+// Groups of 16 neighbouring rows and of one adapter; id: that of lane i's, -2 for no row.
+__device__ __forceinline__ Group group_of_neighbours(const LoraArgs& p, int row0, int id, int slot) {
+  const int i = threadIdx.x & 15;
   const uint32_t all = (uint32_t)(__ballot(id >= -1) & 0xFFFF);
   int count = 0;
   for (uint32_t left = all; left; ++count) left &= ~(uint32_t)__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctz(left)));
   Group g{};
   int mine = slot % count;
-  g.part = slot / count, g.parts = (slots - 1 - mine) / count + 1;
+  g.part = slot / count, g.parts = (p.slots - 1 - mine) / count + 1;
   for (uint32_t left = all; mine >= 0; --mine) {
     g.adapter = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
     g.rows = (uint32_t)__ballot(id == g.adapter) & left;
     left &= ~g.rows;
   }
+  g.row = row0 + (g.rows >> i & 1 ? i : __builtin_ctz(g.rows));
+  return g;
+}
+// Groups of the adapter's rows wherever they are, in their order, by one wave and 64 rows at a time: lanes with the same adapter find
+// each other by its bits.
+__device__ __forceinline__ Group group_of_all(const LoraArgs& p, GroupLds& lds, int number) {
+  const int t = threadIdx.x, rows = (int)p.M;
+  for (int e = t; e <= p.L; e += 64) lds.seen[e] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  int groups = 0;
+#pragma unroll 1
+  for (int m = t; m - t < rows; m += 64) {
+    const bool has = m < rows;
+    const int id = has ? lds.key[m] : -1, e = id < 0 ? p.L : id;
+    uint64_t same = __ballot(has);
+    for (int bit = 1; bit <= p.L; bit <<= 1) {
+      const uint64_t set = __ballot(e & bit);
+      same &= e & bit ? set : ~set;
+    }
+    const int ahead = __popcll(same & ((1ull << t) - 1)), before = lds.seen[e], rank = before + ahead;
+    __builtin_amdgcn_wave_barrier();
+    if (has) lds.rank[m] = rank;
+    if (has && ahead == 0) lds.seen[e] = before + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    groups += __popcll(__ballot(has && (rank & 15) == 0));
+  }
+  const int mine = number % groups;
+  int left = mine, adapter = 0, rank0 = -1, count = 0;
+#pragma unroll 1
+  for (int m = t; m - t < rows; m += 64) {
+    const bool has = m < rows;
+    const int id = has ? lds.key[m] : -2, rank = has ? lds.rank[m] : 0;
+    if (rank0 < 0) {
+      const uint64_t first = __ballot(has && (rank & 15) == 0);
+      const int n = __popcll(first);
+      if (left >= n) {
+        left -= n;
+        continue;
+      }
+      const int lane = __builtin_ctzll(__ballot((first >> t & 1) && __popcll(first & ((1ull << t) - 1)) == left));
+      adapter = __builtin_amdgcn_readlane(id, lane), rank0 = __builtin_amdgcn_readlane(rank, lane);
+      if (t < 16) lds.row[t] = m - t + lane;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    const bool in = id == adapter && rank >= rank0 && rank < rank0 + 16;
+    if (in) lds.row[rank - rank0] = m;
+    count += __popcll(__ballot(in));
+  }
+  Group g{};
+  g.adapter = adapter, g.rows = (1u << count) - 1, g.part = number / groups, g.parts = (p.tiles * p.slots - 1 - mine) / groups + 1;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  g.row = lds.row[t & 15];
+  return g;
+}
+// Neighbours where most have the same adapter, as in prompts, or the rows are few: the search costs 1 to 2 us of a prompt (200 rows 9.1,
+// 8.2 without it) and saves single tokens the passes over the same adapter in other tiles (64 adapters: 256 rows, rank 64 51 -> 30 us,
+// 500 rows, N = 24576, rank 16 84 -> 34; 128 rows, rank 16 12.1 -> 10.7, but 20 requests of as many 8.9 -> 10.2).
+__device__ __forceinline__ Group group_of(const LoraArgs& p, GroupLds& lds, int number) {
+  const int t = threadIdx.x, i = t & 15, row0 = number % p.tiles * 16, slot = number / p.tiles, m = row0 + i, rows = (int)p.M;
+  if (rows <= kTogether || p.L > kMostCounted) {
+    const Group g = group_of_neighbours(p, row0, m < rows ? lora_id(p, m) : -2, slot);
+    if (t < 16) lds.row[t] = g.row;
+    return g;
+  }
+  for (int at = t; at < rows; at += (int)blockDim.x) lds.key[at] = lora_id(p, at);
+  __syncthreads();
+  Group g;
+  if (t < 64) {
+    int runs = 1;
+    for (int at = t + 1; at - t < rows; at += 64) runs += __popcll(__ballot(at < rows && lds.key[at] != lds.key[at - 1]));
+    g = runs > 2 * p.tiles ? group_of_all(p, lds, number) : group_of_neighbours(p, row0, m < rows ? lds.key[m] : -2, slot);
+    if (t < 16) lds.row[t] = g.row;
+    if (t == 0) lds.adapter = g.adapter, lds.rows = g.rows, lds.part = g.part, lds.parts = g.parts;
+  }
+  __syncthreads();
+  g.adapter = __builtin_amdgcn_readfirstlane(lds.adapter), g.rows = __builtin_amdgcn_readfirstlane(lds.rows);
+  g.part = __builtin_amdgcn_readfirstlane(lds.part), g.parts = __builtin_amdgcn_readfirstlane(lds.parts), g.row = lds.row[i];
   return g;
 }
 // The neighbouring lane's value (lanes 0 and 1 swap, 2 and 3, ...), and the largest of 16 lanes.
@@ -114,21 +201,20 @@ union RankLds {
   uint16_t stage[WAVES][(1 + RT) * 16][kUnit + 8];  // rows 16 bytes apart from whole banks
   f32x4 part[WAVES][RT][64];
 };
-// RT tiles of 16 ranks, from tile0 on, of adapter `cur` by the rows `rows` of 16 and a share of K, whose units the waves take in
+// RT tiles of 16 ranks, from tile0 on, of adapter `cur` by the rows row(0 .. 15) and a share of K, whose units the waves take in
 // turn; the waves' sums come to lie in LDS.  A wave's next unit is on its way in registers (more of them made every size slower:
 // one row, K = N = 4096, rank 16 6.6 us with two, 7.3 with four, 6.3 as it is).  Loads cover whole lines, eight lanes each; a wave passes them through LDS of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and
 // 32 + 8 q .. of rank i and of row i.  (Straight from memory in that order a load's neighbouring lanes are in different lines:
 // 4096 rows, K = 4096, rank 64 42 us instead of 12.)
-template <typename T, int RT, int WAVES>
-__device__ __forceinline__ void tile_ranks(const LoraArgs& p, RankLds<RT, WAVES>& lds, int64_t m0, uint32_t rows, int cur, int tile0,
-                                           int begin, int units) {
+template <typename T, int RT, int WAVES, class Row>
+__device__ __forceinline__ void tile_ranks(const LoraArgs& p, RankLds<RT, WAVES>& lds, Row row, int cur, int tile0, int begin, int units) {
   constexpr int TILES = 1 + RT;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, r8 = lane >> 3, c8 = 8 * (lane & 7);
-  // two rows of each tile a lane; for rows of other adapters a row that is read anyway
+  // two rows of each tile a lane
   const uint16_t* from[TILES][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    from[0][h] = p.x + (m0 + (rows >> (r8 + 8 * h) & 1 ? r8 + 8 * h : __builtin_ctz(rows))) * p.ldx + c8;
+    from[0][h] = p.x + row(r8 + 8 * h) * p.ldx + c8;
 #pragma unroll
     for (int r = 0; r < RT; ++r) from[1 + r][h] = p.a + cur * p.a_stride + (int64_t)min(16 * (tile0 + r) + r8 + 8 * h, p.R - 1) * p.K + c8;
   }
@@ -195,22 +281,23 @@ __device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank,
   if (std::is_same<T, f16>::value && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = h.power;
 }
 
-// Few rows: a block has an adapter of the tile and a share of K; those that share the adapter cut the share further, into
+// Few rows: a block has a group of rows and a share of K; those that share the group cut the share further, into
 // sub-shares (lora_shares).
 __device__ __forceinline__ int lora_shares(const LoraArgs& p, int parts) { return min(parts, p.shares / p.splits); }
 template <typename T, int RT, int W>
 __global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {
   __shared__ __attribute__((aligned(16))) RankLds<RT, 4> lds;
-  const int i = threadIdx.x & 15, tile0 = blockIdx.y * RT;
-  const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16;
-  const Group g = group_of(m0 + i < p.M ? lora_id(p, m0 + i) : -2, blockIdx.x / p.tiles, p.slots);
+  __shared__ GroupLds groups;
+  const int tile0 = blockIdx.y * RT;
+  const Group g = group_of(p, groups, blockIdx.x);
   const int shares = lora_shares(p, g.parts), share = blockIdx.z * shares + g.part;
   if (g.adapter < 0 || g.part >= shares) return;
   const int units = (p.K + kUnit - 1) / kUnit, per = (units + p.splits * shares - 1) / (p.splits * shares);
-  tile_ranks<T, RT, 4>(p, lds, m0, g.rows, g.adapter, tile0, share * per, min((share + 1) * per, units));
+  tile_ranks<T, RT, 4>(p, lds, [&](int r) { return (int64_t)__shfl(g.row, r); }, g.adapter, tile0, share * per, min((share + 1) * per, units));
   for_ranks<RT, 4, W>(lds, [&](int row, int rank, float f) {
     rank += 16 * tile0;
-    if (rank < p.ranks && (g.rows >> row & 1)) p.partial[((int64_t)share * p.M + m0 + row) * p.ranks + rank] = f;
+    const int64_t m = __shfl(g.row, row);
+    if (rank < p.ranks && (g.rows >> row & 1)) p.partial[(share * p.M + m) * p.ranks + rank] = f;
   });
 }
 
@@ -231,7 +318,9 @@ __global__ void __launch_bounds__(64 * many_waves(RT)) lora_ranks_kernel(LoraArg
     const uint32_t rows = (uint32_t)(__ballot(id == cur) & 0xFFFF);
     left &= ~rows;
     if (n % p.slots != slot) continue;
-    tile_ranks<T, RT, WAVES>(p, lds, m0, rows, cur, tile0, 0, (p.K + kUnit - 1) / kUnit);
+    // for rows of other adapters a row that is read anyway
+    tile_ranks<T, RT, WAVES>(p, lds, [&](int r) { return m0 + (rows >> r & 1 ? r : __builtin_ctz(rows)); }, cur, tile0, 0,
+                             (p.K + kUnit - 1) / kUnit);
     for_ranks<RT, WAVES, W>(lds, [&](int row, int rank, float f) {
       rank += 16 * tile0;
       if (rank < p.ranks) put_rank<T, W>(p, m0 + row, rank, f, p.scales ? p.scales[cur] : 1.f, rows >> row & 1);
@@ -255,15 +344,16 @@ __global__ void __launch_bounds__(256) lora_ranks_short_kernel(LoraArgs p) {
 }
 
 // ------------------------------------------------------------------ columns
-// Columns behind p.whole, one by one, of the rows `rows` of `count`; parts(row) and power(row, tile) give a row's v.
-template <typename T, int W, class Parts, class Power>
-__device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b, int64_t m0, int count, uint64_t rows, bool adapter,
-                                            Parts parts, Power power) {
+// Columns behind p.whole, one by one, of the rows at(0), ... of `rows`, which has `count` bits; parts(row) and power(row, tile)
+// give a row's v.
+template <typename T, int W, class At, class Parts, class Power>
+__device__ __forceinline__ void odd_columns(const LoraArgs& p, const uint16_t* b, At at, int count, uint64_t rows, bool adapter, Parts parts,
+                                            Power power) {
   const int odd = p.N - p.whole;
-  for (int at = threadIdx.x; at < count * odd; at += blockDim.x) {
-    const int row = at / odd, col = p.whole + at - row * odd;
+  for (int n = threadIdx.x; n < count * odd; n += blockDim.x) {
+    const int row = n / odd, col = p.whole + n - row * odd;
     if (!(rows >> row & 1)) continue;
-    const int64_t m = m0 + row;
+    const int64_t m = at(row);
     float s = 0.f;
     if (adapter) {
       const uint16_t* const v = parts(row);
@@ -303,7 +393,7 @@ __device__ __forceinline__ u32x4 added(const u32x4& base, const f32x4& d0, const
   return o;
 }
 
-// Few rows: 16 by p.cols columns, B straight from memory.  A wave takes 32 columns at a time as two tiles of 16, tile c of them
+// Few rows: a group by p.cols columns, B straight from memory.  A wave takes 32 columns at a time as two tiles of 16, tile c of them
 // the columns 8 (i / 4) + 4 c + i % 4, so that lane (q, i) ends with the eight columns 8 q .. 8 q + 7 of row i.  RT tiles of W
 // ranks at a time.  Base and B of the first columns are on their way while v is made ready: the shares of the first launch are
 // added up or, OWN > 0, all OWN tiles of 16 ranks computed by the block itself, for all of its columns.
@@ -314,18 +404,17 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
   __shared__ __attribute__((aligned(16))) RankLds<OWN ? OWN : 1, OWN ? WAVES : 1> own;
   extern __shared__ u32x4 dynamic_lds[];  // v: [16][ld], of each W ranks the high parts, then the low parts
   __shared__ float power[16][16];
+  __shared__ GroupLds groups;
   uint16_t* const v = (uint16_t*)dynamic_lds;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / W, ld = 2 * p.ranks + 8;
-  const int64_t m0 = (int64_t)(blockIdx.x % p.tiles) * 16, m = m0 + i;
-  const int id = m < p.M ? lora_id(p, m) : -2;
-  const Group g = group_of(id, blockIdx.x / p.tiles, p.slots);
+  const Group g = group_of(p, groups, blockIdx.x);
   if (g.adapter < 0 && p.out == p.base && p.ldo == p.ldb) return;  // in place already
   const int cur = g.adapter, part = blockIdx.y * g.parts + g.part, parts = gridDim.y * g.parts;
   const int steps = (p.whole + STEP - 1) / STEP, cols = (steps + parts - 1) / parts * STEP;
   const int begin = min(part * cols, p.whole) + wave * 32, end = min((part + 1) * cols, p.whole);
   if (part * cols >= p.whole && part + 1 < parts) return;  // nothing left
-  const uint32_t rows = g.rows;
-  const bool mine = id == cur;
+  const int64_t m = g.row;
+  const bool mine = g.rows >> i & 1;
   const uint16_t* const b = p.b + max(cur, 0) * p.b_stride;
   // of the last tile's eight ranks of this lane those that exist, as a mask of their bits
   const int there = p.R - (p.ranks - W) - first_rank<W>(q);
@@ -355,7 +444,7 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
     const float scale = p.scales ? p.scales[cur] : 1.f;
     const int shares = p.splits * lora_shares(p, g.parts);
     if constexpr (OWN > 0) {
-      tile_ranks<T, OWN, WAVES>(p, own, m0, rows, cur, 0, 0, (p.K + kUnit - 1) / kUnit);
+      tile_ranks<T, OWN, WAVES>(p, own, [&](int r) { return (int64_t)__shfl(g.row, r); }, cur, 0, 0, (p.K + kUnit - 1) / kUnit);
       for_ranks<OWN, WAVES, W>(own, [&](int row, int rank, float f) {
         if (rank >= p.ranks) return;
         const Parts two = tile_parts<T, W>(rank < p.R ? f * scale : 0.f);
@@ -367,8 +456,8 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
     // a wave has a row's tile, lane (q, i) the shares q, q + 4, ... of ranks i and 16 + i
     for (int j = wave; j < 16 * tiles && !OWN; j += 4) {
       const int row = j & 15, r = j >> 4;
-      if (!(rows >> row & 1)) continue;
-      const float* const at = p.partial + (m0 + row) * p.ranks + W * r + i;
+      if (!(g.rows >> row & 1)) continue;
+      const float* const at = p.partial + (int64_t)__builtin_amdgcn_readlane(g.row, row) * p.ranks + W * r + i;
       float part[SUB][4], f[SUB];
 #pragma unroll
       for (int h = 0; h < SUB; ++h)
@@ -424,9 +513,11 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
     }
     if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
   }
-  if (part + 1 == parts)
-    odd_columns<T, W>(p, b, m0, 16, rows, cur >= 0, [&](int row) { return v + row * ld; },
-                      [&](int row, int r) { return power[row][r]; });
+  if (part + 1 == parts && p.N > p.whole) {
+    __syncthreads();  // groups.row
+    odd_columns<T, W>(p, b, [&](int row) { return (int64_t)groups.row[row]; }, 16, g.rows, cur >= 0,
+                      [&](int row) { return v + row * ld; }, [&](int row, int r) { return power[row][r]; });
+  }
 }
 
 // Many rows: 64 by p.cols columns, 64 of them at a time: their B goes through LDS once for the four waves, which have 16 rows
@@ -574,11 +665,12 @@ __global__ void __launch_bounds__(256, 3) lora_columns_kernel(LoraArgs p) {
         }
     }
     if (y + 1 == p.ranges) {
+      auto at = [&](int row) { return m0 + row; };
       auto parts = [&](int row) { return p.v + (m0 + row) * 2 * p.ranks; };
       auto powers = [&](int row, int r) { return std::is_same<T, f16>::value ? p.powers[(m0 + row) * tiles + r] : 1.f; };
 #pragma unroll
-      for (int g = 0; g < 2; ++g) odd_columns<T, W>(p, p.b + max(cur[g], 0) * p.b_stride, m0, 64, rows[g], true, parts, powers);
-      if (!in_place) odd_columns<T, W>(p, p.b, m0, 64, none, false, parts, powers);
+      for (int g = 0; g < 2; ++g) odd_columns<T, W>(p, p.b + max(cur[g], 0) * p.b_stride, at, 64, rows[g], true, parts, powers);
+      if (!in_place) odd_columns<T, W>(p, p.b, at, 64, none, false, parts, powers);
     }
     none = 0;
   }
@@ -606,11 +698,10 @@ struct LoraPlan {
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
   const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit), ranks = lora_ranks(R);
-  // Up to here rows may be single tokens of as many requests: 256 rows, N = 6144, rank 16, 64 adapters 22 us, by the kernels for many
-  // rows 44, rank 64 51 and 82, 500 rows, N = 4096, rank 32 36 and 59.  Prompts of so many rows gain less or lose some: 256 of four
-  // requests 8.9 and 11.3, rank 64 17.3 and 19.2, 500 of three, rank 32 12.7 and 12.1, N = 24576 25 and 21, 300, rank 128 28 and 19;
-  // 600 rows 14 and 11.
-  l.many = M > 512;
+  // Up to here rows may be single tokens of as many requests: 256 rows, N = 6144, rank 16, 64 adapters 17 us, by the kernels for many
+  // rows 44, rank 64 30 and 82, 500 rows, N = 4096, rank 32 27 and 59.  Prompts of so many rows gain less or lose some: 256 of four
+  // requests 9.7 and 11.3, rank 64 18.5 and 19.2, 500 of three, rank 32 15.1 and 12.1, 300, rank 128 28 and 19.
+  l.many = M > kFewRows;
   // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little but wait
   // for LDS (8192 rows of 6 requests 48 us with 4, 54 with 16).
   l.slots = (int)(l.many ? 4 : std::min<int64_t>(16, M));

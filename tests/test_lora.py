@@ -57,7 +57,9 @@ CASES = [  # rows, requests, K, N, rank, adapters, without
     (16, 1, 12288, 4100, 128, 1, 0.0), (100, 3, 7, 90, 5, 2, 0.2), (20, 2, 6, 300, 200, 2, 0.2), (200, 200, 300, 200, 64, 30, 0.1),
     (1100, 1100, 64, 72, 64, 50, 0.1), (64, 1, 600, 24600, 16, 1, 0.0),
     (512, 512, 128, 256, 256, 9, 0.1), (511, 2, 5000, 70, 40, 3, 0.1), (520, 520, 300, 200, 64, 30, 0.1), (600, 3, 7, 90, 5, 2, 0.2),
-    (700, 3, 6, 50, 200, 2, 0.2), (514, 3, 1025, 65, 64, 3, 0.2)]
+    (700, 3, 6, 50, 200, 2, 0.2), (514, 3, 1025, 65, 64, 3, 0.2),
+    (300, 300, 40, 24, 8, 1024, 0.1), (300, 300, 40, 27, 8, 1025, 0.1), (400, 400, 64, 40, 16, 1, 0.5), (512, 512, 64, 100, 16, 2, 0.3),
+    (129, 129, 64, 33, 64, 3, 0.3), (257, 40, 1000, 65, 8, 600, 0.1), (500, 500, 7, 30, 20, 3, 0.3), (480, 480, 4100, 300, 64, 30, 0.1)]
 
 
 @pytest.mark.gpu
