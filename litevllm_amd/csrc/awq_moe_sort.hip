@@ -126,6 +126,7 @@ __device__ __forceinline__ int block_scan(int c, int* carry, int* tot) {
   return first;
 }
 
+// A block counts a segment: 16384 routes 2.8 us, 131072 4.8, its launch and one round of loads and LDS adds.
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
   __shared__ int count[1025];
   for (int e = threadIdx.x; e <= a.E; e += kSortThreads) count[e] = 0;
