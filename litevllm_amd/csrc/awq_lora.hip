@@ -4,9 +4,9 @@
 //
 // Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once).  Rows go in tiles of 16 that the matrix cores
 // take; a tile looks up which adapters its rows have and is worked on once for each: once where the rows of a request lie
-// together, as in prompts, up to 16 times in a batch of single tokens, whose rows are put together by adapter where there are some
-// hundred of them.  Its blocks (`slots`) share these and, where it has fewer
-// adapters than blocks, an adapter's columns or K.  The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
+// together, as in prompts, up to 16 times in a batch of single tokens, whose rows are put together by adapter where there are more
+// than some (group_of).  Its blocks (`slots`) share these and, where it has fewer adapters than blocks, an adapter's columns or K.
+// The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
 //
 // v enters the second product as two 16-bit numbers, v = high + low: 16 bits of mantissa at least for bf16, 21 for fp16, and
 // one rounding for the output.  Both halves meet the same B: ranks go in tiles of W = 32, an instruction for the high parts and
@@ -20,6 +20,10 @@ namespace awq {
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));  // 16 bytes at any address of a 16-bit element
 
+// A block's group of few rows as the first launch found it, for the second (see Group).
+struct GroupRecord {
+  int adapter, rows, part, parts, row[16];
+};
 struct LoraArgs {
   const uint16_t *base, *x, *a, *b;
   const void* ids;
@@ -28,6 +32,7 @@ struct LoraArgs {
   float* partial;  // few rows: [shares][M][ranks], s_l not in it yet
   uint16_t* v;     // many rows: [M][2 ranks], of each W ranks the high parts, then the low parts
   float* powers;   // and [M][ranks / W]: 2^e (fp16)
+  GroupRecord* records;  // NULL where there is no first launch that finds them
   int64_t ldb, ldx, ldo, a_stride, b_stride;
   int64_t M;
   int N, K, R, L, id64;
@@ -47,7 +52,7 @@ __device__ __forceinline__ int lora_id(const LoraArgs& p, int64_t m) {
 }
 // Few rows go in groups of up to 16 of the same adapter, the rows without one as if they had the same.  A block has the group of its
 // number or, where there are fewer groups than blocks, shares one with others as number `part` of `parts`.
-constexpr int kFewRows = 512, kTogether = 128, kMostCounted = 1024;
+constexpr int kFewRows = 512, kTogether = 64, kMostCounted = 1024;
 struct Group {
   int adapter;     // -1: none
   uint32_t rows;   // which of the 16 exist
@@ -57,9 +62,17 @@ struct Group {
 struct GroupLds {
   int seen[kMostCounted + 1];  // an adapter's rows so far
   int key[kFewRows], rank[kFewRows];  // a row's adapter (-1), and its number among the adapter's rows
-  int row[16];
-  int adapter, rows, part, parts;
+  GroupRecord found;
 };
+__device__ __forceinline__ Group recorded(const GroupRecord& r) {
+  return {__builtin_amdgcn_readfirstlane(r.adapter), (uint32_t)__builtin_amdgcn_readfirstlane(r.rows), __builtin_amdgcn_readfirstlane(r.part),
+          __builtin_amdgcn_readfirstlane(r.parts), r.row[threadIdx.x & 15]};
+}
+// By one wave.
+__device__ __forceinline__ void record(const Group& g, GroupRecord& r) {
+  if (threadIdx.x < 16) r.row[threadIdx.x] = g.row;
+  if (threadIdx.x == 0) r.adapter = g.adapter, r.rows = (int)g.rows, r.part = g.part, r.parts = g.parts;
+}
 // Groups of 16 neighbouring rows and of one adapter; id: that of lane i's, -2 for no row.
 __device__ __forceinline__ Group group_of_neighbours(const LoraArgs& p, int row0, int id, int slot) {
   const int i = threadIdx.x & 15;
@@ -115,43 +128,39 @@ __device__ __forceinline__ Group group_of_all(const LoraArgs& p, GroupLds& lds, 
       }
       const int lane = __builtin_ctzll(__ballot((first >> t & 1) && __popcll(first & ((1ull << t) - 1)) == left));
       adapter = __builtin_amdgcn_readlane(id, lane), rank0 = __builtin_amdgcn_readlane(rank, lane);
-      if (t < 16) lds.row[t] = m - t + lane;
+      if (t < 16) lds.found.row[t] = m - t + lane;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     const bool in = id == adapter && rank >= rank0 && rank < rank0 + 16;
-    if (in) lds.row[rank - rank0] = m;
+    if (in) lds.found.row[rank - rank0] = m;
     count += __popcll(__ballot(in));
   }
   Group g{};
   g.adapter = adapter, g.rows = (1u << count) - 1, g.part = number / groups, g.parts = (p.tiles * p.slots - 1 - mine) / groups + 1;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  g.row = lds.row[t & 15];
+  g.row = lds.found.row[t & 15];
   return g;
 }
-// Neighbours where most have the same adapter, as in prompts, or the rows are few: the search costs 1 to 2 us of a prompt (200 rows 9.1,
-// 8.2 without it) and saves single tokens the passes over the same adapter in other tiles (64 adapters: 256 rows, rank 64 51 -> 30 us,
-// 500 rows, N = 24576, rank 16 84 -> 34; 128 rows, rank 16 12.1 -> 10.7, but 20 requests of as many 8.9 -> 10.2).
+// Neighbours where most have the same adapter, as in prompts, or the rows are few: the search costs a prompt about 1 us (128 rows, rank
+// 16 7.4, 6.9 without it, rank 64 12.7 and 12.3, 200 rows 9.1 and 8.2) and saves single tokens the passes over the same adapter in other
+// tiles (64 adapters: 128 rows, rank 16 11.0 and 12.3, rank 64 21.9 and 28.1, 256 rows, rank 64 25.9 and 51, 500 rows, N = 24576, rank
+// 16 34 and 84; 64 rows, rank 32 13.1 and 13.4, their prompts 9.6 and 9.2).
 __device__ __forceinline__ Group group_of(const LoraArgs& p, GroupLds& lds, int number) {
   const int t = threadIdx.x, i = t & 15, row0 = number % p.tiles * 16, slot = number / p.tiles, m = row0 + i, rows = (int)p.M;
   if (rows <= kTogether || p.L > kMostCounted) {
     const Group g = group_of_neighbours(p, row0, m < rows ? lora_id(p, m) : -2, slot);
-    if (t < 16) lds.row[t] = g.row;
+    record(g, lds.found);
     return g;
   }
   for (int at = t; at < rows; at += (int)blockDim.x) lds.key[at] = lora_id(p, at);
   __syncthreads();
-  Group g;
   if (t < 64) {
     int runs = 1;
     for (int at = t + 1; at - t < rows; at += 64) runs += __popcll(__ballot(at < rows && lds.key[at] != lds.key[at - 1]));
-    g = runs > 2 * p.tiles ? group_of_all(p, lds, number) : group_of_neighbours(p, row0, m < rows ? lds.key[m] : -2, slot);
-    if (t < 16) lds.row[t] = g.row;
-    if (t == 0) lds.adapter = g.adapter, lds.rows = g.rows, lds.part = g.part, lds.parts = g.parts;
+    record(runs > 2 * p.tiles ? group_of_all(p, lds, number) : group_of_neighbours(p, row0, m < rows ? lds.key[m] : -2, slot), lds.found);
   }
   __syncthreads();
-  g.adapter = __builtin_amdgcn_readfirstlane(lds.adapter), g.rows = __builtin_amdgcn_readfirstlane(lds.rows);
-  g.part = __builtin_amdgcn_readfirstlane(lds.part), g.parts = __builtin_amdgcn_readfirstlane(lds.parts), g.row = lds.row[i];
-  return g;
+  return recorded(lds.found);
 }
 // The neighbouring lane's value (lanes 0 and 1 swap, 2 and 3, ...), and the largest of 16 lanes.
 __device__ __forceinline__ u32x4 from_neighbour(u32x4 v) {
@@ -282,7 +291,8 @@ __device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank,
 }
 
 // Few rows: a block has a group of rows and a share of K; those that share the group cut the share further, into
-// sub-shares (lora_shares).  29 rows, K = 12288, rank 12: 5.2 us, latency.
+// sub-shares (lora_shares).  29 rows, K = 12288, rank 12: 5.2 us, latency.  What
+// it found out about a block's group is left for the second launch (the same rows, N = 5001: 12.0 -> 10.5 us for both).
 __device__ __forceinline__ int lora_shares(const LoraArgs& p, int parts) { return min(parts, p.shares / p.splits); }
 template <typename T, int RT, int W>
 __global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {
@@ -290,6 +300,7 @@ __global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {
   __shared__ GroupLds groups;
   const int tile0 = blockIdx.y * RT;
   const Group g = group_of(p, groups, blockIdx.x);
+  if (blockIdx.y == 0 && blockIdx.z == 0) record(g, p.records[blockIdx.x]);
   const int shares = lora_shares(p, g.parts), share = blockIdx.z * shares + g.part;
   if (g.adapter < 0 || g.part >= shares) return;
   const int units = (p.K + kUnit - 1) / kUnit, per = (units + p.splits * shares - 1) / (p.splits * shares);
@@ -408,7 +419,9 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
   __shared__ GroupLds groups;
   uint16_t* const v = (uint16_t*)dynamic_lds;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, q = lane >> 4, i = lane & 15, tiles = p.ranks / W, ld = 2 * p.ranks + 8;
-  const Group g = group_of(p, groups, blockIdx.x);
+  const bool found = OWN == 0 && p.records;
+  const Group g = found ? recorded(p.records[blockIdx.x]) : group_of(p, groups, blockIdx.x);
+  if (found) record(g, groups.found);
   if (g.adapter < 0 && p.out == p.base && p.ldo == p.ldb) return;  // in place already
   const int cur = g.adapter, part = blockIdx.y * g.parts + g.part, parts = gridDim.y * g.parts;
   const int steps = (p.whole + STEP - 1) / STEP, cols = (steps + parts - 1) / parts * STEP;
@@ -515,8 +528,8 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
     if (mine && c0 + 8 * q < end) *(u32x4_any*)(p.out + m * p.ldo + c0 + 8 * q) = added<T>(now, sum[0], sum[1]);
   }
   if (part + 1 == parts && p.N > p.whole) {
-    __syncthreads();  // groups.row
-    odd_columns<T, W>(p, b, [&](int row) { return (int64_t)groups.row[row]; }, 16, g.rows, cur >= 0,
+    __syncthreads();  // groups.found
+    odd_columns<T, W>(p, b, [&](int row) { return (int64_t)groups.found.row[row]; }, 16, g.rows, cur >= 0,
                       [&](int row) { return v + row * ld; }, [&](int row, int r) { return power[row][r]; });
   }
 }
@@ -701,8 +714,8 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t R) {
   LoraPlan l{};
   const int64_t tiles = cdiv(M, 16), units = cdiv(K, kUnit), ranks = lora_ranks(R);
   // Up to here rows may be single tokens of as many requests: 256 rows, N = 6144, rank 16, 64 adapters 17 us, by the kernels for many
-  // rows 44, rank 64 30 and 82, 500 rows, N = 4096, rank 32 27 and 59.  Prompts of so many rows gain less or lose some: 256 of four
-  // requests 9.7 and 11.3, rank 64 18.5 and 19.2, 500 of three, rank 32 15.1 and 12.1, 300, rank 128 28 and 19.
+  // rows 44, rank 64 26 and 82, 500 rows, N = 4096, rank 32 22 and 59.  Prompts of so many rows gain less or lose some: 256 of four
+  // requests 9.7 and 11.3, rank 64 17.5 and 19.2, 500 of three, rank 32 14.1 and 12.1, 300, rank 128 31 and 19.
   l.many = M > kFewRows;
   // Of many rows a tile has one adapter or two if they are prompts, but may have 16; blocks that find none cost little but wait
   // for LDS (8192 rows of 6 requests 48 us with 4, 54 with 16).
@@ -720,7 +733,8 @@ size_t lora_workspace_bytes(int64_t M, int64_t K, int64_t R) {
   const LoraPlan l = lora_plan(M, K, R);
   const size_t values = (size_t)M * (size_t)lora_ranks(R);
   if (l.own) return 0;
-  return l.many ? values * 4 + values / (size_t)lora_tile(R) * 4 : (size_t)l.shares * values * 4;
+  if (l.many) return values * 4 + values / (size_t)lora_tile(R) * 4;
+  return (size_t)l.shares * values * 4 + (size_t)(cdiv(M, 16) * l.slots) * sizeof(GroupRecord);
 }
 
 template <typename T>
@@ -779,6 +793,7 @@ int launch_lora(const LoraCall& c, hipStream_t st) {
   const LoraPlan l = lora_plan(c.M, c.K, c.R);
   p.tiles = (int)cdiv(c.M, 16), p.slots = l.slots, p.splits = l.splits, p.shares = l.shares;
   p.partial = (float*)c.workspace;
+  if (!l.many && !l.own && c.K >= 8) p.records = (GroupRecord*)(p.partial + (size_t)l.shares * (size_t)(c.M * p.ranks));
   p.v = (uint16_t*)c.workspace, p.powers = (float*)(p.v + (size_t)c.M * 2 * p.ranks);
   return c.dtype == AWQ_DTYPE_F16 ? lora_typed<f16>(p, l, st) : lora_typed<bf16>(p, l, st);
 }
