@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(64 * few_waves(OWN > 0), OWN ? 1 : 2) lora_col
 // load and store of base and out covers whole lines of 128 bytes.  Two adapters at a time, so that a tile where one request ends
 // and the next begins takes no longer; the rows without an adapter go with the first two.
 // Neighbouring blocks have neighbouring columns, so that (in eights) an XCD reads the same columns' B for all row tiles.
-// 4096 rows, N = 24576, rank 64: 99 us, base and out at 4.1 TB/s; 82 without the products and their B.
+// 4096 rows, N = 24576, rank 64: 97 us, base and out at 4.1 TB/s; 82 without the products and their B.
 template <typename T, int RT, int W, bool THROUGH>
 __global__ void __launch_bounds__(256, 3) lora_columns_kernel(LoraArgs p) {
   constexpr int ROWS = 64, SUB = W / 16, LD = W * RT + 8, ROW = W * RT / 8, PIECES = 64 * ROW, EACH = (PIECES + 255) / 256;
