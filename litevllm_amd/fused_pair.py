@@ -23,9 +23,12 @@ from .tensor import AWQWeight, PackedInt4Weight
 
 def _lora_is_active(lora_mapping: Any) -> bool:
     """True only when some request carries an adapter (``_fused_awq_pair.py:45-58``): a list of
-    Nones (plain requests) keeps fusion on."""
+    Nones (plain requests) keeps fusion on.  A tensor is the rows' ids of :meth:`AWQConfig.apply`: active whatever they
+    are, since what they hold is on the device, and 0 is an adapter."""
     if lora_mapping is None:
         return False
+    if isinstance(lora_mapping, torch.Tensor):
+        return lora_mapping.numel() > 0
     count = getattr(lora_mapping, "adapter_count", None)
     if count is not None:
         return int(count) > 0

@@ -80,3 +80,20 @@ def test_fused_pair_matches_oracle_and_separate_calls(M, zeros):
                      ops.gemm(x, b.qweight, b.scales, b.qzeros, G, bias=b.bias, layout="autoawq")], 1)
     rep2 = O.error_report(y.cpu().numpy(), sep.cpu().numpy())
     assert rep2["max_ulp"] <= 1.0, rep2
+
+
+@pytest.mark.parametrize("ids", [[0], [0, 1], [-1], [-1, 4, 0]])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_ids_of_rows_keep_pairs_apart(ids, dtype):
+    """The ids that AWQConfig.apply takes, instead of a mapping: the pairs would leave the adapters out.  Adapter 0 is one too."""
+    from litevllm_amd import try_fused_awq_gate_up_activation
+    p = make_awq_problem(1, 128, 64, 64, seed=1)
+    x, own, ids = torch.zeros(len(ids), 128, dtype=torch.float16), nn.Module(), torch.tensor(ids, dtype=dtype)
+    assert try_fused_awq_pair_matmul(x, _lin(p), _lin(p), own, "k", lora_mapping=ids) is None
+    assert not hasattr(own, "_fused_awq_pair_k")
+    # sizes that do not match are looked at next, so ids that are let through end there
+    lin, taken = SimpleNamespace(input_size=128, output_size=64), []
+    other = type("Looked", (), {"input_size": property(lambda self: taken.append(1) or 128), "output_size": 64, "bias": torch.zeros(64)})()
+    assert try_fused_awq_gate_up_activation(x, lin, other, activation="silu", lora_mapping=ids) is None
+    assert not taken
+    assert not _lora_is_active(ids[:0])
