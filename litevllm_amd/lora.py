@@ -127,6 +127,15 @@ class LoRAAdapters(nn.Module):
         self.lora_b = nn.Parameter(lora_b, requires_grad=False)
         self.scales = None if scales is None else nn.Parameter(scales, requires_grad=False)
 
+    def _apply(self, fn, recurse=True):
+        """A cast of the module is one of the adapters: the scales keep their 32 bits, as 16 / 12 in bf16 would be off by 2^-9 in
+        every value that they weight, and go along to another device."""
+        before = None if self.scales is None else self.scales.data
+        super()._apply(fn, recurse)
+        if before is not None and self.scales.dtype is not before.dtype:
+            self.scales.data = before.to(self.scales.device)
+        return self
+
     @classmethod
     def stack(cls, adapters: Sequence[tuple[torch.Tensor, torch.Tensor, float]]) -> "LoRAAdapters":
         """Of ``(A [r, K], B [N, r], scale)`` of any ranks, zeros behind the lower ones."""
@@ -147,5 +156,5 @@ class LoRAAdapters(nn.Module):
         """:func:`lora_add` with these adapters."""
         scales = self.scales
         if scales is not None and scales.dtype is not torch.float32:
-            scales = scales.float()  # the module was cast as a whole
+            scales = scales.float()  # given so
         return lora_add(base, x, self.lora_a, self.lora_b, ids, scales, out)

@@ -426,3 +426,25 @@ def test_entry_refuses():
     assert call(m=0) == call(n=0) == L.OK
     for m, k, r in ((0, 8, 4), (-1, 8, 4), (2, 0, 4), (2, 8, 0), (2, 8, 257), ((1 << 30) + 1, 8, 4), (2, (1 << 24) + 1, 4)):
         assert lib.awq_w4a16_lora_workspace_bytes(m, k, r) == 0
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.float16),
+                                  lambda m: torch.nn.ModuleList([m]).bfloat16()[0], lambda m: m.double().half(), lambda m: m.half().float()])
+def test_scales_keep_their_bits_when_the_module_is_cast(cast):
+    """16 / 12 is not a bf16 number, and 2^20 is past fp16's range."""
+    from litevllm_amd import LoRAAdapters
+    layer = LoRAAdapters.stack([(torch.ones(12, 8), torch.ones(10, 12), 16 / 12), (torch.ones(4, 8), torch.ones(10, 4), 2.0 ** 20)])
+    want, state = layer.scales.detach().clone(), {k: v.clone() for k, v in layer.state_dict().items()}
+    got = cast(layer)
+    assert got.scales.dtype == torch.float32 and torch.equal(got.scales, want) and not got.scales.requires_grad
+    assert isinstance(got.scales, torch.nn.Parameter) and [k for k, _ in got.named_parameters()] == ["lora_a", "lora_b", "scales"]
+    got.load_state_dict(state)
+    assert torch.equal(got.scales, want)
+    assert cast(LoRAAdapters(torch.ones(1, 4, 8), torch.ones(1, 10, 4))).scales is None
+
+
+def test_scales_follow_the_module_to_another_device():
+    from litevllm_amd import LoRAAdapters
+    layer = LoRAAdapters(torch.ones(1, 4, 8), torch.ones(1, 10, 4), torch.ones(1)).to("meta", torch.bfloat16)
+    assert layer.scales.is_meta and layer.scales.dtype == torch.float32 and layer.lora_a.dtype == torch.bfloat16
+    assert layer.to_empty(device="cpu").scales.shape == (1,)
