@@ -36,7 +36,7 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
     ``out`` may be ``base`` itself, and lie over ``x`` or parts of ``base`` (which are copied first), over
     no other operand.  Rows of the same adapter are cheapest next to each other, as a
     request's tokens are.  Results are bitwise reproducible.  Not differentiable: a backward through the result
-    raises, and so does a call with ``out`` where an input requires a gradient."""
+    raises, and so does a call with ``out`` where an input or ``out`` requires a gradient."""
     dev = ops._require_device(base, x, lora_a, lora_b, ids, scales, out)
     a_shape, b_shape, x_shape, dtype = lora_a.shape, lora_b.shape, x.shape, x.dtype
     if len(a_shape) != 3 or len(b_shape) != 3 or a_shape[0] != b_shape[0] or a_shape[1] != b_shape[2]:
@@ -65,7 +65,7 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
         raise ValueError(f"ids must be {tuple(lead)}, got {tuple(ids.shape)}")
     if scales is not None and (scales.dtype is not torch.float32 or scales.shape != (adapters,)):
         raise ValueError(f"scales must be fp32 [{adapters}], got {scales.dtype} {tuple(scales.shape)}")
-    asked = _derivative_asked("lora_add", out, base, x, lora_a, lora_b, scales)
+    asked = _derivative_asked("lora_add", out, base, x, lora_a, lora_b, scales, out)  # out's graph would not hear of the call
     m = ids.numel()
     given = out is not None
     if not given:

@@ -448,3 +448,22 @@ def test_scales_follow_the_module_to_another_device():
     layer = LoRAAdapters(torch.ones(1, 4, 8), torch.ones(1, 10, 4), torch.ones(1)).to("meta", torch.bfloat16)
     assert layer.scales.is_meta and layer.scales.dtype == torch.float32 and layer.lora_a.dtype == torch.bfloat16
     assert layer.to_empty(device="cpu").scales.shape == (1,)
+
+
+@pytest.mark.gpu
+def test_out_that_a_backward_goes_through_is_refused():
+    """A result that a graph already holds would keep the derivative of what was there before."""
+    from litevllm_amd import lora_add
+    g = torch.Generator().manual_seed(11)
+    x, base, a, b = _whole(g, 6, 32).half(), _whole(g, 6, 40).half(), _whole(g, 2, 4, 32).half(), _whole(g, 2, 40, 4).half()
+    ids, w = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.ones(6, 40, dtype=torch.float16, device="cuda", requires_grad=True)
+    want, y = lora_add(base, x, a, b, ids), w * 2
+    for out in (w, y, y[:]):
+        before = out.detach().clone()
+        with pytest.raises(RuntimeError, match="require a gradient"):
+            lora_add(base, x, a, b, ids, out=out)
+        assert torch.equal(out.detach(), before)
+    y.sum().backward()
+    assert bool((w.grad == 2).all())
+    with torch.no_grad():
+        assert torch.equal(lora_add(base, x, a, b, ids, out=w), want)
