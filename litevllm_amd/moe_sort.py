@@ -93,7 +93,8 @@ class _Sort(torch.autograd.Function):
 class _Unsort(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, places, offsets):
-        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, places, offsets)
+        of_rows, of_weights, _, _ = ctx.needs_input_grad  # what each gradient reads, so that the rest may change
+        ctx.save_for_backward(rows if of_weights else None, weights if of_rows else None, places, offsets if of_rows else None)
         ctx.of = (rows.shape, rows.dtype, places.shape, None if weights is None else weights.dtype, offsets.shape,
                   ops.dtype_code(rows.dtype), L.DTYPE_NONE if weights is None else ops.dtype_code(weights.dtype))
         return _unsorted(rows, weights, places)
@@ -104,7 +105,7 @@ class _Unsort(torch.autograd.Function):
         shape, dtype, routes, wdtype, experts, code, wcode = ctx.of
         on = upstream.get_device()
         if places.shape != routes or places.dtype is not torch.int32 or places.get_device() != on or (
-                offsets.shape != experts or offsets.dtype is not torch.int32 or offsets.get_device() != on) or (
+                offsets is not None and (offsets.shape != experts or offsets.dtype is not torch.int32 or offsets.get_device() != on)) or (
                 rows is not None and (rows.shape != shape or rows.dtype is not dtype or rows.get_device() != on)) or (
                 weights is not None and (weights.shape != routes or weights.dtype is not wdtype or weights.get_device() != on)):
             raise _elsewhere("moe_unsort")
@@ -114,8 +115,8 @@ class _Unsort(torch.autograd.Function):
         grad_weights = upstream.new_empty(routes, dtype=wdtype) if want_weights else None
         read, w, places, offsets = (None if t is None else t.contiguous() for t in (rows, weights, places, offsets))
         _call(upstream.device, "awq_w4a16_moe_unsort_grad", flat.data_ptr(), ld, ops._ptr(read), places.data_ptr(),
-              offsets.data_ptr() + 4 * (experts[0] - 1), ops._ptr(w), wcode, ops._ptr(grad_rows), ops._ptr(grad_weights), routes[0],
-              shape[1], routes[1], code)
+              None if offsets is None else offsets.data_ptr() + 4 * (experts[0] - 1), ops._ptr(w), wcode, ops._ptr(grad_rows),
+              ops._ptr(grad_weights), routes[0], shape[1], routes[1], code)
         if torch.is_grad_enabled():
             inputs = upstream, rows, weights
             grad_rows, grad_weights = (None if g is None else _Refused.apply("moe_unsort is not differentiable twice", g, *inputs)

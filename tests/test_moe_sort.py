@@ -498,3 +498,24 @@ def test_a_training_step_of_a_routed_layer():
     want = [ref.detach(), *torch.autograd.grad(ref, (xd, wd, gd), up.double())]
     for a, b in zip(got, want):
         assert torch.equal(a.double(), b)
+
+
+@pytest.mark.gpu
+def test_a_backward_in_the_weights_alone_needs_only_the_rows():
+    """dw = <dout, rows>: weights and offsets may change in front of it, as beside any product whose other factor is constant."""
+    from litevllm_amd import moe_sort, moe_unsort
+    x, w, ids, up = _whole(80, 30, 24), _whole(81, 30, 3).requires_grad_(True), _ids(82, 30, 7, 3, 0.2), _whole(83, 30, 24)
+    rows, routes = moe_sort(x, ids, 7)
+    want, = torch.autograd.grad(moe_unsort(rows, w, routes), w, up)
+    out = moe_unsort(rows, w, routes)
+    with torch.no_grad():
+        w.mul_(3)
+        routes.offsets.zero_()
+    got, = torch.autograd.grad(out, w, up)
+    assert torch.equal(got, want)
+    rows, routes = moe_sort(x, ids, 7)
+    out = moe_unsort(rows.requires_grad_(True), w, routes)  # rows' gradient needs them
+    with torch.no_grad():
+        w.mul_(3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, w, up)
