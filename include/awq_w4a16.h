@@ -505,7 +505,8 @@ int awq_w4a16_moe_unsort_grad(const void* upstream, int64_t ldu, const void* row
 /* ---- low-rank adapters of many requests -------------------------------------------------
  * What the reference adds behind a layer's quantised product (lite_linear.py:65-78), for all rows in one call:
  *   out[m] = base[m] + s[l] (x[m] A_l^T) B_l^T,  l = ids[m];  out[m] = base[m] for an id outside [0, L).
- * Sums in fp32; x A^T enters the second product with 16 bits of mantissa (bf16) or 21 (fp16); one rounding.
+ * Sums in fp32, one rounding of the result; x A^T enters the second product off by at most 2^-17 of itself (bf16), or
+ * 2^-22 of itself or 2^-38 of the row's largest of 32 neighbouring ranks, whichever is more (fp16).
  *   x: [M, K], base (NULL: zeros) and out: [M, N], all of dtype (F16 or BF16), row strides ldx, ldb, ldo;  lora_a: [L, R, K] and
  *   lora_b: [L, N, R], dense but for the stride between adapters;  ids: [M] int32 or int64;  scales: [L] or NULL (1).
  *   R <= 256; M, N and K <= 2^24.  Two bytes are alignment enough; 16 are faster.  out may be base (with its stride) and

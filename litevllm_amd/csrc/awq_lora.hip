@@ -8,10 +8,13 @@
 // than some (group_of).  Its blocks (`slots`) share these and, where it has fewer adapters than blocks, an adapter's columns or K.
 // The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
 //
-// v enters the second product as two 16-bit numbers, v = high + low: 16 bits of mantissa at least for bf16, 21 for fp16, and
-// one rounding for the output.  Both halves meet the same B: ranks go in tiles of W = 32, an instruction for the high parts and
-// one for the low parts, or of 16 (rank 16 and less), high and low parts in one instruction of depth 32.  fp16 takes v / 2^e
-// instead, with an e of its own for a row's tile that puts the largest value at 2^13 .. 2^14: v may pass fp16's range.
+// v enters the second product as two 16-bit numbers, v = high + low, and the output is rounded once.  Both halves meet the same B:
+// ranks go in tiles of W = 32, an instruction for the high parts and one for the low parts, or of 16 (rank 16 and less), high and
+// low parts in one instruction of depth 32.  fp16 takes v / 2^e instead, with an e of its own for a row's tile that puts the
+// largest value at 2^13 .. 2^14: v may pass fp16's range.
+// high + low is off from v by at most 2^-17 of v in bf16 (two times eight bits and low's sign; for v above 2^-109, where low is a
+// normal number).  In fp16 that is 2^-22 of v down to 2^-16 of the tile's largest value; below, low ends with fp16's smallest
+// step, 2^-24 in units of 2^e, and the error stays at 2^-38 of that largest value: a rank 2^26 below it still has 12 bits.
 #include <algorithm>
 
 #include "awq_launch.h"

@@ -32,7 +32,8 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
 
     ``x [..., K]``, ``base [..., N]`` (None: zeros), fp16 or bf16; ``lora_a [L, R, K]`` and ``lora_b [L, N, R]`` in their type, R up
     to 256 (adapters of lower ranks: zeros, :meth:`LoRAAdapters.stack`); ``ids [...]`` int32 or int64; ``scales`` fp32 ``[L]`` or
-    None (1).  Sums in fp32, ``x @ A^T`` enters the second product with 16 bits of mantissa (bf16) or 21 (fp16), one rounding.
+    None (1).  Sums in fp32, one rounding of the result; ``x @ A^T`` enters the second product off by at most 2^-17 of itself
+    (bf16), or 2^-22 of itself or 2^-38 of the row's largest of 32 neighbouring ranks, whichever is more (fp16).
     ``out`` may be ``base`` itself, and lie over ``x`` or parts of ``base`` (which are copied first), over
     no other operand.  Rows of the same adapter are cheapest next to each other, as a
     request's tokens are.  Results are bitwise reproducible.  Not differentiable: a backward through the result

@@ -467,3 +467,39 @@ def test_out_that_a_backward_goes_through_is_refused():
     assert bool((w.grad == 2).all())
     with torch.no_grad():
         assert torch.equal(lora_add(base, x, a, b, ids, out=w), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("r", [16, 40])
+@pytest.mark.parametrize("m,k", [(3, 64), (100, 4200), (600, 64), (1, 5), (600, 5)])
+def test_low_rank_values_far_apart(m, k, r, dtype):
+    """Values of v a factor of up to 2^34 apart in a row, columns of B that are zero at the large ones.  Each is off by
+    2^-17 of itself in bf16; in fp16 by 2^-22 of itself or 2^-38 of the largest of the 16 or 32 ranks beside it (its low half
+    ends at 2^-24 where that largest is 2^13 at least), whichever is more.  Every rank has an input of its own, so v is one product."""
+    from litevllm_amd import lora_add
+    g, dt, n = torch.Generator().manual_seed(m + r), DTYPES[dtype], 90
+    at = torch.arange(r) % k                                 # a rank's input
+    steps = (torch.arange(r) * 7 % 18).double()
+    mantissa = lambda *s: 1 + torch.rand(*s, generator=g, dtype=torch.float64)
+    x, a, b = torch.zeros(m, k, dtype=torch.float64), torch.zeros(1, r, k, dtype=torch.float64), torch.zeros(1, n, r, dtype=torch.float64)
+    scale = torch.zeros(k, dtype=torch.float64)
+    scale[at] = 9 - steps                                     # ranks that share an input (k < r) have one exponent of it
+    x[:] = mantissa(m, k) * 2.0 ** scale
+    a[0, torch.arange(r), at] = mantissa(r) * 2.0 ** (9 - steps)
+    one = torch.arange(n) % r                                 # a column's rank; some have more
+    b[0, torch.arange(n), one] = mantissa(n) * 2.0 ** (steps - 11 - scale[at])[one]  # v B is about 1/4
+    b[0, ::5, :] += (torch.rand(n, r, generator=g, dtype=torch.float64) < 0.1)[::5] * 2.0 ** -18
+    x, a, b = (t.to(dt).cuda() for t in (x, a, b))
+    ids = torch.zeros(m, dtype=torch.int32, device="cuda")
+    want = _reference(None, x, a, b, ids, None)
+    v = (x.double() @ a[0].double().t().contiguous()).abs()
+    w, f = 16 if r <= 16 else 32, torch.finfo(dt)
+    top = torch.cat([v[:, i:i + w].amax(1, keepdim=True).expand(m, min(w, r - i)) for i in range(0, r, w)], 1)
+    off = v * 2.0 ** -17 if dt == torch.bfloat16 else torch.maximum(v * 2.0 ** -22, top * 2.0 ** -38)
+    weight = b[0].double().abs().t().contiguous()
+    terms = v @ weight
+    tol = off @ weight + terms * (r + 8) * 2.0 ** -23 + want.abs() * f.eps / 2 + f.smallest_normal * f.eps
+    got = lora_add(None, x, a, b, ids)
+    bad = (got.double() - want).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - want).abs() / tol).max()))
