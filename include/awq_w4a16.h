@@ -510,7 +510,8 @@ int awq_w4a16_moe_unsort_grad(const void* upstream, int64_t ldu, const void* row
  *   x: [M, K], base (NULL: zeros) and out: [M, N], all of dtype (F16 or BF16), row strides ldx, ldb, ldo;  lora_a: [L, R, K] and
  *   lora_b: [L, N, R], dense but for the stride between adapters;  ids: [M] int32 or int64;  scales: [L] or NULL (1).
  *   R <= 256; M, N and K <= 2^24.  Two bytes are alignment enough; 16 are faster.  out may be base (with its stride) and
- *   lies apart from everything else.  Results are bitwise reproducible.
+ *   lies apart from everything else.  The same call gives the same bits; the order of a row's fp32 sums may follow M and the
+ *   adapters of the other rows.
  *   workspace: 16-byte aligned, no zeroing needed; calls that may overlap must not share one. */
 size_t awq_w4a16_lora_workspace_bytes(int64_t M, int64_t K, int64_t R);
 int awq_w4a16_lora_add(const void* base, int64_t ldb, const void* x, int64_t ldx, const void* lora_a, int64_t a_stride,

@@ -34,10 +34,11 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
     to 256 (adapters of lower ranks: zeros, :meth:`LoRAAdapters.stack`); ``ids [...]`` int32 or int64; ``scales`` fp32 ``[L]`` or
     None (1).  Sums in fp32, one rounding of the result; ``x @ A^T`` enters the second product off by at most 2^-17 of itself
     (bf16), or 2^-22 of itself or 2^-38 of the row's largest of 32 neighbouring ranks, whichever is more (fp16).
-    ``out`` may be ``base`` itself, and lie over ``x`` or parts of ``base`` (which are copied first), over
-    no other operand.  Rows of the same adapter are cheapest next to each other, as a
-    request's tokens are.  Results are bitwise reproducible.  Not differentiable: a backward through the result
-    raises, and so does a call with ``out`` where an input or ``out`` requires a gradient."""
+    ``out`` may be ``base`` itself, and lie over ``x`` or parts of ``base`` (which are copied first), over no other operand.
+    Rows of the same adapter are cheapest next to each other, as a request's tokens are.  The same call gives the same bits; the
+    order of a row's fp32 sums, and so its last bit, may follow how many rows the call has and which adapters they name.
+    Not differentiable: a backward through the result raises, and so does a call with ``out`` where an input or ``out``
+    requires a gradient."""
     dev = ops._require_device(base, x, lora_a, lora_b, ids, scales, out)
     a_shape, b_shape, x_shape, dtype = lora_a.shape, lora_b.shape, x.shape, x.dtype
     if len(a_shape) != 3 or len(b_shape) != 3 or a_shape[0] != b_shape[0] or a_shape[1] != b_shape[2]:

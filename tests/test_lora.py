@@ -503,3 +503,22 @@ def test_low_rank_values_far_apart(m, k, r, dtype):
     got = lora_add(None, x, a, b, ids)
     bad = (got.double() - want).abs() > tol
     assert not bool(bad.any()), (int(bad.sum()), float(((got.double() - want).abs() / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,k,r", [(29, 12288, 12), (100, 4096, 64), (300, 5000, 40)])
+def test_a_row_among_other_neighbours(m, k, r, dtype):
+    """Two launches: which blocks share K, and so the order of fp32 sums, follows the adapters of the batch.  A row keeps its
+    value but for those sums, each within _check_random's bound of the exact value."""
+    from litevllm_amd import lora_add
+    g, dt, n = torch.Generator().manual_seed(m), DTYPES[dtype], 72
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    x, base, a, b = rnd(m, k), rnd(m, n), rnd(m, r, k), rnd(m, n, r)
+    own, shared = torch.arange(m, device="cuda"), torch.full((m,), 5, device="cuda")
+    shared[m // 2:] = 3
+    for ids in (own, shared, own.flip(0), torch.where(own == 5, 5, -1)):
+        got = _check_random(base, x, a, b, ids, None)
+        assert torch.equal(lora_add(base, x, a, b, ids), got)
+    order = torch.randperm(m, generator=g).cuda()
+    _check_random(base[order], x[order], a, b, shared[order], None)
