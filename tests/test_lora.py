@@ -522,3 +522,22 @@ def test_a_row_among_other_neighbours(m, k, r, dtype):
         assert torch.equal(lora_add(base, x, a, b, ids), got)
     order = torch.randperm(m, generator=g).cuda()
     _check_random(base[order], x[order], a, b, shared[order], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("m,requests,n,r", [(1400, 5, 24581, 20), (1401, 60, 24576, 64), (530, 3, 65003, 130), (1100, 2, 32011, 16), (9000, 40, 4100, 7)])
+def test_results_that_pass_the_caches(m, requests, n, r, dtype):
+    """2^25 results and more from a base, with rows of no adapter and odd columns; in place the same."""
+    from litevllm_amd import lora_add
+    g, dt, adapters, k = torch.Generator().manual_seed(m), DTYPES[dtype], 7, 64
+    assert m * n >= 2 ** 25
+    x, a, b = _whole(g, m, k, size=1).to(dt), _whole(g, adapters, r, k, size=1).to(dt), _whole(g, adapters, n, r, size=1).to(dt)
+    base, ids = _whole(g, m, n, size=100).to(dt), _ids(g, m, adapters, requests, 0.3)
+    got = _check_exact(base, x, a, b, ids, None)
+    assert torch.equal(lora_add(base, x, a, b, ids, out=base), got)
+    wide = torch.full((m, n + 9), 7.0, dtype=dt, device="cuda")  # rows apart, at other alignments
+    lora_add(None, x, a, b, ids, out=wide[:, 4:n + 4])
+    assert bool((wide[:, :4] == 7).all()) and bool((wide[:, n + 4:] == 7).all())
+    want = _reference(None, x, a, b, ids, None)
+    assert torch.equal(wide[:, 4:n + 4], want.to(dt))
