@@ -541,3 +541,41 @@ def test_results_that_pass_the_caches(m, requests, n, r, dtype):
     assert bool((wide[:, :4] == 7).all()) and bool((wide[:, n + 4:] == 7).all())
     want = _reference(None, x, a, b, ids, None)
     assert torch.equal(wide[:, 4:n + 4], want.to(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["awq", "symmetric", "mxfp4", "dense"])
+def test_layers_with_adapters_take_the_types_of_the_adapters(kind):
+    """bf16 as fp16; rows of 32 bits, which dense layers and unpacked int4 take, are refused instead of rounded, and so are
+    adapters of another type than the rows."""
+    from litevllm_amd import AWQConfig, LoRAAdapters, mxfp4_quantize
+    from oracle.gen import make_awq_problem
+    m, k, n = 24, 256, 384
+    g = torch.Generator().manual_seed(12)
+    rnd = lambda *s: torch.randn(*s, generator=g).cuda()
+    cfg, layer = AWQConfig(group_size=128, layout="autoawq"), SimpleNamespace(prefix="model.layers.0.self_attn.o_proj", bias=None)
+    if kind in ("awq", "symmetric"):
+        p = make_awq_problem(M=m, K=k, N=n, group_size=128, seed=5)
+        layer.qweight, layer.scales = (torch.from_numpy(p[i]).cuda() for i in ("qweight", "scales"))
+        layer.qzeros = torch.from_numpy(p["qzeros"]).cuda() if kind == "awq" else None
+    elif kind == "mxfp4":
+        layer.qweight, layer.scales = mxfp4_quantize(rnd(n, k))
+    else:
+        layer.qweight, layer.weight = None, (rnd(n, k) * 0.05).bfloat16()
+    layer.lora_adapters = LoRAAdapters.stack([(rnd(8, k) * 0.05, rnd(n, 8), 2.0), (rnd(12, k) * 0.05, rnd(n, 12), 0.7)]).bfloat16()
+    x, ids = rnd(m, k).bfloat16(), _ids(g, m, 2, m, 0.3)
+    with torch.no_grad():
+        plain = cfg.apply(layer, x)
+        got = cfg.apply(layer, x, lora_ids=ids)
+    assert plain.dtype == got.dtype == torch.bfloat16
+    a, b, s = layer.lora_adapters.lora_a.data, layer.lora_adapters.lora_b.data, layer.lora_adapters.scales.data
+    want, terms = _reference(plain, x, a, b, ids, s), _reference(None, x.abs(), a.abs(), b.abs(), ids, s)
+    tol = want.abs() * 2.0 ** -8 + terms * ((k + 20) * 2.0 ** -23 + 2.0 ** -17) + 2.0 ** -130
+    assert bool(((got.double() - want).abs() <= tol).all())
+    for rows in (x.float(), x.half()):
+        if kind == "dense":
+            layer.weight = layer.weight.to(rows.dtype)
+        if kind != "mxfp4" or rows.dtype == torch.float16:
+            cfg.apply(layer, rows)  # without ids it is taken
+            with pytest.raises(TypeError):
+                cfg.apply(layer, rows, lora_ids=ids)
