@@ -1,6 +1,6 @@
 """The tokens' rows in the order of the experts that :func:`moe_route` chose, and back at the tokens with the routing's weights,
-for experts whose products the grouped kernels do not take (dense ones, ones that are trained, low-rank adapters of
-experts by :func:`lora_add`)."""
+for experts whose products the grouped kernels do not take: dense ones, ones that are trained, and, where nothing is trained,
+experts with low-rank adapters of their own (:func:`lora_add`, which has no derivative)."""
 from __future__ import annotations
 
 from typing import NamedTuple
