@@ -33,8 +33,10 @@ class QuantizationConfig:
 
 def _with_lora(layer: nn.Module, y: torch.Tensor, x: torch.Tensor, ids: torch.Tensor | None) -> torch.Tensor:
     """``y`` with the layer's adapters for the rows' ``ids``; without either as it is: not every layer has adapters."""
+    if ids is None:
+        return y
     adapters = getattr(layer, "lora_adapters", None)
-    if ids is None or adapters is None:
+    if adapters is None:
         return y
     # y is this call's own: it takes the sum itself where no derivative can be asked for
     return adapters.add(y, x, ids, out=None if torch.is_grad_enabled() else y)

@@ -579,3 +579,20 @@ def test_layers_with_adapters_take_the_types_of_the_adapters(kind):
             cfg.apply(layer, rows)  # without ids it is taken
             with pytest.raises(TypeError):
                 cfg.apply(layer, rows, lora_ids=ids)
+
+
+def test_calls_without_ids_do_not_look_for_adapters():
+    """A missing attribute of a module costs a call about 1 us."""
+    from litevllm_amd import AWQConfig
+
+    class Layer(torch.nn.Module):
+        bias, looked = None, 0
+
+        @property
+        def lora_adapters(self):
+            self.looked += 1
+    layer = Layer()
+    layer._quant_weight = SimpleNamespace(matmul=lambda x, bias, config: x)
+    x = torch.ones(1, 8)
+    assert AWQConfig().apply(layer, x) is x and layer.looked == 0
+    assert AWQConfig().apply(layer, x, lora_ids=torch.zeros(1, dtype=torch.int32)) is x and layer.looked == 1
