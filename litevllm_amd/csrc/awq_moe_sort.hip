@@ -78,7 +78,7 @@ __device__ __forceinline__ u32x4 packed(const float* v) {
 
 // Which token and piece a thread has: rows of at most half a block's pieces share blocks, longer ones take one or several.
 struct RowGrid {
-  int pieces, per_block;  // tokens of a block; 1 where a row has blocks of its own
+  int pieces, per_block;  // tokens of a block, two at least; 1 where a row has blocks of its own
 };
 struct TokenPiece {
   int64_t token;
@@ -383,7 +383,7 @@ static RowLaunch row_launch(int64_t T, int64_t H, int vec) {
   const int pieces = (int)cdiv(H, vec), ny = (int)cdiv(pieces, 256);
   if (pieces <= 128) {
     const int per = 256 / pieces;
-    return {{pieces, per == 1 ? 2 : per}, dim3((unsigned)cdiv(T, per)), dim3(256)};
+    return {{pieces, per}, dim3((unsigned)cdiv(T, per)), dim3(256)};
   }
   return {{pieces, 1}, dim3((unsigned)T, (unsigned)ny), dim3((unsigned)(cdiv(cdiv(pieces, ny), 64) * 64))};
 }
