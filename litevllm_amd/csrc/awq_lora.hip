@@ -2,10 +2,11 @@
 //
 //   l = ids[m];  v[m] = s_l x[m] A_l^T  (rank values);  out[m] = base[m] + v[m] B_l^T;  out[m] = base[m] without an adapter
 //
-// Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once).  Rows go in tiles of 16 that the matrix cores
-// take; a tile looks up which adapters its rows have and is worked on once for each: once where the rows of a request lie
-// together, as in prompts, up to 16 times in a batch of single tokens, whose rows are put together by adapter where there are more
-// than some (group_of).  Its blocks (`slots`) share these and, where it has fewer adapters than blocks, an adapter's columns or K.
+// Two launches: the ranks (x and A once, sums in fp32) and the columns (base and B once); one for few rows whose adapters are
+// small, where the blocks of columns compute their v themselves (lora_plan).  Rows go in tiles of 16 that the matrix cores take; a
+// tile looks up which adapters its rows have and is worked on once for each: once where the rows of a request lie together,
+// as in prompts, up to 16 times in a batch of single tokens, whose rows are put together by adapter from 65 to 512 rows
+// (group_of).  Its blocks (`slots`) share these and, where it has fewer adapters than blocks, an adapter's columns or K.
 // The matrix cores do not mix rows, so the other rows of a tile only cost idle lanes.
 //
 // v enters the second product as two 16-bit numbers, v = high + low, and the output is rounded once.  Both halves meet the same B:
@@ -68,8 +69,8 @@ struct GroupLds {
   GroupRecord found;
 };
 __device__ __forceinline__ Group recorded(const GroupRecord& r) {
-  return {__builtin_amdgcn_readfirstlane(r.adapter), (uint32_t)__builtin_amdgcn_readfirstlane(r.rows), __builtin_amdgcn_readfirstlane(r.part),
-          __builtin_amdgcn_readfirstlane(r.parts), r.row[threadIdx.x & 15]};
+  return {__builtin_amdgcn_readfirstlane(r.adapter), (uint32_t)__builtin_amdgcn_readfirstlane(r.rows),
+          __builtin_amdgcn_readfirstlane(r.part), __builtin_amdgcn_readfirstlane(r.parts), r.row[threadIdx.x & 15]};
 }
 // By one wave.
 __device__ __forceinline__ void record(const Group& g, GroupRecord& r) {
@@ -215,9 +216,10 @@ union RankLds {
 };
 // RT tiles of 16 ranks, from tile0 on, of adapter `cur` by the rows row(0 .. 15) and a share of K, whose units the waves take in
 // turn; the waves' sums come to lie in LDS.  A wave's next unit is on its way in registers (more of them made every size slower:
-// one row, K = N = 4096, rank 16 6.6 us with two, 7.3 with four, 6.3 as it is).  Loads cover whole lines, eight lanes each; a wave passes them through LDS of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and
-// 32 + 8 q .. of rank i and of row i.  (Straight from memory in that order a load's neighbouring lanes are in different lines:
-// 4096 rows, K = 4096, rank 64 42 us instead of 12.)
+// one row, K = N = 4096, rank 16 6.6 us with two, 7.3 with four, 6.3 as it is).  Loads cover whole lines, eight lanes each; a
+// wave passes them through LDS of its own into the matrix cores' order, where lane (q, i) holds values 8 q .. 8 q + 7 and 32 + 8 q
+// .. of rank i and of row i.  (Straight from memory in that order a load's neighbouring lanes are in different lines: 4096 rows,
+// K = 4096, rank 64 42 us instead of 12.)
 template <typename T, int RT, int WAVES, class Row>
 __device__ __forceinline__ void tile_ranks(const LoraArgs& p, RankLds<RT, WAVES>& lds, Row row, int cur, int tile0, int begin, int units) {
   constexpr int TILES = 1 + RT;
@@ -293,9 +295,9 @@ __device__ __forceinline__ void put_rank(const LoraArgs& p, int64_t m, int rank,
   if (std::is_same<T, f16>::value && rank % W == 0) p.powers[m * (p.ranks / W) + rank / W] = h.power;
 }
 
-// Few rows: a block has a group of rows and a share of K; those that share the group cut the share further, into
-// sub-shares (lora_shares).  29 rows, K = 12288, rank 12: 5.2 us, latency.  What
-// it found out about a block's group is left for the second launch (the same rows, N = 5001: 12.0 -> 10.5 us for both).
+// Few rows: a block has a group of rows and a share of K; those that share the group cut the share further, into sub-shares
+// (lora_shares).  29 rows, K = 12288, rank 12: 5.2 us, latency.  What it found out about a block's group is left for the
+// second launch (the same rows, N = 5001: 12.0 -> 10.5 us for both).
 __device__ __forceinline__ int lora_shares(const LoraArgs& p, int parts) { return min(parts, p.shares / p.splits); }
 template <typename T, int RT, int W>
 __global__ void __launch_bounds__(256) lora_ranks_few_kernel(LoraArgs p) {

@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
 }
 
 // A block places the routes of its tokens and copies their rows.  Bound by its chain (ids, counts, scan, places, rows): 4 tokens 4.3
-// us, of 2048 tokens, top 8, H = 2048 with the counts' launch 19.5, a copy of the same bytes 15.  For that it counts the routes in front of its own and all of
-// them, by expert: in LDS where they are few, else those in front of it in its segment and the rest from the segments' counts.
-// Its own, at most kMostOwn, are placed by one wave, 64 at a time in their order; lanes of the same expert find each
-// other by its bits.
+// us, 2048 tokens, top 8, H = 2048 with the counts' launch 19.5, where a copy of the same bytes takes 15.  To place its routes it
+// counts those in front of its own and all of them, by expert: in LDS where they are few, else those in front of it in its segment
+// and the rest from the segments' counts.  Its own, at most kMostOwn, are placed by one wave, 64 at a time in their order; lanes
+// of the same expert find each other by its bits.
 constexpr int kMostOwn = 1024;
 template <int ES>  // 0: no rows
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(SortArgs a) {
