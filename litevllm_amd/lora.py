@@ -122,7 +122,7 @@ def lora_add(base: torch.Tensor | None, x: torch.Tensor, lora_a: torch.Tensor, l
 class LoRAAdapters(nn.Module):
     """The adapters of a linear layer: ``lora_a [L, R, K]``, ``lora_b [L, N, R]`` and ``scales`` fp32 ``[L]`` (alpha / rank; None:
     1).  As ``layer.lora_adapters`` :meth:`AWQConfig.apply` adds them to the layer's product for the ids that a call names; the
-    rows are of the adapters' type, fp16 or bf16."""
+    rows are of the adapters' type, fp16 or bf16.  The scales stay fp32 when the module is cast."""
 
     def __init__(self, lora_a: torch.Tensor, lora_b: torch.Tensor, scales: torch.Tensor | None = None):
         super().__init__()
